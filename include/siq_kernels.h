@@ -1,7 +1,7 @@
 /*
  * siq_kernels.h -- C ABI of the SiQ-VL training hot path on MI355X (gfx950).
  *
- * Five operators, all hand-written HIP behind this plain-C boundary:
+ * Hand-written HIP operators behind this plain-C boundary:
  *   1. varlen (cu_seqlens-packed) flash attention, forward and backward,
  *      causal GQA (Qwen2.5 decoder) or bidirectional (SigLIP tower);
  *   2. fused lm_head linear + cross-entropy, forward and backward, without
@@ -11,7 +11,9 @@
  *   4. the pixel-shuffle projector (vision features to text embeddings),
  *      forward and backward, with the shuffle folded into the GEMM loads;
  *   5. the splice of the projected vision rows into the token embeddings,
- *      fused with the embedding gather, and its embedding-table gradient.
+ *      fused with the embedding gather, and its embedding-table gradient;
+ *   6. activations kept in 8 bits for the backward pass, and the gated MLP
+ *      activation over them.
  *
  * Conventions
  *  - Every entry point returns an int status (SIQ_OK = 0, < 0 on error) and
@@ -54,6 +56,10 @@ enum siq_status {
 /* Element types of the entry points that take more than one. */
 #define SIQ_DTYPE_BF16 0
 #define SIQ_DTYPE_FP32 1
+
+/* Formats of 8-bit storage (siq_pack8). */
+#define SIQ_FORMAT_INT8 0
+#define SIQ_FORMAT_E4M3 1
 
 /* Version of this ABI (SIQ_ABI_VERSION of the library that was built). */
 int siq_abi_version(void);
@@ -388,6 +394,52 @@ size_t siq_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab);
 int siq_embedding_bwd(const void* grad, const int64_t* input_ids, int64_t n_tokens, int64_t vocab, int64_t hidden,
                       int dtype, int64_t skip_id0, int64_t skip_id1, void* dweight, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Activations in 8 bits for the backward pass.
+ *
+ * No counterpart in the reference, which keeps them in bf16 (and, with
+ * gradient_checkpointing, one input for each decoder layer:
+ * scripts/train.py:714).
+ *
+ * siq_pack8: x [numel] (dtype SIQ_DTYPE_BF16 or _FP32, contiguous) in codes
+ * [numel] bytes and scales [ceil(numel / 32)] bytes, one for each 32
+ * neighbours.  With a the largest magnitude of the 32, the scale byte b is the
+ * biased exponent of a, one more where a would round past the largest code:
+ *   SIQ_FORMAT_INT8: x = code * 2^(b - 133), code a signed byte in [-127, 127];
+ *   SIQ_FORMAT_E4M3: x = code * 2^(b - 135), code an OCP e4m3 number.
+ * b is at least 7 (int8) or 9 (e4m3), so steps are normal numbers: groups
+ * whose largest magnitude lies below 2^-120 (2^-118) lose precision.  Codes are
+ * rounded to nearest even, by at most half a step (int8; fp32 magnitudes
+ * above 1.99 * 2^127: one step) or half a unit of their last place (e4m3).
+ * b = 255 marks a group that holds an infinity or a NaN: all of it unpacks to
+ * NaN.  siq_unpack8 writes code * step, exactly.
+ * All pointers 16-byte aligned; numel at most 2^35.  No workspace.
+ *
+ * siq_swiglu8_fwd: h = silu(gate) up of rows x cols elements (the gated MLP
+ * activation of transformers' Qwen2MLP), and gate and
+ * up packed as siq_pack8 packs the contiguous [rows, cols] tensors; the four
+ * packed outputs may be NULL together (nothing is kept: evaluation).  Rows are
+ * gate_stride / up_stride elements apart (halves of one product); unless both
+ * strides equal cols, they must be multiples of 16 bytes and cols of 8.  h is
+ * contiguous.
+ * siq_swiglu8_bwd: with g, u the unpacked values and s = 1 / (1 + exp(-g)),
+ *   dup = dh g s,  dgate = dh u s (1 + g (1 - s)),  h = g s u
+ * (h only if not NULL: the down projection's input for its weight gradient).
+ * dh and h contiguous, dgate and dup with row strides as above.
+ * Everything in fp32, rounded once to dtype.
+ * ------------------------------------------------------------------------- */
+int siq_pack8(const void* x, int64_t numel, int dtype, int format, void* codes, void* scales, void* stream);
+
+int siq_unpack8(const void* codes, const void* scales, int64_t numel, int dtype, int format, void* x, void* stream);
+
+int siq_swiglu8_fwd(const void* gate, const void* up, int64_t rows, int64_t cols, int64_t gate_stride,
+                    int64_t up_stride, int dtype, int format, void* h, void* gate_codes, void* gate_scales,
+                    void* up_codes, void* up_scales, void* stream);
+
+int siq_swiglu8_bwd(const void* dh, const void* gate_codes, const void* gate_scales, const void* up_codes,
+                    const void* up_scales, int64_t rows, int64_t cols, int64_t dgate_stride, int64_t dup_stride,
+                    int dtype, int format, void* dgate, void* dup, void* h, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Measurement support (no reference counterpart).

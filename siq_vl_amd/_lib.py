@@ -6,6 +6,7 @@ naming the build step, never a silent CPU or PyTorch path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -17,6 +18,7 @@ from . import build as _build
 
 _LOCK = threading.Lock()
 _LIB: ctypes.CDLL | None = None
+_HERE = contextlib.nullcontext()
 
 SIQ_OK = 0
 SIQ_ERR_INVALID_ARGUMENT = -1
@@ -104,6 +106,18 @@ _PROTOS = {
     "siq_embedding_bwd_workspace_bytes": (_size, [_i64, _i64]),
     "siq_embedding_bwd": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _i64, _i64, _c_void_p, _c_void_p,
                                  _size, _c_void_p]),
+    "siq_pack8": (_i32, [_c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p]),
+    "siq_unpack8": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p]),
+    "siq_swiglu8_fwd": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p],
+    ),
+    "siq_swiglu8_bwd": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i32, _i32, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p],
+    ),
     "siq_probe_clock": (_i32, [_c_void_p, _i64, _c_void_p]),
     "siq_rope_fwd": (
         _i32,
@@ -165,6 +179,12 @@ def check(rc: int, what: str) -> None:
     if rc in (SIQ_ERR_INVALID_ARGUMENT, SIQ_ERR_UNSUPPORTED, SIQ_ERR_ALIGNMENT, SIQ_ERR_WORKSPACE):
         raise ValueError(text)
     raise RuntimeError(text)
+
+
+def on_device(device):
+    """A context in which ``device`` is the current GPU (none is entered when it
+    is already): kernels go to the current one, whatever their stream."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def int64_array(values) -> ctypes.Array:

@@ -1,0 +1,337 @@
+"""8-bit storage of activations on the GPU against the oracle in 64 bits: codes and scales bit for bit, the gated MLP
+activation and its gradients within the rounding of their type, and the ways they are called."""
+
+import gc
+import weakref
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import pack8 as op
+from siq_vl_amd import checkpoint8 as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+# half a step of the output type, relative to the value
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def awkward(n, dtype, seed=0):
+    """Values over many orders, with zero groups, groups of one large value, ties, subnormals and the type's ends."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, generator=g) * torch.exp2(torch.randint(-20, 20, (n,), generator=g).float())
+    fill = [0.0, -0.0, 127.5, 127.0, 0.5, 1.5, 2.5, 464.0, 465.0, 448.0, 1e-40, -1e-38, 1.18e-38, 3.3e38, -3.38e38, 63.75]
+    for i, v in enumerate(fill):
+        for at in (i * 37 % n, (i * 37 + 64) % n):
+            x[at] = v
+    for k in range(0, n - 96, 96):
+        if (k // 96) % 3 == 0:
+            x[k:k + 32] = 0.0
+        elif (k // 96) % 3 == 1:  # small beside one large
+            x[k:k + 32] = x[k:k + 32].clamp(-1, 1) * 0.01
+            x[k + 5] = 1.0 + (k % 7)
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n", [1, 7, 8, 31, 32, 33, 255, 4096, 4101, 70_003])
+def test_pack_is_the_oracles_bit_for_bit(n, dtype, fmt):
+    print(f"pack n={n} {dtype} {fmt}", flush=True)
+    x = awkward(n, DTYPES[dtype], seed=n)
+    p = K.pack8(x.to(DEV), fmt)
+    codes, scales = op.encode(np64(x), fmt)
+    assert np.array_equal(p.scales.cpu().numpy(), scales)
+    assert np.array_equal(p.codes.cpu().numpy(), codes)
+    y = K.unpack8(p)
+    assert y.dtype == x.dtype and y.shape == x.shape
+    assert np.array_equal(np64(y), op.decode(codes, scales, fmt))
+    other = torch.float32 if x.dtype == torch.bfloat16 else torch.bfloat16
+    assert np.array_equal(np64(K.unpack8(p, other)), op.decode(codes, scales, fmt))
+    assert p.nbytes == n + (n + 31) // 32
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_a_group_with_infinity_or_nan_unpacks_to_nan(fmt, dtype):
+    x = torch.ones(5 * 32 + 3, dtype=DTYPES[dtype])
+    x[40], x[100], x[162] = float("inf"), float("nan"), float("-inf")
+    y = K.unpack8(K.pack8(x.to(DEV), fmt)).cpu()
+    bad = torch.zeros(x.numel(), dtype=torch.bool)
+    bad[32:64] = bad[96:128] = bad[160:] = True
+    assert bool(y[bad].isnan().all()) and bool((y[~bad] == 1).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_every_code_at_every_step(fmt):
+    low = 7 if fmt == "int8" else 9
+    scales = torch.arange(low, 256, dtype=torch.uint8)
+    codes = torch.arange(256, dtype=torch.uint8).repeat(scales.numel(), 1)
+    s8 = scales.repeat_interleave(8)
+    p = K.Packed8(codes.flatten().to(DEV), s8.to(DEV), torch.Size(codes.shape), torch.float32, fmt)
+    want = op.decode(codes.flatten().numpy(), s8.numpy(), fmt).reshape(codes.shape)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(K.unpack8(p).cpu().numpy(), want.astype(np.float32), equal_nan=True)
+
+
+def test_pack_of_views_and_empty_tensors():
+    x = torch.randn(64, 96, device=DEV, dtype=torch.bfloat16)
+    for v in (x.T, x[:, 1:], x[3:, ::2], x.flatten()[5:]):
+        a, b = K.pack8(v), K.pack8(v.contiguous().clone())
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales) and a.shape == v.shape
+    p = K.pack8(x[:0])
+    assert p.nbytes == 0 and K.unpack8(p).shape == (0, 96)
+    h = K.swiglu8(x[:0].requires_grad_(), x[:0])
+    assert h.shape == (0, 96) and torch.autograd.grad(h.sum(), [h])[0].shape == (0, 96)
+    one = K.unpack8(K.pack8(torch.tensor(3.0, device=DEV)))
+    assert one.shape == () and float(one) == 3.0
+
+
+def fp32_part(g):
+    """Relative error of the fp32 sigmoid: the exponential's argument is off by 1.45 |g| half steps and a rounding of
+    its own, the exponential, the sum, the reciprocal and the products after it by a step each."""
+    return (1.5 * np.abs(g) + 16) * 2.0 ** -24
+
+
+def close(name, got, want, size, dtype, g):
+    """``size``: the magnitude that the fp32 roundings are relative to (more than |want| where terms cancel)."""
+    tiny = 2.0 ** -126  # results below the normal numbers
+    err = np.abs(np64(got) - want)
+    tol = HALF[dtype] * np.abs(want) + (1 + HALF[dtype]) * fp32_part(g) * size + tiny
+    assert (err <= tol).all(), f"{name}: worst {np.max(err / tol):.3f} of what rounding allows"
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,cols,form", [(1, 1, "two"), (1, 33, "two"), (3, 64, "two"), (5, 77, "two"), (130, 264, "two"),
+                                            (1, 64, "views"), (7, 40, "views"), (61, 200, "views"), (9, 36, "views"),
+                                            (1, 24, "one"), (33, 72, "one"), (5, 31, "one"), (1003, 3584, "one")])
+def test_swiglu_and_its_gradients(rows, cols, form, dtype, fmt):
+    print(f"swiglu {rows} x {cols} {form} {dtype} {fmt}", flush=True)
+    dt = DTYPES[dtype]
+    gen = torch.Generator().manual_seed(rows * 1000 + cols)
+    both = (2.5 * torch.randn(rows, 2 * cols, generator=gen)).to(dt)
+    both[0, 0], both[-1, -1], both[rows // 2, cols // 2] = 90.0, -0.0, -95.0
+    dh = torch.randn(rows, cols, generator=gen).to(dt)
+    g, u = both[:, :cols], both[:, cols:]
+    leaf = both.to(DEV).requires_grad_()
+    if form == "one":
+        h = K.swiglu8(leaf, format=fmt)
+    elif form == "views":
+        h = K.swiglu8(leaf[:, :cols], leaf[:, cols:], fmt)
+    else:
+        h = K.swiglu8(leaf[:, :cols].contiguous(), leaf[:, cols:].contiguous(), fmt)
+    grad, = torch.autograd.grad(h, [leaf], dh.to(DEV))
+    assert h.dtype == dt and grad.shape == leaf.shape
+    g64, u64, d64 = np64(g), np64(u), np64(dh)
+    close("h", h, op.swiglu(g64, u64), np.abs(op.swiglu(g64, u64)), dt, g64)
+    gq, uq = op.rounded(g64, fmt), op.rounded(u64, fmt)
+    dg, du = op.swiglu_bwd(d64, gq, uq)
+    s = 1 / (1 + np.exp(-gq))
+    close("dgate", grad[:, :cols], dg, np.abs(d64 * uq * s) * (1 + np.abs(gq) * (1 + s)), dt, gq)
+    close("dup", grad[:, cols:], du, np.abs(du), dt, gq)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_swiglu_keeps_what_pack_gives_and_recomputes_h(fmt):
+    g, u = torch.randn(2, 37, 160, device=DEV, dtype=torch.bfloat16)
+    h, stores = K.swiglu8_fwd(g, u, fmt)
+    pg, pu = K.pack8(g, fmt), K.pack8(u, fmt)
+    for a, b in zip(stores, (pg.codes, pg.scales, pu.codes, pu.scales)):
+        assert torch.equal(a, b)
+    lone, none = K.swiglu8_fwd(g, u, fmt, keep=False)
+    assert none is None and torch.equal(lone, h)
+    dh = torch.randn_like(h)
+    dgate, dup, h2 = K.swiglu8_bwd(dh, stores, fmt, need_h=True)
+    assert torch.equal(h2, K.swiglu8_fwd(K.unpack8(pg), K.unpack8(pu), fmt)[0])
+    for need, fused in ((False, False), (True, True), (False, True)):
+        a, b, c = K.swiglu8_bwd(dh, stores, fmt, need_h=need, fused=fused)
+        assert torch.equal(a, torch.cat([dgate, dup], -1) if fused else dgate)
+        assert torch.equal(c, h2) if need else c is None
+    with pytest.raises(ValueError, match="do not belong"):
+        K.swiglu8_bwd(dh[:, :128], stores, fmt)
+
+
+def test_swiglu_gradient_is_a_difference():
+    """Against central differences of the forward in fp32 at values that 8 bits hold exactly."""
+    g = (torch.randint(-64, 65, (256,)) / 16).float().to(DEV)
+    u = (torch.randint(-64, 65, (256,)) / 16).float().to(DEV)
+    g[::32] = u[::32] = 4.0  # every group's step is 1 / 16
+    assert torch.equal(K.unpack8(K.pack8(g)), g) and torch.equal(K.unpack8(K.pack8(u)), u)
+    gr, ur = g.clone().requires_grad_(), u.clone().requires_grad_()
+    dg, du = torch.autograd.grad(K.swiglu8(gr, ur).sum(), [gr, ur])
+
+    def h(a, b):
+        return K.swiglu8(a, b).double()
+
+    eps = 2.0 ** -7
+    num_g = (h(g + eps, u) - h(g - eps, u)) / (2 * eps)
+    num_u = (h(g, u + eps) - h(g, u - eps)) / (2 * eps)
+    # rounding: |h| <= 16, two values off by 24 half steps each over 2 eps; truncation: eps^2 / 6 of the third
+    # derivative of silu (at most 0.6) times |u| <= 4; h is linear in u
+    rounding = 16 * 2 * 24 * 2.0 ** -24 / (2 * eps)
+    assert float((dg - num_g).abs().max()) <= rounding + eps ** 2 / 6 * 0.6 * 4 + 1e-4
+    assert float((du - num_u).abs().max()) <= rounding + 1e-4
+
+
+def test_swiglu_linear_matches_the_parts():
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    g, u = (torch.randn(2, 50, 96, generator=gen, device=DEV).to(torch.bfloat16).requires_grad_() for _ in range(2))
+    w = (0.1 * torch.randn(40, 96, generator=gen, device=DEV)).to(torch.bfloat16).requires_grad_()
+    dy = torch.randn(2, 50, 40, generator=gen, device=DEV).to(torch.bfloat16)
+    y = K.swiglu8_linear(g, u, w)
+    assert torch.equal(y, torch.nn.functional.linear(K.swiglu8(g, u), w))
+    dg, du, dw = torch.autograd.grad(y, [g, u, w], dy)
+    dg2, du2 = torch.autograd.grad(K.swiglu8(g, u), [g, u], dy @ w)
+    assert torch.equal(dg, dg2) and torch.equal(du, du2)
+    hq = op.swiglu(op.rounded(np64(g), "int8"), op.rounded(np64(u), "int8")).reshape(-1, 96)
+    want = np64(dy).reshape(-1, 40).T @ hq
+    # h and the result rounded to bf16; 100 products summed in fp32
+    tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 300 * 2.0 ** -24) * (np.abs(np64(dy)).reshape(-1, 40).T @ np.abs(hq))
+    assert (np.abs(np64(dw) - want) <= 1.01 * tol).all()
+    frozen = K.swiglu8_linear(g, u, w.detach())
+    assert torch.equal(torch.autograd.grad(frozen, [g], dy)[0], dg)
+    with torch.no_grad():
+        assert K.swiglu8_linear(g, u, w).grad_fn is None and torch.equal(K.swiglu8_linear(g, u, w), y)
+
+
+def test_checkpoint_gradients_are_those_at_the_unpacked_input():
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(96, 96, device=DEV, dtype=torch.bfloat16)
+    drop = torch.nn.Dropout(0.5)
+
+    def block(t, scale):
+        return drop(torch.tanh(lin(t))) * scale + t
+
+    x = torch.randn(33, 96, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    s = torch.rand(96, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(33, 96, device=DEV, dtype=torch.bfloat16)
+    for fmt in ("int8", "e4m3"):
+        torch.manual_seed(5)
+        y = K.checkpoint8(block, x, s, format=fmt)
+        torch.manual_seed(5)
+        assert torch.equal(y, block(x, s))  # the forward is the input's own, dropout included
+        got = torch.autograd.grad(y, [x, s, lin.weight], dy, retain_graph=True)
+        again = torch.autograd.grad(y, [x, s, lin.weight], dy)
+        xq = K.unpack8(K.pack8(x, fmt)).requires_grad_()
+        torch.manual_seed(5)
+        want = torch.autograd.grad(block(xq, s), [xq, s, lin.weight], dy)
+        for a, b, c in zip(got, want, again):
+            assert torch.equal(a, b) and torch.equal(a, c)
+    with torch.no_grad():
+        assert K.checkpoint8(block, x, s).grad_fn is None
+
+
+def test_checkpoint_does_not_keep_its_input():
+    w = torch.randn(64, 64, device=DEV).requires_grad_()
+    leaf = torch.randn(2048, 64, device=DEV).requires_grad_()
+    x = leaf * 2
+    ref = weakref.ref(x)
+    y = K.checkpoint8(lambda t: torch.relu(t @ w), x)
+    del x
+    gc.collect()
+    assert ref() is None
+    y.sum().backward()
+    assert leaf.grad is not None and w.grad is not None
+
+
+def test_checkpoint_of_an_input_without_gradient():
+    w = torch.randn(64, 64, device=DEV, requires_grad=True)
+    x = torch.randn(20, 64, device=DEV)
+    y = K.checkpoint8(lambda t: (t @ w).relu(), x)
+    dw, = torch.autograd.grad(y.sum(), [w])
+    assert torch.equal(dw, torch.autograd.grad((K.unpack8(K.pack8(x)) @ w).relu().sum(), [w])[0])
+
+
+def test_calls_on_another_stream_and_two_at_once():
+    g, u = torch.randn(2, 4099, 520, device=DEV, dtype=torch.bfloat16)
+    dh = torch.randn(4099, 520, device=DEV, dtype=torch.bfloat16)
+    want_h, want_s = K.swiglu8_fwd(g, u)
+    want = K.swiglu8_bwd(dh, want_s)[:2]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for st in streams:
+        with torch.cuda.stream(st):
+            h, s = K.swiglu8_fwd(g, u)
+            got.append((h, *K.swiglu8_bwd(dh, s)[:2], K.unpack8(K.pack8(g))))
+    torch.cuda.synchronize()
+    for h, a, b, x in got:
+        assert torch.equal(h, want_h) and torch.equal(a, want[0]) and torch.equal(b, want[1])
+        assert torch.equal(x, K.unpack8(K.pack8(g)))
+
+
+def test_captured_calls_replay_on_new_values():
+    g, u, dh = (torch.randn(300, 264, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    K.swiglu8_bwd(dh, K.swiglu8_fwd(g, u)[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, s = K.swiglu8_fwd(g, u, "e4m3")
+        dg, du, _ = K.swiglu8_bwd(dh, s, "e4m3")
+        x = K.unpack8(K.pack8(g, "e4m3"))
+    for i in range(3):
+        for t in (g, u, dh):
+            t.copy_(torch.randn_like(t) * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        h2, s2 = K.swiglu8_fwd(g, u, "e4m3")
+        dg2, du2, _ = K.swiglu8_bwd(dh, s2, "e4m3")
+        assert torch.equal(h, h2) and torch.equal(dg, dg2) and torch.equal(du, du2)
+        assert torch.equal(x, K.unpack8(K.pack8(g, "e4m3")))
+
+
+def tiny_qwen2():
+    transformers = pytest.importorskip("transformers")
+    from siq_vl_amd import attention
+
+    attention.register()
+    cfg = transformers.Qwen2Config(vocab_size=256, hidden_size=256, intermediate_size=512, num_hidden_layers=2,
+                                   num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
+    torch.manual_seed(1)
+    model = transformers.Qwen2ForCausalLM(cfg).to(DEV, torch.bfloat16)
+    model.config._attn_implementation = "siq_varlen"
+    return model.train()
+
+
+def _loss_and_grads(model, ids):
+    model.zero_grad()
+    loss = model(input_ids=ids, labels=ids, use_cache=False).loss
+    loss.backward()
+    return float(loss.detach()), {n: p.grad.double() for n, p in model.named_parameters()}
+
+
+@pytest.mark.parametrize("which", ["mlp", "mlp frozen", "layers"])
+def test_on_a_qwen2_model(which):
+    """A training step of a small model: the forward is bitwise the stock one (layers) or within bf16 rounding of it
+    (mlp: the activation is rounded once instead of twice); the gradients differ by what 8-bit storage costs."""
+    model = tiny_qwen2()
+    ids = torch.randint(0, 256, (2, 65), device=DEV)
+    loss0, grads0 = _loss_and_grads(model, ids)
+    if which == "layers":
+        assert K.enable_8bit_checkpoints(model) >= 2
+    else:
+        assert K.enable_8bit_mlp(model) == 2
+        if which == "mlp frozen":
+            for mod in model.model.layers:
+                mod.mlp.down_proj.weight.requires_grad_(False)
+                grads0.pop(next(n for n, p in model.named_parameters() if p is mod.mlp.down_proj.weight))
+    model.zero_grad()
+    loss = model(input_ids=ids, labels=ids, use_cache=False).loss
+    loss.backward()
+    grads = {n: p.grad.double() for n, p in model.named_parameters() if p.requires_grad}
+    assert grads.keys() == grads0.keys()
+    if which == "layers":
+        assert float(loss.detach()) == loss0
+    else:
+        assert abs(float(loss.detach()) - loss0) <= 2.0 ** -7 * loss0
+    # int8 groups of 32 normal values: a step of at most max / 64, about 3 / 64, so rounding noise of at most
+    # 3 / 64 / sqrt(12) = 1.4% of the values; two layers of it and the bf16 roundings stay below 10% of a gradient
+    for n, g in grads.items():
+        rel = float((g - grads0[n]).norm() / grads0[n].norm())
+        assert rel <= 0.1, (n, rel)
