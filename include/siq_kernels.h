@@ -13,7 +13,9 @@
  *   5. the splice of the projected vision rows into the token embeddings,
  *      fused with the embedding gather, and its embedding-table gradient;
  *   6. activations kept in 8 bits for the backward pass, and the gated MLP
- *      activation over them.
+ *      activation over them;
+ *   7. the losses of preference and policy training on packed
+ *      log-probabilities, forward and backward.
  *
  * Conventions
  *  - Every entry point returns an int status (SIQ_OK = 0, < 0 on error) and
@@ -440,6 +442,78 @@ int siq_swiglu8_fwd(const void* gate, const void* up, int64_t rows, int64_t cols
 int siq_swiglu8_bwd(const void* dh, const void* gate_codes, const void* gate_scales, const void* up_codes,
                     const void* up_scales, int64_t rows, int64_t cols, int64_t dgate_stride, int64_t dup_stride,
                     int dtype, int format, void* dgate, void* dup, void* h, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Losses of preference and policy training.
+ *
+ * No counterpart in the reference, which ends at supervised fine-tuning: what
+ * follows it trains on pairs of answers, or on sampled ones with advantages,
+ * over the same packed batches.  Inputs are fp32 per-token log-probabilities of
+ * packed sequences (cu_seqlens int32 [sequences + 1]; cu[0] is taken as 0, and
+ * tokens behind cu[sequences] belong to none: they count nowhere and their
+ * gradient is zero), mask [tokens] bytes (0: the token does not count, whatever
+ * its values; NULL: all count).  Sums are in fp64 and in a fixed order, no
+ * atomics.  grad_loss: the loss's upstream gradient, a device scalar.
+ *
+ * siq_pref_fwd: the loss of paired sequences.  Pair i is sequences 2 i (chosen)
+ * and 2 i + 1 (rejected) (SIQ_ORDER_INTERLEAVED), or i and pairs + i
+ * (SIQ_ORDER_HALVES).  A sequence's score is the sum over its counted tokens
+ * of policy - reference (reference NULL: of policy), divided by their number
+ * when length_normalized (by 1 where none counts); x = score of chosen -
+ * score of rejected:
+ *   SIQ_PREF_SIGMOID: (1 - e) softplus(-beta x) + e softplus(beta x), e =
+ *     label_smoothing;   SIQ_PREF_IPO: (x - 1 / (2 beta))^2;
+ *   SIQ_PREF_HINGE: max(0, 1 - beta x).
+ * *loss = their sum / pairs, or / *divisor (a device scalar) if not NULL;
+ * chosen_rewards / rejected_rewards [pairs] = beta * score; coef [2 pairs] =
+ * the loss's gradient with respect to a counted token of each sequence, which
+ * siq_pref_bwd spreads over the tokens (dpolicy [tokens], written in full).
+ *
+ * siq_policy_fwd: the clipped policy loss.  r = exp(logp - old_logp); a token's
+ * objective is min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), and for A < 0
+ * not below dual_clip * A (dual_clip 0: no such bound); its loss is -objective +
+ * kl_coef * kl with x = reference - logp and kl = -x (SIQ_KL_K1), x^2 / 2 (_K2)
+ * or e^x - 1 - x (_K3).  advantages A: [tokens] (advantage_per_token) or
+ * [seqs].  SIQ_AGG_TOKEN: the mean over counted tokens; SIQ_AGG_SEQUENCE: the
+ * mean over sequences of their counted tokens' mean (0 where none counts);
+ * with divisor its value replaces the number of counted tokens, or of
+ * sequences.  cu_seqlens NULL: one sequence.  A token exactly at a border is
+ * not cut.  stats [3] = loss, mean kl and share of cut tokens over counted ones
+ * (all 0 where none counts); dtoken [tokens] (16-byte aligned) and weight
+ * [seqs] (SIQ_AGG_TOKEN: [1]) are what siq_policy_bwd multiplies:
+ * dlogps = grad_loss weight dtoken (dlogps 16-byte aligned).
+ * ------------------------------------------------------------------------- */
+#define SIQ_PREF_SIGMOID 0
+#define SIQ_PREF_IPO 1
+#define SIQ_PREF_HINGE 2
+#define SIQ_ORDER_INTERLEAVED 0
+#define SIQ_ORDER_HALVES 1
+#define SIQ_AGG_TOKEN 0
+#define SIQ_AGG_SEQUENCE 1
+#define SIQ_KL_K1 0
+#define SIQ_KL_K2 1
+#define SIQ_KL_K3 2
+
+size_t siq_pref_workspace_bytes(int64_t pairs, int64_t tokens);
+
+int siq_pref_fwd(const float* policy, const float* reference, const void* mask, const int32_t* cu_seqlens,
+                 int64_t pairs, int64_t tokens, int loss_type, int order, double beta, double label_smoothing,
+                 int length_normalized, const float* divisor, float* loss, float* chosen_rewards,
+                 float* rejected_rewards, float* coef, void* workspace, size_t workspace_bytes, void* stream);
+
+int siq_pref_bwd(const float* grad_loss, const float* coef, const void* mask, const int32_t* cu_seqlens, int64_t pairs,
+                 int64_t tokens, float* dpolicy, void* stream);
+
+size_t siq_policy_workspace_bytes(int64_t seqs, int64_t tokens);
+
+int siq_policy_fwd(const float* logps, const float* old_logps, const float* advantages, const void* mask,
+                   const float* reference, const int32_t* cu_seqlens, int64_t seqs, int64_t tokens,
+                   int advantage_per_token, int aggregation, int kl_type, double clip_low, double clip_high,
+                   double dual_clip, double kl_coef, const float* divisor, float* stats, float* dtoken, float* weight,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* weight, const int32_t* cu_seqlens,
+                   int64_t seqs, int64_t tokens, int aggregation, float* dlogps, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Measurement support (no reference counterpart).

@@ -31,6 +31,7 @@ _c_void_p = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _size = ctypes.c_size_t
 
 _PROTOS = {
@@ -118,6 +119,20 @@ _PROTOS = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i32, _i32, _c_void_p,
          _c_void_p, _c_void_p, _c_void_p],
     ),
+    "siq_pref_workspace_bytes": (_size, [_i64, _i64]),
+    "siq_pref_fwd": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _i32, _f64, _f64, _i32, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
+    ),
+    "siq_pref_bwd": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p]),
+    "siq_policy_workspace_bytes": (_size, [_i64, _i64]),
+    "siq_policy_fwd": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _i32, _i32, _f64, _f64,
+         _f64, _f64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
+    ),
+    "siq_policy_bwd": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p]),
     "siq_probe_clock": (_i32, [_c_void_p, _i64, _c_void_p]),
     "siq_rope_fwd": (
         _i32,

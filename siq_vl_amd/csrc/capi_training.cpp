@@ -2,9 +2,13 @@
 // policy training adds: host-side validation and launches, as in capi.cpp.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+#include <limits>
+
 #include "../../include/siq_kernels.h"
 #include "capi_internal.h"
 #include "pack8.h"
+#include "policy.h"
 
 using namespace siq_capi;
 
@@ -48,6 +52,26 @@ int check_rows(int64_t rows, int64_t cols, int64_t ld0, int64_t ld1, int dtype, 
                   (long long)ld[i]);
   if (cols % 8 != 0)
     return fail(SIQ_ERR_UNSUPPORTED, "cols (%lld) must be a multiple of 8 where rows are not contiguous", (long long)cols);
+  return SIQ_OK;
+}
+
+constexpr int64_t kMaxSeqs = int64_t(1) << 24;
+
+int check_packed(int64_t seqs, int64_t tokens) {
+  if (seqs < 1 || seqs > kMaxSeqs)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "the number of sequences must be in [1, 2^24] (got %lld)", (long long)seqs);
+  if (tokens < 0 || tokens >= (int64_t(1) << 31))
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "tokens must be in [0, 2^31) (got %lld)", (long long)tokens);
+  return SIQ_OK;
+}
+
+int check_not_null(const void* p, const char* name) {
+  return p == nullptr ? fail(SIQ_ERR_INVALID_ARGUMENT, "%s must not be NULL", name) : SIQ_OK;
+}
+
+int check_ws(const void* ws, size_t bytes, size_t need) {
+  if (ws == nullptr || bytes < need || !aligned16(ws))
+    return fail(SIQ_ERR_WORKSPACE, "workspace needs %zu bytes (16-byte aligned), got %zu", need, bytes);
   return SIQ_OK;
 }
 
@@ -139,6 +163,143 @@ int siq_swiglu8_bwd(const void* dh, const void* gate_codes, const void* gate_sca
   a.f32 = dtype == SIQ_DTYPE_FP32;
   a.e4m3 = format == SIQ_FORMAT_E4M3;
   return launched(siq::launch_swiglu8_bwd(a, static_cast<hipStream_t>(stream)), "swiglu8 backward");
+}
+
+size_t siq_pref_workspace_bytes(int64_t pairs, int64_t tokens) {
+  if (pairs < 1 || pairs > kMaxSeqs / 2 || tokens < 0 || tokens >= (int64_t(1) << 31)) return 0;
+  return siq::pref_workspace_bytes(pairs, tokens);
+}
+
+int siq_pref_fwd(const float* policy, const float* reference, const void* mask, const int32_t* cu_seqlens,
+                 int64_t pairs, int64_t tokens, int loss_type, int order, double beta, double label_smoothing,
+                 int length_normalized, const float* divisor, float* loss, float* chosen_rewards,
+                 float* rejected_rewards, float* coef, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if (pairs < 1 || pairs > kMaxSeqs / 2)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "pairs must be in [1, 2^23] (got %lld)", (long long)pairs);
+  if ((rc = check_packed(2 * pairs, tokens))) return rc;
+  if (loss_type < SIQ_PREF_SIGMOID || loss_type > SIQ_PREF_HINGE)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "loss_type must be SIQ_PREF_SIGMOID, _IPO or _HINGE");
+  if (order != SIQ_ORDER_INTERLEAVED && order != SIQ_ORDER_HALVES)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "order must be SIQ_ORDER_INTERLEAVED or SIQ_ORDER_HALVES");
+  if (!(beta > 0.) || !std::isfinite(beta)) return fail(SIQ_ERR_INVALID_ARGUMENT, "beta must be positive and finite");
+  if (!(label_smoothing >= 0. && label_smoothing <= 0.5))
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "label_smoothing must be in [0, 0.5]");
+  if (label_smoothing != 0. && loss_type != SIQ_PREF_SIGMOID)
+    return fail(SIQ_ERR_UNSUPPORTED, "label_smoothing goes with SIQ_PREF_SIGMOID only");
+  if ((rc = check_not_null(cu_seqlens, "cu_seqlens")) || (rc = check_not_null(loss, "loss")) ||
+      (rc = check_not_null(chosen_rewards, "chosen_rewards")) ||
+      (rc = check_not_null(rejected_rewards, "rejected_rewards")) || (rc = check_not_null(coef, "coef")))
+    return rc;
+  if (tokens > 0 && (rc = check_not_null(policy, "policy"))) return rc;
+  if ((rc = check_ws(workspace, workspace_bytes, siq::pref_workspace_bytes(pairs, tokens)))) return rc;
+  siq::PrefArgs a{};
+  a.seq = {cu_seqlens, 2 * pairs, tokens};
+  a.policy = policy;
+  a.reference = reference;
+  a.mask = static_cast<const uint8_t*>(mask);
+  a.pairs = pairs;
+  a.type = loss_type;
+  a.halves = order == SIQ_ORDER_HALVES;
+  a.normalized = length_normalized != 0;
+  a.beta = beta;
+  a.smoothing = label_smoothing;
+  a.divisor = divisor;
+  a.loss = loss;
+  a.chosen = chosen_rewards;
+  a.rejected = rejected_rewards;
+  a.coef = coef;
+  a.ws = workspace;
+  return launched(siq::pref_fwd(a, static_cast<hipStream_t>(stream)), "preference loss");
+}
+
+int siq_pref_bwd(const float* grad_loss, const float* coef, const void* mask, const int32_t* cu_seqlens, int64_t pairs,
+                 int64_t tokens, float* dpolicy, void* stream) {
+  int rc;
+  if (pairs < 1 || pairs > kMaxSeqs / 2)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "pairs must be in [1, 2^23] (got %lld)", (long long)pairs);
+  if ((rc = check_packed(2 * pairs, tokens))) return rc;
+  if (tokens == 0) return ok();
+  if ((rc = check_not_null(grad_loss, "grad_loss")) || (rc = check_not_null(coef, "coef")) ||
+      (rc = check_not_null(cu_seqlens, "cu_seqlens")) || (rc = check_not_null(dpolicy, "dpolicy")))
+    return rc;
+  return launched(siq::pref_bwd({cu_seqlens, 2 * pairs, tokens}, grad_loss, coef, static_cast<const uint8_t*>(mask),
+                                dpolicy, static_cast<hipStream_t>(stream)),
+                  "preference loss backward");
+}
+
+size_t siq_policy_workspace_bytes(int64_t seqs, int64_t tokens) {
+  if (seqs < 1 || seqs > kMaxSeqs || tokens < 0 || tokens >= (int64_t(1) << 31)) return 0;
+  return siq::policy_workspace_bytes(seqs, tokens);
+}
+
+int siq_policy_fwd(const float* logps, const float* old_logps, const float* advantages, const void* mask,
+                   const float* reference, const int32_t* cu_seqlens, int64_t seqs, int64_t tokens,
+                   int advantage_per_token, int aggregation, int kl_type, double clip_low, double clip_high,
+                   double dual_clip, double kl_coef, const float* divisor, float* stats, float* dtoken, float* weight,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_packed(seqs, tokens))) return rc;
+  if (aggregation != SIQ_AGG_TOKEN && aggregation != SIQ_AGG_SEQUENCE)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "aggregation must be SIQ_AGG_TOKEN or SIQ_AGG_SEQUENCE");
+  if (kl_type < SIQ_KL_K1 || kl_type > SIQ_KL_K3)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "kl_type must be SIQ_KL_K1, _K2 or _K3");
+  if (!(clip_low >= 0. && clip_low <= 1.)) return fail(SIQ_ERR_INVALID_ARGUMENT, "clip_low must be in [0, 1]");
+  if (!(clip_high >= 0.)) return fail(SIQ_ERR_INVALID_ARGUMENT, "clip_high must be >= 0");
+  if (!(dual_clip == 0. || dual_clip > 1.))
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "dual_clip must be 0 (none) or above 1");
+  if (!std::isfinite(kl_coef)) return fail(SIQ_ERR_INVALID_ARGUMENT, "kl_coef must be finite");
+  if (kl_coef != 0. && reference == nullptr && tokens > 0)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "a KL term needs the reference's log-probabilities");
+  if (cu_seqlens == nullptr && seqs != 1)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "without cu_seqlens there is one sequence");
+  if ((rc = check_not_null(stats, "stats")) || (rc = check_not_null(weight, "weight"))) return rc;
+  if (tokens > 0) {
+    if ((rc = check_not_null(logps, "logps")) || (rc = check_not_null(old_logps, "old_logps")) ||
+        (rc = check_not_null(advantages, "advantages")) || (rc = check_ptr(dtoken, "dtoken")))
+      return rc;
+  }
+  if ((rc = check_ws(workspace, workspace_bytes, siq::policy_workspace_bytes(seqs, tokens)))) return rc;
+  siq::PolicyArgs a{};
+  a.seq = {cu_seqlens, seqs, tokens};
+  a.logps = logps;
+  a.old = old_logps;
+  a.advantages = advantages;
+  a.mask = static_cast<const uint8_t*>(mask);
+  a.reference = reference;
+  a.per_token = advantage_per_token != 0;
+  a.by_sequence = aggregation == SIQ_AGG_SEQUENCE;
+  a.kl = reference == nullptr ? siq::kKlNone : kl_type;
+  a.log_low = std::log1p(-clip_low);
+  a.log_high = std::log1p(clip_high);
+  a.log_dual = dual_clip == 0. ? std::numeric_limits<double>::infinity() : std::log(dual_clip);
+  a.low = (float)(1. - clip_low);
+  a.high = (float)(1. + clip_high);
+  a.dual = (float)dual_clip;
+  a.kl_coef = (float)kl_coef;
+  a.divisor = divisor;
+  a.stats = stats;
+  a.dtoken = dtoken;
+  a.weight = weight;
+  a.ws = workspace;
+  return launched(siq::policy_fwd(a, static_cast<hipStream_t>(stream)), "policy loss");
+}
+
+int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* weight, const int32_t* cu_seqlens,
+                   int64_t seqs, int64_t tokens, int aggregation, float* dlogps, void* stream) {
+  int rc;
+  if ((rc = check_packed(seqs, tokens))) return rc;
+  if (aggregation != SIQ_AGG_TOKEN && aggregation != SIQ_AGG_SEQUENCE)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "aggregation must be SIQ_AGG_TOKEN or SIQ_AGG_SEQUENCE");
+  if (cu_seqlens == nullptr && seqs != 1)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "without cu_seqlens there is one sequence");
+  if (tokens == 0) return ok();
+  if ((rc = check_not_null(grad_loss, "grad_loss")) || (rc = check_not_null(weight, "weight")) ||
+      (rc = check_ptr(dtoken, "dtoken")) || (rc = check_ptr(dlogps, "dlogps")))
+    return rc;
+  return launched(siq::policy_bwd({cu_seqlens, seqs, tokens}, aggregation == SIQ_AGG_SEQUENCE, grad_loss, dtoken, weight,
+                                  dlogps, static_cast<hipStream_t>(stream)),
+                  "policy loss backward");
 }
 
 }  // extern "C"
