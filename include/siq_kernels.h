@@ -15,7 +15,8 @@
  *   6. activations kept in 8 bits for the backward pass, and the gated MLP
  *      activation over them;
  *   7. the losses of preference and policy training on packed
- *      log-probabilities, forward and backward.
+ *      log-probabilities, forward and backward, and those log-probabilities
+ *      from hidden states without the logits.
  *
  * Conventions
  *  - Every entry point returns an int status (SIQ_OK = 0, < 0 on error) and
@@ -252,6 +253,39 @@ size_t siq_flce_loss_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab);
 int siq_flce_loss(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
                   int64_t vocab, int64_t ignore_index, int reduction, const float* divisor, float* loss,
                   int64_t* count, int64_t* bad_labels, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log-probabilities of the labels, without the logits (no counterpart in the
+ * reference, whose loss is their mean; preference and policy losses weight each
+ * of them):
+ *   logp[i] = z_iy - log sum_j exp(z_ij),  z = hidden weight^T / temperature,
+ * fp32 [n]; 0 where the label is ignore_index or, counted in *bad_labels,
+ * outside [0, vocab).  *count = rows that count.  Operands as for
+ * siq_flce_fwd_bwd.
+ * siq_flp_bwd: with dlogp [n] the upstream gradients (those of rows that do not
+ * count are not read),
+ *   dhidden = dZ weight,  dweight = dZ^T hidden,
+ *   dZ_ij = dlogp_i / temperature (1[j = y_i] - exp(z_ij - lse_i)),
+ * either of the two may be NULL (not computed); dhidden must not overlap hidden.
+ * `saved` (siq_flp_saved_bytes) non-NULL: the forward keeps every row's softmax
+ * numerators (n x vocab bf16) there and the backward, given the same buffer and
+ * inputs, starts from them; it is only read, so a second backward may follow.
+ * NULL in both: the backward forms the logits again, chunk_tokens rows at a
+ * time, as siq_flce_fwd_bwd does (chunk_tokens is not used with saved). */
+size_t siq_flp_saved_bytes(int64_t n, int64_t vocab);
+
+size_t siq_flp_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int keep);
+
+int siq_flp_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim, int64_t vocab,
+                int64_t ignore_index, double temperature, float* logp, int64_t* count, int64_t* bad_labels, void* saved,
+                size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t siq_flp_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight,
+                                   int have_saved);
+
+int siq_flp_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* dlogp, int64_t n,
+                int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, const void* saved,
+                size_t saved_bytes, void* dhidden, void* dweight, int64_t chunk_tokens, void* workspace,
+                size_t workspace_bytes, void* stream);
 
 /* dst = src * (*scalar) over numel bf16 elements, rounded once from fp32
  * (a device fp32 scalar, read on the device): applies the upstream gradient

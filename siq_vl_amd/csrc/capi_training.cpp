@@ -7,6 +7,7 @@
 
 #include "../../include/siq_kernels.h"
 #include "capi_internal.h"
+#include "flce.h"
 #include "pack8.h"
 #include "policy.h"
 
@@ -73,6 +74,47 @@ int check_ws(const void* ws, size_t bytes, size_t need) {
   if (ws == nullptr || bytes < need || !aligned16(ws))
     return fail(SIQ_ERR_WORKSPACE, "workspace needs %zu bytes (16-byte aligned), got %zu", need, bytes);
   return SIQ_OK;
+}
+
+// Sizes of a log-probability call (0: fine).
+int check_flp(int64_t n, int64_t hdim, int64_t vocab) {
+  if (n < 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "n must be >= 0");
+  if (hdim <= 0 || vocab <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "hdim and vocab must be positive");
+  if (hdim % 64 != 0) return fail(SIQ_ERR_UNSUPPORTED, "hdim (%lld) must be a multiple of 64", (long long)hdim);
+  if (vocab % 8 != 0) return fail(SIQ_ERR_UNSUPPORTED, "vocab (%lld) must be a multiple of 8", (long long)vocab);
+  if (n >= (int64_t(1) << 31) || vocab >= (int64_t(1) << 31) || hdim >= (int64_t(1) << 20))
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "n and vocab must be < 2^31, hdim < 2^20");
+  return SIQ_OK;
+}
+
+int check_flp_call(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
+                   int64_t vocab, double temperature, const void* saved, size_t saved_bytes) {
+  int rc;
+  if ((rc = check_flp(n, hdim, vocab)) || (rc = check_ptr(weight, "weight"))) return rc;
+  if (!(temperature > 0.) || !std::isfinite(temperature) || !std::isfinite((float)(1.4426950408889634 / temperature)) ||
+      (float)(1. / temperature) == 0.f)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "temperature must be positive and finite");
+  if (n > 0 && ((rc = check_ptr(hidden, "hidden")) || (rc = check_not_null(labels, "labels")))) return rc;
+  if (saved != nullptr && (saved_bytes < siq::flp_saved_bytes(n, vocab) || !aligned16(saved)))
+    return fail(SIQ_ERR_WORKSPACE, "saved needs %zu bytes (16-byte aligned), got %zu", siq::flp_saved_bytes(n, vocab),
+                saved_bytes);
+  return SIQ_OK;
+}
+
+siq::FlpArgs flp_args(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
+                      int64_t vocab, int64_t ignore_index, double temperature, void* saved, void* ws) {
+  siq::FlpArgs a{};
+  a.hidden = static_cast<const siq::bf16*>(hidden);
+  a.weight = static_cast<const siq::bf16*>(weight);
+  a.labels = labels;
+  a.n = n;
+  a.hdim = hdim;
+  a.vocab = vocab;
+  a.ignore_index = ignore_index;
+  a.temperature = temperature;
+  a.saved = saved;
+  a.ws = ws;
+  return a;
 }
 
 int launched(hipError_t e, const char* what) {
@@ -300,6 +342,64 @@ int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* wei
   return launched(siq::policy_bwd({cu_seqlens, seqs, tokens}, aggregation == SIQ_AGG_SEQUENCE, grad_loss, dtoken, weight,
                                   dlogps, static_cast<hipStream_t>(stream)),
                   "policy loss backward");
+}
+
+size_t siq_flp_saved_bytes(int64_t n, int64_t vocab) {
+  if (n < 0 || vocab <= 0) return 0;
+  return siq::flp_saved_bytes(n, vocab);
+}
+
+size_t siq_flp_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int keep) {
+  if (n < 0 || hdim <= 0 || vocab <= 0) return 0;
+  return siq::flp_fwd_workspace_bytes(n, hdim, vocab, keep != 0);
+}
+
+size_t siq_flp_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight,
+                                   int have_saved) {
+  if (n < 0 || hdim <= 0 || vocab <= 0 || chunk_tokens <= 0) return 0;
+  return siq::flp_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, need_dweight != 0, have_saved != 0);
+}
+
+int siq_flp_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim, int64_t vocab,
+                int64_t ignore_index, double temperature, float* logp, int64_t* count, int64_t* bad_labels, void* saved,
+                size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, saved, saved_bytes)) ||
+      (rc = check_not_null(count, "count")) || (rc = check_not_null(bad_labels, "bad_labels")))
+    return rc;
+  if (n > 0 && (rc = check_not_null(logp, "logp"))) return rc;
+  if ((rc = check_ws(workspace, workspace_bytes, siq::flp_fwd_workspace_bytes(n, hdim, vocab, saved != nullptr)))) return rc;
+  siq::FlpArgs a = flp_args(hidden, weight, labels, n, hdim, vocab, ignore_index, temperature, saved, workspace);
+  a.logp = logp;
+  a.count = count;
+  a.bad_labels = bad_labels;
+  return launched(siq::flp_fwd(a, static_cast<hipStream_t>(stream)), "log-probabilities");
+}
+
+int siq_flp_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* dlogp, int64_t n,
+                int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, const void* saved,
+                size_t saved_bytes, void* dhidden, void* dweight, int64_t chunk_tokens, void* workspace,
+                size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, saved, saved_bytes))) return rc;
+  if (chunk_tokens <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "chunk_tokens must be positive");
+  if (n > 0 && (rc = check_not_null(dlogp, "dlogp"))) return rc;
+  if (dhidden != nullptr && !aligned16(dhidden)) return fail(SIQ_ERR_ALIGNMENT, "dhidden is not 16-byte aligned");
+  if (dweight != nullptr && !aligned16(dweight)) return fail(SIQ_ERR_ALIGNMENT, "dweight is not 16-byte aligned");
+  if (dhidden == nullptr && dweight == nullptr) return ok();
+  const char *h0 = static_cast<const char*>(hidden), *d0 = static_cast<const char*>(dhidden);
+  const size_t bytes = sizeof(siq::bf16) * (size_t)n * (size_t)hdim;
+  if (n > 0 && dhidden != nullptr && d0 < h0 + bytes && h0 < d0 + bytes)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "dhidden must not overlap hidden");
+  const size_t need = siq::flp_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, dweight != nullptr, saved != nullptr);
+  if ((rc = check_ws(workspace, workspace_bytes, need))) return rc;
+  siq::FlpArgs a = flp_args(hidden, weight, labels, n, hdim, vocab, ignore_index, temperature, const_cast<void*>(saved),
+                            workspace);
+  a.dlogp = dlogp;
+  a.dhidden = static_cast<siq::bf16*>(dhidden);
+  a.dweight = static_cast<siq::bf16*>(dweight);
+  a.chunk = chunk_tokens;
+  return launched(siq::flp_bwd(a, static_cast<hipStream_t>(stream)), "log-probabilities backward");
 }
 
 }  // extern "C"

@@ -86,6 +86,7 @@ struct LogitsArgs {
   int64_t V, nc, c0, ldp;
   int nI, nJ;
   int store_e;            // 0: loss only, E is not needed
+  float zscale, invt;     // log2(e) / temperature, 1 / temperature
 };
 
 __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
         bf16x8 e8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float e = exp2f_fast(__builtin_fmaf(acc[a][b][8 * jj + i], kLog2e, -m2));
+          const float e = exp2f_fast(__builtin_fmaf(acc[a][b][8 * jj + i], p.zscale, -m2));
           sum += e;
           e8[i] = (bf16)e;
         }
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (hit && r0 == wave_row(a, 0) + 16 * (r >> 3) + (r & 7)) zsel = acc[a][b][r];
-      if (hit) p.zy[tok] = zsel;
+      if (hit) p.zy[tok] = zsel * p.invt;
     }
     const float sum = numerators(b, ref[b], p.store_e && tv);
     if (h == 0) red[wi * 256 + col] = sum;
@@ -186,8 +187,8 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[a][b][r]);
-    // log2 units (scaling by log2 e > 0 commutes with the max)
-    mx = half_max(mx) * kLog2e;
+    // log2 units (scaling by log2 e / temperature > 0 commutes with the max)
+    mx = half_max(mx) * p.zscale;
     if (h == 0) red[wi * 256 + wave_col(b, wj) + l32] = mx;
   }
   __syncthreads();
@@ -226,8 +227,10 @@ struct RowArgs {
   bf16* H;               // [nc, hdim] compacted rows: scaled by f (need_dw)
   float* f;              // [nc] factors of E
   float* wt;             // [nc] weights of the label terms
-  float* loss_row;       // [nc] (chunk slice)
-  const float* invden;
+  float* loss_row;       // [nc] (chunk slice), or nullptr
+  float* logp;           // [n] log-probabilities of the labels by original row, or nullptr
+  const int32_t* rows;   // compacted row -> original row (chunk slice; with logp)
+  const float* invden;   // nullptr: 1
   const int64_t* nvalid;
   uint64_t* keys;        // [nsort, kIdChunk] rows sorted by label
   int32_t* slot;         // [V] cleared
@@ -249,6 +252,17 @@ struct RowArgs {
 // 0.58 ms, 2048 x 896 2.48 -> 1.17 ms, 16384 x 1536 13.5 -> 10.6 ms; no row
 // redone: 0.52, 0.92 and 9.4 ms either way.
 constexpr int kRowThreads = 1024, kRowRows = 64, kRowGroups = 256, kRowSeg = 64;
+// One sorted run: the labels of rows [base, base + kIdChunk) below nv (1024 threads).
+__device__ __forceinline__ void sort_labels(uint64_t* sk, const int64_t* y, int64_t base, int64_t nv, uint64_t* keys) {
+  const int len = (int)max((int64_t)0, min((int64_t)kIdChunk, nv - base));
+  int np2 = 64;
+  while (np2 < len) np2 <<= 1;
+  for (int i = threadIdx.x; i < np2; i += kRowThreads)
+    sk[i] = i < len ? ((uint64_t)y[base + i] << 32) | (uint32_t)i : kNoKey;
+  __syncthreads();
+  sort_keys(sk, np2);
+  for (int i = threadIdx.x; i < kIdChunk; i += kRowThreads) keys[base + i] = i < np2 ? sk[i] : kNoKey;
+}
 __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) {
   constexpr int NWR = kRowThreads / 64, U = 8;
   __shared__ union {
@@ -262,15 +276,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t nv = min(p.nc, *p.nvalid - p.c0);  // valid rows of the chunk
   if ((int)blockIdx.x < p.nsort) {
-    const int64_t base = (int64_t)blockIdx.x * kIdChunk;
-    const int len = (int)max((int64_t)0, min((int64_t)kIdChunk, nv - base));
-    int np2 = 64;
-    while (np2 < len) np2 <<= 1;
-    for (int i = tid; i < np2; i += kRowThreads)
-      sh.sk[i] = i < len ? ((uint64_t)p.y[base + i] << 32) | (uint32_t)i : kNoKey;
-    __syncthreads();
-    sort_keys(sh.sk, np2);
-    for (int i = tid; i < kIdChunk; i += kRowThreads) p.keys[base + i] = i < np2 ? sh.sk[i] : kNoKey;
+    sort_labels(sh.sk, p.y, (int64_t)blockIdx.x * kIdChunk, nv, p.keys);
     return;
   }
   const int blk = (int)blockIdx.x - p.nsort, groups = ((int)gridDim.x - p.nsort) / p.parts;
@@ -336,10 +342,13 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
     }
     const float lse2 = top + __log2f(sum);
     const bool mine = r0 + lane < nv && part == 0;
-    if (mine) p.loss_row[row] = lse2 * kLn2 - p.zy[row];
+    if (mine && p.loss_row != nullptr) p.loss_row[row] = lse2 * kLn2 - p.zy[row];
+    // (relative to the row's reference, so that a likely label's does not cancel)
+    if (mine && p.logp != nullptr)
+      p.logp[p.rows[row]] = kLn2 * (__builtin_fmaf(p.zy[row], kLog2e, -top) - __log2f(sum));
     if (p.grads) {
       // (a power of two in rows whose E is rounded once more below: then f H is exact)
-      const float g = *p.invden;
+      const float g = p.invden != nullptr ? *p.invden : 1.f;
       const float f = redone ? __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(g)) : exp2f_fast(top - lse2) * g;
       if (mine) {
         p.f[row] = f;
@@ -358,7 +367,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
   // rows with redone tiles: E of every tile times what makes it the gradient over f (8 columns never straddle a
   // tile); this part's tiles, kRowSeg of them at a time, four rows at once
   constexpr int CT = 256, UE = 4;
-  const float lse2 = sh.r.lse[lane], gm = __builtin_amdgcn_frexp_mantf(*p.invden);
+  const float lse2 = sh.r.lse[lane], gm = __builtin_amdgcn_frexp_mantf(p.invden != nullptr ? *p.invden : 1.f);
   const int64_t tper = (p.nvt + p.parts - 1) / p.parts, te = min(p.nvt, (part + 1) * tper);
   for (int64_t tb = part * tper; sh.r.n > 0 && tb < te; tb += kRowSeg) {
     const int nt = (int)min((int64_t)kRowSeg, te - tb);
@@ -749,6 +758,7 @@ struct DwArgs {
   const int64_t* nvalid;
   int64_t hdim, V, c0, chunk;
   int nI, nJ;
+  int two_in_bf16;  // over two chunks the first one's sum waits in dw
 };
 
 __global__ __launch_bounds__(NT) void flce_dw_kernel(const DwArgs p) {
@@ -762,13 +772,14 @@ __global__ __launch_bounds__(NT) void flce_dw_kernel(const DwArgs p) {
   // row at all) stores bf16 directly.  Over two chunks the first one's sum is
   // kept in dW itself, in bf16, and the second adds to it: dW is rounded
   // twice, and the fp32 [V, hdim] round trip (twice dW's size, written and
-  // read back) is saved.  Over more chunks the sum stays in fp32.
+  // read back) is saved.  Over more chunks the sum stays in fp32, as it does
+  // over two where rows' weights differ in sign and the sums may cancel.
   // mode 0: bf16 store; 1: fp32 store; 2: fp32 add; 3: fp32 add + bf16
   // store; 4: bf16 add.
   const int64_t nvt_all = *p.nvalid;
   if (p.c0 > 0 && p.c0 >= nvt_all) return;
   const bool last = p.c0 + p.chunk >= nvt_all;
-  const bool two = nvt_all <= 2 * p.chunk;
+  const bool two = p.two_in_bf16 && nvt_all <= 2 * p.chunk;
   const int mode = p.c0 == 0 ? (last || two ? 0 : 1) : (two ? 4 : (last ? 3 : 2));
   // tokens past the last 64-row step with a valid row are skipped (those up to
   // it are zero rows: flce_gather_kernel)
@@ -917,15 +928,16 @@ __global__ __launch_bounds__(1024) void flce_compact_kernel(const int64_t* __res
 // ignore_index and 0 after them, up to the next multiple of 256 and at least
 // BK - 1 of them: dW reduces over whole k-steps counted from the chunk's first
 // row, wherever that lies, so its last one reads up to BK - 1 rows past the
-// valid ones.  And dH = 0 on every row whose label does not count.  One wave
-// per row, 16 bytes per lane per step.
+// valid ones.  And dH = 0 (and logp = 0) on every row whose label does not
+// count.  One wave per row, 16 bytes per lane per step.
 __global__ __launch_bounds__(256) void flce_gather_kernel(const bf16* __restrict__ H, const bf16* __restrict__ W,
                                                           const int64_t* __restrict__ y,
                                                           const int32_t* __restrict__ rows,
                                                           const int64_t* __restrict__ nvalid, int64_t n, int64_t hdim,
-                                                          int64_t V, int64_t ignore_index, bf16* __restrict__ Hc,
-                                                          int64_t* __restrict__ yc, float* __restrict__ ref,
-                                                          bf16* __restrict__ dh) {
+                                                          int64_t V, int64_t ignore_index, float zscale,
+                                                          bf16* __restrict__ Hc, int64_t* __restrict__ yc,
+                                                          float* __restrict__ ref, bf16* __restrict__ dh,
+                                                          float* __restrict__ logp) {
   const int lane = threadIdx.x & 63;
   const int64_t nvec = hdim / 8, nv = *nvalid;
   const int64_t npad = min(((n + 255) / 256) * 256, max(((nv + 255) / 256) * 256, nv + BK - 1));
@@ -948,14 +960,16 @@ __global__ __launch_bounds__(256) void flce_gather_kernel(const bf16* __restrict
     for (int o = 32; o >= 1; o >>= 1) dot += __shfl_xor(dot, o);
     if (lane == 0) {
       yc[k] = yk;
-      ref[k] = dot * kLog2e;
+      ref[k] = dot * zscale;
     }
   }
-  if (dh == nullptr) return;  // loss only
+  if (dh == nullptr && logp == nullptr) return;  // loss only
   for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < n; t += wstep) {
     const int64_t v = y[t];
     if (v != ignore_index && v >= 0 && v < V) continue;
-    for (int64_t c = lane; c < nvec; c += 64) st_bf16x8(dh + t * hdim + 8 * c, zero_bf16x8());
+    if (logp != nullptr && lane == 0) logp[t] = 0.f;
+    if (dh != nullptr)
+      for (int64_t c = lane; c < nvec; c += 64) st_bf16x8(dh + t * hdim + 8 * c, zero_bf16x8());
   }
 }
 
@@ -1074,6 +1088,116 @@ Layout layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool need_dh, b
   return L;
 }
 
+// ---------------------------------------------------------------- weighted rows
+// Log-probabilities of the labels have one upstream gradient g a row instead of
+// one for all, known only in the backward:  dZ = g / temperature (onehot -
+// softmax).  Everything before that does not depend on g, so the forward may keep E
+// with the row's factor and label weight at g = -temperature (f0, w0: the
+// cross-entropy's for a loss weighted by 1); this pass makes f = -g f0 /
+// temperature and w likewise, and for dW the rows scaled by f and the labels
+// sorted, as the row pass does.  Rows are read from the caller's hidden states
+// in their original order and written compacted; zero rows follow the valid
+// ones up to the k-step in which dW ends.
+struct WeighArgs {
+  const bf16* H;          // [n, hdim] all rows
+  const int32_t* rows;    // chunk's compacted row -> row of H
+  const int64_t* y;       // chunk labels
+  const float* f0;        // [nc]
+  const float* w0;
+  const float* g;         // [n] upstream gradients, by original row
+  const int64_t* nvalid;
+  const int64_t* labels;  // [n] all labels, with dh: rows that do not count are zeroed
+  bf16* dh;               // or nullptr
+  bf16* Hs;               // [nc, hdim] (nsort > 0)
+  float* f;               // [nc]
+  float* wt;
+  uint64_t* keys;         // [nsort, kIdChunk]
+  int32_t* slot;          // [V] cleared
+  int64_t n, nc, c0, V, hdim, ignore_index;
+  float scale;            // -1 / temperature
+  int nsort;              // sorting workgroups (0 without dW)
+};
+__global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs p) {
+  constexpr int NWR = kRowThreads / 64;
+  __shared__ uint64_t sk[kIdChunk];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t nv = min(p.nc, *p.nvalid - p.c0);
+  if ((int)blockIdx.x < p.nsort) {
+    sort_labels(sk, p.y, (int64_t)blockIdx.x * kIdChunk, nv, p.keys);
+    return;
+  }
+  const int64_t blk = (int64_t)blockIdx.x - p.nsort, nblk = (int64_t)gridDim.x - p.nsort, nvec = p.hdim / 8;
+  if (p.nsort > 0)
+    for (int64_t v = blk * kRowThreads + tid; v < p.V; v += nblk * kRowThreads) p.slot[v] = 0;
+  if (p.nsort > 0) {
+    const int64_t end = nv > 0 ? min(p.nc, (nv + BK - 1) / BK * BK) : 0;
+    for (int64_t k = blk * NWR + w; k < end; k += nblk * NWR) {
+      const bool real = k < nv;
+      const int64_t src = real ? p.rows[k] : 0;
+      const float f = real ? p.f0[k] * (p.scale * p.g[src]) : 0.f;
+      for (int64_t c = lane; c < nvec; c += 64) {
+        bf16x8 x = zero_bf16x8();
+        if (real) {
+          x = ld_bf16x8(p.H + src * p.hdim + 8 * c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = (bf16)((float)x[i] * f);
+        }
+        st_bf16x8(p.Hs + k * p.hdim + 8 * c, x);
+      }
+    }
+  }
+  for (int64_t k = blk * kRowThreads + tid; k < nv; k += nblk * kRowThreads) {
+    const float g = p.scale * p.g[p.rows[k]];
+    p.f[k] = p.f0[k] * g;
+    p.wt[k] = p.w0[k] * g;
+  }
+  if (p.dh == nullptr) return;
+  for (int64_t t = blk * NWR + w; t < p.n; t += nblk * NWR) {
+    const int64_t v = p.labels[t];
+    if (v != p.ignore_index && v >= 0 && v < p.V) continue;
+    for (int64_t c = lane; c < nvec; c += 64) st_bf16x8(p.dh + t * p.hdim + 8 * c, zero_bf16x8());
+  }
+}
+
+// ---------------------------------------------------------------- launches
+unsigned row_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, 4096); }
+
+void launch_logits(LogitsArgs& lg, hipStream_t stream) {
+  lg.nI = (int)((lg.V + kVT - 1) / kVT);
+  lg.nJ = (int)((lg.nc + BJ - 1) / BJ);
+  const int grid = ((lg.nI * lg.nJ + kXcds - 1) / kXcds) * kXcds;
+  hipLaunchKernelGGL(flce_logits_kernel, dim3(grid), dim3(NT), 0, stream, lg);
+}
+
+void launch_row(RowArgs& rw, hipStream_t stream) {
+  const int64_t groups = (rw.nc + kRowRows - 1) / kRowRows;
+  rw.parts = rw.grads ? (int)std::max<int64_t>(kRowGroups / groups, 1) : 1;
+  hipLaunchKernelGGL(flce_row_kernel, dim3((unsigned)(rw.nsort + groups * rw.parts)), dim3(kRowThreads), 0, stream, rw);
+}
+
+void launch_dh(DhArgs& dh, hipStream_t stream) {
+  dh.nI = (int)((dh.hdim + BI - 1) / BI);
+  const int64_t units = dh_slots(dh.c0, dh.nc, dh.nI, dh.splits, dh.run);
+  const int64_t grid = kXcds * dh.nI * ((units + kXcds - 1) / kXcds);
+  hipLaunchKernelGGL(flce_dh_kernel, dim3((unsigned)grid), dim3(NT), 0, stream, dh);
+  if (dh.splits == 1) return;
+  const int64_t blocks = std::min<int64_t>((dh.nc * dh.hdim / 8 + 255) / 256, 4096);
+  hipLaunchKernelGGL(flce_dh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh);
+}
+
+void launch_dw(DwArgs& dw, hipStream_t stream) {
+  dw.nI = (int)((dw.hdim + BI - 1) / BI);
+  dw.nJ = (int)((dw.V + kVT - 1) / kVT);
+  const int grid = ((dw.nI * dw.nJ + kXcds - 1) / kXcds) * kXcds;
+  hipLaunchKernelGGL(flce_dw_kernel, dim3(grid), dim3(NT), 0, stream, dw);
+}
+
+// (a fill kernel, so that the call stays graph-capturable)
+void launch_zero(bf16* x, int64_t numel, hipStream_t stream) {
+  const int64_t nvec = numel / 8, blocks = std::min<int64_t>((nvec + 255) / 256, 4096);
+  hipLaunchKernelGGL(zero_bf16_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, x, nvec);
+}
+
 }  // namespace
 
 size_t flce_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dh, bool need_dw) {
@@ -1109,10 +1233,8 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(flce_compact_kernel, dim3(1), dim3(1024), 0, stream, a.labels, a.n, V, a.ignore_index,
                      a.reduction, a.divisor, rows, nvalid, a.count, a.bad_labels, invden);
   if (a.n > 0) {
-    int64_t blocks = (a.n + 3) / 4;
-    if (blocks > 4096) blocks = 4096;
-    hipLaunchKernelGGL(flce_gather_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a.hidden, a.weight, a.labels, rows,
-                       nvalid, a.n, Hd, V, a.ignore_index, hcomp, ycomp, ref, grads ? a.dhidden : nullptr);
+    hipLaunchKernelGGL(flce_gather_kernel, dim3(row_blocks(a.n)), dim3(256), 0, stream, a.hidden, a.weight, a.labels, rows,
+                       nvalid, a.n, Hd, V, a.ignore_index, kLog2e, hcomp, ycomp, ref, grads ? a.dhidden : nullptr, nullptr);
   }
   // chunks of compacted rows: the host sizes them for n rows; those past the
   // valid count return at once
@@ -1137,14 +1259,10 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     lg.V = V;
     lg.nc = nc;
     lg.ldp = L.chunk;
-    lg.nI = (int)L.nvt;
-    lg.nJ = (int)((nc + BJ - 1) / BJ);
     lg.store_e = grads ? 1 : 0;
-    {
-      const int total = lg.nI * lg.nJ;
-      const int grid = ((total + kXcds - 1) / kXcds) * kXcds;
-      hipLaunchKernelGGL(flce_logits_kernel, dim3(grid), dim3(NT), 0, stream, lg);
-    }
+    lg.zscale = kLog2e;
+    lg.invt = 1.f;
+    launch_logits(lg, stream);
 
     RowArgs rw{};
     rw.mpart = mpart;
@@ -1169,9 +1287,7 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     rw.ldp = L.chunk;
     rw.nsort = L.nsort;
     rw.grads = grads ? 1 : 0;
-    const int64_t groups = (nc + kRowRows - 1) / kRowRows;
-    rw.parts = grads ? (int)std::max<int64_t>(kRowGroups / groups, 1) : 1;
-    hipLaunchKernelGGL(flce_row_kernel, dim3((unsigned)(L.nsort + groups * rw.parts)), dim3(kRowThreads), 0, stream, rw);
+    launch_row(rw, stream);
     if (!grads) continue;
     auto label_sums = [&]() {
       LabelArgs la{};
@@ -1204,21 +1320,10 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     dh.c0 = c0;
     dh.hdim = Hd;
     dh.nc = nc;
-    dh.nI = (int)((Hd + BI - 1) / BI);
     dh.splits = L.splits;
     dh.prow = L.prow;
     dh.run = L.run;
-    {
-      const int64_t units = dh_slots(c0, nc, dh.nI, L.splits, L.run);
-      const int64_t grid = kXcds * dh.nI * ((units + kXcds - 1) / kXcds);
-      hipLaunchKernelGGL(flce_dh_kernel, dim3((unsigned)grid), dim3(NT), 0, stream, dh);
-    }
-    if (L.splits > 1) {
-      const int64_t nvec = nc * Hd / 8;
-      int64_t blocks = (nvec + 255) / 256;
-      if (blocks > 4096) blocks = 4096;
-      hipLaunchKernelGGL(flce_dh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh);
-    }
+    launch_dh(dh, stream);
 
     if (a.dweight != nullptr) {
       if (!in_place) label_sums();
@@ -1234,22 +1339,267 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
       dw.c0 = c0;
       dw.hdim = Hd;
       dw.V = V;
-      dw.nI = (int)((Hd + BI - 1) / BI);
-      dw.nJ = (int)L.nvt;
       dw.chunk = L.chunk;
-      const int total = dw.nI * dw.nJ;
-      const int grid = ((total + kXcds - 1) / kXcds) * kXcds;
-      hipLaunchKernelGGL(flce_dw_kernel, dim3(grid), dim3(NT), 0, stream, dw);
+      dw.two_in_bf16 = 1;
+      launch_dw(dw, stream);
     }
   }
-  if (grads && a.n == 0 && a.dweight != nullptr) {
-    // no rows: d loss / d W is zero (a fill kernel, so the call stays graph-capturable)
-    const int64_t nvec = V * Hd / 8;
-    int64_t blocks = (nvec + 255) / 256;
-    if (blocks > 4096) blocks = 4096;
-    hipLaunchKernelGGL(zero_bf16_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a.dweight, nvec);
-  }
+  if (grads && a.n == 0 && a.dweight != nullptr) launch_zero(a.dweight, V * Hd, stream);
   hipLaunchKernelGGL(flce_loss_kernel, dim3(1), dim3(1024), 0, stream, loss_row, a.n, nvalid, invden, a.loss);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- log-probabilities of the labels
+namespace {
+
+// What the forward keeps for the backward.
+struct FlpSaved {
+  size_t nvalid, rows, yc, f0, w0, E, total;
+};
+FlpSaved flp_saved(int64_t n, int64_t V) {
+  FlpSaved S{};
+  size_t off = 256;  // nvalid at 0
+  S.rows = off;
+  off += al(sizeof(int32_t) * (size_t)n);
+  S.yc = off;
+  off += al(sizeof(int64_t) * (size_t)((n + 255) / 256 * 256));
+  S.f0 = off;
+  off += al(sizeof(float) * (size_t)n);
+  S.w0 = off;
+  off += al(sizeof(float) * (size_t)n);
+  S.E = off;
+  off += al(sizeof(bf16) * (size_t)n * (size_t)V);
+  S.total = off;
+  return S;
+}
+
+// Workspace of either direction; parts that a call does not need have no size.
+struct FlpLayout {
+  size_t scal, spart, mpart, zy, ref, hc, saved, part, f, wt, acc32, keys, slot, next, lsum, total;
+  int64_t chunk, nchunks, nvt;
+  int splits, prow, run, nsort;
+};
+// logits: the logits product and its row pass run (not: E comes from the
+// forward); grads: the gradient products.
+FlpLayout flp_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool logits, bool grads, bool need_dw,
+                     bool have_saved) {
+  FlpLayout L{};
+  L.chunk = std::max<int64_t>(std::min(chunk, n), 1);
+  L.nchunks = (n + L.chunk - 1) / L.chunk;
+  L.nvt = (V + kVT - 1) / kVT;
+  const size_t npad = (size_t)((std::max<int64_t>(n, 1) + 255) / 256 * 256);
+  size_t off = 256;  // scal: an unused divisor, the count and the bad labels of a backward
+  auto take = [&](bool on, size_t bytes) {
+    const size_t at = off;
+    if (on) off += al(bytes);
+    return at;
+  };
+  L.spart = take(logits, sizeof(float) * (size_t)(L.chunk * L.nvt));
+  L.mpart = take(logits, sizeof(float) * (size_t)(L.chunk * L.nvt));
+  L.zy = take(logits, sizeof(float) * (size_t)L.chunk);
+  L.ref = take(logits, sizeof(float) * npad);
+  L.hc = take(logits || need_dw, sizeof(bf16) * npad * (size_t)hdim);
+  // a state of its own, with one chunk's E (the backward's) or none (a forward that keeps nothing)
+  L.saved = take(!have_saved, flp_saved(n, 0).total + (grads ? sizeof(bf16) * (size_t)(L.chunk * V) : 0));
+  L.splits = dh_splits(hdim, L.chunk);
+  L.prow = (int)std::min<int64_t>(L.chunk, BJ);
+  L.run = dh_run(V);
+  int64_t slots = 0;
+  if (grads && L.splits > 1)
+    for (int64_t c0 = 0; c0 < n; c0 += L.chunk)
+      slots = std::max(slots, dh_slots(c0, std::min(L.chunk, n - c0), (int)((hdim + BI - 1) / BI), L.splits, L.run));
+  L.part = take(slots > 0, sizeof(float) * (size_t)(slots * L.prow * hdim));
+  L.f = take(grads, sizeof(float) * (size_t)L.chunk);
+  L.wt = take(grads, sizeof(float) * (size_t)L.chunk);
+  L.nsort = need_dw ? (int)((L.chunk + kIdChunk - 1) / kIdChunk) : 0;
+  L.acc32 = take(need_dw && L.nchunks > 1, sizeof(float) * (size_t)(V * hdim));
+  L.keys = take(need_dw, sizeof(uint64_t) * (size_t)L.nsort * kIdChunk);
+  L.slot = take(need_dw, sizeof(int32_t) * (size_t)V);
+  L.next = take(need_dw, sizeof(int32_t) * (size_t)L.nsort * kIdChunk);
+  L.lsum = take(need_dw, sizeof(float) * (size_t)(L.chunk * hdim));
+  L.total = off;
+  return L;
+}
+
+template <class T>
+T* at(void* base, size_t off) {
+  return reinterpret_cast<T*>(static_cast<char*>(base) + off);
+}
+
+float zscale_of(const FlpArgs& a) { return (float)(1.4426950408889634 / a.temperature); }
+
+// The valid rows' list and their compacted hidden states, labels and references.
+void flp_compact(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSaved& S, float* logp, int64_t* count,
+                 int64_t* bad, bf16* dh, hipStream_t stream) {
+  hipLaunchKernelGGL(flce_compact_kernel, dim3(1), dim3(1024), 0, stream, a.labels, a.n, a.vocab, a.ignore_index, 0,
+                     nullptr, at<int32_t>(saved, S.rows), at<int64_t>(saved, S.nvalid), count, bad,
+                     at<float>(a.ws, L.scal));
+  if (a.n > 0)
+    hipLaunchKernelGGL(flce_gather_kernel, dim3(row_blocks(a.n)), dim3(256), 0, stream, a.hidden, a.weight, a.labels,
+                       at<int32_t>(saved, S.rows), at<int64_t>(saved, S.nvalid), a.n, a.hdim, a.vocab, a.ignore_index,
+                       zscale_of(a), at<bf16>(a.ws, L.hc), at<int64_t>(saved, S.yc),
+                       at<float>(a.ws, L.ref), dh, logp);
+}
+
+// Logits and row pass of the chunk at c0: E (unless nullptr) with f0 and w0, logp (unless nullptr).
+void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSaved& S, int64_t c0, bf16* E, float* f0,
+                float* w0, float* logp, hipStream_t stream) {
+  const int64_t nc = std::min(L.chunk, a.n - c0);
+  LogitsArgs lg{};
+  lg.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
+  lg.H = GOp{at<bf16>(a.ws, L.hc) + c0 * a.hdim, a.hdim, nc, a.hdim};
+  lg.y = at<int64_t>(saved, S.yc) + c0;
+  lg.ref = at<float>(a.ws, L.ref) + c0;
+  lg.E = E;
+  lg.mpart = at<float>(a.ws, L.mpart);
+  lg.spart = at<float>(a.ws, L.spart);
+  lg.zy = at<float>(a.ws, L.zy);
+  lg.nvalid = at<int64_t>(saved, S.nvalid);
+  lg.c0 = c0;
+  lg.V = a.vocab;
+  lg.nc = nc;
+  lg.ldp = L.chunk;
+  lg.store_e = E != nullptr ? 1 : 0;
+  lg.zscale = zscale_of(a);
+  lg.invt = (float)(1. / a.temperature);
+  launch_logits(lg, stream);
+
+  RowArgs rw{};
+  rw.mpart = lg.mpart;
+  rw.spart = lg.spart;
+  rw.ref = lg.ref;
+  rw.zy = lg.zy;
+  rw.y = lg.y;
+  rw.E = E;
+  rw.f = f0;
+  rw.wt = w0;
+  rw.logp = logp;
+  rw.rows = at<int32_t>(saved, S.rows) + c0;
+  rw.nvalid = lg.nvalid;
+  rw.c0 = c0;
+  rw.nc = nc;
+  rw.nvt = L.nvt;
+  rw.V = a.vocab;
+  rw.hdim = a.hdim;
+  rw.ldp = L.chunk;
+  rw.grads = lg.store_e;
+  launch_row(rw, stream);
+}
+
+}  // namespace
+
+size_t flp_saved_bytes(int64_t n, int64_t vocab) { return flp_saved(n, vocab).total; }
+
+size_t flp_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, bool keep) {
+  return flp_layout(n, hdim, vocab, keep ? n : kLossChunk, true, false, false, keep).total;
+}
+
+size_t flp_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw, bool have_saved) {
+  return flp_layout(n, hdim, vocab, have_saved ? n : chunk, !have_saved, true, need_dw, have_saved).total;
+}
+
+hipError_t flp_fwd(const FlpArgs& a, hipStream_t stream) {
+  const bool keep = a.saved != nullptr;
+  const FlpLayout L = flp_layout(a.n, a.hdim, a.vocab, keep ? a.n : kLossChunk, true, false, false, keep);
+  const FlpSaved S = flp_saved(a.n, keep ? a.vocab : 0);
+  char* saved = keep ? static_cast<char*>(a.saved) : at<char>(a.ws, L.saved);
+  flp_compact(a, L, saved, S, a.logp, a.count, a.bad_labels, nullptr, stream);
+  for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk)
+    flp_logits(a, L, saved, S, c0, keep ? at<bf16>(saved, S.E) : nullptr, at<float>(saved, S.f0), at<float>(saved, S.w0),
+               a.logp, stream);
+  return hipGetLastError();
+}
+
+hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
+  const bool have = a.saved != nullptr, need_dw = a.dweight != nullptr;
+  const FlpLayout L = flp_layout(a.n, a.hdim, a.vocab, have ? a.n : a.chunk, !have, true, need_dw, have);
+  const FlpSaved S = flp_saved(a.n, have ? a.vocab : 0);
+  char* saved = have ? static_cast<char*>(a.saved) : at<char>(a.ws, L.saved);
+  bf16* E = at<bf16>(saved, S.E);  // of all rows, or of one chunk
+  if (a.n == 0) {
+    if (need_dw) launch_zero(a.dweight, a.vocab * a.hdim, stream);
+    return hipGetLastError();
+  }
+  if (!have) flp_compact(a, L, saved, S, nullptr, at<int64_t>(a.ws, L.scal) + 1, at<int64_t>(a.ws, L.scal) + 2, a.dhidden, stream);
+  const int64_t* nvalid = at<int64_t>(saved, S.nvalid);
+  for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
+    const int64_t nc = std::min(L.chunk, a.n - c0);
+    float *f0 = at<float>(saved, S.f0) + c0, *w0 = at<float>(saved, S.w0) + c0;
+    if (!have) flp_logits(a, L, saved, S, c0, E, f0, w0, nullptr, stream);
+    bf16* Hs = at<bf16>(a.ws, L.hc) + c0 * a.hdim;
+    WeighArgs wg{};
+    wg.H = a.hidden;
+    wg.rows = at<int32_t>(saved, S.rows) + c0;
+    wg.y = at<int64_t>(saved, S.yc) + c0;
+    wg.f0 = f0;
+    wg.w0 = w0;
+    wg.g = a.dlogp;
+    wg.nvalid = nvalid;
+    wg.labels = a.labels;
+    wg.dh = have ? a.dhidden : nullptr;
+    wg.Hs = Hs;
+    wg.f = at<float>(a.ws, L.f);
+    wg.wt = at<float>(a.ws, L.wt);
+    wg.keys = at<uint64_t>(a.ws, L.keys);
+    wg.slot = at<int32_t>(a.ws, L.slot);
+    wg.n = a.n;
+    wg.nc = nc;
+    wg.c0 = c0;
+    wg.V = a.vocab;
+    wg.hdim = a.hdim;
+    wg.ignore_index = a.ignore_index;
+    wg.scale = (float)(-1. / a.temperature);
+    wg.nsort = L.nsort;
+    const int64_t blocks = std::min<int64_t>((nc + kRowThreads / 64 - 1) / (kRowThreads / 64), 1024);
+    hipLaunchKernelGGL(flce_weigh_kernel, dim3((unsigned)(L.nsort + blocks)), dim3(kRowThreads), 0, stream, wg);
+
+    if (a.dhidden != nullptr) {
+      DhArgs dh{};
+      dh.Wt = GOp{a.weight, a.hdim, a.vocab, a.hdim};
+      dh.E = GOp{E, a.vocab, nc, a.vocab};
+      dh.dh = a.dhidden;
+      dh.part = at<float>(a.ws, L.part);
+      dh.f = wg.f;
+      dh.wt = wg.wt;
+      dh.y = wg.y;
+      dh.rows = at<int32_t>(saved, S.rows);
+      dh.nvalid = nvalid;
+      dh.c0 = c0;
+      dh.hdim = a.hdim;
+      dh.nc = nc;
+      dh.splits = L.splits;
+      dh.prow = L.prow;
+      dh.run = L.run;
+      launch_dh(dh, stream);
+    }
+    if (need_dw) {
+      LabelArgs la{};
+      la.keys = wg.keys;
+      la.H = a.hidden;
+      la.rows = wg.rows;
+      la.wt = wg.wt;
+      la.lsum = at<float>(a.ws, L.lsum);
+      la.slot = wg.slot;
+      la.next = at<int32_t>(a.ws, L.next);
+      la.hdim = a.hdim;
+      la.nsort = L.nsort;
+      hipLaunchKernelGGL(flce_label_kernel, dim3((unsigned)nc), dim3(256), 0, stream, la);
+      DwArgs dw{};
+      dw.Ht = GOp{Hs, a.hdim, nc, a.hdim};
+      dw.Et = GOp{E, a.vocab, nc, a.vocab};
+      dw.slot = la.slot;
+      dw.next = la.next;
+      dw.lsum = la.lsum;
+      dw.dw = a.dweight;
+      dw.acc32 = at<float>(a.ws, L.acc32);
+      dw.nvalid = nvalid;
+      dw.c0 = c0;
+      dw.hdim = a.hdim;
+      dw.V = a.vocab;
+      dw.chunk = L.chunk;
+      launch_dw(dw, stream);
+    }
+  }
   return hipGetLastError();
 }
 

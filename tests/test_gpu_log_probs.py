@@ -1,0 +1,252 @@
+"""Log-probabilities of labels on the GPU against the oracle in 64 bits, kept and recomputed, alone and with the losses
+that read them."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import log_probs as olp
+from oracle import policy as op
+from siq_vl_amd import cross_entropy as C
+from siq_vl_amd import log_probs as LP
+from siq_vl_amd import policy as P
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def make(n, hdim, vocab, seed=0, ignored=0.3, wscale=0.05, lean=0.0):
+    g = torch.Generator().manual_seed(seed)
+    w = (wscale * torch.randn(vocab, hdim, generator=g)).to(torch.bfloat16)
+    y = torch.randint(0, vocab, (n,), generator=g)
+    h = torch.randn(n, hdim, generator=g) + lean * torch.rand(n, 1, generator=g) * w[y].float() / (wscale ** 2 * hdim)
+    y[torch.rand(n, generator=g) < ignored] = -100
+    up = torch.randn(n, generator=g) * torch.rand(n, generator=g)
+    up[torch.rand(n, generator=g) < 0.2] = 0.0
+    return h.to(torch.bfloat16), w, y, up
+
+
+def check(h, w, y, up, temperature=1.0, keep=True, chunk=None, need_dw=True, rounds=1.0):
+    hd, wd, yd = h.to(DEV), w.to(DEV), y.to(DEV)
+    logp, count, bad, saved = LP.flp_fwd(hd, wd, yd, temperature=temperature, keep=keep)
+    assert (saved is not None) == keep
+    dh, dw = LP.flp_bwd(hd, wd, yd, up.to(DEV), temperature=temperature, saved=saved, need_dweight=need_dw,
+                        chunk_tokens=chunk)
+    torch.cuda.synchronize()
+    ref = olp.linear_log_probs(np64(h), np64(w), y.numpy(), np64(up), temperature)
+    assert int(count) == ref["count"] and int(bad) == ref["bad"]
+    assert (np.abs(np64(logp) - ref["logp"]) <= ref["logp_off"]).all()
+    out = (y == -100) | (y < 0) | (y >= w.shape[0])
+    assert bool((logp.cpu()[out] == 0).all()) and bool((dh.cpu()[out] == 0).all())
+    assert (np.abs(np64(dh) - ref["dh"]) <= rounds * ref["dh_off"]).all()
+    if need_dw:
+        assert (np.abs(np64(dw) - ref["dw"]) <= rounds * ref["dw_off"]).all()
+    else:
+        assert dw is None
+    return logp, dh, dw
+
+
+@pytest.mark.parametrize("keep,chunk", [(True, None), (False, None), (False, 128), (False, 64), (False, 100)])
+@pytest.mark.parametrize("n,hdim,vocab", [(1, 64, 8), (3, 64, 1000), (255, 320, 264), (257, 128, 2000), (300, 896, 1000)])
+def test_against_the_oracle(n, hdim, vocab, keep, chunk):
+    print(f"logp n={n} h={hdim} V={vocab} keep={keep} chunk={chunk}", flush=True)
+    h, w, y, up = make(n, hdim, vocab, seed=n, ignored=0.3 if n > 1 else 0.0)
+    check(h, w, y, up, 1.0, keep, chunk)
+    check(h, w, y, up, 0.7, keep, chunk)
+    check(h, w, y, up, 1.9, keep, chunk, need_dw=False)
+
+
+@pytest.mark.parametrize("keep", [True, False])
+def test_likely_labels_keep_their_digits(keep):
+    h, w, y, up = make(400, 256, 1000, seed=5, lean=40.0)
+    logp, _, _ = check(h, w, y, up, 1.0, keep)
+    assert float(logp[y.to(DEV) >= 0].max()) > -1e-3
+
+
+@pytest.mark.parametrize("keep", [True, False])
+def test_labels_far_below_the_largest_logit(keep):
+    """Logits a hundred apart: whole tiles are formed again relative to their own maximum, and rounded twice."""
+    h, w, y, up = make(300, 128, 1000, seed=6, wscale=2.0)
+    logp, _, _ = check(h, w, y, up, 1.0, keep, rounds=2.0)
+    assert float(logp.min()) < -60
+    check(h, w, y, up, 0.25, keep, rounds=2.0)
+
+
+@pytest.mark.parametrize("keep", [True, False])
+def test_one_label_for_all_rows_and_labels_at_the_ends(keep):
+    h, w, y, up = make(700, 128, 264, seed=7)
+    y[y >= 0] = 17
+    check(h, w, y, up, 1.0, keep)
+    y[::2], y[1::2] = 0, 263
+    check(h, w, y, up, 1.0, keep)
+
+
+@pytest.mark.parametrize("keep", [True, False])
+def test_nothing_counts_no_rows_and_bad_labels(keep):
+    h, w, y, up = make(300, 128, 1000, seed=8)
+    y[:] = -100
+    _, dh, dw = check(h, w, y, up, 1.0, keep)
+    assert bool((dw == 0).all())
+    logp, count, bad, saved = LP.flp_fwd(h[:0].to(DEV), w.to(DEV), y[:0].to(DEV), keep=keep)
+    dh, dw = LP.flp_bwd(h[:0].to(DEV), w.to(DEV), y[:0].to(DEV), up[:0].to(DEV), saved=saved)
+    assert logp.shape == (0,) and int(count) == 0 and dh.shape == (0, 128) and bool((dw == 0).all())
+    y[:] = 5
+    y[3], y[200] = 1000, -7
+    check(h, w, y, up, 1.0, keep)
+    with pytest.raises(C.LabelError):
+        LP.fused_linear_log_probs(h.to(DEV), w.to(DEV), y.to(DEV), validate="sync")
+    # upstream gradients of rows that do not count are not read
+    up[3] = up[200] = float("nan")
+    dh, dw = LP.flp_bwd(h.to(DEV), w.to(DEV), y.to(DEV), up.to(DEV))
+    assert not bool(dh.isnan().any()) and not bool(dw.isnan().any())
+
+
+def test_mean_is_the_cross_entropy_and_its_gradients_bitwise():
+    h, w, y, _ = make(600, 320, 2000, seed=9)
+    hd, wd, yd = h.to(DEV), w.to(DEV), y.to(DEV)
+    loss, count, _, dh, dw = C.flce_fwd_bwd(hd, wd, yd, chunk_tokens=1024)
+    logp, _, _, saved = LP.flp_fwd(hd, wd, yd, keep=True)
+    assert abs(float(loss) + float(logp.double().sum()) / int(count)) <= 1e-6 * float(loss)
+    up = torch.full((600,), -1.0, device=DEV) / count.float()
+    for s in (saved, None):
+        dh2, dw2 = LP.flp_bwd(hd, wd, yd, up, saved=s, chunk_tokens=1024)
+        assert torch.equal(dh, dh2) and torch.equal(dw, dw2)
+
+
+def test_kept_and_recomputed_agree_and_repeat():
+    h, w, y, up = make(900, 256, 3008, seed=10)
+    hd, wd, yd, ud = h.to(DEV), w.to(DEV), y.to(DEV), up.to(DEV)
+    a = LP.flp_fwd(hd, wd, yd, keep=True)
+    b = LP.flp_fwd(hd, wd, yd, keep=False)
+    assert torch.equal(a[0], b[0])
+    before = a[3].clone()
+    first = LP.flp_bwd(hd, wd, yd, ud, saved=a[3])
+    assert torch.equal(a[3], before)  # only read
+    for s, chunk in ((a[3], None), (None, 1024)):
+        again = LP.flp_bwd(hd, wd, yd, ud, saved=s, chunk_tokens=chunk)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    assert torch.equal(LP.flp_bwd(hd, wd, yd, ud, saved=a[3], need_dweight=False)[0], first[0])
+    only_w = LP.flp_bwd(hd, wd, yd, ud, saved=a[3], need_dhidden=False)
+    assert only_w[0] is None and torch.equal(only_w[1], first[1])
+
+
+def test_autograd_shapes_types_frozen_and_retained():
+    h, w, y, up = make(60, 128, 520, seed=11)
+    hg = h.view(4, 15, 128).to(DEV).requires_grad_()
+    wg, yd, ud = w.to(DEV).requires_grad_(), y.view(4, 15).to(DEV), up.view(4, 15).to(DEV)
+    want = LP.flp_bwd(hg.detach().view(60, 128), wg.detach(), yd.view(-1), ud.view(-1), temperature=1.3)
+    for keep_bytes in (1 << 30, 0):
+        logp = LP.fused_linear_log_probs(hg, wg, yd, temperature=1.3, keep_bytes=keep_bytes)
+        assert logp.shape == (4, 15) and logp.dtype == torch.float32
+        got = torch.autograd.grad(logp, [hg, wg], ud, retain_graph=True)
+        again = torch.autograd.grad(logp, [hg, wg], ud)
+        assert torch.equal(got[0].view(60, 128), want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+    frozen = LP.fused_linear_log_probs(hg, wg.detach(), yd, temperature=1.3)
+    assert torch.equal(torch.autograd.grad(frozen, [hg], ud)[0].view(60, 128), want[0])
+    head = LP.fused_linear_log_probs(hg.detach(), wg, yd, temperature=1.3)
+    assert torch.equal(torch.autograd.grad(head, [wg], ud)[0], want[1])
+    with torch.no_grad():
+        lone = LP.fused_linear_log_probs(hg, wg, yd, temperature=1.3)
+    assert lone.grad_fn is None and torch.equal(lone, logp)
+    # a broadcast upstream gradient, and fp32 master copies
+    g1, = torch.autograd.grad(LP.fused_linear_log_probs(hg, wg.detach(), yd).sum(), [hg])
+    g2, = torch.autograd.grad(LP.fused_linear_log_probs(hg, wg.detach(), yd), [hg], torch.ones(4, 15, device=DEV))
+    assert torch.equal(g1, g2)
+    h32, w32 = hg.detach().float().requires_grad_(), wg.detach().float().requires_grad_()
+    got = torch.autograd.grad(LP.fused_linear_log_probs(h32, w32, yd, temperature=1.3), [h32, w32], ud)
+    assert got[0].dtype == torch.float32 and torch.equal(got[0].view(60, 128), want[0].float())
+    assert torch.equal(got[1], want[1].float())
+
+
+def test_gradient_is_a_difference():
+    """One direction in ``hidden``, central differences of the fp32 log-probabilities."""
+    h, w, y, up = make(64, 128, 520, seed=12, ignored=0.1)
+    g = torch.Generator().manual_seed(1)
+    h = (h.float() * 8).round().div(8).to(torch.bfloat16)  # steps of 1 / 8 below 16: moved by 1 / 16 exactly
+    d = (torch.randint(-1, 2, h.shape, generator=g) / 16).to(torch.bfloat16)
+    hd, wd, yd, ud = h.to(DEV), w.to(DEV), y.to(DEV), up.to(DEV).double()
+    assert torch.equal((hd + d.to(DEV)).float(), hd.float() + d.to(DEV).float())
+    up_, down = (LP.flp_fwd(hd + s * d.to(DEV), wd, yd)[0].double() for s in (1, -1))
+    num = ((up_ - down) * ud / 2).cpu().numpy()
+    dh, _ = LP.flp_bwd(hd, wd, yd, up.to(DEV), need_dweight=False)
+    got = (dh.double() * d.to(DEV).double()).sum(1).cpu().numpy()
+    ref = olp.linear_log_probs(np64(h), np64(w), y.numpy(), np64(up))
+    # a row's move changes its logits by s = |w| |d| at most, typically 0.05 * 128^0.5 / 20: the third derivative of a
+    # log-sum-exp is at most 2 s^3 / 6; plus what rounding makes of the gradient and of the two values
+    s = np.abs(np64(d)) @ np.abs(np64(w)).T
+    spread = np.linalg.norm(np64(d), axis=1) * np.linalg.norm(np64(w), axis=1).max()
+    bound = np.abs(np64(up)) * (spread ** 3 / 3 + ref["logp_off"]) + (ref["dh_off"] * np.abs(np64(d))).sum(1) + 1e-9
+    assert s.max() > 0 and (np.abs(num - got) <= bound).all()
+
+
+def chain(kind, h, w, y, cu, mask, old, ref, adv, dtype64=False):
+    """Hidden states to loss and gradients, as a training step runs it."""
+    hg, wg = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    logp = LP.fused_linear_log_probs(hg, wg, y.to(DEV))
+    if kind == "pref":
+        loss = P.preference_loss(logp, ref, cu, mask=mask, beta=0.5).loss
+    else:
+        loss = P.policy_loss(logp, old, adv, cu, mask=mask, reference_logps=ref, kl_coef=0.1, aggregation="sequence").loss
+    loss.backward()
+    return float(loss.detach()), hg.grad, wg.grad
+
+
+@pytest.mark.parametrize("kind", ["pref", "policy"])
+def test_a_run_from_hidden_states_to_the_loss(kind):
+    lengths = [70, 130, 1, 99, 0, 200]
+    n = sum(lengths)
+    h, w, y, _ = make(n, 256, 1000, seed=13, ignored=0.4)
+    cu = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    base = olp.linear_log_probs(np64(h), np64(w), y.numpy())["logp"]
+    rng = np.random.default_rng(3)
+    old, ref = (np.float32(base + 0.2 * rng.standard_normal(n)) for _ in range(2))
+    adv = np.float32(rng.standard_normal(len(lengths)))
+    mask = (y != -100).numpy()
+    cu_t, mask_t, old_t, ref_t, adv_t = (torch.tensor(v, device=DEV) for v in (cu, mask, old, ref, adv))
+    loss, dh, dw = chain(kind, h, w, y, cu_t, mask_t, old_t, ref_t, adv_t)
+    if kind == "pref":
+        want, _, _, g = op.preference(base, ref, cu, mask, beta=0.5)
+    else:
+        want, _, _, g = op.policy(base, old, adv, cu, mask, ref, kl_coef=0.1, aggregation="sequence")
+    out = olp.linear_log_probs(np64(h), np64(w), y.numpy(), g)
+    # what the log-probabilities' own error does to the weights: sums of up to 200 of them in the pairs' margins
+    wobble = 1 + 300 * out["logp_off"].max()
+    assert abs(loss - want) <= 300 * out["logp_off"].max() * (1 + abs(want))
+    assert (np.abs(np64(dh) - out["dh"]) <= wobble * out["dh_off"] + (wobble - 1) * np.abs(out["dh"])).all()
+    assert (np.abs(np64(dw) - out["dw"]) <= wobble * out["dw_off"] + (wobble - 1) * np.abs(out["dw"]).max()).all()
+
+
+def test_streams_and_captured_calls():
+    h, w, y, up = make(500, 128, 1000, seed=14)
+    hd, wd, yd, ud = h.to(DEV), w.to(DEV), y.to(DEV), up.to(DEV)
+
+    def call(keep):
+        logp, _, _, saved = LP.flp_fwd(hd, wd, yd, keep=keep)
+        return (logp, *LP.flp_bwd(hd, wd, yd, ud, saved=saved, chunk_tokens=128))
+
+    want = [call(True), call(False)]
+    torch.cuda.synchronize()
+    got = []
+    for st in [torch.cuda.Stream() for _ in range(2)]:
+        with torch.cuda.stream(st):
+            got.append([call(True), call(False)])
+    torch.cuda.synchronize()
+    for pair in got:
+        for a, b in zip(pair, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [call(True), call(False)]
+    for i in range(3):
+        hd.copy_(torch.randn_like(hd))
+        yd.copy_(yd.roll(1))
+        ud.copy_(torch.randn_like(ud))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, [call(True), call(False)]):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
