@@ -81,12 +81,13 @@ struct LogitsArgs {
   bf16* E;                // [nc, V]
   float* spart;           // [nvt, ldp] tile sum of exp2(z2 - ref); negated for a redone tile
   float* mpart;           // [nvt, ldp] a redone tile's own reference
-  float* zy;              // [nc] label logit (natural units)
+  float* zy;              // [nc] label logit (natural units); label_apart: log2 units, relative to ref
   const int64_t* nvalid;  // valid (compacted) rows in all chunks
   int64_t V, nc, c0, ldp;
   int nI, nJ;
   int store_e;            // 0: loss only, E is not needed
-  float zscale, invt;     // log2(e) / temperature, 1 / temperature
+  int label_apart;        // the label is left out of E and of the sums
+  float zscale;           // log2(e) / temperature
 };
 
 __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
@@ -160,8 +161,11 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
       for (int a = 0; a < 4; ++a)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (hit && r0 == wave_row(a, 0) + 16 * (r >> 3) + (r & 7)) zsel = acc[a][b][r];
-      if (hit) p.zy[tok] = zsel * p.invt;
+          if (hit && r0 == wave_row(a, 0) + 16 * (r >> 3) + (r & 7)) {
+            zsel = acc[a][b][r];
+            if (p.label_apart) acc[a][b][r] = -INFINITY;
+          }
+      if (hit) p.zy[tok] = p.label_apart ? __builtin_fmaf(zsel, p.zscale, -ref[b]) : zsel;
     }
     const float sum = numerators(b, ref[b], p.store_e && tv);
     if (h == 0) red[wi * 256 + col] = sum;
@@ -221,15 +225,15 @@ struct RowArgs {
   const float* spart;    // [nvt, ldp] tile sums (negative: redone, relative to mpart)
   const float* mpart;
   const float* ref;      // [nc] row references (log2 units)
-  const float* zy;
+  const float* zy;       // [nc] as the logits kernel left it
   const int64_t* y;      // chunk labels
   bf16* E;               // [nc, V]
   bf16* H;               // [nc, hdim] compacted rows: scaled by f (need_dw)
   float* f;              // [nc] factors of E
   float* wt;             // [nc] weights of the label terms
-  float* loss_row;       // [nc] (chunk slice), or nullptr
-  float* logp;           // [n] log-probabilities of the labels by original row, or nullptr
-  const int32_t* rows;   // compacted row -> original row (chunk slice; with logp)
+  float* loss_row;       // [nc] (chunk slice; not with label_apart)
+  float* logp;           // [n] log-probabilities of the labels by original row (label_apart), or nullptr
+  const int32_t* rows;   // compacted row -> original row (chunk slice; label_apart)
   const float* invden;   // nullptr: 1
   const int64_t* nvalid;
   uint64_t* keys;        // [nsort, kIdChunk] rows sorted by label
@@ -238,6 +242,7 @@ struct RowArgs {
   int nsort;             // sorting workgroups (0 without dW)
   int parts;             // workgroups per 64 rows
   int grads;             // 0: loss only (E was never stored)
+  int label_apart;
 };
 
 // Workgroups [0, nsort) sort the chunk's labels; the others take 64 rows each,
@@ -340,20 +345,32 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       for (int i = 0; i < NWR; ++i)
         if (sh.r.redone[i][lane] > 0.f) sum += sh.r.redone[i][lane] * exp2f_fast(sh.r.mx[i][lane] - top);
     }
-    const float lse2 = top + __log2f(sum);
     const bool mine = r0 + lane < nv && part == 0;
-    if (mine && p.loss_row != nullptr) p.loss_row[row] = lse2 * kLn2 - p.zy[row];
-    // (relative to the row's reference, so that a likely label's does not cancel)
-    if (mine && p.logp != nullptr)
-      p.logp[p.rows[row]] = kLn2 * (__builtin_fmaf(p.zy[row], kLog2e, -top) - __log2f(sum));
+    float lse2, w0, f0;  // log2 sum, (probability of the label) - 1, what E times it is a probability
+    if (p.label_apart) {
+      // `sum` is that of the other columns: with t its ratio to the label's term the label's probability is 1 / (1 + t),
+      // and both its logarithm and its distance from 1 keep their digits where t is small.  Redone tiles are 2^60 above
+      // the label: there only the sum counts.
+      const float d = p.zy[row], t = sum * exp2f_fast(-d), all = sum + exp2f_fast(d);
+      const float lp = redone ? -kLn2 * (__log2f(sum) + (top - rf - d)) : -log1pf(t);
+      lse2 = top + __log2f(redone ? sum : all);
+      f0 = 1.f / all;
+      w0 = redone ? -1.f : -t / (1.f + t);
+      if (mine && p.logp != nullptr) p.logp[p.rows[row]] = lp;
+    } else {
+      lse2 = top + __log2f(sum);
+      f0 = exp2f_fast(top - lse2);
+      w0 = exp2f_fast(__builtin_fmaf(p.zy[row], kLog2e, -lse2)) - 1.f;
+      if (mine) p.loss_row[row] = lse2 * kLn2 - p.zy[row];
+    }
     if (p.grads) {
       // (a power of two in rows whose E is rounded once more below: then f H is exact)
       const float g = p.invden != nullptr ? *p.invden : 1.f;
-      const float f = redone ? __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(g)) : exp2f_fast(top - lse2) * g;
+      const float f = redone ? __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(g)) : f0 * g;
       if (mine) {
         p.f[row] = f;
-        p.wt[row] = (exp2f_fast(__builtin_fmaf(p.zy[row], kLog2e, -lse2)) - 1.f) * g;
-        if (!redone) p.E[row * p.V + p.y[row]] = (bf16)0.f;
+        p.wt[row] = w0 * g;
+        if (!redone && !p.label_apart) p.E[row * p.V + p.y[row]] = (bf16)0.f;
       }
       sh.r.f[lane] = f;
       sh.r.lse[lane] = lse2;
@@ -1261,7 +1278,6 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     lg.ldp = L.chunk;
     lg.store_e = grads ? 1 : 0;
     lg.zscale = kLog2e;
-    lg.invt = 1.f;
     launch_logits(lg, stream);
 
     RowArgs rw{};
@@ -1461,7 +1477,7 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   lg.ldp = L.chunk;
   lg.store_e = E != nullptr ? 1 : 0;
   lg.zscale = zscale_of(a);
-  lg.invt = (float)(1. / a.temperature);
+  lg.label_apart = 1;
   launch_logits(lg, stream);
 
   RowArgs rw{};
@@ -1483,6 +1499,7 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   rw.hdim = a.hdim;
   rw.ldp = L.chunk;
   rw.grads = lg.store_e;
+  rw.label_apart = 1;
   launch_row(rw, stream);
 }
 
