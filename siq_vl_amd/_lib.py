@@ -209,6 +209,14 @@ def check(rc: int, what: str) -> None:
     raise RuntimeError(text)
 
 
+def first_order(what: str) -> None:
+    """Raises in a backward that is itself recorded (``create_graph=True``): the
+    kernels' gradients carry no graph, and a second derivative would come out
+    as if they were constants."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative (create_graph=True)")
+
+
 def on_device(device):
     """A context in which ``device`` is the current GPU (none is entered when it
     is already): kernels go to the current one, whatever their stream."""

@@ -204,8 +204,8 @@ class _Swiglu8(torch.autograd.Function):
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        _lib.first_order("swiglu8")
         dgate, dup, _ = swiglu8_bwd(dh, ctx.saved_tensors, ctx.fmt)
         return dgate, dup, None
 
@@ -220,8 +220,8 @@ class _Swiglu8Fused(torch.autograd.Function):
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        _lib.first_order("swiglu8")
         return swiglu8_bwd(dh, ctx.saved_tensors, ctx.fmt, fused=True)[0], None
 
 
@@ -250,8 +250,8 @@ class _Swiglu8Linear(torch.autograd.Function):
         return torch.nn.functional.linear(h, weight)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _lib.first_order("swiglu8_linear")
         weight, *stores = ctx.saved_tensors
         need_in, need_w = any(ctx.needs_input_grad[:2]), ctx.needs_input_grad[2]
         dgate, dup, h = swiglu8_bwd(dy @ weight, stores, ctx.fmt, need_h=need_w)

@@ -94,8 +94,8 @@ class _FusedLinearLogProbs(torch.autograd.Function):
         return logp.view(labels.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dlogp):
+        _lib.first_order("fused_linear_log_probs")
         hidden, weight, labels, *saved = ctx.saved_tensors
         dh, dw = flp_bwd(hidden.reshape(-1, hidden.shape[-1]), weight, labels.reshape(-1), dlogp.reshape(-1),
                          ctx.ignore_index, ctx.temperature, saved[0] if saved else None, ctx.needs_input_grad[0],

@@ -111,11 +111,14 @@ class _Preference(torch.autograd.Function):
         ctx.save_for_backward(coef, cu, *(() if mask is None else (mask,)))
         ctx.shape, ctx.pairs = policy.shape, pairs
         ctx.mark_non_differentiable(chosen, rejected)
+        ctx.set_materialize_grads(False)
         return loss, chosen, rejected
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, *_):
+        _lib.first_order("preference_loss")
+        if grad_loss is None:
+            return (None,) * 10
         coef, cu, *mask = ctx.saved_tensors
         grad = grad_loss.to(torch.float32)
         dev = coef.device
@@ -182,11 +185,14 @@ class _Policy(torch.autograd.Function):
         ctx.shape, ctx.seqs, ctx.aggregation = logps.shape, seqs, aggregation
         loss, kl, cut = stats.unbind()
         ctx.mark_non_differentiable(kl, cut)
+        ctx.set_materialize_grads(False)
         return loss, kl, cut
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, *_):
+        _lib.first_order("policy_loss")
+        if grad_loss is None:
+            return (None,) * 14
         dtoken, weight, *cu = ctx.saved_tensors
         grad = grad_loss.to(torch.float32)
         dev = dtoken.device

@@ -335,3 +335,11 @@ def test_on_a_qwen2_model(which):
     for n, g in grads.items():
         rel = float((g - grads0[n]).norm() / grads0[n].norm())
         assert rel <= 0.1, (n, rel)
+
+
+def test_a_second_derivative_is_refused():
+    g = torch.randn(4, 64, device=DEV, requires_grad=True)
+    w = torch.randn(8, 64, device=DEV)
+    for y in (K.swiglu8(g, g), K.swiglu8(g), K.swiglu8_linear(g, g, w)):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y.sum(), [g], create_graph=True)

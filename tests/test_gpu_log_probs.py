@@ -277,3 +277,10 @@ def test_streams_and_captured_calls():
         torch.cuda.synchronize()
         for a, b in zip(captured, [call(True), call(False)]):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_a_second_derivative_is_refused():
+    h, w, y, _ = make(20, 64, 264)
+    hg = h.to(DEV).requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(LP.fused_linear_log_probs(hg, w.to(DEV), y.to(DEV)).sum(), [hg], create_graph=True)

@@ -341,3 +341,12 @@ def test_captured_losses_replay_on_new_values():
         want = call(lp_t.clone().copy_(leaf.detach()).requires_grad_())
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_a_second_derivative_is_refused():
+    cu, _, pi, old, _ = batch([4, 6])
+    pi_t, old_t, cu_t = gpu(pi, old, cu)
+    pi_t.requires_grad_()
+    for loss in (P.preference_loss(pi_t, old_t, cu_t).loss, P.policy_loss(pi_t, old_t, torch.ones(2, device=DEV), cu_t).loss):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(loss, [pi_t], create_graph=True)
