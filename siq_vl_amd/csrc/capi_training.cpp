@@ -82,8 +82,8 @@ int check_flp(int64_t n, int64_t hdim, int64_t vocab) {
   if (hdim <= 0 || vocab <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "hdim and vocab must be positive");
   if (hdim % 64 != 0) return fail(SIQ_ERR_UNSUPPORTED, "hdim (%lld) must be a multiple of 64", (long long)hdim);
   if (vocab % 8 != 0) return fail(SIQ_ERR_UNSUPPORTED, "vocab (%lld) must be a multiple of 8", (long long)vocab);
-  if (n >= (int64_t(1) << 31) || vocab >= (int64_t(1) << 31) || hdim >= (int64_t(1) << 20))
-    return fail(SIQ_ERR_INVALID_ARGUMENT, "n and vocab must be < 2^31, hdim < 2^20");
+  if (n >= (int64_t(1) << 31) || vocab >= (int64_t(1) << 23) || hdim >= (int64_t(1) << 20))
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "n must be < 2^31, vocab < 2^23 and hdim < 2^20");
   return SIQ_OK;
 }
 

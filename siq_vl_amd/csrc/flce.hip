@@ -1176,6 +1176,317 @@ __global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// The products of a call of few rows (one short answer, a decoding step's
+// tokens) read the whole weight for little arithmetic: 32 NB columns of a tile
+// are rows of the call, where the general kernels' tiles have 256 of which most
+// would be padding.  Smaller stages let two workgroups share a CU, so loads are
+// in flight while the other one waits at a barrier.  k-steps of 64 in two
+// buffers: the next one is loading while this one is multiplied.
+
+// One k-step's loads of an operand with k contiguous: ROWS rows x 64 k (swizzled
+// as gemm.h's KC halves), 8 rows an instruction, dealt over NWV waves.
+template <int ROWS, int NWV>
+struct FewRows {
+  static constexpr int PER = ROWS / 8 / NWV;
+  uint32_t off[PER];
+  __device__ __forceinline__ void init(int64_t ld, int64_t last, int lane, int w) {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int r = 8 * (PER * w + q) + lane / 8;
+      off[q] = 2 * (uint32_t)(min((int64_t)r, last) * ld + 8 * ((lane % 8) ^ swz_kc(r)));
+    }
+  }
+  __device__ __forceinline__ void issue(const bf16* base, bf16* lds, int wu) const {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) dma16(base, off[q], lds + (PER * wu + q) * 512);
+  }
+};
+
+constexpr int kFewRows = 128;  // rows of a call (NB = 2: 64) that take these kernels
+
+// The logits kernel over 256 vocabulary rows x 32 NB rows of the call: eight
+// waves, 32 vocabulary rows each.  Same outputs; always with the label apart.
+template <int NB>
+__global__ __launch_bounds__(NT) void flce_logits_few_kernel(const LogitsArgs p) {
+  constexpr int TOK = 32 * NB, STAGE = (BI + TOK) * BK, NWV = NT / 64;
+  __shared__ __align__(16) bf16 smem[2 * STAGE];
+  const int64_t i0 = (int64_t)blockIdx.x * BI;
+  if (*p.nvalid <= p.c0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  const int64_t vbase = i0 + 32 * w + 8 * h;  // accumulator r: vocabulary row vbase + 16 (r / 8) + r % 8
+  FewRows<BI, NWV> la;
+  FewRows<TOK, NWV> lb;
+  la.init(p.W.ld, p.V - 1 - i0, lane, w);
+  lb.init(p.H.ld, p.nc - 1, lane, w);
+  const bf16 *wb = p.W.base + i0 * p.W.ld, *hb = p.H.base;
+  HalfRead<true, true, 1> ra;
+  HalfRead<true, false, NB> rb;
+  ra.init(lane, 32 * w);
+  rb.init(lane, 0);
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = zero16();
+  const int n = (int)(p.W.cols / BK);
+  auto issue = [&](int s) {
+    bf16* st = smem + (s & 1) * STAGE;
+    lb.issue(hb + (int64_t)s * BK, st + BI * BK, wu);
+    la.issue(wb + (int64_t)s * BK, st, wu);
+  };
+  issue(0);
+  float ref[NB];
+  int rel[NB];  // the token's label, counted from vbase (-1: not in this wave's rows)
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t tok = min((int64_t)(32 * b + l32), p.nc - 1);
+    ref[b] = p.ref[tok];
+    const int64_t d = p.y[tok] - vbase;
+    rel[b] = d >= 0 && d < 32 && (d & 8) == 0 ? (int)d : -1;
+  }
+  for (int s = 0; s < n; ++s) {
+    if (s + 1 < n) {
+      issue(s + 1);
+      wait_vmcnt<FewRows<BI, NWV>::PER + FewRows<TOK, NWV>::PER>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    phase_barrier();
+    const bf16 *A = smem + (s & 1) * STAGE, *B = A + BI * BK;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const bf16x8 a = ra.read(A, 0, ks);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, rb.read(B, b, ks), acc[b]);
+    }
+    wait_lds();
+    phase_barrier();
+  }
+  // (in the stages' place: two workgroups share a CU's LDS)
+  float *red = reinterpret_cast<float*>(smem), *tot = red + NWV * TOK, *top = tot + TOK;  // [NWV][TOK], [TOK], [TOK]
+  if (i0 + BI > p.V) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (vbase + 16 * (r >> 3) + (r & 7) >= p.V) acc[b][r] = -INFINITY;
+  }
+  auto numerators = [&](int b, float m2, bool store) {
+    const int64_t tok = 32 * b + l32;
+    float sum = 0.f;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      const int64_t v0 = vbase + 16 * jj;
+      bf16x8 e8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = exp2f_fast(__builtin_fmaf(acc[b][8 * jj + i], p.zscale, -m2));
+        sum += e;
+        e8[i] = (bf16)e;
+      }
+      if (store && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e8);
+    }
+    return half_sum(sum);
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t tok = 32 * b + l32;
+    const bool tv = tok < p.nc, hit = tv && rel[b] >= 0;
+    if (__any(hit)) {
+      float zsel = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (hit && rel[b] == 16 * (r >> 3) + (r & 7)) {
+          zsel = acc[b][r];
+          acc[b][r] = -INFINITY;
+        }
+      if (hit) p.zy[tok] = __builtin_fmaf(zsel, p.zscale, -ref[b]);
+    }
+    const float sum = numerators(b, ref[b], p.store_e && tv);
+    if (h == 0) red[w * TOK + 32 * b + l32] = sum;
+  }
+  __syncthreads();
+  // a thread a token: the tile's sum
+  bool redo = false;
+  if (tid < TOK) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < NWV; ++k) t += red[k * TOK + tid];
+    tot[tid] = t;
+    redo = tid < p.nc && !(t < kRefLimit);
+    if (tid < p.nc) p.spart[(int64_t)blockIdx.x * p.ldp + tid] = t;
+  }
+  if (!__syncthreads_or(redo)) return;
+  // tokens whose reference is too low: the same relative to the tile's maximum
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[b][r]);
+    mx = half_max(mx) * p.zscale;
+    if (h == 0) red[w * TOK + 32 * b + l32] = mx;
+  }
+  __syncthreads();
+  if (tid < TOK) {
+    float m = red[tid];
+#pragma unroll
+    for (int k = 1; k < NWV; ++k) m = fmaxf(m, red[k * TOK + tid]);
+    top[tid] = m;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int tok = 32 * b + l32;
+    const float sum = numerators(b, top[tok], p.store_e && tok < p.nc && !(tot[tok] < kRefLimit));
+    if (h == 0) red[w * TOK + tok] = sum;
+  }
+  __syncthreads();
+  if (tid < TOK && tid < p.nc && !(tot[tid] < kRefLimit)) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < NWV; ++k) t += red[k * TOK + tid];
+    p.spart[(int64_t)blockIdx.x * p.ldp + tid] = -t;
+    p.mpart[(int64_t)blockIdx.x * p.ldp + tid] = top[tid];
+  }
+}
+
+// dH of few rows: 128 hidden features x 32 NB rows of the call x a range of the
+// vocabulary a workgroup, four waves of 32 features.  About 512 workgroups (two
+// a CU); block b runs on XCD b % 8, and the tiles of one range, which share its
+// columns of E, follow one another there.
+constexpr int kFewBI = 128, kFewThreads = 256, kFewPerXcd = 64;
+int few_splits(int64_t hdim, int64_t V) {
+  const int64_t nI = (hdim + kFewBI - 1) / kFewBI, steps = (V + BK - 1) / BK;
+  return (int)(kXcds * std::min(std::max<int64_t>(kFewPerXcd / nI, 1), (steps + kXcds - 1) / kXcds));
+}
+template <int NB>
+__global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p) {
+  constexpr int TOK = 32 * NB, STAGE = (kFewBI + TOK) * BK, NWV = kFewThreads / 64, QA = 16 / NWV;
+  __shared__ __align__(16) bf16 smem[2 * STAGE];
+  if (*p.nvalid <= p.c0) return;
+  const int x = (int)(blockIdx.x % kXcds), k = (int)(blockIdx.x / kXcds);
+  const int ti = k % p.nI, split = x + kXcds * (k / p.nI);
+  const int64_t i0 = (int64_t)ti * kFewBI, V = p.E.cols;
+  const int64_t S = (V + BK - 1) / BK, per = (S + p.splits - 1) / p.splits;
+  const int64_t kb = min(split * per * BK, V), ke = min((split + 1) * per * BK, V);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  const int ld = (int)p.Wt.ld;
+  uint32_t oa[QA];
+  int ra0[QA];  // k row of the stage
+#pragma unroll
+  for (int q = 0; q < QA; ++q) {
+    const int r = 4 * (QA * w + q) + lane / 16;
+    ra0[q] = r;
+    oa[q] = 2 * (uint32_t)(r * ld + min(8 * ((lane % 16) ^ swz_nkc(r)), (int)min(p.hdim - 8 - i0, (int64_t)(kFewBI - 8))));
+  }
+  FewRows<TOK, NWV> lb;
+  lb.init(p.E.ld, p.nc - 1, lane, w);
+  HalfRead<false, true, 1> ra;
+  HalfRead<true, false, NB> rb;
+  ra.init(lane, 32 * w);
+  rb.init(lane, 0);
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = zero16();
+  const int n = (int)((ke - kb + BK - 1) / BK);
+  auto issue = [&](int s) {
+    bf16* st = smem + (s & 1) * STAGE;
+    const int64_t k0 = kb + (int64_t)s * BK;
+    const int kval = (int)min(ke - k0, (int64_t)BK);
+    // past the last row of the weight and the last columns of E: valid ones again (E's are zeroed below)
+#pragma unroll
+    for (int q = 0; q < QA; ++q)
+      dma16(p.Wt.base + k0 * ld + i0, oa[q] - 2 * (uint32_t)(max(0, ra0[q] - (kval - 1)) * ld), st + (QA * wu + q) * 512);
+    const bf16* eb = p.E.base + k0;
+#pragma unroll
+    for (int q = 0; q < lb.PER; ++q) {
+      const int r = 8 * (lb.PER * w + q) + lane / 8, c = 8 * ((lane % 8) ^ swz_kc(r));
+      dma16(eb, lb.off[q] - 2 * (uint32_t)max(0, c - (kval - 8)), st + kFewBI * BK + (lb.PER * wu + q) * 512);
+    }
+  };
+  if (n > 0) issue(0);
+  for (int s = 0; s < n; ++s) {
+    if (s + 1 < n) {
+      issue(s + 1);
+      wait_vmcnt<QA + FewRows<TOK, NWV>::PER>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    phase_barrier();
+    bf16 *A = smem + (s & 1) * STAGE, *B = A + kFewBI * BK;
+    const int kval = (int)min(ke - kb - (int64_t)s * BK, (int64_t)BK);
+    if (kval < BK) {
+      for (int i = tid; i < TOK * 8; i += kFewThreads) {
+        const int r = i / 8, c = i % 8;
+        if (8 * c >= kval) st_bf16x8(B + r * BK + 8 * (c ^ swz_kc(r)), zero_bf16x8());
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const bf16x8 a = ra.read(A, 0, ks);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, rb.read(B, b, ks), acc[b]);
+    }
+    wait_lds();
+    phase_barrier();
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t tok = 32 * b + l32;
+    if (tok >= p.nc) continue;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      const int64_t hh = i0 + 32 * w + 16 * jj + 8 * h;
+      if (hh >= p.hdim) continue;
+      float* dst = p.part + ((int64_t)split * p.prow + tok) * p.hdim + hh;
+      f32x4 lo, hi;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = acc[b][8 * jj + i];
+        hi[i] = acc[b][8 * jj + 4 + i];
+      }
+      *reinterpret_cast<f32x4*>(dst) = lo;
+      *reinterpret_cast<f32x4*>(dst + 4) = hi;
+    }
+  }
+}
+
+// The sum over the ranges, with the factor and the label term: a workgroup a row
+// and 256 features, thirty-two lanes of 8 features x eight that share the ranges.
+__global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const DhArgs p) {
+  __shared__ __align__(16) float sh[8][32][8];
+  const int64_t nv = min(p.nc, *p.nvalid - p.c0), r = blockIdx.y;
+  if (r >= nv) return;
+  const int g = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 256 + 8 * g, stride = (int64_t)p.prow * p.hdim;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+  if (col < p.hdim) {
+    const float* src = p.part + r * p.hdim + col;
+#pragma unroll 4
+    for (int s = q; s < p.splits; s += 8) {
+      a += *reinterpret_cast<const f32x4*>(src + s * stride);
+      b += *reinterpret_cast<const f32x4*>(src + s * stride + 4);
+    }
+  }
+  *reinterpret_cast<f32x4*>(&sh[q][g][0]) = a;
+  *reinterpret_cast<f32x4*>(&sh[q][g][4]) = b;
+  __syncthreads();
+  if (q != 0 || col >= p.hdim) return;
+  const bf16x8 l = ld_bf16x8(p.Wt.base + p.y[r] * p.hdim + col);
+  const float f = p.f[r], wt = p.wt[r];
+  bf16x8 o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += sh[k][g][i];
+    o[i] = (bf16)__builtin_fmaf(f, t, wt * (float)l[i]);
+  }
+  st_bf16x8(p.dh + (int64_t)p.rows[p.c0 + r] * p.hdim + col, o);
+}
+
 // ---------------------------------------------------------------- launches
 unsigned row_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, 4096); }
 
@@ -1200,6 +1511,25 @@ void launch_dh(DhArgs& dh, hipStream_t stream) {
   if (dh.splits == 1) return;
   const int64_t blocks = std::min<int64_t>((dh.nc * dh.hdim / 8 + 255) / 256, 4096);
   hipLaunchKernelGGL(flce_dh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh);
+}
+
+void launch_logits_few(LogitsArgs& lg, hipStream_t stream) {
+  const dim3 grid((unsigned)((lg.V + kVT - 1) / kVT));
+  if (lg.nc <= 64)
+    hipLaunchKernelGGL(flce_logits_few_kernel<2>, grid, dim3(NT), 0, stream, lg);
+  else
+    hipLaunchKernelGGL(flce_logits_few_kernel<4>, grid, dim3(NT), 0, stream, lg);
+}
+
+void launch_dh_few(DhArgs& dh, hipStream_t stream) {
+  dh.nI = (int)((dh.hdim + kFewBI - 1) / kFewBI);
+  const dim3 grid((unsigned)(dh.nI * dh.splits));
+  if (dh.nc <= 64)
+    hipLaunchKernelGGL(flce_dh_few_kernel<2>, grid, dim3(kFewThreads), 0, stream, dh);
+  else
+    hipLaunchKernelGGL(flce_dh_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, dh);
+  hipLaunchKernelGGL(flce_dh_few_sum_kernel, dim3((unsigned)((dh.hdim + 255) / 256), (unsigned)dh.nc), dim3(256), 0, stream,
+                     dh);
 }
 
 void launch_dw(DwArgs& dw, hipStream_t stream) {
@@ -1394,6 +1724,7 @@ struct FlpLayout {
   size_t scal, spart, mpart, zy, ref, hc, saved, part, f, wt, acc32, keys, slot, next, lsum, total;
   int64_t chunk, nchunks, nvt;
   int splits, prow, run, nsort;
+  bool few;
 };
 // logits: the logits product and its row pass run (not: E comes from the
 // forward); grads: the gradient products.
@@ -1417,11 +1748,12 @@ FlpLayout flp_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool log
   L.hc = take(logits || need_dw, sizeof(bf16) * npad * (size_t)hdim);
   // a state of its own, with one chunk's E (the backward's) or none (a forward that keeps nothing)
   L.saved = take(!have_saved, flp_saved(n, 0).total + (grads ? sizeof(bf16) * (size_t)(L.chunk * V) : 0));
-  L.splits = dh_splits(hdim, L.chunk);
+  L.few = L.chunk <= kFewRows;
+  L.splits = L.few ? few_splits(hdim, V) : dh_splits(hdim, L.chunk);
   L.prow = (int)std::min<int64_t>(L.chunk, BJ);
   L.run = dh_run(V);
-  int64_t slots = 0;
-  if (grads && L.splits > 1)
+  int64_t slots = grads && L.few ? L.splits : 0;
+  if (grads && !L.few && L.splits > 1)
     for (int64_t c0 = 0; c0 < n; c0 += L.chunk)
       slots = std::max(slots, dh_slots(c0, std::min(L.chunk, n - c0), (int)((hdim + BI - 1) / BI), L.splits, L.run));
   L.part = take(slots > 0, sizeof(float) * (size_t)(slots * L.prow * hdim));
@@ -1478,7 +1810,10 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   lg.store_e = E != nullptr ? 1 : 0;
   lg.zscale = zscale_of(a);
   lg.label_apart = 1;
-  launch_logits(lg, stream);
+  if (L.few)
+    launch_logits_few(lg, stream);
+  else
+    launch_logits(lg, stream);
 
   RowArgs rw{};
   rw.mpart = lg.mpart;
@@ -1587,7 +1922,10 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       dh.splits = L.splits;
       dh.prow = L.prow;
       dh.run = L.run;
-      launch_dh(dh, stream);
+      if (L.few)
+        launch_dh_few(dh, stream);
+      else
+        launch_dh(dh, stream);
     }
     if (need_dw) {
       LabelArgs la{};

@@ -51,7 +51,7 @@ def check(h, w, y, up, temperature=1.0, keep=True, chunk=None, need_dw=True, rou
 
 
 @pytest.mark.parametrize("keep,chunk", [(True, None), (False, None), (False, 128), (False, 64), (False, 100)])
-@pytest.mark.parametrize("n,hdim,vocab", [(1, 64, 8), (3, 64, 1000), (255, 320, 264), (257, 128, 2000), (300, 896, 1000)])
+@pytest.mark.parametrize("n,hdim,vocab", [(64, 64, 2000), (65, 192, 1000), (128, 320, 4104), (129, 320, 4104), (1, 64, 8), (3, 64, 1000), (255, 320, 264), (257, 128, 2000), (300, 896, 1000)])
 def test_against_the_oracle(n, hdim, vocab, keep, chunk):
     print(f"logp n={n} h={hdim} V={vocab} keep={keep} chunk={chunk}", flush=True)
     h, w, y, up = make(n, hdim, vocab, seed=n, ignored=0.3 if n > 1 else 0.0)
@@ -67,18 +67,20 @@ def test_likely_labels_keep_their_digits(keep):
     assert float(logp[y.to(DEV) >= 0].max()) > -1e-3
 
 
+@pytest.mark.parametrize("n", [50, 100, 300])
 @pytest.mark.parametrize("keep", [True, False])
-def test_labels_far_below_the_largest_logit(keep):
+def test_labels_far_below_the_largest_logit(n, keep):
     """Logits a hundred apart: whole tiles are formed again relative to their own maximum, and rounded twice."""
-    h, w, y, up = make(300, 128, 1000, seed=6, wscale=2.0)
+    h, w, y, up = make(n, 128, 1000, seed=6, wscale=2.0)
     logp, _, _ = check(h, w, y, up, 1.0, keep, rounds=2.0)
     assert float(logp.min()) < -60
     check(h, w, y, up, 0.25, keep, rounds=2.0)
 
 
 @pytest.mark.parametrize("keep", [True, False])
-def test_one_label_for_all_rows_and_labels_at_the_ends(keep):
-    h, w, y, up = make(700, 128, 264, seed=7)
+@pytest.mark.parametrize("n", [40, 700])
+def test_one_label_for_all_rows_and_labels_at_the_ends(n, keep):
+    h, w, y, up = make(n, 128, 264, seed=7)
     y[y >= 0] = 17
     check(h, w, y, up, 1.0, keep)
     y[::2], y[1::2] = 0, 263

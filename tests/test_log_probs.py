@@ -60,7 +60,7 @@ def _bwd(lib, **kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(n=-1), INVALID), (dict(n=2 ** 31), INVALID), (dict(hdim=0), INVALID), (dict(hdim=100), UNSUPPORTED),
-    (dict(vocab=1001), UNSUPPORTED), (dict(vocab=2 ** 31), INVALID), (dict(h=None), INVALID), (dict(h=FAKE + 8), ALIGN),
+    (dict(vocab=1001), UNSUPPORTED), (dict(vocab=2 ** 23), INVALID), (dict(h=None), INVALID), (dict(h=FAKE + 8), ALIGN),
     (dict(w=None), INVALID), (dict(w=FAKE + 2), ALIGN), (dict(y=None), INVALID), (dict(t=0.0), INVALID),
     (dict(t=-1.0), INVALID), (dict(t=float("inf")), INVALID), (dict(t=float("nan")), INVALID), (dict(t=1e-45), INVALID),
     (dict(saved=FAKE, sb=100), WS), (dict(saved=FAKE + 8, sb=1 << 30), WS), (dict(ws=None), WS), (dict(wb=64), WS),
