@@ -36,23 +36,27 @@ class DeferredChecks:
         host = torch.empty(counts.shape, dtype=counts.dtype, pin_memory=True)
         host.copy_(counts, non_blocking=True)
         ev = torch.cuda.Event()
-        ev.record(torch.cuda.current_stream(counts.device))
+        stream = torch.cuda.current_stream(counts.device)
+        ev.record(stream)
         with self._lock:
-            self._pending.append((ev, host, judge))
+            self._pending.append((ev, (counts.device, stream.cuda_stream), host, judge))
 
     def check(self, block: bool = False) -> None:
         """Judges every tracked call whose counts have landed (all of them when
         ``block``); the first bad one raises, and each call is judged once."""
         landed = []
+        behind = set()  # streams with a call that has not landed: later ones there have not either, and are not asked
         with self._lock:
             keep = []
-            for ev, host, judge in self._pending:
+            for call in self._pending:
+                ev, where, host, judge = call
                 if block:
                     ev.synchronize()
-                if ev.query():
+                if where not in behind and ev.query():
                     landed.append((host, judge))
                 else:
-                    keep.append((ev, host, judge))
+                    behind.add(where)
+                    keep.append(call)
             self._pending[:] = keep
         for host, judge in landed:
             judge(host.reshape(-1).tolist())

@@ -1487,6 +1487,162 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const DhArgs p) {
   st_bf16x8(p.dh + (int64_t)p.rows[p.c0 + r] * p.hdim + col, o);
 }
 
+// dW of few rows, one chunk: 128 hidden features x 128 vocabulary rows a
+// workgroup, four waves of 64 x 64, all of the call's rows (STEPS k-steps of 64)
+// loaded at once.  There is next to nothing to multiply: it is bound by writing
+// dW, so small workgroups, several a CU, whose stores overlap the others' loads.
+// Rows past the valid ones are zeroed in LDS.
+template <int STEPS>
+__global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p) {
+  constexpr int TILE = 128, OP = BK * TILE, QA = 4;
+  __shared__ __align__(16) bf16 smem[2 * STEPS * OP];
+  int ti, tj;
+  if (!tile_of(p.nI, p.nJ, p.nI, ti, tj)) return;
+  const int64_t i0 = (int64_t)ti * TILE, j0 = (int64_t)tj * TILE;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int wi = w & 1, wj = w >> 1, wu = __builtin_amdgcn_readfirstlane(w);
+  const int nc = (int)p.Ht.rows, nv = (int)min((int64_t)nc, *p.nvalid);
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) acc[a][b] = zero16();
+  int slot[2] = {0, 0};
+  if (nv > 0) {
+    const int ca = (int)min(p.hdim - 8 - i0, (int64_t)(TILE - 8)), cb = (int)min(p.V - 8 - j0, (int64_t)(TILE - 8));
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (BK * s >= nv) break;
+#pragma unroll
+      for (int q = 0; q < QA; ++q) {
+        const int r = 4 * (QA * w + q) + lane / 16, c = 8 * ((lane % 16) ^ swz_nkc(r)), row = min(BK * s + r, nc - 1);
+        bf16* dst = smem + 2 * s * OP + (QA * wu + q) * 512;
+        dma16(p.Ht.base + i0, 2 * (uint32_t)(row * (int)p.hdim + min(c, ca)), dst);
+        dma16(p.Et.base + j0, 2 * ((uint32_t)row * (uint32_t)p.V + (uint32_t)min(c, cb)), dst + OP);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) slot[b] = p.slot[min(j0 + 64 * wj + 32 * b + l32, p.V - 1)];
+    HalfRead<false, true, 2> ra;
+    HalfRead<false, false, 2> rb;
+    ra.init(lane, 64 * wi);
+    rb.init(lane, 64 * wj);
+    wait_vmcnt<0>();
+    __syncthreads();
+    const int full = nv / BK, tail = nv - full * BK;
+    if (tail > 0) {
+      bf16* B = smem + (2 * full + 1) * OP;
+      for (int i = tail * 16 + tid; i < BK * 16; i += kFewThreads) st_bf16x8(B + 8 * i, zero_bf16x8());
+      __syncthreads();
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (BK * s >= nv) break;
+      const bf16 *A = smem + 2 * s * OP, *B = A + OP;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        bf16x8 a[2], b[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          a[t] = ra.read(A, t, ks);
+          b[t] = rb.read(B, t, ks);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) acc[x][y] = mfma32(a[x], b[y], acc[x][y]);
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int64_t v = j0 + 64 * wj + 32 * b + l32;
+    if (v >= p.V) continue;
+    for (int sl = slot[b]; sl > 0; sl = p.next[sl - 1]) {
+      const float* lt = p.lsum + (int64_t)(sl - 1) * p.hdim;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int64_t hh = i0 + 64 * wi + 32 * a + 16 * jj + 8 * h;
+          if (hh >= p.hdim) continue;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(lt + hh), hi = *reinterpret_cast<const f32x4*>(lt + hh + 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[a][b][8 * jj + i] += lo[i];
+            acc[a][b][8 * jj + 4 + i] += hi[i];
+          }
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const int64_t hh = i0 + 64 * wi + 32 * a + 16 * jj + 8 * h;
+        if (hh < p.hdim) st_bf16x8(p.dw + v * p.hdim + hh, pack8(acc[a][b], 8 * jj));
+      }
+  }
+}
+
+// The valid rows' list, as flce_compact_kernel's, and their compacted operands,
+// as flce_gather_kernel's, in one launch: with at most kFewRows labels every wave
+// finds the row that it copies by itself.  Wave k takes the k-th valid row, and
+// clears what belongs to row k if that does not count.
+__global__ __launch_bounds__(256) void flce_few_rows_kernel(const bf16* __restrict__ H, const bf16* __restrict__ W,
+                                                            const int64_t* __restrict__ y, int n, int64_t hdim,
+                                                            int64_t V, int64_t ignore_index, float zscale,
+                                                            int32_t* __restrict__ rows, int64_t* __restrict__ nvalid,
+                                                            int64_t* __restrict__ count, int64_t* __restrict__ bad,
+                                                            bf16* __restrict__ Hc, int64_t* __restrict__ yc,
+                                                            float* __restrict__ ref, bf16* __restrict__ dh,
+                                                            float* __restrict__ logp) {
+  constexpr int G = kFewRows / 64;
+  const int lane = threadIdx.x & 63, k = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+  int64_t v[G];
+  uint64_t m[G];
+  int nv = 0, nbad = 0, src = -1;
+#pragma unroll
+  for (int g = 0; g < G; ++g) v[g] = 64 * g + lane < n ? y[64 * g + lane] : ignore_index;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const bool ok = v[g] >= 0 && v[g] < V && v[g] != ignore_index;
+    m[g] = __ballot(ok);
+    nbad += __popcll(__ballot(v[g] != ignore_index && !ok));
+    const int rank = nv + __popcll(m[g] & (lane ? ~0ull >> (64 - lane) : 0ull));
+    const uint64_t mine = __ballot(ok && rank == k);
+    if (mine != 0) src = 64 * g + (int)__builtin_ctzll(mine);
+    nv += __popcll(m[g]);
+  }
+  if (k == 0 && lane == 0) {
+    *nvalid = *count = nv;
+    *bad = nbad;
+  }
+  if (k >= n) return;
+  const int64_t nvec = hdim / 8, yk = src >= 0 ? y[src] : ignore_index;
+  float dot = 0.f;
+  for (int64_t c = lane; c < nvec; c += 64) {
+    bf16x8 x = zero_bf16x8();
+    if (src >= 0) {
+      x = ld_bf16x8(H + src * hdim + 8 * c);
+      const bf16x8 wy = ld_bf16x8(W + yk * hdim + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = __builtin_fmaf((float)x[i], (float)wy[i], dot);
+    }
+    st_bf16x8(Hc + (int64_t)k * hdim + 8 * c, x);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) dot += __shfl_xor(dot, o);
+  if (lane == 0) {
+    if (src >= 0) rows[k] = src;
+    yc[k] = yk;
+    ref[k] = dot * zscale;
+  }
+  if ((m[k / 64] >> (k % 64)) & 1) return;
+  if (logp != nullptr && lane == 0) logp[k] = 0.f;
+  if (dh != nullptr)
+    for (int64_t c = lane; c < nvec; c += 64) st_bf16x8(dh + (int64_t)k * hdim + 8 * c, zero_bf16x8());
+}
+
 // ---------------------------------------------------------------- launches
 unsigned row_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, 4096); }
 
@@ -1530,6 +1686,16 @@ void launch_dh_few(DhArgs& dh, hipStream_t stream) {
     hipLaunchKernelGGL(flce_dh_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, dh);
   hipLaunchKernelGGL(flce_dh_few_sum_kernel, dim3((unsigned)((dh.hdim + 255) / 256), (unsigned)dh.nc), dim3(256), 0, stream,
                      dh);
+}
+
+void launch_dw_few(DwArgs& dw, hipStream_t stream) {
+  dw.nI = (int)((dw.hdim + 127) / 128);
+  dw.nJ = (int)((dw.V + 127) / 128);
+  const int grid = ((dw.nI * dw.nJ + kXcds - 1) / kXcds) * kXcds;
+  if (dw.Ht.rows <= BK)
+    hipLaunchKernelGGL(flce_dw_few_kernel<1>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
+  else
+    hipLaunchKernelGGL(flce_dw_few_kernel<2>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
 }
 
 void launch_dw(DwArgs& dw, hipStream_t stream) {
@@ -1779,6 +1945,13 @@ float zscale_of(const FlpArgs& a) { return (float)(1.4426950408889634 / a.temper
 // The valid rows' list and their compacted hidden states, labels and references.
 void flp_compact(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSaved& S, float* logp, int64_t* count,
                  int64_t* bad, bf16* dh, hipStream_t stream) {
+  if (a.n > 0 && a.n <= kFewRows) {
+    hipLaunchKernelGGL(flce_few_rows_kernel, dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, stream, a.hidden, a.weight,
+                       a.labels, (int)a.n, a.hdim, a.vocab, a.ignore_index, zscale_of(a), at<int32_t>(saved, S.rows),
+                       at<int64_t>(saved, S.nvalid), count, bad, at<bf16>(a.ws, L.hc), at<int64_t>(saved, S.yc),
+                       at<float>(a.ws, L.ref), dh, logp);
+    return;
+  }
   hipLaunchKernelGGL(flce_compact_kernel, dim3(1), dim3(1024), 0, stream, a.labels, a.n, a.vocab, a.ignore_index, 0,
                      nullptr, at<int32_t>(saved, S.rows), at<int64_t>(saved, S.nvalid), count, bad,
                      at<float>(a.ws, L.scal));
@@ -1952,7 +2125,10 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       dw.hdim = a.hdim;
       dw.V = a.vocab;
       dw.chunk = L.chunk;
-      launch_dw(dw, stream);
+      if (L.few && L.nchunks == 1)
+        launch_dw_few(dw, stream);
+      else
+        launch_dw(dw, stream);
     }
   }
   return hipGetLastError();
