@@ -64,7 +64,7 @@ def _format(fmt: str) -> int:
 def _check(t: torch.Tensor, name: str) -> None:
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must live on the GPU, got {t.device}")
 
 
@@ -125,7 +125,7 @@ def unpack8(packed: Packed8, dtype: torch.dtype | None = None) -> torch.Tensor:
 # --------------------------------------------------------------------------- gated MLP activation
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A [rows, cols] view of ``t`` that the kernels read in place, or a contiguous copy."""
-    t = t.reshape(-1, t.shape[-1])
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     step = 4 if t.dtype == torch.float32 else 8
     if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % step == 0
                              and t.shape[1] % 8 == 0):

@@ -1203,7 +1203,11 @@ struct FewRows {
   }
 };
 
-constexpr int kFewRows = 128;  // rows of a call (NB = 2: 64) that take these kernels
+// Rows of a call (NB = 2: 64) that take these kernels.  Forward and dH with a
+// frozen head over 151936 columns of 896, against the general kernels: 48 rows
+// 65 and 54 us (124 and 124), 128 rows 91 and 74 us, 129 rows (general) 110 and
+// 110 us.
+constexpr int kFewRows = 128;
 
 // The logits kernel over 256 vocabulary rows x 32 NB rows of the call: eight
 // waves, 32 vocabulary rows each.  Same outputs; always with the label apart.
@@ -1487,15 +1491,16 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const DhArgs p) {
   st_bf16x8(p.dh + (int64_t)p.rows[p.c0 + r] * p.hdim + col, o);
 }
 
-// dW of few rows, one chunk: 128 hidden features x 128 vocabulary rows a
-// workgroup, four waves of 64 x 64, all of the call's rows (STEPS k-steps of 64)
-// loaded at once.  There is next to nothing to multiply: it is bound by writing
-// dW, so small workgroups, several a CU, whose stores overlap the others' loads.
-// Rows past the valid ones are zeroed in LDS.
-template <int STEPS>
+// dW of at most 64 rows (one k-step): 128 hidden features x 128 vocabulary rows a
+// workgroup, four waves of 64 x 64.  There is next to nothing to multiply: it is
+// bound by writing dW, so small workgroups, four a CU, whose stores overlap the
+// others' loads, and whole rows leave at once.  48 x 896 over 151936 columns: 65
+// us (4.2 TB/s), the general kernel 89; two k-steps (128 x 1536) were no faster
+// than the general kernel, 190 and 183 us.  Rows past the valid ones are zeroed
+// in LDS.
 __global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p) {
   constexpr int TILE = 128, OP = BK * TILE, QA = 4;
-  __shared__ __align__(16) bf16 smem[2 * STEPS * OP];
+  __shared__ __align__(16) bf16 smem[2 * OP];
   int ti, tj;
   if (!tile_of(p.nI, p.nJ, p.nI, ti, tj)) return;
   const int64_t i0 = (int64_t)ti * TILE, j0 = (int64_t)tj * TILE;
@@ -1511,15 +1516,11 @@ __global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p
   if (nv > 0) {
     const int ca = (int)min(p.hdim - 8 - i0, (int64_t)(TILE - 8)), cb = (int)min(p.V - 8 - j0, (int64_t)(TILE - 8));
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      if (BK * s >= nv) break;
-#pragma unroll
-      for (int q = 0; q < QA; ++q) {
-        const int r = 4 * (QA * w + q) + lane / 16, c = 8 * ((lane % 16) ^ swz_nkc(r)), row = min(BK * s + r, nc - 1);
-        bf16* dst = smem + 2 * s * OP + (QA * wu + q) * 512;
-        dma16(p.Ht.base + i0, 2 * (uint32_t)(row * (int)p.hdim + min(c, ca)), dst);
-        dma16(p.Et.base + j0, 2 * ((uint32_t)row * (uint32_t)p.V + (uint32_t)min(c, cb)), dst + OP);
-      }
+    for (int q = 0; q < QA; ++q) {
+      const int r = 4 * (QA * w + q) + lane / 16, c = 8 * ((lane % 16) ^ swz_nkc(r)), row = min(r, nc - 1);
+      bf16* dst = smem + (QA * wu + q) * 512;
+      dma16(p.Ht.base + i0, 2 * (uint32_t)(row * (int)p.hdim + min(c, ca)), dst);
+      dma16(p.Et.base + j0, 2 * ((uint32_t)row * (uint32_t)p.V + (uint32_t)min(c, cb)), dst + OP);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) slot[b] = p.slot[min(j0 + 64 * wj + 32 * b + l32, p.V - 1)];
@@ -1529,29 +1530,24 @@ __global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p
     rb.init(lane, 64 * wj);
     wait_vmcnt<0>();
     __syncthreads();
-    const int full = nv / BK, tail = nv - full * BK;
-    if (tail > 0) {
-      bf16* B = smem + (2 * full + 1) * OP;
-      for (int i = tail * 16 + tid; i < BK * 16; i += kFewThreads) st_bf16x8(B + 8 * i, zero_bf16x8());
+    const bf16* A = smem;
+    bf16* B = smem + OP;
+    if (nv < BK) {
+      for (int i = nv * 16 + tid; i < BK * 16; i += kFewThreads) st_bf16x8(B + 8 * i, zero_bf16x8());
       __syncthreads();
     }
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      if (BK * s >= nv) break;
-      const bf16 *A = smem + 2 * s * OP, *B = A + OP;
+    for (int ks = 0; ks < 4; ++ks) {
+      bf16x8 a[2], b[2];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        bf16x8 a[2], b[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          a[t] = ra.read(A, t, ks);
-          b[t] = rb.read(B, t, ks);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) acc[x][y] = mfma32(a[x], b[y], acc[x][y]);
+      for (int t = 0; t < 2; ++t) {
+        a[t] = ra.read(A, t, ks);
+        b[t] = rb.read(B, t, ks);
       }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) acc[x][y] = mfma32(a[x], b[y], acc[x][y]);
     }
   }
 #pragma unroll
@@ -1574,13 +1570,25 @@ __global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p
           }
         }
     }
+  }
+  // through LDS, [128 v][128 h] with the 16-byte chunks of a row turned by the row, so that rows leave whole
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
-        const int64_t hh = i0 + 64 * wi + 32 * a + 16 * jj + 8 * h;
-        if (hh < p.hdim) st_bf16x8(p.dw + v * p.hdim + hh, pack8(acc[a][b], 8 * jj));
+        const int r = 64 * wj + 32 * b + l32, c = 8 * wi + 4 * a + 2 * jj + h;
+        st_bf16x8(smem + r * TILE + 8 * (c ^ (r & 15)), pack8(acc[a][b], 8 * jj));
       }
+  __syncthreads();
+  const int c = tid % 16;
+  if (i0 + 8 * c >= p.hdim) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 16 * i + tid / 16;
+    if (j0 + r < p.V) st_bf16x8(p.dw + (j0 + r) * p.hdim + i0 + 8 * c, ld_bf16x8(smem + r * TILE + 8 * (c ^ (r & 15))));
   }
 }
 
@@ -1692,10 +1700,7 @@ void launch_dw_few(DwArgs& dw, hipStream_t stream) {
   dw.nI = (int)((dw.hdim + 127) / 128);
   dw.nJ = (int)((dw.V + 127) / 128);
   const int grid = ((dw.nI * dw.nJ + kXcds - 1) / kXcds) * kXcds;
-  if (dw.Ht.rows <= BK)
-    hipLaunchKernelGGL(flce_dw_few_kernel<1>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
-  else
-    hipLaunchKernelGGL(flce_dw_few_kernel<2>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
+  hipLaunchKernelGGL(flce_dw_few_kernel, dim3(grid), dim3(kFewThreads), 0, stream, dw);
 }
 
 void launch_dw(DwArgs& dw, hipStream_t stream) {
@@ -2125,7 +2130,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       dw.hdim = a.hdim;
       dw.V = a.vocab;
       dw.chunk = L.chunk;
-      if (L.few && L.nchunks == 1)
+      if (a.n <= BK && L.nchunks == 1)
         launch_dw_few(dw, stream);
       else
         launch_dw(dw, stream);

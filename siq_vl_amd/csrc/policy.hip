@@ -20,8 +20,9 @@
 // bound by memory for long batches and by launches for short ones: a pass over
 // the tokens that leaves one partial sum a slice, and one workgroup that adds
 // those up in a fixed order and turns them into the loss and the sequences'
-// weights.  No atomics: results are bitwise reproducible.  Sums are in 64 bits:
-// a margin is a difference of two sums of thousands of terms.
+// weights; where there are few slices that workgroup makes them too, in one
+// launch (kOneLaunch).  No atomics: results are bitwise reproducible.  Sums are
+// in 64 bits: a margin is a difference of two sums of thousands of terms.
 #include "common.h"
 #include "policy.h"
 
@@ -33,6 +34,7 @@ constexpr int kThreads = 256;
 constexpr int kPer = 8;                    // tokens a thread has in flight
 constexpr int kSlice = kThreads * kPer;    // tokens of a slice at most
 constexpr int kSumThreads = 1024;
+constexpr int kOneLaunch = kSumThreads / 64;  // slices that the one workgroup takes, a wave each
 
 // Slices.  The token axis is cut at multiples of kSlice and at sequence ends.
 // Going along it, each cut raises the sequence s, the window w = t / kSlice, or
@@ -103,31 +105,56 @@ struct PrefPart {
   double sum, count;
 };
 
+// Sum of policy - reference and number of the slice's counted tokens that
+// thread `tid` of G sees.
+template <int G>
+__device__ __forceinline__ void pref_slice(const PrefArgs& p, const Slice& c, int tid, double (&x)[2]) {
+  x[0] = x[1] = 0.;
+  for (int64_t t0 = c.begin + tid; t0 < c.end; t0 += G * kPer) {
+    float a[kPer], r[kPer];
+    bool m[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t t = t0 + i * G;
+      m[i] = t < c.end && (p.mask == nullptr || p.mask[t] != 0);
+      a[i] = t < c.end ? p.policy[t] : 0.f;
+      r[i] = t < c.end && p.reference != nullptr ? p.reference[t] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      x[0] += m[i] ? (double)a[i] - (double)r[i] : 0.;
+      x[1] += m[i] ? 1. : 0.;
+    }
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void pref_slice_kernel(const PrefArgs p, PrefPart* __restrict__ part) {
   const Slice c = slice_of(p.seq, blockIdx.x);
   if (c.begin >= c.end || c.s >= p.seq.seqs) return;
-  float a[kPer], r[kPer];
-  bool m[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t t = c.begin + i * kThreads + threadIdx.x;
-    m[i] = t < c.end && (p.mask == nullptr || p.mask[t] != 0);
-    a[i] = t < c.end ? p.policy[t] : 0.f;
-    r[i] = t < c.end && p.reference != nullptr ? p.reference[t] : 0.f;
-  }
-  double x[2] = {0., 0.};
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    x[0] += m[i] ? (double)a[i] - (double)r[i] : 0.;
-    x[1] += m[i] ? 1. : 0.;
-  }
+  double x[2];
+  pref_slice<kThreads>(p, c, threadIdx.x, x);
   block_sum<kThreads, 2>(x);
   if (threadIdx.x == 0) part[blockIdx.x] = PrefPart{x[0], x[1]};
 }
 
-__global__ __launch_bounds__(kSumThreads) void pref_pair_kernel(const PrefArgs p, const PrefPart* __restrict__ part,
-                                                                PrefPart* __restrict__ total, int lanes) {
+// ONE: the slices (nslices <= kOneLaunch) are made here.
+template <bool ONE>
+__global__ __launch_bounds__(kSumThreads) void pref_pair_kernel(const PrefArgs p, PrefPart* __restrict__ part,
+                                                                PrefPart* __restrict__ total, int lanes, int nslices) {
   const int tid = threadIdx.x;
+  if (ONE) {
+    const int b = tid >> 6;
+    if (b < nslices) {
+      const Slice c = slice_of(p.seq, b);
+      if (c.begin < c.end && c.s < p.seq.seqs) {
+        double x[2];
+        pref_slice<64>(p, c, tid & 63, x);
+        const PrefPart q{wave_sum(x[0]), wave_sum(x[1])};
+        if ((tid & 63) == 0) part[b] = q;
+      }
+    }
+    __syncthreads();
+  }
   const int64_t n = 2 * p.pairs;
   for (int64_t s = tid / lanes; s < n; s += kSumThreads / lanes) {
     int64_t first, last;
@@ -201,81 +228,108 @@ struct PolicyPart {
   double loss, kl, count, cut;
 };
 
+// Sums of the slice's counted tokens that thread `tid` of G sees (loss, kl,
+// count, cut), and every token's gradient.  tail: behind the last sequence.
+template <int G>
+__device__ __forceinline__ void policy_slice(const PolicyArgs& p, const Slice& c, bool tail, int tid, double (&x)[4]) {
+  x[0] = x[1] = x[2] = x[3] = 0.;
+  const float seq_adv = tail || p.per_token ? 0.f : p.advantages[c.s];
+  for (int64_t t0 = c.begin + tid; t0 < c.end; t0 += G * kPer) {
+    float lp[kPer], old[kPer], ref[kPer], adv[kPer];
+    bool m[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t t = t0 + i * G;
+      const bool in = t < c.end;
+      m[i] = in && !tail && (p.mask == nullptr || p.mask[t] != 0);
+      lp[i] = in ? p.logps[t] : 0.f;
+      old[i] = in ? p.old[t] : 0.f;
+      ref[i] = in && p.kl != kKlNone ? p.reference[t] : 0.f;
+      adv[i] = in && p.per_token ? p.advantages[t] : seq_adv;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t t = t0 + i * G;
+      const double d = (double)lp[i] - (double)old[i];
+      const float A = adv[i], r = exp2f_fast((float)d * kLog2e);
+      const bool over = A > 0.f && d > p.log_high, under = A < 0.f && d < p.log_low, far = A < 0.f && d > p.log_dual;
+      const bool cut = over || under || far;
+      const float obj = A * (over ? p.high : under ? p.low : far ? p.dual : r);
+      float loss = -obj, g = cut ? 0.f : -A * r, kl = 0.f;
+      if (p.kl != kKlNone) {
+        const float y = (float)((double)ref[i] - (double)lp[i]);
+        float dkl;
+        if (p.kl == kKl3) {
+          // e^y - 1 - y: by its Taylor series up to |y| = 1/2 (the rest is below 2e-9 of it), where the difference would cancel
+          float e1;
+          if (fabsf(y) <= 0.5f) {
+            float q = 1.f / 362880.f;
+            q = __builtin_fmaf(q, y, 1.f / 40320.f);
+            q = __builtin_fmaf(q, y, 1.f / 5040.f);
+            q = __builtin_fmaf(q, y, 1.f / 720.f);
+            q = __builtin_fmaf(q, y, 1.f / 120.f);
+            q = __builtin_fmaf(q, y, 1.f / 24.f);
+            q = __builtin_fmaf(q, y, 1.f / 6.f);
+            q = __builtin_fmaf(q, y, 0.5f);
+            kl = q * y * y;
+            e1 = y + kl;
+          } else {
+            e1 = exp2f_fast(y * kLog2e) - 1.f;
+            kl = e1 - y;
+          }
+          dkl = -e1;
+        } else if (p.kl == kKl2) {
+          kl = 0.5f * y * y;
+          dkl = -y;
+        } else {
+          kl = -y;
+          dkl = 1.f;
+        }
+        loss = __builtin_fmaf(p.kl_coef, kl, loss);
+        g = __builtin_fmaf(p.kl_coef, dkl, g);
+      }
+      if (m[i]) {
+        x[0] += (double)loss;
+        x[1] += (double)kl;
+        x[2] += 1.;
+        x[3] += cut ? 1. : 0.;
+      }
+      if (t < c.end) p.dtoken[t] = m[i] ? g : 0.f;
+    }
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void policy_slice_kernel(const PolicyArgs p, PolicyPart* __restrict__ part) {
   const Slice c = slice_of(p.seq, blockIdx.x);
   if (c.begin >= c.end) return;
-  const bool tail = c.s >= p.seq.seqs;  // behind the last sequence
-  const float seq_adv = tail || p.per_token ? 0.f : p.advantages[c.s];
-  float lp[kPer], old[kPer], ref[kPer], adv[kPer];
-  bool m[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t t = c.begin + i * kThreads + threadIdx.x;
-    const bool in = t < c.end;
-    m[i] = in && !tail && (p.mask == nullptr || p.mask[t] != 0);
-    lp[i] = in ? p.logps[t] : 0.f;
-    old[i] = in ? p.old[t] : 0.f;
-    ref[i] = in && p.kl != kKlNone ? p.reference[t] : 0.f;
-    adv[i] = in && p.per_token ? p.advantages[t] : seq_adv;
-  }
-  double x[4] = {0., 0., 0., 0.};
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t t = c.begin + i * kThreads + threadIdx.x;
-    const double d = (double)lp[i] - (double)old[i];
-    const float A = adv[i], r = exp2f_fast((float)d * kLog2e);
-    const bool over = A > 0.f && d > p.log_high, under = A < 0.f && d < p.log_low, far = A < 0.f && d > p.log_dual;
-    const bool cut = over || under || far;
-    const float obj = A * (over ? p.high : under ? p.low : far ? p.dual : r);
-    float loss = -obj, g = cut ? 0.f : -A * r, kl = 0.f;
-    if (p.kl != kKlNone) {
-      const float y = (float)((double)ref[i] - (double)lp[i]);
-      float dkl;
-      if (p.kl == kKl3) {
-        // e^y - 1 - y: by its Taylor series up to |y| = 1/2 (the rest is below 2e-9 of it), where the difference would cancel
-        float e1;
-        if (fabsf(y) <= 0.5f) {
-          float q = 1.f / 362880.f;
-          q = __builtin_fmaf(q, y, 1.f / 40320.f);
-          q = __builtin_fmaf(q, y, 1.f / 5040.f);
-          q = __builtin_fmaf(q, y, 1.f / 720.f);
-          q = __builtin_fmaf(q, y, 1.f / 120.f);
-          q = __builtin_fmaf(q, y, 1.f / 24.f);
-          q = __builtin_fmaf(q, y, 1.f / 6.f);
-          q = __builtin_fmaf(q, y, 0.5f);
-          kl = q * y * y;
-          e1 = y + kl;
-        } else {
-          e1 = exp2f_fast(y * kLog2e) - 1.f;
-          kl = e1 - y;
-        }
-        dkl = -e1;
-      } else if (p.kl == kKl2) {
-        kl = 0.5f * y * y;
-        dkl = -y;
-      } else {
-        kl = -y;
-        dkl = 1.f;
-      }
-      loss = __builtin_fmaf(p.kl_coef, kl, loss);
-      g = __builtin_fmaf(p.kl_coef, dkl, g);
-    }
-    if (m[i]) {
-      x[0] += (double)loss;
-      x[1] += (double)kl;
-      x[2] += 1.;
-      x[3] += cut ? 1. : 0.;
-    }
-    if (t < c.end) p.dtoken[t] = m[i] ? g : 0.f;
-  }
+  const bool tail = c.s >= p.seq.seqs;
+  double x[4];
+  policy_slice<kThreads>(p, c, tail, threadIdx.x, x);
   if (tail) return;
   block_sum<kThreads, 4>(x);
   if (threadIdx.x == 0) part[blockIdx.x] = PolicyPart{x[0], x[1], x[2], x[3]};
 }
 
-__global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArgs p, const PolicyPart* __restrict__ part,
-                                                                 int lanes) {
+// ONE: the slices (nslices <= kOneLaunch) are made here.
+template <bool ONE>
+__global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArgs p, PolicyPart* __restrict__ part,
+                                                                 int lanes, int nslices) {
   const int tid = threadIdx.x;
+  if (ONE) {
+    const int b = tid >> 6;
+    if (b < nslices) {
+      const Slice c = slice_of(p.seq, b);
+      const bool tail = c.s >= p.seq.seqs;
+      if (c.begin < c.end) {
+        double x[4];
+        policy_slice<64>(p, c, tail, tid & 63, x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = wave_sum(x[k]);
+        if ((tid & 63) == 0 && !tail) part[b] = PolicyPart{x[0], x[1], x[2], x[3]};
+      }
+    }
+    __syncthreads();
+  }
   const double div = p.divisor != nullptr ? (double)*p.divisor : (double)p.seq.seqs;
   double x[4] = {0., 0., 0., 0.};  // loss, kl, count, cut
   for (int64_t s = tid / lanes; s < p.seq.seqs; s += kSumThreads / lanes) {
@@ -341,9 +395,13 @@ hipError_t pref_fwd(const PrefArgs& a, hipStream_t stream) {
   const int64_t n = slices(a.seq.seqs, a.seq.tokens);
   PrefPart* part = static_cast<PrefPart*>(a.ws);
   PrefPart* total = reinterpret_cast<PrefPart*>(static_cast<char*>(a.ws) + al(sizeof(PrefPart) * (size_t)n));
-  hipLaunchKernelGGL(pref_slice_kernel, dim3((unsigned)n), dim3(kThreads), 0, stream, a, part);
-  hipLaunchKernelGGL(pref_pair_kernel, dim3(1), dim3(kSumThreads), 0, stream, a, part, total,
-                     lanes_for(a.seq.seqs, a.seq.tokens));
+  const int lanes = lanes_for(a.seq.seqs, a.seq.tokens);
+  if (n <= kOneLaunch) {
+    hipLaunchKernelGGL(pref_pair_kernel<true>, dim3(1), dim3(kSumThreads), 0, stream, a, part, total, lanes, (int)n);
+  } else {
+    hipLaunchKernelGGL(pref_slice_kernel, dim3((unsigned)n), dim3(kThreads), 0, stream, a, part);
+    hipLaunchKernelGGL(pref_pair_kernel<false>, dim3(1), dim3(kSumThreads), 0, stream, a, part, total, lanes, 0);
+  }
   return hipGetLastError();
 }
 
@@ -360,10 +418,14 @@ size_t policy_workspace_bytes(int64_t seqs, int64_t tokens) {
 
 hipError_t policy_fwd(const PolicyArgs& a, hipStream_t stream) {
   PolicyPart* part = static_cast<PolicyPart*>(a.ws);
-  hipLaunchKernelGGL(policy_slice_kernel, dim3((unsigned)slices(a.seq.seqs, a.seq.tokens)), dim3(kThreads), 0, stream, a,
-                     part);
-  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(kSumThreads), 0, stream, a, part,
-                     lanes_for(a.seq.seqs, a.seq.tokens));
+  const int64_t n = slices(a.seq.seqs, a.seq.tokens);
+  const int lanes = lanes_for(a.seq.seqs, a.seq.tokens);
+  if (n <= kOneLaunch) {
+    hipLaunchKernelGGL(policy_sum_kernel<true>, dim3(1), dim3(kSumThreads), 0, stream, a, part, lanes, (int)n);
+  } else {
+    hipLaunchKernelGGL(policy_slice_kernel, dim3((unsigned)n), dim3(kThreads), 0, stream, a, part);
+    hipLaunchKernelGGL(policy_sum_kernel<false>, dim3(1), dim3(kSumThreads), 0, stream, a, part, lanes, 0);
+  }
   return hipGetLastError();
 }
 

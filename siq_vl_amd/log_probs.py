@@ -30,6 +30,12 @@ DEFAULT_KEEP_BYTES = 8 << 30
 def flp_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = IGNORE_INDEX,
             temperature: float = 1.0, keep: bool = False):
     """Raw forward: ``(logp fp32 [n], count, bad_labels, saved | None)``."""
+    logp, counts, saved = _forward(hidden, weight, labels, ignore_index, temperature, keep)
+    return logp, counts[0], counts[1], saved
+
+
+def _forward(hidden, weight, labels, ignore_index, temperature, keep):
+    """``(logp, [count, bad_labels] int64, saved | None)``."""
     _check_operands(hidden, weight, labels)
     for name, t in (("weight", weight), ("labels", labels)):
         if t.device != hidden.device:
@@ -39,16 +45,15 @@ def flp_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ig
     L = _lib.lib()
     logp = torch.empty(n, dtype=torch.float32, device=dev)
     counts = torch.empty(2, dtype=torch.int64, device=dev)
-    count, bad = counts.unbind()
     saved = torch.empty(L.siq_flp_saved_bytes(n, vocab), dtype=torch.uint8, device=dev) if keep else None
     ws = torch.empty(L.siq_flp_fwd_workspace_bytes(n, hdim, vocab, int(keep)), dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         rc = L.siq_flp_fwd(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), n, hdim, vocab, int(ignore_index),
-                           float(temperature), logp.data_ptr(), count.data_ptr(), bad.data_ptr(),
+                           float(temperature), logp.data_ptr(), counts.data_ptr(), counts.data_ptr() + 8,
                            saved.data_ptr() if keep else None, saved.numel() if keep else 0, ws.data_ptr(), ws.numel(),
                            _lib.stream(dev))
     _lib.check(rc, "siq_flp_fwd")
-    return logp, count, bad, saved
+    return logp, counts, saved
 
 
 def flp_bwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, dlogp: torch.Tensor,
@@ -82,13 +87,17 @@ def flp_bwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, dl
     return dh, dw
 
 
+def _rows(hidden: torch.Tensor) -> torch.Tensor:
+    return hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+
+
 class _FusedLinearLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, temperature, chunk_tokens, keep_bytes, validate):
-        h2, y = hidden.reshape(-1, hidden.shape[-1]), labels.reshape(-1)
+        h2, y = _rows(hidden), labels if labels.dim() == 1 else labels.reshape(-1)
         keep = _lib.lib().siq_flp_saved_bytes(h2.shape[0], weight.shape[0]) <= keep_bytes
-        logp, _, bad, saved = flp_fwd(h2, weight, y, ignore_index, temperature, keep)
-        _track_bad(bad, weight.shape[0], ignore_index, validate)
+        logp, counts, saved = _forward(h2, weight, y, ignore_index, temperature, keep)
+        _track_bad(counts[1], weight.shape[0], ignore_index, validate)
         ctx.save_for_backward(hidden, weight, labels, *((saved,) if keep else ()))
         ctx.ignore_index, ctx.temperature, ctx.chunk_tokens = ignore_index, temperature, chunk_tokens
         return logp.view(labels.shape)
@@ -97,7 +106,7 @@ class _FusedLinearLogProbs(torch.autograd.Function):
     def backward(ctx, dlogp):
         _lib.first_order("fused_linear_log_probs")
         hidden, weight, labels, *saved = ctx.saved_tensors
-        dh, dw = flp_bwd(hidden.reshape(-1, hidden.shape[-1]), weight, labels.reshape(-1), dlogp.reshape(-1),
+        dh, dw = flp_bwd(_rows(hidden), weight, labels.reshape(-1), dlogp.reshape(-1),
                          ctx.ignore_index, ctx.temperature, saved[0] if saved else None, ctx.needs_input_grad[0],
                          ctx.needs_input_grad[1], ctx.chunk_tokens)
         return None if dh is None else dh.view(hidden.shape), dw, *(None,) * 6
@@ -125,8 +134,8 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
     h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
     w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
     if not torch.is_grad_enabled() or not (h.requires_grad or w.requires_grad):
-        logp, _, bad, _ = flp_fwd(h.reshape(-1, h.shape[-1]), w, labels.reshape(-1), int(ignore_index), temperature)
-        _track_bad(bad, w.shape[0], int(ignore_index), validate)
+        logp, counts, _ = _forward(_rows(h), w, labels.reshape(-1), int(ignore_index), temperature, False)
+        _track_bad(counts[1], w.shape[0], int(ignore_index), validate)
         return logp.view(labels.shape)
     return _FusedLinearLogProbs.apply(h, w, labels, int(ignore_index), float(temperature), chunk_tokens, int(keep_bytes),
                                       validate)

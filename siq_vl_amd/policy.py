@@ -54,7 +54,7 @@ def _choice(name: str, value: str, of: dict) -> int:
 def _logps(name: str, t: torch.Tensor, like: torch.Tensor | None = None, frozen: bool = False) -> torch.Tensor:
     if t.dtype != torch.float32:
         raise ValueError(f"{name} must be float32, got {t.dtype}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must live on the GPU, got {t.device}")
     if like is not None and (t.shape != like.shape or t.device != like.device):
         raise ValueError(f"{name} must be {tuple(like.shape)} on {like.device}, got {tuple(t.shape)} on {t.device}")
@@ -98,9 +98,8 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, policy, reference, cu, mask, loss_type, order, beta, smoothing, normalized, divisor):
         dev, tokens, pairs = policy.device, policy.numel(), (cu.numel() - 1) // 2
-        out = torch.empty(4 * pairs, dtype=torch.float32, device=dev)
-        chosen, rejected, coef = out.split((pairs, pairs, 2 * pairs))
-        loss = torch.empty((), dtype=torch.float32, device=dev)
+        loss, chosen, rejected = policy.new_empty(()), policy.new_empty(pairs), policy.new_empty(pairs)
+        coef = policy.new_empty(2 * pairs)
         L = _lib.lib()
         ws = torch.empty(L.siq_pref_workspace_bytes(pairs, tokens), dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
@@ -170,9 +169,7 @@ class _Policy(torch.autograd.Function):
                 kl_coef, divisor):
         dev, tokens = logps.device, logps.numel()
         seqs = 1 if cu is None else cu.numel() - 1
-        stats = torch.empty(3, dtype=torch.float32, device=dev)
-        dtoken = torch.empty(tokens, dtype=torch.float32, device=dev)
-        weight = torch.empty(seqs if aggregation else 1, dtype=torch.float32, device=dev)
+        stats, dtoken, weight = logps.new_empty(3), logps.new_empty(tokens), logps.new_empty(seqs if aggregation else 1)
         L = _lib.lib()
         ws = torch.empty(L.siq_policy_workspace_bytes(seqs, tokens), dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
