@@ -23,6 +23,8 @@
 // weights; where there are few slices that workgroup makes them too, in one
 // launch (kOneLaunch).  No atomics: results are bitwise reproducible.  Sums are
 // in 64 bits: a margin is a difference of two sums of thousands of terms.
+#include <type_traits>
+
 #include "common.h"
 #include "policy.h"
 
@@ -51,14 +53,17 @@ __device__ __forceinline__ int64_t seq_start(const Packed& p, int64_t s) {
 struct Slice {
   int64_t s, begin, end;
 };
+// A wave searches together, 64 offsets at a step: with 700 sequences two loads
+// that wait for one another instead of ten.
 __device__ __forceinline__ Slice slice_of(const Packed& p, int64_t b) {
+  const int lane = threadIdx.x & 63;
   int64_t lo = 0, hi = p.seqs + 1;  // first slice of lo <= b; of hi: past it
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (mid + seq_start(p, mid) / kSlice <= b)
-      lo = mid;
-    else
-      hi = mid;
+    const int64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+    const uint64_t past = __ballot(at >= hi || at + seq_start(p, at) / kSlice > b);
+    const int64_t k = past != 0 ? (int64_t)__builtin_ctzll(past) : 64;
+    hi = min(hi, lo + (k + 1) * step);
+    lo += k * step;
   }
   const int64_t w = b - lo;
   return Slice{lo, max(seq_start(p, lo), w * kSlice), min(seq_start(p, lo + 1), (w + 1) * kSlice)};
@@ -109,23 +114,26 @@ struct PrefPart {
 // thread `tid` of G sees.
 template <int G>
 __device__ __forceinline__ void pref_slice(const PrefArgs& p, const Slice& c, int tid, double (&x)[2]) {
-  x[0] = x[1] = 0.;
+  x[0] = 0.;
+  int n = 0;
   for (int64_t t0 = c.begin + tid; t0 < c.end; t0 += G * kPer) {
     float a[kPer], r[kPer];
     bool m[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t t = t0 + i * G;
-      m[i] = t < c.end && (p.mask == nullptr || p.mask[t] != 0);
-      a[i] = t < c.end ? p.policy[t] : 0.f;
-      r[i] = t < c.end && p.reference != nullptr ? p.reference[t] : 0.f;
+      // (past the end the last token again, not counted: loads without branches are all in flight at once)
+      const int64_t t = t0 + i * G, at = min(t, c.end - 1);
+      m[i] = (p.mask == nullptr || p.mask[at] != 0) && t < c.end;
+      a[i] = p.policy[at];
+      r[i] = p.reference != nullptr ? p.reference[at] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       x[0] += m[i] ? (double)a[i] - (double)r[i] : 0.;
-      x[1] += m[i] ? 1. : 0.;
+      n += m[i] ? 1 : 0;
     }
   }
+  x[1] = (double)n;
 }
 
 __global__ __launch_bounds__(kThreads) void pref_slice_kernel(const PrefArgs p, PrefPart* __restrict__ part) {
@@ -228,90 +236,105 @@ struct PolicyPart {
   double loss, kl, count, cut;
 };
 
+// Estimate of the KL divergence at y = reference - logp, and its derivative by logp.
+template <int KL>
+__device__ __forceinline__ void kl_term(float y, float& kl, float& dkl) {
+  if (KL == kKl3) {
+    // e^y - 1 - y: by its Taylor series up to |y| = 1/2 (the rest is below 2e-9 of it), where the difference would
+    // cancel; both are formed and one is taken, so that a wave's lanes stay together
+    float q = 1.f / 362880.f;
+    q = __builtin_fmaf(q, y, 1.f / 40320.f);
+    q = __builtin_fmaf(q, y, 1.f / 5040.f);
+    q = __builtin_fmaf(q, y, 1.f / 720.f);
+    q = __builtin_fmaf(q, y, 1.f / 120.f);
+    q = __builtin_fmaf(q, y, 1.f / 24.f);
+    q = __builtin_fmaf(q, y, 1.f / 6.f);
+    q = __builtin_fmaf(q, y, 0.5f);
+    const float near = q * y * y, e1 = exp2f_fast(y * kLog2e) - 1.f;
+    const bool small = fabsf(y) <= 0.5f;
+    kl = small ? near : e1 - y;
+    dkl = -(small ? y + near : e1);
+  } else if (KL == kKl2) {
+    kl = 0.5f * y * y;
+    dkl = -y;
+  } else {
+    kl = -y;
+    dkl = 1.f;
+  }
+}
+
 // Sums of the slice's counted tokens that thread `tid` of G sees (loss, kl,
 // count, cut), and every token's gradient.  tail: behind the last sequence.
-template <int G>
+template <int G, int KL>
 __device__ __forceinline__ void policy_slice(const PolicyArgs& p, const Slice& c, bool tail, int tid, double (&x)[4]) {
-  x[0] = x[1] = x[2] = x[3] = 0.;
+  x[0] = x[1] = 0.;
+  int count = 0, cuts = 0;
   const float seq_adv = tail || p.per_token ? 0.f : p.advantages[c.s];
   for (int64_t t0 = c.begin + tid; t0 < c.end; t0 += G * kPer) {
     float lp[kPer], old[kPer], ref[kPer], adv[kPer];
-    bool m[kPer];
+    uint8_t mk[kPer];
+    // (past the end the last token again, not counted: loads without branches are all in flight at once)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t t = t0 + i * G;
-      const bool in = t < c.end;
-      m[i] = in && !tail && (p.mask == nullptr || p.mask[t] != 0);
-      lp[i] = in ? p.logps[t] : 0.f;
-      old[i] = in ? p.old[t] : 0.f;
-      ref[i] = in && p.kl != kKlNone ? p.reference[t] : 0.f;
-      adv[i] = in && p.per_token ? p.advantages[t] : seq_adv;
+      const int64_t at = min(t0 + i * G, c.end - 1);
+      lp[i] = p.logps[at];
+      old[i] = p.old[at];
+      if (KL != kKlNone) ref[i] = p.reference[at];
+    }
+    if (p.per_token) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) adv[i] = p.advantages[min(t0 + i * G, c.end - 1)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) adv[i] = seq_adv;
+    }
+    if (p.mask != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) mk[i] = p.mask[min(t0 + i * G, c.end - 1)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) mk[i] = 1;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int64_t t = t0 + i * G;
+      const bool m = t < c.end && !tail && mk[i] != 0;
       const double d = (double)lp[i] - (double)old[i];
       const float A = adv[i], r = exp2f_fast((float)d * kLog2e);
       const bool over = A > 0.f && d > p.log_high, under = A < 0.f && d < p.log_low, far = A < 0.f && d > p.log_dual;
       const bool cut = over || under || far;
-      const float obj = A * (over ? p.high : under ? p.low : far ? p.dual : r);
-      float loss = -obj, g = cut ? 0.f : -A * r, kl = 0.f;
-      if (p.kl != kKlNone) {
-        const float y = (float)((double)ref[i] - (double)lp[i]);
-        float dkl;
-        if (p.kl == kKl3) {
-          // e^y - 1 - y: by its Taylor series up to |y| = 1/2 (the rest is below 2e-9 of it), where the difference would cancel
-          float e1;
-          if (fabsf(y) <= 0.5f) {
-            float q = 1.f / 362880.f;
-            q = __builtin_fmaf(q, y, 1.f / 40320.f);
-            q = __builtin_fmaf(q, y, 1.f / 5040.f);
-            q = __builtin_fmaf(q, y, 1.f / 720.f);
-            q = __builtin_fmaf(q, y, 1.f / 120.f);
-            q = __builtin_fmaf(q, y, 1.f / 24.f);
-            q = __builtin_fmaf(q, y, 1.f / 6.f);
-            q = __builtin_fmaf(q, y, 0.5f);
-            kl = q * y * y;
-            e1 = y + kl;
-          } else {
-            e1 = exp2f_fast(y * kLog2e) - 1.f;
-            kl = e1 - y;
-          }
-          dkl = -e1;
-        } else if (p.kl == kKl2) {
-          kl = 0.5f * y * y;
-          dkl = -y;
-        } else {
-          kl = -y;
-          dkl = 1.f;
-        }
+      float loss = -(A * (over ? p.high : under ? p.low : far ? p.dual : r)), g = cut ? 0.f : -A * r;
+      if (KL != kKlNone) {
+        float kl, dkl;
+        kl_term<KL>((float)((double)ref[i] - (double)lp[i]), kl, dkl);
         loss = __builtin_fmaf(p.kl_coef, kl, loss);
         g = __builtin_fmaf(p.kl_coef, dkl, g);
+        x[1] += (double)(m ? kl : 0.f);
       }
-      if (m[i]) {
-        x[0] += (double)loss;
-        x[1] += (double)kl;
-        x[2] += 1.;
-        x[3] += cut ? 1. : 0.;
-      }
-      if (t < c.end) p.dtoken[t] = m[i] ? g : 0.f;
+      x[0] += (double)(m ? loss : 0.f);
+      count += m ? 1 : 0;
+      cuts += m && cut ? 1 : 0;
+      if (t < c.end) p.dtoken[t] = m ? g : 0.f;
     }
   }
+  x[2] = (double)count;
+  x[3] = (double)cuts;
 }
 
+template <int KL>
 __global__ __launch_bounds__(kThreads) void policy_slice_kernel(const PolicyArgs p, PolicyPart* __restrict__ part) {
   const Slice c = slice_of(p.seq, blockIdx.x);
   if (c.begin >= c.end) return;
   const bool tail = c.s >= p.seq.seqs;
   double x[4];
-  policy_slice<kThreads>(p, c, tail, threadIdx.x, x);
+  policy_slice<kThreads, KL>(p, c, tail, threadIdx.x, x);
   if (tail) return;
   block_sum<kThreads, 4>(x);
   if (threadIdx.x == 0) part[blockIdx.x] = PolicyPart{x[0], x[1], x[2], x[3]};
 }
 
 // ONE: the slices (nslices <= kOneLaunch) are made here.
-template <bool ONE>
+template <bool ONE, int KL>
 __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArgs p, PolicyPart* __restrict__ part,
                                                                  int lanes, int nslices) {
   const int tid = threadIdx.x;
@@ -322,7 +345,7 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArg
       const bool tail = c.s >= p.seq.seqs;
       if (c.begin < c.end) {
         double x[4];
-        policy_slice<64>(p, c, tail, tid & 63, x);
+        policy_slice<64, KL>(p, c, tail, tid & 63, x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = wave_sum(x[k]);
         if ((tid & 63) == 0 && !tail) part[b] = PolicyPart{x[0], x[1], x[2], x[3]};
@@ -420,11 +443,27 @@ hipError_t policy_fwd(const PolicyArgs& a, hipStream_t stream) {
   PolicyPart* part = static_cast<PolicyPart*>(a.ws);
   const int64_t n = slices(a.seq.seqs, a.seq.tokens);
   const int lanes = lanes_for(a.seq.seqs, a.seq.tokens);
-  if (n <= kOneLaunch) {
-    hipLaunchKernelGGL(policy_sum_kernel<true>, dim3(1), dim3(kSumThreads), 0, stream, a, part, lanes, (int)n);
-  } else {
-    hipLaunchKernelGGL(policy_slice_kernel, dim3((unsigned)n), dim3(kThreads), 0, stream, a, part);
-    hipLaunchKernelGGL(policy_sum_kernel<false>, dim3(1), dim3(kSumThreads), 0, stream, a, part, lanes, 0);
+  auto run = [&](auto kl) {
+    constexpr int KL = decltype(kl)::value;
+    if (n <= kOneLaunch) {
+      hipLaunchKernelGGL((policy_sum_kernel<true, KL>), dim3(1), dim3(kSumThreads), 0, stream, a, part, lanes, (int)n);
+    } else {
+      hipLaunchKernelGGL(policy_slice_kernel<KL>, dim3((unsigned)n), dim3(kThreads), 0, stream, a, part);
+      hipLaunchKernelGGL((policy_sum_kernel<false, kKlNone>), dim3(1), dim3(kSumThreads), 0, stream, a, part, lanes, 0);
+    }
+  };
+  switch (a.kl) {
+    case kKl1:
+      run(std::integral_constant<int, kKl1>());
+      break;
+    case kKl2:
+      run(std::integral_constant<int, kKl2>());
+      break;
+    case kKl3:
+      run(std::integral_constant<int, kKl3>());
+      break;
+    default:
+      run(std::integral_constant<int, kKlNone>());
   }
   return hipGetLastError();
 }
