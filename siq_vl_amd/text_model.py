@@ -11,6 +11,10 @@ of ``Qwen2ForCausalLM.forward`` (transformers models/qwen2/modeling_qwen2.py:
   straight into ``fused_linear_cross_entropy`` with the labels shifted as
   ``ForCausalLMLoss`` shifts them (loss/loss_utils.py:63-64, or the given
   ``shift_labels``) and ``num_items_in_batch`` honoured; ``logits`` is None;
+* with ``labels`` and ``return_log_probs=True`` (preference and policy training,
+  ``siq_vl_amd.policy``): instead of a loss, the log-probabilities of the shifted
+  labels (``fused_linear_log_probs``, at ``temperature``) in the output's
+  ``log_probs``, [batch, seqlen], 0 where the shifted label is ignored;
 * without ``labels`` (``generate``): the original logits path;
 * with ``labels`` but no gradient (evaluation under ``torch.no_grad``): the
   loss-only kernel, no logits and no gradient work.
@@ -21,18 +25,35 @@ of ``Qwen2ForCausalLM.forward`` (transformers models/qwen2/modeling_qwen2.py:
 
 from __future__ import annotations
 
+import functools
 import types
+from dataclasses import dataclass
 from typing import Any
 
 import torch
 
 from .cross_entropy import IGNORE_INDEX, fused_linear_cross_entropy, shift_labels
+from .log_probs import fused_linear_log_probs
+
+
+@functools.cache
+def _output_with_log_probs():
+    from transformers.modeling_outputs import CausalLMOutputWithPast
+
+    @dataclass
+    class CausalLMOutputWithLogProbs(CausalLMOutputWithPast):
+        log_probs: torch.Tensor | None = None
+
+    return CausalLMOutputWithLogProbs
 
 
 def fused_causal_lm_forward(self, input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
-                            inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0, **kwargs: Any):
+                            inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0,
+                            return_log_probs: bool = False, temperature: float = 1.0, **kwargs: Any):
     from transformers.modeling_outputs import CausalLMOutputWithPast
 
+    if return_log_probs and labels is None and kwargs.get("shift_labels") is None:
+        raise ValueError("return_log_probs needs labels: they say which tokens' log-probabilities are wanted")
     outputs = self.model(
         input_ids=input_ids,
         attention_mask=attention_mask,
@@ -45,13 +66,20 @@ def fused_causal_lm_forward(self, input_ids=None, attention_mask=None, position_
     # the same positions the stock forward turns into logits (all of them for logits_to_keep=0)
     slice_indices = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
     hidden = outputs.last_hidden_state[:, slice_indices, :]
-    if labels is None:
+    if labels is None and not return_log_probs:
         logits = self.lm_head(hidden)
         return CausalLMOutputWithPast(loss=None, logits=logits, past_key_values=outputs.past_key_values,
                                       hidden_states=outputs.hidden_states, attentions=outputs.attentions)
     targets = kwargs.get("shift_labels")
     if targets is None:
         targets = shift_labels(labels, IGNORE_INDEX)
+    if return_log_probs:
+        targets = targets.to(hidden.device)
+        logps = fused_linear_log_probs(hidden, self.lm_head.weight, targets.view(hidden.shape[:-1]), IGNORE_INDEX,
+                                       temperature, chunk_tokens=getattr(self, "siq_ce_chunk_tokens", None))
+        return _output_with_log_probs()(loss=None, logits=None, past_key_values=outputs.past_key_values,
+                                        hidden_states=outputs.hidden_states, attentions=outputs.attentions,
+                                        log_probs=logps)
     loss = fused_linear_cross_entropy(
         hidden.reshape(-1, hidden.shape[-1]),
         self.lm_head.weight,

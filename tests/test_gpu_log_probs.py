@@ -286,3 +286,56 @@ def test_a_second_derivative_is_refused():
     hg = h.to(DEV).requires_grad_()
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(LP.fused_linear_log_probs(hg, w.to(DEV), y.to(DEV)).sum(), [hg], create_graph=True)
+
+
+def test_a_preference_step_of_a_packed_model():
+    """Two pairs of answers in one packed batch through a small Qwen2: the model's log-probabilities are those of its own
+    logits, and the loss's gradient reaches every parameter as through the logits."""
+    transformers = pytest.importorskip("transformers")
+    from siq_vl_amd import attention
+    from siq_vl_amd.cross_entropy import shift_labels
+    from siq_vl_amd.text_model import enable_fused_cross_entropy
+
+    attention.register()
+    cfg = transformers.Qwen2Config(vocab_size=264, hidden_size=256, intermediate_size=512, num_hidden_layers=2,
+                                   num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512)
+    torch.manual_seed(2)
+    model = transformers.Qwen2ForCausalLM(cfg).to(DEV, torch.bfloat16).train()
+    model.config._attn_implementation = "siq_varlen"
+    lengths = [30, 41, 17, 50]
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32, device=DEV)
+    ids = torch.randint(0, 264, (1, sum(lengths)), device=DEV)
+    labels = ids.clone()
+    for a, n in zip(cu[:-1].tolist(), lengths):
+        labels[0, a:a + n // 3] = -100  # the prompt; the first label of a sequence is no target of the one before
+    pos = torch.cat([torch.arange(n) for n in lengths]).to(DEV)[None]
+    inputs = dict(input_ids=ids, position_ids=pos, use_cache=False, cu_seq_lens_q=cu, cu_seq_lens_k=cu,
+                  max_length_q=50, max_length_k=50)
+    targets = shift_labels(labels)
+    mask = targets != -100
+    ref = torch.randn(1, sum(lengths), device=DEV) - 5.5
+    logits = model(**inputs).logits
+    z = torch.log_softmax(logits.float(), -1).gather(-1, targets.clamp(min=0)[..., None])[..., 0]
+    want = torch.where(mask, z, 0.0)
+    P.preference_loss(want, ref, cu, mask=mask, beta=0.1).loss.backward()
+    grads = {n: p.grad.double() for n, p in model.named_parameters()}
+    model.zero_grad()
+    enable_fused_cross_entropy(model)
+    with pytest.raises(ValueError, match="labels"):
+        model(**inputs, return_log_probs=True)
+    out = model(**inputs, labels=labels, return_log_probs=True)
+    assert out.loss is None and out.logits is None and out.log_probs.shape == (1, sum(lengths))
+    # the stock path rounds its logits to bf16: half a step of the largest of them, twice
+    off = 2 * 2.0 ** -8 * float(logits.abs().max()) + 1e-4
+    assert float((out.log_probs - want).abs().max()) <= off
+    P.preference_loss(out.log_probs, ref, cu, mask=mask, beta=0.1).loss.backward()
+    for n, p in model.named_parameters():
+        # the same in bf16 activations and gradients, the logits' gradient not rounded: a few roundings of 2^-8
+        rel = float((p.grad.double() - grads[n]).norm() / grads[n].norm())
+        assert rel <= 0.05, (n, rel)
+    with torch.no_grad():  # a reference model's pass
+        lone = model(**inputs, labels=labels, return_log_probs=True).log_probs
+    assert torch.equal(lone, out.log_probs)
+    warm = model(**inputs, labels=labels, return_log_probs=True, temperature=2.0).log_probs
+    assert not torch.equal(warm, lone)
+    assert model(**inputs, labels=labels).loss is not None
