@@ -512,10 +512,11 @@ int siq_swiglu8_bwd(const void* dh, const void* gate_codes, const void* gate_sca
  * mean over sequences of their counted tokens' mean (0 where none counts);
  * with divisor its value replaces the number of counted tokens, or of
  * sequences.  cu_seqlens NULL: one sequence.  A token exactly at a border is
- * not cut.  stats [3] = loss, mean kl and share of cut tokens over counted ones
- * (all 0 where none counts); dtoken [tokens] (16-byte aligned) and weight
- * [seqs] (SIQ_AGG_TOKEN: [1]) are what siq_policy_bwd multiplies:
- * dlogps = grad_loss weight dtoken (dlogps 16-byte aligned).
+ * not cut.  *loss, *mean_kl and *clip_fraction (the share of cut tokens), the
+ * latter two over counted tokens, are 0 where none counts; dtoken [tokens]
+ * (16-byte aligned) and weight [seqs] (SIQ_AGG_TOKEN: [1]) are what
+ * siq_policy_bwd multiplies: dlogps = grad_loss weight dtoken (dlogps 16-byte
+ * aligned).
  * ------------------------------------------------------------------------- */
 #define SIQ_PREF_SIGMOID 0
 #define SIQ_PREF_IPO 1
@@ -543,8 +544,8 @@ size_t siq_policy_workspace_bytes(int64_t seqs, int64_t tokens);
 int siq_policy_fwd(const float* logps, const float* old_logps, const float* advantages, const void* mask,
                    const float* reference, const int32_t* cu_seqlens, int64_t seqs, int64_t tokens,
                    int advantage_per_token, int aggregation, int kl_type, double clip_low, double clip_high,
-                   double dual_clip, double kl_coef, const float* divisor, float* stats, float* dtoken, float* weight,
-                   void* workspace, size_t workspace_bytes, void* stream);
+                   double dual_clip, double kl_coef, const float* divisor, float* loss, float* mean_kl,
+                   float* clip_fraction, float* dtoken, float* weight, void* workspace, size_t workspace_bytes, void* stream);
 
 int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* weight, const int32_t* cu_seqlens,
                    int64_t seqs, int64_t tokens, int aggregation, float* dlogps, void* stream);

@@ -278,8 +278,8 @@ size_t siq_policy_workspace_bytes(int64_t seqs, int64_t tokens) {
 int siq_policy_fwd(const float* logps, const float* old_logps, const float* advantages, const void* mask,
                    const float* reference, const int32_t* cu_seqlens, int64_t seqs, int64_t tokens,
                    int advantage_per_token, int aggregation, int kl_type, double clip_low, double clip_high,
-                   double dual_clip, double kl_coef, const float* divisor, float* stats, float* dtoken, float* weight,
-                   void* workspace, size_t workspace_bytes, void* stream) {
+                   double dual_clip, double kl_coef, const float* divisor, float* loss, float* mean_kl,
+                   float* clip_fraction, float* dtoken, float* weight, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_packed(seqs, tokens))) return rc;
   if (aggregation != SIQ_AGG_TOKEN && aggregation != SIQ_AGG_SEQUENCE)
@@ -295,7 +295,9 @@ int siq_policy_fwd(const float* logps, const float* old_logps, const float* adva
     return fail(SIQ_ERR_INVALID_ARGUMENT, "a KL term needs the reference's log-probabilities");
   if (cu_seqlens == nullptr && seqs != 1)
     return fail(SIQ_ERR_INVALID_ARGUMENT, "without cu_seqlens there is one sequence");
-  if ((rc = check_not_null(stats, "stats")) || (rc = check_not_null(weight, "weight"))) return rc;
+  if ((rc = check_not_null(loss, "loss")) || (rc = check_not_null(mean_kl, "mean_kl")) ||
+      (rc = check_not_null(clip_fraction, "clip_fraction")) || (rc = check_not_null(weight, "weight")))
+    return rc;
   if (tokens > 0) {
     if ((rc = check_not_null(logps, "logps")) || (rc = check_not_null(old_logps, "old_logps")) ||
         (rc = check_not_null(advantages, "advantages")) || (rc = check_ptr(dtoken, "dtoken")))
@@ -320,7 +322,9 @@ int siq_policy_fwd(const float* logps, const float* old_logps, const float* adva
   a.dual = (float)dual_clip;
   a.kl_coef = (float)kl_coef;
   a.divisor = divisor;
-  a.stats = stats;
+  a.loss = loss;
+  a.mean_kl = mean_kl;
+  a.clip_fraction = clip_fraction;
   a.dtoken = dtoken;
   a.weight = weight;
   a.ws = workspace;

@@ -1869,6 +1869,10 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
 // ---------------------------------------------------------------- log-probabilities of the labels
 namespace {
 
+// Rows at a time where the numerators of all rows are kept: they bound what is
+// held for a row besides (tile sums, label sums).
+constexpr int64_t kKeepChunk = 65536;
+
 // What the forward keeps for the backward.
 struct FlpSaved {
   size_t nvalid, rows, yc, f0, w0, E, total;
@@ -2021,31 +2025,30 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
 size_t flp_saved_bytes(int64_t n, int64_t vocab) { return flp_saved(n, vocab).total; }
 
 size_t flp_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, bool keep) {
-  return flp_layout(n, hdim, vocab, keep ? n : kLossChunk, true, false, false, keep).total;
+  return flp_layout(n, hdim, vocab, keep ? kKeepChunk : kLossChunk, true, false, false, keep).total;
 }
 
 size_t flp_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw, bool have_saved) {
-  return flp_layout(n, hdim, vocab, have_saved ? n : chunk, !have_saved, true, need_dw, have_saved).total;
+  return flp_layout(n, hdim, vocab, have_saved ? kKeepChunk : chunk, !have_saved, true, need_dw, have_saved).total;
 }
 
 hipError_t flp_fwd(const FlpArgs& a, hipStream_t stream) {
   const bool keep = a.saved != nullptr;
-  const FlpLayout L = flp_layout(a.n, a.hdim, a.vocab, keep ? a.n : kLossChunk, true, false, false, keep);
+  const FlpLayout L = flp_layout(a.n, a.hdim, a.vocab, keep ? kKeepChunk : kLossChunk, true, false, false, keep);
   const FlpSaved S = flp_saved(a.n, keep ? a.vocab : 0);
   char* saved = keep ? static_cast<char*>(a.saved) : at<char>(a.ws, L.saved);
   flp_compact(a, L, saved, S, a.logp, a.count, a.bad_labels, nullptr, stream);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk)
-    flp_logits(a, L, saved, S, c0, keep ? at<bf16>(saved, S.E) : nullptr, at<float>(saved, S.f0), at<float>(saved, S.w0),
-               a.logp, stream);
+    flp_logits(a, L, saved, S, c0, keep ? at<bf16>(saved, S.E) + c0 * a.vocab : nullptr, at<float>(saved, S.f0) + c0,
+               at<float>(saved, S.w0) + c0, a.logp, stream);
   return hipGetLastError();
 }
 
 hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
   const bool have = a.saved != nullptr, need_dw = a.dweight != nullptr;
-  const FlpLayout L = flp_layout(a.n, a.hdim, a.vocab, have ? a.n : a.chunk, !have, true, need_dw, have);
+  const FlpLayout L = flp_layout(a.n, a.hdim, a.vocab, have ? kKeepChunk : a.chunk, !have, true, need_dw, have);
   const FlpSaved S = flp_saved(a.n, have ? a.vocab : 0);
   char* saved = have ? static_cast<char*>(a.saved) : at<char>(a.ws, L.saved);
-  bf16* E = at<bf16>(saved, S.E);  // of all rows, or of one chunk
   if (a.n == 0) {
     if (need_dw) launch_zero(a.dweight, a.vocab * a.hdim, stream);
     return hipGetLastError();
@@ -2054,6 +2057,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
   const int64_t* nvalid = at<int64_t>(saved, S.nvalid);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
     const int64_t nc = std::min(L.chunk, a.n - c0);
+    bf16* E = at<bf16>(saved, S.E) + (have ? c0 * a.vocab : 0);  // of all rows, or of one chunk
     float *f0 = at<float>(saved, S.f0) + c0, *w0 = at<float>(saved, S.w0) + c0;
     if (!have) flp_logits(a, L, saved, S, c0, E, f0, w0, nullptr, stream);
     bf16* Hs = at<bf16>(a.ws, L.hc) + c0 * a.hdim;
@@ -2066,7 +2070,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
     wg.g = a.dlogp;
     wg.nvalid = nvalid;
     wg.labels = a.labels;
-    wg.dh = have ? a.dhidden : nullptr;
+    wg.dh = have && c0 == 0 ? a.dhidden : nullptr;
     wg.Hs = Hs;
     wg.f = at<float>(a.ws, L.f);
     wg.wt = at<float>(a.ws, L.wt);

@@ -49,7 +49,9 @@ struct PolicyArgs {
   float low, high, dual;               // those ratios
   float kl_coef;
   const float* divisor;     // or nullptr: counted tokens, or sequences
-  float* stats;             // loss, mean kl, share of cut tokens
+  float* loss;
+  float* mean_kl;
+  float* clip_fraction;     // share of cut tokens
   float* dtoken;            // [tokens] gradient of a token's loss
   float* weight;            // [seqs] (by_sequence) or [1]: its share in the loss
   void* ws;

@@ -384,9 +384,9 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArg
     x[0] *= w;
     p.weight[0] = (float)w;
   }
-  p.stats[0] = (float)x[0];
-  p.stats[1] = (float)(x[1] * per);
-  p.stats[2] = (float)(x[3] * per);
+  *p.loss = (float)x[0];
+  *p.mean_kl = (float)(x[1] * per);
+  *p.clip_fraction = (float)(x[3] * per);
 }
 
 // dlogps = grad weight dtoken, one weight for all tokens.

@@ -30,12 +30,12 @@ DEFAULT_KEEP_BYTES = 8 << 30
 def flp_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = IGNORE_INDEX,
             temperature: float = 1.0, keep: bool = False):
     """Raw forward: ``(logp fp32 [n], count, bad_labels, saved | None)``."""
-    logp, counts, saved = _forward(hidden, weight, labels, ignore_index, temperature, keep)
+    logp, counts, saved = _forward(hidden, weight, labels, ignore_index, temperature, keep, labels.shape)
     return logp, counts[0], counts[1], saved
 
 
-def _forward(hidden, weight, labels, ignore_index, temperature, keep):
-    """``(logp, [count, bad_labels] int64, saved | None)``."""
+def _forward(hidden, weight, labels, ignore_index, temperature, keep, shape):
+    """``(logp of that shape, [count, bad_labels] int64, saved | None)``."""
     _check_operands(hidden, weight, labels)
     for name, t in (("weight", weight), ("labels", labels)):
         if t.device != hidden.device:
@@ -43,7 +43,7 @@ def _forward(hidden, weight, labels, ignore_index, temperature, keep):
     (n, hdim), vocab, dev = hidden.shape, weight.shape[0], hidden.device
     hidden, weight, labels = hidden.contiguous(), weight.contiguous(), labels.contiguous()
     L = _lib.lib()
-    logp = torch.empty(n, dtype=torch.float32, device=dev)
+    logp = torch.empty(shape, dtype=torch.float32, device=dev)
     counts = torch.empty(2, dtype=torch.int64, device=dev)
     saved = torch.empty(L.siq_flp_saved_bytes(n, vocab), dtype=torch.uint8, device=dev) if keep else None
     ws = torch.empty(L.siq_flp_fwd_workspace_bytes(n, hdim, vocab, int(keep)), dtype=torch.uint8, device=dev)
@@ -96,11 +96,11 @@ class _FusedLinearLogProbs(torch.autograd.Function):
     def forward(ctx, hidden, weight, labels, ignore_index, temperature, chunk_tokens, keep_bytes, validate):
         h2, y = _rows(hidden), labels if labels.dim() == 1 else labels.reshape(-1)
         keep = _lib.lib().siq_flp_saved_bytes(h2.shape[0], weight.shape[0]) <= keep_bytes
-        logp, counts, saved = _forward(h2, weight, y, ignore_index, temperature, keep)
+        logp, counts, saved = _forward(h2, weight, y, ignore_index, temperature, keep, labels.shape)
         _track_bad(counts[1], weight.shape[0], ignore_index, validate)
         ctx.save_for_backward(hidden, weight, labels, *((saved,) if keep else ()))
         ctx.ignore_index, ctx.temperature, ctx.chunk_tokens = ignore_index, temperature, chunk_tokens
-        return logp.view(labels.shape)
+        return logp
 
     @staticmethod
     def backward(ctx, dlogp):
@@ -134,9 +134,9 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
     h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
     w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
     if not torch.is_grad_enabled() or not (h.requires_grad or w.requires_grad):
-        logp, counts, _ = _forward(_rows(h), w, labels.reshape(-1), int(ignore_index), temperature, False)
+        logp, counts, _ = _forward(_rows(h), w, labels.reshape(-1), int(ignore_index), temperature, False, labels.shape)
         _track_bad(counts[1], w.shape[0], int(ignore_index), validate)
-        return logp.view(labels.shape)
+        return logp
     return _FusedLinearLogProbs.apply(h, w, labels, int(ignore_index), float(temperature), chunk_tokens, int(keep_bytes),
                                       validate)
 

@@ -169,18 +169,18 @@ class _Policy(torch.autograd.Function):
                 kl_coef, divisor):
         dev, tokens = logps.device, logps.numel()
         seqs = 1 if cu is None else cu.numel() - 1
-        stats, dtoken, weight = logps.new_empty(3), logps.new_empty(tokens), logps.new_empty(seqs if aggregation else 1)
+        loss, kl, cut = logps.new_empty(()), logps.new_empty(()), logps.new_empty(())
+        dtoken, weight = logps.new_empty(tokens), logps.new_empty(seqs if aggregation else 1)
         L = _lib.lib()
         ws = torch.empty(L.siq_policy_workspace_bytes(seqs, tokens), dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
             rc = L.siq_policy_fwd(logps.data_ptr(), old.data_ptr(), advantages.data_ptr(), _ptr(mask), _ptr(reference),
                                   _ptr(cu), seqs, tokens, per_token, aggregation, kl_type, low, high, dual, kl_coef,
-                                  _ptr(divisor), stats.data_ptr(), dtoken.data_ptr(), weight.data_ptr(), ws.data_ptr(),
-                                  ws.numel(), _lib.stream(dev))
+                                  _ptr(divisor), loss.data_ptr(), kl.data_ptr(), cut.data_ptr(), dtoken.data_ptr(),
+                                  weight.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream(dev))
         _lib.check(rc, "siq_policy_fwd")
         ctx.save_for_backward(dtoken, weight, *(() if cu is None else (cu,)))
         ctx.shape, ctx.seqs, ctx.aggregation = logps.shape, seqs, aggregation
-        loss, kl, cut = stats.unbind()
         ctx.mark_non_differentiable(kl, cut)
         ctx.set_materialize_grads(False)
         return loss, kl, cut

@@ -332,9 +332,8 @@ def test_on_a_qwen2_model(which):
         assert abs(float(loss.detach()) - loss0) <= 2.0 ** -7 * loss0
     # int8 groups of 32 normal values: a step of at most max / 64, about 3 / 64, so rounding noise of at most
     # 3 / 64 / sqrt(12) = 1.4% of the values; two layers of it and the bf16 roundings stay below 10% of a gradient
-    for n, g in grads.items():
-        rel = float((g - grads0[n]).norm() / grads0[n].norm())
-        assert rel <= 0.1, (n, rel)
+    worst = max(float((g - grads0[n]).norm() / grads0[n].norm()) for n, g in grads.items())
+    assert 1e-4 < worst <= 0.1  # (0: nothing was kept in 8 bits)
 
 
 def test_a_second_derivative_is_refused():

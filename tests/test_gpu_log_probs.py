@@ -146,6 +146,37 @@ def test_near_certain_labels_are_exact_relative_to_their_distance_from_certainty
     assert (np.abs(np64(dh) + p @ np64(w)) <= (2 * 2.0 ** -8 + off[:, None]) * size).all()
 
 
+def test_more_kept_rows_than_one_pass_takes():
+    """70,000 rows of a small vocabulary: kept numerators in two passes of 65,536 rows, against chunks that are formed again."""
+    n, hdim, vocab = 70_000, 64, 264
+    g = torch.Generator(device=DEV).manual_seed(4)
+    h = torch.randn(n, hdim, generator=g, device=DEV).to(torch.bfloat16)
+    w = (0.1 * torch.randn(vocab, hdim, generator=g, device=DEV)).to(torch.bfloat16)
+    y = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    y[torch.rand(n, generator=g, device=DEV) < 0.02] = -100
+    up = torch.randn(n, generator=g, device=DEV)
+    a, b = LP.flp_fwd(h, w, y, keep=True), LP.flp_fwd(h, w, y, keep=False)
+    assert torch.equal(a[0], b[0]) and int(a[1]) == int(b[1])
+    dh, dw = LP.flp_bwd(h, w, y, up, saved=a[3])
+    dh2, dw2 = LP.flp_bwd(h, w, y, up, chunk_tokens=4096)
+    # the exact gradients in 64 bits, and what rounding may make of each (see the oracle)
+    at = y >= 0
+    p = torch.softmax(h.double() @ w.double().T.contiguous(), 1) * (up.double() * at)[:, None]
+    dz = -p
+    dz[at.nonzero()[:, 0], y[at]] += up.double()[at]
+    want = dz @ w.double()
+    off = 1.05 * (2.0 ** -8 * (p.abs() @ w.double().abs() + want.abs()) + 1e-4 * up.double().abs()[:, None])
+    for got in (dh, dh2):
+        assert bool(((got.double() - want).abs() <= off).all()) and bool((got[~at] == 0).all())
+    want = dz.T.contiguous() @ h.double()
+    # E and the scaled rows rounded, sums of n products in fp32 (eight at once), the label terms' weights
+    label = torch.zeros_like(want).index_add_(0, y[at], (up.double().abs()[:, None] * h.double().abs())[at])
+    off = (2.0 ** -7 + n / 8 * 2.0 ** -24) * (p.abs().T.contiguous() @ h.double().abs()) + 2.0 ** -8 * want.abs()
+    off = 1.05 * off + (1e-4 + n / 8 * 2.0 ** -24) * label
+    for got in (dw, dw2):
+        assert bool(((got.double() - want).abs() <= off).all())
+
+
 def test_kept_and_recomputed_agree_and_repeat():
     h, w, y, up = make(900, 256, 3008, seed=10)
     hd, wd, yd, ud = h.to(DEV), w.to(DEV), y.to(DEV), up.to(DEV)
@@ -168,6 +199,9 @@ def test_autograd_shapes_types_frozen_and_retained():
     hg = h.view(4, 15, 128).to(DEV).requires_grad_()
     wg, yd, ud = w.to(DEV).requires_grad_(), y.view(4, 15).to(DEV), up.view(4, 15).to(DEV)
     want = LP.flp_bwd(hg.detach().view(60, 128), wg.detach(), yd.view(-1), ud.view(-1), temperature=1.3)
+    scaled = LP.fused_linear_log_probs(hg, wg, yd)
+    scaled *= 2.0  # the result is no view of anything: it may be changed in place
+    torch.autograd.grad(scaled.sum(), [hg])
     for keep_bytes in (1 << 30, 0):
         logp = LP.fused_linear_log_probs(hg, wg, yd, temperature=1.3, keep_bytes=keep_bytes)
         assert logp.shape == (4, 15) and logp.dtype == torch.float32

@@ -283,6 +283,18 @@ def test_bad_offsets_touch_nothing_else():
     assert np.isclose(float(P.preference_loss(lp_t, ref_t, cu, mask=mask_t).loss), good[0], rtol=1e-6)
 
 
+def test_losses_may_be_changed_in_place():
+    cu, _, pi, old, ref = batch([30, 40])
+    pi_t, old_t, ref_t, cu_t = gpu(pi, old, ref, cu)
+    pi_t.requires_grad_()
+    for f in (lambda: P.preference_loss(pi_t, ref_t, cu_t).loss, lambda: P.policy_loss(pi_t, old_t, old_t[:2], cu_t).loss):
+        want, = torch.autograd.grad(f(), [pi_t])
+        loss = f()
+        loss /= 4  # gradient accumulation
+        got, = torch.autograd.grad(loss, [pi_t])
+        assert torch.equal(got * 4, want)
+
+
 def test_two_streams_a_retained_graph_and_reproducibility():
     cu, mask, lp, old, ref = batch(LENGTHS["slices"], seed=6)
     lp_t, old_t, ref_t, mask_t, cu_t = gpu(lp, old, ref, mask, cu)

@@ -71,11 +71,11 @@ def test_preference_validation(lib, kw, code):
 
 def _policy(lib, **kw):
     a = dict(lp=FAKE, old=FAKE, adv=FAKE, mask=FAKE, ref=FAKE, cu=FAKE, seqs=3, tokens=100, per=0, agg=0, kl=2, low=0.2,
-             high=0.2, dual=0.0, coef=0.1, div=None, stats=FAKE, dtoken=FAKE, weight=FAKE, ws=FAKE,
+             high=0.2, dual=0.0, coef=0.1, div=None, loss=FAKE, mean=FAKE, frac=FAKE, dtoken=FAKE, weight=FAKE, ws=FAKE,
              bytes=lib.siq_policy_workspace_bytes(3, 100))
     a.update(kw)
     return lib.siq_policy_fwd(*(a[k] for k in ("lp", "old", "adv", "mask", "ref", "cu", "seqs", "tokens", "per", "agg", "kl",
-                                               "low", "high", "dual", "coef", "div", "stats", "dtoken", "weight", "ws",
+                                               "low", "high", "dual", "coef", "div", "loss", "mean", "frac", "dtoken", "weight", "ws",
                                                "bytes")), None)
 
 
@@ -83,7 +83,7 @@ def _policy(lib, **kw):
     (dict(seqs=0), INVALID), (dict(seqs=2 ** 24 + 1), INVALID), (dict(tokens=-1), INVALID), (dict(agg=2), INVALID),
     (dict(kl=3), INVALID), (dict(kl=-1), INVALID), (dict(low=1.5), INVALID), (dict(low=-0.1), INVALID),
     (dict(high=-0.1), INVALID), (dict(high=float("nan")), INVALID), (dict(dual=1.0), INVALID), (dict(dual=0.5), INVALID),
-    (dict(coef=float("nan")), INVALID), (dict(ref=None), INVALID), (dict(cu=None), INVALID), (dict(stats=None), INVALID),
+    (dict(coef=float("nan")), INVALID), (dict(ref=None), INVALID), (dict(cu=None), INVALID), (dict(loss=None), INVALID), (dict(mean=None), INVALID), (dict(frac=None), INVALID),
     (dict(weight=None), INVALID), (dict(lp=None), INVALID), (dict(adv=None), INVALID), (dict(dtoken=None), INVALID),
     (dict(dtoken=FAKE + 4), ALIGN), (dict(bytes=0), WS),
 ])
