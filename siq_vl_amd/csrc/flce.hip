@@ -1457,29 +1457,45 @@ __global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p
   }
 }
 
-// The sum over the ranges, with the factor and the label term: a workgroup a row
-// and 256 features, thirty-two lanes of 8 features x eight that share the ranges.
-__global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const DhArgs p) {
+// The sum over the ranges, with the row's factor and label term: a workgroup a
+// row and 256 features, thirty-two lanes of 8 features x eight that share the
+// ranges.  Row r of the call is cleared where it does not count.
+struct FewSumArgs {
+  DhArgs dh;
+  const float* f0;        // as WeighArgs: dH alone needs no pass of its own for them
+  const float* w0;
+  const float* g;
+  const int64_t* labels;  // of all rows, or nullptr: nothing is cleared
+  int64_t ignore_index;
+  float scale;
+};
+__global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const FewSumArgs a) {
   __shared__ __align__(16) float sh[8][32][8];
+  const DhArgs& p = a.dh;
   const int64_t nv = min(p.nc, *p.nvalid - p.c0), r = blockIdx.y;
-  if (r >= nv) return;
   const int g = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 256 + 8 * g, stride = (int64_t)p.prow * p.hdim;
-  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+  if (a.labels != nullptr && q == 1 && col < p.hdim) {
+    const int64_t v = a.labels[r];
+    if (v == a.ignore_index || v < 0 || v >= p.E.cols) st_bf16x8(p.dh + r * p.hdim + col, zero_bf16x8());
+  }
+  if (r >= nv) return;
+  f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
   if (col < p.hdim) {
     const float* src = p.part + r * p.hdim + col;
 #pragma unroll 4
     for (int s = q; s < p.splits; s += 8) {
-      a += *reinterpret_cast<const f32x4*>(src + s * stride);
-      b += *reinterpret_cast<const f32x4*>(src + s * stride + 4);
+      lo += *reinterpret_cast<const f32x4*>(src + s * stride);
+      hi += *reinterpret_cast<const f32x4*>(src + s * stride + 4);
     }
   }
-  *reinterpret_cast<f32x4*>(&sh[q][g][0]) = a;
-  *reinterpret_cast<f32x4*>(&sh[q][g][4]) = b;
+  *reinterpret_cast<f32x4*>(&sh[q][g][0]) = lo;
+  *reinterpret_cast<f32x4*>(&sh[q][g][4]) = hi;
   __syncthreads();
   if (q != 0 || col >= p.hdim) return;
+  const int64_t row = p.rows[p.c0 + r];
   const bf16x8 l = ld_bf16x8(p.Wt.base + p.y[r] * p.hdim + col);
-  const float f = p.f[r], wt = p.wt[r];
+  const float gr = a.scale * a.g[row], f = a.f0[r] * gr, wt = a.w0[r] * gr;
   bf16x8 o;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -1488,7 +1504,7 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const DhArgs p) {
     for (int k = 0; k < 8; ++k) t += sh[k][g][i];
     o[i] = (bf16)__builtin_fmaf(f, t, wt * (float)l[i]);
   }
-  st_bf16x8(p.dh + (int64_t)p.rows[p.c0 + r] * p.hdim + col, o);
+  st_bf16x8(p.dh + row * p.hdim + col, o);
 }
 
 // dW of at most 64 rows (one k-step): 128 hidden features x 128 vocabulary rows a
@@ -1685,7 +1701,8 @@ void launch_logits_few(LogitsArgs& lg, hipStream_t stream) {
     hipLaunchKernelGGL(flce_logits_few_kernel<4>, grid, dim3(NT), 0, stream, lg);
 }
 
-void launch_dh_few(DhArgs& dh, hipStream_t stream) {
+void launch_dh_few(FewSumArgs& a, hipStream_t stream) {
+  DhArgs& dh = a.dh;
   dh.nI = (int)((dh.hdim + kFewBI - 1) / kFewBI);
   const dim3 grid((unsigned)(dh.nI * dh.splits));
   if (dh.nc <= 64)
@@ -1693,7 +1710,7 @@ void launch_dh_few(DhArgs& dh, hipStream_t stream) {
   else
     hipLaunchKernelGGL(flce_dh_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, dh);
   hipLaunchKernelGGL(flce_dh_few_sum_kernel, dim3((unsigned)((dh.hdim + 255) / 256), (unsigned)dh.nc), dim3(256), 0, stream,
-                     dh);
+                     a);
 }
 
 void launch_dw_few(DwArgs& dw, hipStream_t stream) {
@@ -2084,8 +2101,11 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
     wg.ignore_index = a.ignore_index;
     wg.scale = (float)(-1. / a.temperature);
     wg.nsort = L.nsort;
-    const int64_t blocks = std::min<int64_t>((nc + kRowThreads / 64 - 1) / (kRowThreads / 64), 1024);
-    hipLaunchKernelGGL(flce_weigh_kernel, dim3((unsigned)(L.nsort + blocks)), dim3(kRowThreads), 0, stream, wg);
+    const bool few_dh = L.few && L.nchunks == 1 && !need_dw;
+    if (!few_dh) {
+      const int64_t blocks = std::min<int64_t>((nc + kRowThreads / 64 - 1) / (kRowThreads / 64), 1024);
+      hipLaunchKernelGGL(flce_weigh_kernel, dim3((unsigned)(L.nsort + blocks)), dim3(kRowThreads), 0, stream, wg);
+    }
 
     if (a.dhidden != nullptr) {
       DhArgs dh{};
@@ -2104,10 +2124,19 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       dh.splits = L.splits;
       dh.prow = L.prow;
       dh.run = L.run;
-      if (L.few)
-        launch_dh_few(dh, stream);
-      else
+      if (L.few) {
+        FewSumArgs fs{};
+        fs.dh = dh;
+        fs.f0 = f0;
+        fs.w0 = w0;
+        fs.g = a.dlogp;
+        fs.labels = few_dh && have ? a.labels : nullptr;
+        fs.ignore_index = a.ignore_index;
+        fs.scale = wg.scale;
+        launch_dh_few(fs, stream);
+      } else {
         launch_dh(dh, stream);
+      }
     }
     if (need_dw) {
       LabelArgs la{};
