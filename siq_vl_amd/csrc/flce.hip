@@ -1507,104 +1507,152 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const FewSumArgs a
   st_bf16x8(p.dh + row * p.hdim + col, o);
 }
 
-// dW of at most 64 rows (one k-step): 128 hidden features x 128 vocabulary rows a
-// workgroup, four waves of 64 x 64.  There is next to nothing to multiply: it is
-// bound by writing dW, so small workgroups, four a CU, whose stores overlap the
-// others' loads, and whole rows leave at once.  48 x 896 over 151936 columns: 65
-// us (4.2 TB/s), the general kernel 89; two k-steps (128 x 1536) were no faster
-// than the general kernel, 190 and 183 us.  Rows past the valid ones are zeroed
-// in LDS.
+// dW of few rows (STEPS k-steps of 64), one chunk: a workgroup takes 128
+// vocabulary rows and up to kDwTiles tiles of 128 hidden features, four waves of
+// 64 x 64.  There is next to nothing to multiply: it is bound by writing dW.  The
+// numerators' tile is read once into registers; then, tile after tile, the rows'
+// slice of H is multiplied and the result turned in LDS so that whole rows leave,
+// and while they do the next slice is loading.  Rows past the valid ones are
+// zeroed in LDS.
+constexpr int kDwTiles = 4;
+template <int STEPS>
 __global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p) {
   constexpr int TILE = 128, OP = BK * TILE, QA = 4;
-  __shared__ __align__(16) bf16 smem[2 * OP];
-  int ti, tj;
-  if (!tile_of(p.nI, p.nJ, p.nI, ti, tj)) return;
-  const int64_t i0 = (int64_t)ti * TILE, j0 = (int64_t)tj * TILE;
+  __shared__ __align__(16) bf16 smem[(2 + STEPS) * OP];  // numerators, then results: 2 OP; H: STEPS OP
+  static_assert(STEPS <= 2, "the numerators' tile lies where the results go");
+  bf16 *out = smem, *hs = smem + 2 * OP;
+  int part, tj;
+  const int tiles = (p.nI + kDwTiles - 1) / kDwTiles;
+  if (!tile_of(tiles, p.nJ, tiles, part, tj)) return;
+  const int t0 = part * kDwTiles, t1 = min(p.nI, t0 + kDwTiles);
+  const int64_t j0 = (int64_t)tj * TILE;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
   const int wi = w & 1, wj = w >> 1, wu = __builtin_amdgcn_readfirstlane(w);
   const int nc = (int)p.Ht.rows, nv = (int)min((int64_t)nc, *p.nvalid);
-  f32x16 acc[2][2];
+  const int steps = (nv + BK - 1) / BK;  // (0: dW is zero)
+  // this lane's chunk of instruction q of a k-step: k row and column
+  int row[QA], col[QA];
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int q = 0; q < QA; ++q) {
+    row[q] = 4 * (QA * w + q) + lane / 16;
+    col[q] = 8 * ((lane % 16) ^ swz_nkc(row[q]));
+  }
+  auto load_h = [&](int t) {
+    const int last = (int)min(p.hdim - 8 - (int64_t)t * TILE, (int64_t)(TILE - 8));
 #pragma unroll
-    for (int b = 0; b < 2; ++b) acc[a][b] = zero16();
-  int slot[2] = {0, 0};
-  if (nv > 0) {
-    const int ca = (int)min(p.hdim - 8 - i0, (int64_t)(TILE - 8)), cb = (int)min(p.V - 8 - j0, (int64_t)(TILE - 8));
+    for (int s = 0; s < STEPS; ++s) {
+      if (s >= steps) break;
 #pragma unroll
-    for (int q = 0; q < QA; ++q) {
-      const int r = 4 * (QA * w + q) + lane / 16, c = 8 * ((lane % 16) ^ swz_nkc(r)), row = min(r, nc - 1);
-      bf16* dst = smem + (QA * wu + q) * 512;
-      dma16(p.Ht.base + i0, 2 * (uint32_t)(row * (int)p.hdim + min(c, ca)), dst);
-      dma16(p.Et.base + j0, 2 * ((uint32_t)row * (uint32_t)p.V + (uint32_t)min(c, cb)), dst + OP);
+      for (int q = 0; q < QA; ++q)
+        dma16(p.Ht.base + (int64_t)t * TILE, 2 * (uint32_t)(min(BK * s + row[q], nc - 1) * (int)p.hdim + min(col[q], last)),
+              hs + s * OP + (QA * wu + q) * 512);
     }
+  };
+  bf16x8 b[STEPS][4][2];
+  int slot[2] = {0, 0};
+  if (steps > 0) {
+    const int last = (int)min(p.V - 8 - j0, (int64_t)(TILE - 8));
 #pragma unroll
-    for (int b = 0; b < 2; ++b) slot[b] = p.slot[min(j0 + 64 * wj + 32 * b + l32, p.V - 1)];
-    HalfRead<false, true, 2> ra;
-    HalfRead<false, false, 2> rb;
-    ra.init(lane, 64 * wi);
-    rb.init(lane, 64 * wj);
+    for (int s = 0; s < STEPS; ++s) {
+      if (s >= steps) break;
+#pragma unroll
+      for (int q = 0; q < QA; ++q)
+        dma16(p.Et.base + j0, 2 * ((uint32_t)min(BK * s + row[q], nc - 1) * (uint32_t)p.V + (uint32_t)min(col[q], last)),
+              out + s * OP + (QA * wu + q) * 512);
+    }
+    load_h(t0);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) slot[y] = p.slot[min(j0 + 64 * wj + 32 * y + l32, p.V - 1)];
     wait_vmcnt<0>();
     __syncthreads();
-    const bf16* A = smem;
-    bf16* B = smem + OP;
-    if (nv < BK) {
-      for (int i = nv * 16 + tid; i < BK * 16; i += kFewThreads) st_bf16x8(B + 8 * i, zero_bf16x8());
-      __syncthreads();
+    for (int i = nv * 16 + tid; i < steps * BK * 16; i += kFewThreads) st_bf16x8(out + 8 * i, zero_bf16x8());
+    __syncthreads();
+    HalfRead<false, false, 2> rb;
+    rb.init(lane, 64 * wj);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) b[s][ks][y] = s < steps ? rb.read(out + s * OP, y, ks) : zero_bf16x8();
+    wait_lds();
+  }
+  HalfRead<false, true, 2> ra;
+  ra.init(lane, 64 * wi);
+  const int oc = tid % 16, orow = tid / 16;
+  const bool whole = j0 + TILE <= p.V;
+  for (int t = t0; t < t1; ++t) {
+    const int64_t i0 = (int64_t)t * TILE;
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[x][y] = zero16();
+    // this tile's rows have landed (they were asked for before the last results were stored: eight stores a wave, fewer
+    // where the vocabulary ends in the tile), and every wave has read those results, or the numerators, from LDS
+    if (whole)
+      wait_vmcnt<8>();
+    else
+      wait_vmcnt<0>();
+    phase_barrier();
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (s >= steps) break;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        bf16x8 a[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) a[x] = ra.read(hs + s * OP, x, ks);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) acc[x][y] = mfma32(a[x], b[s][ks][y], acc[x][y]);
+      }
     }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      bf16x8 a[2], b[2];
+    for (int y = 0; y < 2; ++y)
+      for (int sl = slot[y]; sl > 0; sl = p.next[sl - 1]) {
+        const float* lt = p.lsum + (int64_t)(sl - 1) * p.hdim;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        a[t] = ra.read(A, t, ks);
-        b[t] = rb.read(B, t, ks);
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const int64_t hh = i0 + 64 * wi + 32 * x + 16 * jj + 8 * h;
+            if (hh >= p.hdim) continue;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(lt + hh), hi = *reinterpret_cast<const f32x4*>(lt + hh + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              acc[x][y][8 * jj + i] += lo[i];
+              acc[x][y][8 * jj + 4 + i] += hi[i];
+            }
+          }
       }
+    // [128 v][128 h], the 16-byte chunks of a row turned by the row
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) acc[x][y] = mfma32(a[x], b[y], acc[x][y]);
-    }
-  }
-#pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int64_t v = j0 + 64 * wj + 32 * b + l32;
-    if (v >= p.V) continue;
-    for (int sl = slot[b]; sl > 0; sl = p.next[sl - 1]) {
-      const float* lt = p.lsum + (int64_t)(sl - 1) * p.hdim;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
-          const int64_t hh = i0 + 64 * wi + 32 * a + 16 * jj + 8 * h;
-          if (hh >= p.hdim) continue;
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(lt + hh), hi = *reinterpret_cast<const f32x4*>(lt + hh + 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc[a][b][8 * jj + i] += lo[i];
-            acc[a][b][8 * jj + 4 + i] += hi[i];
-          }
+          const int r = 64 * wj + 32 * y + l32, c = 8 * wi + 4 * x + 2 * jj + h;
+          st_bf16x8(out + r * TILE + 8 * (c ^ (r & 15)), pack8(acc[x][y], 8 * jj));
         }
+    wait_lds();
+    phase_barrier();
+    if (t + 1 < t1) load_h(t + 1);
+    bf16x8 o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 16 * i + orow;
+      o[i] = ld_bf16x8(out + r * TILE + 8 * (oc ^ (r & 15)));
     }
-  }
-  // through LDS, [128 v][128 h] with the 16-byte chunks of a row turned by the row, so that rows leave whole
-  __syncthreads();
+    wait_lds();
+    if (i0 + 8 * oc < p.hdim) {
+      bf16* dst = p.dw + (j0 + orow) * p.hdim + i0 + 8 * oc;
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        const int r = 64 * wj + 32 * b + l32, c = 8 * wi + 4 * a + 2 * jj + h;
-        st_bf16x8(smem + r * TILE + 8 * (c ^ (r & 15)), pack8(acc[a][b], 8 * jj));
-      }
-  __syncthreads();
-  const int c = tid % 16;
-  if (i0 + 8 * c >= p.hdim) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 16 * i + tid / 16;
-    if (j0 + r < p.V) st_bf16x8(p.dw + (j0 + r) * p.hdim + i0 + 8 * c, ld_bf16x8(smem + r * TILE + 8 * (c ^ (r & 15))));
+      for (int i = 0; i < 8; ++i)
+        if (j0 + 16 * i + orow < p.V) st_bf16x8(dst + (int64_t)(16 * i) * p.hdim, o[i]);
+    }
   }
 }
 
@@ -1716,8 +1764,11 @@ void launch_dh_few(FewSumArgs& a, hipStream_t stream) {
 void launch_dw_few(DwArgs& dw, hipStream_t stream) {
   dw.nI = (int)((dw.hdim + 127) / 128);
   dw.nJ = (int)((dw.V + 127) / 128);
-  const int grid = ((dw.nI * dw.nJ + kXcds - 1) / kXcds) * kXcds;
-  hipLaunchKernelGGL(flce_dw_few_kernel, dim3(grid), dim3(kFewThreads), 0, stream, dw);
+  const int parts = (dw.nI + kDwTiles - 1) / kDwTiles, grid = ((parts * dw.nJ + kXcds - 1) / kXcds) * kXcds;
+  if (dw.Ht.rows <= BK)
+    hipLaunchKernelGGL(flce_dw_few_kernel<1>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
+  else
+    hipLaunchKernelGGL(flce_dw_few_kernel<2>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
 }
 
 void launch_dw(DwArgs& dw, hipStream_t stream) {
@@ -2163,7 +2214,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       dw.hdim = a.hdim;
       dw.V = a.vocab;
       dw.chunk = L.chunk;
-      if (a.n <= BK && L.nchunks == 1)
+      if (L.few && L.nchunks == 1)
         launch_dw_few(dw, stream);
       else
         launch_dw(dw, stream);
