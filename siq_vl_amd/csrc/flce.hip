@@ -1204,9 +1204,8 @@ struct FewRows {
 };
 
 // Rows of a call (NB = 2: 64) that take these kernels.  Forward and dH with a
-// frozen head over 151936 columns of 896, against the general kernels: 48 rows
-// 65 and 54 us (124 and 124), 128 rows 91 and 74 us, 129 rows (general) 110 and
-// 110 us.
+// frozen head over 151936 columns of 896: 48 rows 65 and 50 us, 128 rows 87 and
+// 69 us, 129 rows (the general kernels, which take as long for fewer) 101 and 99.
 constexpr int kFewRows = 128;
 
 // The logits kernel over 256 vocabulary rows x 32 NB rows of the call: eight
@@ -1513,7 +1512,8 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const FewSumArgs a
 // numerators' tile is read once into registers; then, tile after tile, the rows'
 // slice of H is multiplied and the result turned in LDS so that whole rows leave,
 // and while they do the next slice is loading.  Rows past the valid ones are
-// zeroed in LDS.
+// zeroed in LDS.  Over 151936 columns, against the general kernel: 48 rows x 896
+// 57 us (89), 48 x 1536 95 (139), 128 x 1536 131 (183; 467 MB written, 3.6 TB/s).
 constexpr int kDwTiles = 4;
 template <int STEPS>
 __global__ __launch_bounds__(kFewThreads) void flce_dw_few_kernel(const DwArgs p) {

@@ -51,7 +51,7 @@ def check(h, w, y, up, temperature=1.0, keep=True, chunk=None, need_dw=True, rou
 
 
 @pytest.mark.parametrize("keep,chunk", [(True, None), (False, None), (False, 128), (False, 64), (False, 100)])
-@pytest.mark.parametrize("n,hdim,vocab", [(64, 64, 2000), (65, 192, 1000), (128, 320, 4104), (129, 320, 4104), (1, 64, 8), (3, 64, 1000), (255, 320, 264), (257, 128, 2000), (300, 896, 1000)])
+@pytest.mark.parametrize("n,hdim,vocab", [(50, 896, 520), (100, 1152, 1000), (64, 64, 2000), (65, 192, 1000), (128, 320, 4104), (129, 320, 4104), (1, 64, 8), (3, 64, 1000), (255, 320, 264), (257, 128, 2000), (300, 896, 1000)])
 def test_against_the_oracle(n, hdim, vocab, keep, chunk):
     print(f"logp n={n} h={hdim} V={vocab} keep={keep} chunk={chunk}", flush=True)
     h, w, y, up = make(n, hdim, vocab, seed=n, ignored=0.3 if n > 1 else 0.0)
