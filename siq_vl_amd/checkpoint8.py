@@ -335,6 +335,8 @@ def enable_8bit_checkpoints(model: torch.nn.Module, format: str = "int8") -> int
     ``gradient_checkpointing=True`` enables the stock one at its start: leave that
     argument False and call this before."""
     _format(format)
+    if not hasattr(model, "gradient_checkpointing_enable"):
+        raise TypeError("expected a transformers model (gradient_checkpointing_enable)")
     model.gradient_checkpointing_enable(gradient_checkpointing_kwargs={"use_reentrant": False})
     func = functools.partial(_layer_checkpoint, format)
     n = 0

@@ -116,3 +116,8 @@ def test_python_refusals():
         K.unpack8(K.Packed8(codes, scales, torch.Size([64]), torch.float32, "int8"))
     with pytest.raises(ValueError, match="dtype"):
         K.unpack8(K.Packed8(codes, scales, torch.Size([64]), torch.float16, "int8"))
+    with pytest.raises(TypeError, match="transformers"):
+        K.enable_8bit_checkpoints(torch.nn.Linear(2, 2))
+    assert K.enable_8bit_mlp(torch.nn.Linear(2, 2)) == 0
+    with pytest.raises(ValueError, match="format"):
+        K.enable_8bit_mlp(torch.nn.Linear(2, 2), "int4")

@@ -103,3 +103,19 @@ def test_python_refusals():
         LP.fused_linear_log_probs(h, w[:, :32], y)
     with pytest.raises(ValueError, match="bfloat16"):
         LP.flp_bwd(h.float(), w, y, torch.zeros(4))
+
+
+def test_log_probs_of_a_model_need_labels_and_the_gpu():
+    transformers = pytest.importorskip("transformers")
+    from siq_vl_amd.text_model import enable_fused_cross_entropy
+
+    cfg = transformers.Qwen2Config(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=1,
+                                   num_attention_heads=2, num_key_value_heads=1, use_cache=False)
+    model = transformers.Qwen2ForCausalLM(cfg)
+    enable_fused_cross_entropy(model)
+    ids = torch.randint(0, 64, (1, 5))
+    with pytest.raises(ValueError, match="return_log_probs needs labels"):
+        model(input_ids=ids, return_log_probs=True)
+    with pytest.raises(ValueError, match="GPU"):
+        model(input_ids=ids, labels=ids, return_log_probs=True)
+    assert model(input_ids=ids).logits.shape == (1, 5, 64)
