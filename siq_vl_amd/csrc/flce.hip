@@ -351,7 +351,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       // `sum` is that of the other columns: with t its ratio to the label's term the label's probability is 1 / (1 + t),
       // and both its logarithm and its distance from 1 keep their digits where t is small.  Redone tiles are 2^60 above
       // the label: there only the sum counts.
-      const float d = p.zy[row], t = sum * exp2f_fast(-d), all = sum + exp2f_fast(d);
+      const float d = p.zy[row], t = sum == 0.f ? 0.f : sum * exp2f_fast(-d), all = sum + exp2f_fast(d);
       const float lp = redone ? -kLn2 * (__log2f(sum) + (top - rf - d)) : -log1pf(t);
       lse2 = top + __log2f(redone ? sum : all);
       f0 = 1.f / all;

@@ -74,9 +74,8 @@ def fused_causal_lm_forward(self, input_ids=None, attention_mask=None, position_
     if targets is None:
         targets = shift_labels(labels, IGNORE_INDEX)
     if return_log_probs:
-        targets = targets.to(hidden.device)
-        logps = fused_linear_log_probs(hidden, self.lm_head.weight, targets.view(hidden.shape[:-1]), IGNORE_INDEX,
-                                       temperature, chunk_tokens=getattr(self, "siq_ce_chunk_tokens", None))
+        logps = fused_linear_log_probs(hidden, self.lm_head.weight, targets.to(hidden.device), IGNORE_INDEX, temperature,
+                                       chunk_tokens=getattr(self, "siq_ce_chunk_tokens", None))
         return _output_with_log_probs()(loss=None, logits=None, past_key_values=outputs.past_key_values,
                                         hidden_states=outputs.hidden_states, attentions=outputs.attentions,
                                         log_probs=logps)
