@@ -2,12 +2,16 @@
 
 There is no fallback: if the library is missing the caller gets a RuntimeError
 naming the build step, never a silent CPU or PyTorch path.
+
+``native()`` is the extension ``_native.so``, the host side of the short
+operators; it calls this library through the same ABI.
 """
 
 from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib
 import os
 import threading
 from pathlib import Path
@@ -18,6 +22,7 @@ from . import build as _build
 
 _LOCK = threading.Lock()
 _LIB: ctypes.CDLL | None = None
+_NATIVE = None
 _HERE = contextlib.nullcontext()
 
 SIQ_OK = 0
@@ -196,6 +201,26 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _LIB = handle
     return _LIB
+
+
+def native():
+    """Loads the extension once and gives it the library's entry points; raises
+    if either has not been built."""
+    global _NATIVE
+    if _NATIVE is not None:
+        return _NATIVE
+    handle = lib()
+    with _LOCK:
+        if _NATIVE is None:
+            if not _build.NATIVE_PATH.exists():
+                raise RuntimeError(
+                    f"{_build.NATIVE_PATH} is missing: build the HIP kernels first "
+                    "(python -c 'import __graft_entry__ as g; g.build()' or python -m siq_vl_amd.build)"
+                )
+            module = importlib.import_module("._native", __package__)
+            module.bind({name: ctypes.cast(getattr(handle, name), _c_void_p).value for name in module.entries()})
+            _NATIVE = module
+    return _NATIVE
 
 
 def check(rc: int, what: str) -> None:

@@ -68,37 +68,9 @@ def _check(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must live on the GPU, got {t.device}")
 
 
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
-def _align(n: int) -> int:
-    return (n + 255) & ~255
-
-
-def _stores(numel: int, count: int, device: torch.device) -> list[torch.Tensor]:
-    """``count`` pairs of code and scale bytes for ``numel`` elements each, in one allocation."""
-    groups = (numel + GROUP - 1) // GROUP
-    step = _align(numel) + _align(groups)
-    buf = torch.empty(step * count, dtype=torch.uint8, device=device)
-    out = []
-    for i in range(count):
-        at = i * step
-        out += [buf[at:at + numel], buf[at + _align(numel):at + _align(numel) + groups]]
-    return out
-
-
 def pack8(x: torch.Tensor, format: str = "int8") -> Packed8:
     """``x`` (bf16 or fp32, any shape) in 8 bits, in memory order."""
-    fmt = _format(format)
-    _check(x, "x")
-    x = _flat(x.detach())
-    codes, scales = _stores(x.numel(), 1, x.device)
-    with _lib.on_device(x.device):
-        rc = _lib.lib().siq_pack8(x.data_ptr(), x.numel(), _DTYPES[x.dtype], fmt, codes.data_ptr(), scales.data_ptr(),
-                                  _lib.stream(x.device))
-    _lib.check(rc, "siq_pack8")
+    codes, scales = _lib.native().pack8(x, _format(format))
     return Packed8(codes, scales, x.shape, x.dtype, format)
 
 
@@ -106,139 +78,29 @@ def unpack8(packed: Packed8, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The values that ``packed`` stands for (``dtype``: bf16 or fp32, the packed tensor's by default)."""
     fmt = _format(packed.format)
     dtype = packed.dtype if dtype is None else dtype
-    numel = packed.shape.numel()
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
-    for name, t, n in (("codes", packed.codes, numel), ("scales", packed.scales, (numel + GROUP - 1) // GROUP)):
-        if t.dtype != torch.uint8 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name} must be {n} contiguous uint8, got {tuple(t.shape)} {t.dtype}")
-        if t.device.type != "cuda" or t.device != packed.codes.device:
-            raise ValueError(f"codes and scales must live on one GPU, got {packed.codes.device} and {t.device}")
-    x = torch.empty(packed.shape, dtype=dtype, device=packed.codes.device)
-    with _lib.on_device(x.device):
-        rc = _lib.lib().siq_unpack8(packed.codes.data_ptr(), packed.scales.data_ptr(), numel, _DTYPES[dtype], fmt,
-                                    x.data_ptr(), _lib.stream(x.device))
-    _lib.check(rc, "siq_unpack8")
-    return x
+    return _lib.native().unpack8(packed.codes, packed.scales, packed.shape, dtype == torch.float32, fmt)
 
 
 # --------------------------------------------------------------------------- gated MLP activation
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A [rows, cols] view of ``t`` that the kernels read in place, or a contiguous copy."""
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    step = 4 if t.dtype == torch.float32 else 8
-    if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % step == 0
-                             and t.shape[1] % 8 == 0):
-        return t.clone() if t.data_ptr() % 16 else t
-    return t.contiguous()
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 and not t.is_contiguous() else t.shape[1]
-
-
 def swiglu8_fwd(gate: torch.Tensor, up: torch.Tensor, format: str = "int8", keep: bool = True):
     """Raw forward on ``[..., cols]``: ``(h, stores)`` with ``stores`` the packed
     gate and up (codes, scales, codes, scales), or None without ``keep``."""
-    fmt = _format(format)
-    for name, t in (("gate", gate), ("up", up)):
-        _check(t, name)
-        if t.dim() == 0:
-            raise ValueError(f"{name} must have at least one dimension")
-    if gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
-        raise ValueError(f"gate and up must be alike, got {tuple(gate.shape)} {gate.dtype} on {gate.device} and "
-                         f"{tuple(up.shape)} {up.dtype} on {up.device}")
-    h = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-    stores = _stores(h.numel(), 2, h.device) if keep else None
-    if h.numel() == 0:
-        return h, stores
-    g, u = _rows(gate), _rows(up)
-    ptrs = [s.data_ptr() for s in stores] if keep else [None] * 4
-    with _lib.on_device(h.device):
-        rc = _lib.lib().siq_swiglu8_fwd(g.data_ptr(), u.data_ptr(), g.shape[0], g.shape[1], _ld(g), _ld(u),
-                                        _DTYPES[h.dtype], fmt, h.data_ptr(), *ptrs, _lib.stream(h.device))
-    _lib.check(rc, "siq_swiglu8_fwd")
-    return h, stores
+    h, stores = _lib.native().swiglu8_fwd(gate, up, _format(format), keep)
+    return h, stores if keep else None
 
 
 def swiglu8_bwd(dh: torch.Tensor, stores, format: str = "int8", need_h: bool = False, fused: bool = False):
     """Raw backward: ``(dgate, dup, h | None)`` like ``dh``; with ``fused`` both
     gradients side by side in one tensor, ``(dgate_dup [..., 2 * cols], None, h | None)``."""
-    fmt = _format(format)
-    _check(dh, "dh")
-    if dh.dim() == 0:
-        raise ValueError("dh must have at least one dimension")
-    numel, cols = dh.numel(), dh.shape[-1]
-    groups = (numel + GROUP - 1) // GROUP
-    for s, n in zip(stores, (numel, groups, numel, groups), strict=True):
-        if s.dtype != torch.uint8 or s.numel() != n or not s.is_contiguous() or s.device != dh.device:
-            raise ValueError(f"the packed gate and up do not belong to a gradient of shape {tuple(dh.shape)}")
-    rows = numel // cols if cols else 0
-    both = torch.empty(*dh.shape[:-1], 2 * cols, dtype=dh.dtype, device=dh.device) if fused else None
-    # the halves are written in place where their rows start at 16-byte boundaries
-    halves = fused and cols % 8 == 0
-    if halves:
-        dgate, dup, ld = both[..., :cols], both[..., cols:], 2 * cols
-    else:
-        dgate = torch.empty(dh.shape, dtype=dh.dtype, device=dh.device)
-        dup, ld = torch.empty_like(dgate), cols
-    h = torch.empty(dh.shape, dtype=dh.dtype, device=dh.device) if need_h else None
-    if numel:
-        dh = _flat(dh)
-        with _lib.on_device(dh.device):
-            rc = _lib.lib().siq_swiglu8_bwd(dh.data_ptr(), *(s.data_ptr() for s in stores), rows, cols, ld, ld,
-                                            _DTYPES[dh.dtype], fmt, dgate.data_ptr(), dup.data_ptr(),
-                                            None if h is None else h.data_ptr(), _lib.stream(dh.device))
-        _lib.check(rc, "siq_swiglu8_bwd")
-        if fused and not halves:
-            both[..., :cols], both[..., cols:] = dgate, dup
-    return (both, None, h) if fused else (dgate, dup, h)
-
-
-class _Swiglu8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate, up, fmt):
-        h, stores = swiglu8_fwd(gate, up, fmt)
-        ctx.save_for_backward(*stores)
-        ctx.fmt = fmt
-        return h
-
-    @staticmethod
-    def backward(ctx, dh):
-        _lib.first_order("swiglu8")
-        dgate, dup, _ = swiglu8_bwd(dh, ctx.saved_tensors, ctx.fmt)
-        return dgate, dup, None
-
-
-class _Swiglu8Fused(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate_up, fmt):
-        cols = gate_up.shape[-1] // 2
-        h, stores = swiglu8_fwd(gate_up[..., :cols], gate_up[..., cols:], fmt)
-        ctx.save_for_backward(*stores)
-        ctx.fmt = fmt
-        return h
-
-    @staticmethod
-    def backward(ctx, dh):
-        _lib.first_order("swiglu8")
-        return swiglu8_bwd(dh, ctx.saved_tensors, ctx.fmt, fused=True)[0], None
+    return _lib.native().swiglu8_bwd(dh, stores, _format(format), need_h, fused)
 
 
 def swiglu8(gate: torch.Tensor, up: torch.Tensor | None = None, format: str = "int8") -> torch.Tensor:
     """``silu(gate) * up`` that keeps gate and up in 8 bits for its backward.
     With ``up`` None, ``gate`` holds both side by side in its last dimension."""
-    _format(format)
-    if up is None:
-        if gate.dim() == 0 or gate.shape[-1] % 2:
-            raise ValueError(f"gate and up side by side need an even last dimension, got {tuple(gate.shape)}")
-        if torch.is_grad_enabled() and gate.requires_grad:
-            return _Swiglu8Fused.apply(gate, format)
-        cols = gate.shape[-1] // 2
-        return swiglu8_fwd(gate[..., :cols], gate[..., cols:], format, keep=False)[0]
-    if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-        return _Swiglu8.apply(gate, up, format)
-    return swiglu8_fwd(gate, up, format, keep=False)[0]
+    return _lib.native().swiglu8(gate, up, _format(format))
 
 
 class _Swiglu8Linear(torch.autograd.Function):

@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .cross_entropy import IGNORE_INDEX, _check_operands, _track_bad, default_chunk_tokens
+from .cross_entropy import IGNORE_INDEX, _track_bad, default_chunk_tokens
 
 # What the forward may keep for its backward: rows x vocab bf16.  The head's
 # backward is a step's first, so this is held beside all other activations, but
@@ -30,30 +30,8 @@ DEFAULT_KEEP_BYTES = 8 << 30
 def flp_fwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = IGNORE_INDEX,
             temperature: float = 1.0, keep: bool = False):
     """Raw forward: ``(logp fp32 [n], count, bad_labels, saved | None)``."""
-    logp, counts, saved = _forward(hidden, weight, labels, ignore_index, temperature, keep, labels.shape)
+    logp, counts, saved = _lib.native().flp_fwd(hidden, weight, labels, int(ignore_index), float(temperature), bool(keep))
     return logp, counts[0], counts[1], saved
-
-
-def _forward(hidden, weight, labels, ignore_index, temperature, keep, shape):
-    """``(logp of that shape, [count, bad_labels] int64, saved | None)``."""
-    _check_operands(hidden, weight, labels)
-    for name, t in (("weight", weight), ("labels", labels)):
-        if t.device != hidden.device:
-            raise ValueError(f"{name} must live on {hidden.device}, got {t.device}")
-    (n, hdim), vocab, dev = hidden.shape, weight.shape[0], hidden.device
-    hidden, weight, labels = hidden.contiguous(), weight.contiguous(), labels.contiguous()
-    L = _lib.lib()
-    logp = torch.empty(shape, dtype=torch.float32, device=dev)
-    counts = torch.empty(2, dtype=torch.int64, device=dev)
-    saved = torch.empty(L.siq_flp_saved_bytes(n, vocab), dtype=torch.uint8, device=dev) if keep else None
-    ws = torch.empty(L.siq_flp_fwd_workspace_bytes(n, hdim, vocab, int(keep)), dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        rc = L.siq_flp_fwd(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), n, hdim, vocab, int(ignore_index),
-                           float(temperature), logp.data_ptr(), counts.data_ptr(), counts.data_ptr() + 8,
-                           saved.data_ptr() if keep else None, saved.numel() if keep else 0, ws.data_ptr(), ws.numel(),
-                           _lib.stream(dev))
-    _lib.check(rc, "siq_flp_fwd")
-    return logp, counts, saved
 
 
 def flp_bwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, dlogp: torch.Tensor,
@@ -61,55 +39,10 @@ def flp_bwd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, dl
             need_dhidden: bool = True, need_dweight: bool = True, chunk_tokens: int | None = None):
     """Raw backward: ``(dhidden | None, dweight | None)``; ``saved`` is the
     forward's on the same inputs, or None (the logits are formed again)."""
-    _check_operands(hidden, weight, labels)
-    (n, hdim), vocab, dev = hidden.shape, weight.shape[0], hidden.device
-    if dlogp.shape != (n,) or dlogp.dtype != torch.float32:
-        raise ValueError(f"dlogp must be float32 [{n}], got {dlogp.dtype} {tuple(dlogp.shape)}")
-    for name, t in (("weight", weight), ("labels", labels), ("dlogp", dlogp)):
-        if t.device != dev:
-            raise ValueError(f"{name} must live on {dev}, got {t.device}")
-    hidden, weight, labels, dlogp = (t.contiguous() for t in (hidden, weight, labels, dlogp))
-    chunk = default_chunk_tokens(vocab) if chunk_tokens is None else int(chunk_tokens)
-    if chunk <= 0:
-        raise ValueError("chunk_tokens must be positive")
-    L = _lib.lib()
-    dh = torch.empty_like(hidden) if need_dhidden else None
-    dw = torch.empty_like(weight) if need_dweight else None
-    have = saved is not None
-    ws = torch.empty(L.siq_flp_bwd_workspace_bytes(n, hdim, vocab, chunk, int(need_dweight), int(have)),
-                     dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        rc = L.siq_flp_bwd(hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(), dlogp.data_ptr(), n, hdim, vocab,
-                           int(ignore_index), float(temperature), saved.data_ptr() if have else None,
-                           saved.numel() if have else 0, dh.data_ptr() if need_dhidden else None,
-                           dw.data_ptr() if need_dweight else None, chunk, ws.data_ptr(), ws.numel(), _lib.stream(dev))
-    _lib.check(rc, "siq_flp_bwd")
-    return dh, dw
-
-
-def _rows(hidden: torch.Tensor) -> torch.Tensor:
-    return hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
-
-
-class _FusedLinearLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, labels, ignore_index, temperature, chunk_tokens, keep_bytes, validate):
-        h2, y = _rows(hidden), labels if labels.dim() == 1 else labels.reshape(-1)
-        keep = _lib.lib().siq_flp_saved_bytes(h2.shape[0], weight.shape[0]) <= keep_bytes
-        logp, counts, saved = _forward(h2, weight, y, ignore_index, temperature, keep, labels.shape)
-        _track_bad(counts[1], weight.shape[0], ignore_index, validate)
-        ctx.save_for_backward(hidden, weight, labels, *((saved,) if keep else ()))
-        ctx.ignore_index, ctx.temperature, ctx.chunk_tokens = ignore_index, temperature, chunk_tokens
-        return logp
-
-    @staticmethod
-    def backward(ctx, dlogp):
-        _lib.first_order("fused_linear_log_probs")
-        hidden, weight, labels, *saved = ctx.saved_tensors
-        dh, dw = flp_bwd(_rows(hidden), weight, labels.reshape(-1), dlogp.reshape(-1),
-                         ctx.ignore_index, ctx.temperature, saved[0] if saved else None, ctx.needs_input_grad[0],
-                         ctx.needs_input_grad[1], ctx.chunk_tokens)
-        return None if dh is None else dh.view(hidden.shape), dw, *(None,) * 6
+    if hidden.dim() == weight.dim() == 2 and chunk_tokens is None:
+        chunk_tokens = default_chunk_tokens(weight.shape[0])
+    return _lib.native().flp_bwd(hidden, weight, labels, dlogp, int(ignore_index), float(temperature), saved,
+                                 bool(need_dhidden), bool(need_dweight), int(chunk_tokens or 0))
 
 
 def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
@@ -133,12 +66,13 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
         raise ValueError(f"labels must be {tuple(hidden.shape[:-1])}, got {tuple(labels.shape)}")
     h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
     w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
-    if not torch.is_grad_enabled() or not (h.requires_grad or w.requires_grad):
-        logp, counts, _ = _forward(_rows(h), w, labels.reshape(-1), int(ignore_index), temperature, False, labels.shape)
-        _track_bad(counts[1], w.shape[0], int(ignore_index), validate)
-        return logp
-    return _FusedLinearLogProbs.apply(h, w, labels, int(ignore_index), float(temperature), chunk_tokens, int(keep_bytes),
-                                      validate)
+    if chunk_tokens is None:
+        chunk_tokens = default_chunk_tokens(w.shape[0])
+    ignore_index = int(ignore_index)
+    logp, counts = _lib.native().linear_log_probs(h, w, labels, ignore_index, float(temperature), int(chunk_tokens),
+                                                  int(keep_bytes))
+    _track_bad(counts[1], w.shape[0], ignore_index, validate)
+    return logp
 
 
 __all__ = ["DEFAULT_KEEP_BYTES", "flp_bwd", "flp_fwd", "fused_linear_log_probs"]

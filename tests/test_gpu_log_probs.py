@@ -373,3 +373,12 @@ def test_a_preference_step_of_a_packed_model():
     warm = model(**inputs, labels=labels, return_log_probs=True, temperature=2.0).log_probs
     assert not torch.equal(warm, lone)
     assert model(**inputs, labels=labels).loss is not None
+
+
+def test_what_the_forward_kept_is_checked():
+    h, w, y, up = (t.to(DEV) for t in make(40, 64, 1000, seed=1))
+    saved = LP.flp_fwd(h, w, y, keep=True)[3]
+    for other, text in ((saved.cpu(), "saved must live on"), (saved.view(torch.int32), "what the forward kept"),
+                        (saved[:-64], "saved")):
+        with pytest.raises(ValueError, match=text):
+            LP.flp_bwd(h, w, y, up, saved=other)

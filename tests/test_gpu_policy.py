@@ -1,6 +1,8 @@
 """Preference and policy losses on the GPU against the oracle in 64 bits: lengths from none to long, masks that leave
 nothing, values that must not matter, borders, aggregations, and the ways they are called."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -362,3 +364,61 @@ def test_a_second_derivative_is_refused():
     for loss in (P.preference_loss(pi_t, old_t, cu_t).loss, P.policy_loss(pi_t, old_t, torch.ones(2, device=DEV), cu_t).loss):
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(loss, [pi_t], create_graph=True)
+
+
+def test_what_is_reported_beside_the_loss_carries_no_graph():
+    cu, mask, pi, old, ref = batch([40, 60], seed=3)
+    pi_t, old_t, ref_t, mask_t, cu_t = gpu(pi, old, ref, mask, cu)
+    pi_t.requires_grad_()
+    pair = P.preference_loss(pi_t, ref_t, cu_t, mask=mask_t)
+    out = P.policy_loss(pi_t, old_t, torch.ones(2, device=DEV), cu_t, mask=mask_t)
+    assert [t.requires_grad for t in pair] == [True, False, False]
+    assert [t.requires_grad for t in out] == [True, False, False]
+    with torch.no_grad():
+        assert not P.preference_loss(pi_t, ref_t, cu_t, mask=mask_t).loss.requires_grad
+
+
+def test_saved_tensors_go_through_their_hooks():
+    cu, mask, pi, old, ref = batch([40, 2500, 60, 7], seed=5)
+    pi_t, old_t, ref_t, mask_t, cu_t = gpu(pi, old, ref, mask, cu)
+    pi_t.requires_grad_()
+
+    def losses():
+        return [P.preference_loss(pi_t, ref_t, cu_t, mask=mask_t).loss, P.preference_loss(pi_t, None, cu_t).loss,
+                P.policy_loss(pi_t, old_t, torch.ones(4, device=DEV), cu_t, aggregation="sequence").loss,
+                P.policy_loss(pi_t, old_t, pi_t.detach()).loss]
+
+    want = [torch.autograd.grad(loss, [pi_t])[0] for loss in losses()]
+    with torch.autograd.graph.save_on_cpu():
+        kept = losses()
+    for loss, grad in zip(kept, want):
+        assert torch.equal(torch.autograd.grad(loss, [pi_t])[0], grad)
+
+
+def test_two_threads_on_streams_of_their_own():
+    data = [batch([500 + 40 * i, 2100, 0, 900], seed=20 + i) for i in range(2)]
+    torch.cuda.synchronize()
+
+    def step(cu, mask, lp, old, ref):
+        lp_t, old_t, ref_t, mask_t, cu_t = gpu(lp, old, ref, mask, cu)
+        lp_t.requires_grad_()
+        out = P.policy_loss(lp_t, old_t, torch.ones(4, device=DEV), cu_t, mask=mask_t, reference_logps=ref_t, kl_coef=0.1)
+        pair = P.preference_loss(lp_t, ref_t, cu_t, mask=mask_t)
+        return [t.cpu() for t in (out.loss.detach(), pair.loss.detach(),
+                                  *torch.autograd.grad([out.loss, pair.loss], [lp_t]))]
+
+    want, got = [step(*d) for d in data], [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(step(*data[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 20
+        assert all(torch.equal(a, b) for step in got[i] for a, b in zip(step, want[i]))

@@ -120,3 +120,25 @@ def test_python_refusals():
         P.policy_loss(lp, lp, lp, kl_type="k4")
     with pytest.raises(ValueError, match="GPU"):
         P.policy_loss(lp, lp, lp)
+
+
+def test_missing_extension_fails_loudly(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_NATIVE", None)
+    monkeypatch.setattr(_lib._build, "NATIVE_PATH", tmp_path / "absent.so")
+    with pytest.raises(RuntimeError, match="build"):
+        _lib.native()
+
+
+def test_the_extension_calls_entries_of_the_library():
+    native = _lib.native()
+    assert set(native.entries()) <= set(_lib.EXPORTED)
+    with pytest.raises(IndexError):  # refused at the first entry without an address: what is bound stays
+        native.bind({})
+
+
+def test_errors_come_from_the_extension_as_python_errors():
+    x = torch.zeros(3, 4)
+    with pytest.raises(ValueError, match="policy_logps must be float32, got torch.float16"):
+        P.preference_loss(x.half(), None, x)
+    with pytest.raises(TypeError):
+        P.policy_loss(x, None, x)
