@@ -396,7 +396,14 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       m[u] = p.spart[at] < 0.f ? m[u] : rf;
     }
 #pragma unroll
-    for (int u = 0; u < kRowSeg / NWR; ++u) sh.r.fac[w + NWR * u][lane] = exp2f_fast(m[u] - lse2) * gm;
+    for (int u = 0; u < kRowSeg / NWR; ++u) {
+      // (a label of next to no probability: the factor of a tile relative to it may leave fp32's range where its
+      // products with E, up to kRefLimit, do not: 2^100 times it then, marked by its sign)
+      const float d = m[u] - lse2;
+      const bool far = p.label_apart && d < -100.f;
+      const float k = exp2f_fast(far ? d + 100.f : d) * gm;
+      sh.r.fac[w + NWR * u][lane] = far ? -k : k;
+    }
     __syncthreads();
     const int64_t c0 = tb * (kVT / 8);
     const int ne = (int)(min(p.V / 8, (tb + nt) * (kVT / 8)) - c0);
@@ -413,9 +420,9 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
         for (int u = 0; u < UE; ++u) {
           const int c = cc + CT * u;
           if (c >= ne) break;
-          const float k = sh.r.fac[c / (kVT / 8)][r];
+          const float f = sh.r.fac[c / (kVT / 8)][r], k = fabsf(f), far = f < 0.f ? 0x1p-100f : 1.f;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) x[u][q] = c == ych && q == yq ? (bf16)0.f : (bf16)((float)x[u][q] * k);
+          for (int q = 0; q < 8; ++q) x[u][q] = c == ych && q == yq ? (bf16)0.f : (bf16)((float)x[u][q] * k * far);
           st_bf16x8(e + 8 * c, x[u]);
         }
       }

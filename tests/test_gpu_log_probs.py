@@ -382,3 +382,16 @@ def test_what_the_forward_kept_is_checked():
                         (saved[:-64], "saved")):
         with pytest.raises(ValueError, match=text):
             LP.flp_bwd(h, w, y, up, saved=other)
+
+
+@pytest.mark.parametrize("n", [50, 300])
+@pytest.mark.parametrize("keep", [True, False])
+def test_a_label_of_no_probability_beside_columns_of_little(n, keep):
+    """The label 2^-135 of the row's largest column, another tile 2^-83: its columns' gradient is small and not zero."""
+    h, w = torch.zeros(n, 64), torch.zeros(1024, 64)
+    h[:, 0], w[300:400, 0], w[600:640, 0] = 1.0, 36.0, 90.0
+    h[:, 1], w[:, 1] = torch.randn(n, generator=torch.Generator().manual_seed(n)), 0.25
+    y = torch.arange(n) % 256
+    up = 0.5 + torch.rand(n, generator=torch.Generator().manual_seed(1))
+    _, _, dw = check(h.to(torch.bfloat16), w.to(torch.bfloat16), y, up, 1.0, keep, rounds=2.0)
+    assert bool((dw[300:400, 0] < 0).all())
