@@ -239,6 +239,7 @@ struct RowArgs {
   uint64_t* keys;        // [nsort, kIdChunk] rows sorted by label
   int32_t* slot;         // [V] cleared
   int64_t nc, nvt, V, hdim, c0, ldp;
+  int vlog;              // log2 of the eight-column groups of a tile
   int nsort;             // sorting workgroups (0 without dW)
   int parts;             // workgroups per 64 rows
   int grads;             // 0: loss only (E was never stored)
@@ -405,8 +406,8 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       sh.r.fac[w + NWR * u][lane] = far ? -k : k;
     }
     __syncthreads();
-    const int64_t c0 = tb * (kVT / 8);
-    const int ne = (int)(min(p.V / 8, (tb + nt) * (kVT / 8)) - c0);
+    const int64_t c0 = tb << p.vlog;
+    const int ne = (int)(min(p.V / 8, (tb + nt) << p.vlog) - c0);
     for (int i = tid / CT; i < sh.r.n; i += kRowThreads / CT) {
       const int r = sh.r.list[i];
       const int64_t y = p.y[r0 + r] - 8 * c0;
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
         for (int u = 0; u < UE; ++u) {
           const int c = cc + CT * u;
           if (c >= ne) break;
-          const float f = sh.r.fac[c / (kVT / 8)][r], k = fabsf(f), far = f < 0.f ? 0x1p-100f : 1.f;
+          const float f = sh.r.fac[c >> p.vlog][r], k = fabsf(f), far = f < 0.f ? 0x1p-100f : 1.f;
 #pragma unroll
           for (int q = 0; q < 8; ++q) x[u][q] = c == ych && q == yq ? (bf16)0.f : (bf16)((float)x[u][q] * k * far);
           st_bf16x8(e + 8 * c, x[u]);
@@ -1188,8 +1189,9 @@ __global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs
 // tokens) read the whole weight for little arithmetic: 32 NB columns of a tile
 // are rows of the call, where the general kernels' tiles have 256 of which most
 // would be padding.  Smaller stages let two workgroups share a CU, so loads are
-// in flight while the other one waits at a barrier.  k-steps of 64 in two
-// buffers: the next one is loading while this one is multiplied.
+// in flight while the other one waits at a barrier, and the last round of tiles,
+// which leaves CUs idle, is short.
+constexpr int kFewBI = 128, kFewThreads = 256;  // weight rows or features of a tile; threads of its workgroup
 
 // One k-step's loads of an operand with k contiguous: ROWS rows x 64 k (swizzled
 // as gemm.h's KC halves), 8 rows an instruction, dealt over NWV waves.
@@ -1210,23 +1212,66 @@ struct FewRows {
   }
 };
 
+// The k-steps s of n of a few-rows product through STAGES buffers: issue(s, b)
+// asks for step s into buffer b (PER loads a wave), step(s, b) multiplies it.
+// With three buffers two steps are loading at any time, and one barrier a step
+// does: behind it every wave has read the buffer that the next loads go to.
+template <int STAGES, int PER, class I, class C>
+__device__ __forceinline__ void few_steps(int n, I issue, C step) {
+  static_assert(STAGES == 2 || STAGES == 3, "two or three buffers");
+  if (n <= 0) return;
+  issue(0, 0);
+  if constexpr (STAGES == 2) {
+    for (int s = 0; s < n; ++s) {
+      if (s + 1 < n) {
+        issue(s + 1, (s + 1) & 1);
+        wait_vmcnt<PER>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      phase_barrier();
+      step(s, s & 1);
+      wait_lds();
+      phase_barrier();
+    }
+  } else {
+    if (n > 1) issue(1, 1);
+    int b = 0;
+    for (int s = 0; s < n; ++s) {
+      if (s + 1 < n)
+        wait_vmcnt<PER>();
+      else
+        wait_vmcnt<0>();
+      phase_barrier();
+      if (s + 2 < n) issue(s + 2, b == 0 ? 2 : b - 1);
+      step(s, b);
+      wait_lds();
+      b = b == 2 ? 0 : b + 1;
+    }
+    phase_barrier();
+  }
+}
+
 // Rows of a call (NB = 2: 64) that take these kernels.  Forward and dH with a
-// frozen head over 151936 columns of 896: 48 rows 65 and 50 us, 128 rows 87 and
-// 69 us, 129 rows (the general kernels, which take as long for fewer) 101 and 99.
+// frozen head over 151936 columns of 896: 48 rows 61 and 51 us, 128 rows 86 and
+// 69 us, 129 rows (the general kernels, which take as long for fewer) 112 and 102.
 constexpr int kFewRows = 128;
 
-// The logits kernel over 256 vocabulary rows x 32 NB rows of the call: eight
+// The logits kernel over 128 vocabulary rows x 32 NB rows of the call: four
 // waves, 32 vocabulary rows each.  Same outputs; always with the label apart.
+// Bound by reading the weight: 48 rows over 151936 x 896 44.6 us, 6.1 TB/s; 52.6
+// with tiles of 256 rows in two buffers, whose last 82 tiles ran by themselves.
+// (128 rows of the call: two buffers, for two workgroups a CU; 60 us.)
 template <int NB>
-__global__ __launch_bounds__(NT) void flce_logits_few_kernel(const LogitsArgs p) {
-  constexpr int TOK = 32 * NB, STAGE = (BI + TOK) * BK, NWV = NT / 64;
-  __shared__ __align__(16) bf16 smem[2 * STAGE];
-  const int64_t i0 = (int64_t)blockIdx.x * BI;
+__global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const LogitsArgs p) {
+  constexpr int TOK = 32 * NB, STAGE = (kFewBI + TOK) * BK, NWV = kFewThreads / 64, STAGES = NB <= 2 ? 3 : 2;
+  __shared__ __align__(16) bf16 smem[STAGES * STAGE];
+  const int64_t i0 = (int64_t)blockIdx.x * kFewBI;
   if (*p.nvalid <= p.c0) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
   const int64_t vbase = i0 + 32 * w + 8 * h;  // accumulator r: vocabulary row vbase + 16 (r / 8) + r % 8
-  FewRows<BI, NWV> la;
+  FewRows<kFewBI, NWV> la;
   FewRows<TOK, NWV> lb;
   la.init(p.W.ld, p.V - 1 - i0, lane, w);
   lb.init(p.H.ld, p.nc - 1, lane, w);
@@ -1238,13 +1283,6 @@ __global__ __launch_bounds__(NT) void flce_logits_few_kernel(const LogitsArgs p)
   f32x16 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = zero16();
-  const int n = (int)(p.W.cols / BK);
-  auto issue = [&](int s) {
-    bf16* st = smem + (s & 1) * STAGE;
-    lb.issue(hb + (int64_t)s * BK, st + BI * BK, wu);
-    la.issue(wb + (int64_t)s * BK, st, wu);
-  };
-  issue(0);
   float ref[NB];
   int rel[NB];  // the token's label, counted from vbase (-1: not in this wave's rows)
 #pragma unroll
@@ -1254,27 +1292,25 @@ __global__ __launch_bounds__(NT) void flce_logits_few_kernel(const LogitsArgs p)
     const int64_t d = p.y[tok] - vbase;
     rel[b] = d >= 0 && d < 32 && (d & 8) == 0 ? (int)d : -1;
   }
-  for (int s = 0; s < n; ++s) {
-    if (s + 1 < n) {
-      issue(s + 1);
-      wait_vmcnt<FewRows<BI, NWV>::PER + FewRows<TOK, NWV>::PER>();
-    } else {
-      wait_vmcnt<0>();
-    }
-    phase_barrier();
-    const bf16 *A = smem + (s & 1) * STAGE, *B = A + BI * BK;
+  few_steps<STAGES, la.PER + lb.PER>(
+      (int)(p.W.cols / BK),
+      [&](int s, int buf) {
+        bf16* st = smem + buf * STAGE;
+        lb.issue(hb + (int64_t)s * BK, st + kFewBI * BK, wu);
+        la.issue(wb + (int64_t)s * BK, st, wu);
+      },
+      [&](int, int buf) {
+        const bf16 *A = smem + buf * STAGE, *B = A + kFewBI * BK;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const bf16x8 a = ra.read(A, 0, ks);
+        for (int ks = 0; ks < 4; ++ks) {
+          const bf16x8 a = ra.read(A, 0, ks);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, rb.read(B, b, ks), acc[b]);
-    }
-    wait_lds();
-    phase_barrier();
-  }
+          for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, rb.read(B, b, ks), acc[b]);
+        }
+      });
   // (in the stages' place: two workgroups share a CU's LDS)
   float *red = reinterpret_cast<float*>(smem), *tot = red + NWV * TOK, *top = tot + TOK;  // [NWV][TOK], [TOK], [TOK]
-  if (i0 + BI > p.V) {
+  if (i0 + kFewBI > p.V) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1363,8 +1399,9 @@ __global__ __launch_bounds__(NT) void flce_logits_few_kernel(const LogitsArgs p)
 // dH of few rows: 128 hidden features x 32 NB rows of the call x a range of the
 // vocabulary a workgroup, four waves of 32 features.  About 512 workgroups (two
 // a CU); block b runs on XCD b % 8, and the tiles of one range, which share its
-// columns of E, follow one another there.
-constexpr int kFewBI = 128, kFewThreads = 256, kFewPerXcd = 64;
+// columns of E, follow one another there.  Bound by reading the weight: 48 rows
+// over 151936 x 896 45.4 us, 6.0 TB/s; three buffers take as long as two.
+constexpr int kFewPerXcd = 64;
 int few_splits(int64_t hdim, int64_t V) {
   const int64_t nI = (hdim + kFewBI - 1) / kFewBI, steps = (V + BK - 1) / BK;
   return (int)(kXcds * std::min(std::max<int64_t>(kFewPerXcd / nI, 1), (steps + kXcds - 1) / kXcds));
@@ -1400,8 +1437,8 @@ __global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = zero16();
   const int n = (int)((ke - kb + BK - 1) / BK);
-  auto issue = [&](int s) {
-    bf16* st = smem + (s & 1) * STAGE;
+  auto issue = [&](int s, int buf) {
+    bf16* st = smem + buf * STAGE;
     const int64_t k0 = kb + (int64_t)s * BK;
     const int kval = (int)min(ke - k0, (int64_t)BK);
     // past the last row of the weight and the last columns of E: valid ones again (E's are zeroed below)
@@ -1415,16 +1452,8 @@ __global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p
       dma16(eb, lb.off[q] - 2 * (uint32_t)max(0, c - (kval - 8)), st + kFewBI * BK + (lb.PER * wu + q) * 512);
     }
   };
-  if (n > 0) issue(0);
-  for (int s = 0; s < n; ++s) {
-    if (s + 1 < n) {
-      issue(s + 1);
-      wait_vmcnt<QA + FewRows<TOK, NWV>::PER>();
-    } else {
-      wait_vmcnt<0>();
-    }
-    phase_barrier();
-    bf16 *A = smem + (s & 1) * STAGE, *B = A + kFewBI * BK;
+  few_steps<2, QA + lb.PER>(n, issue, [&](int s, int buf) {
+    bf16 *A = smem + buf * STAGE, *B = A + kFewBI * BK;
     const int kval = (int)min(ke - kb - (int64_t)s * BK, (int64_t)BK);
     if (kval < BK) {
       for (int i = tid; i < TOK * 8; i += kFewThreads) {
@@ -1439,9 +1468,7 @@ __global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p
 #pragma unroll
       for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, rb.read(B, b, ks), acc[b]);
     }
-    wait_lds();
-    phase_barrier();
-  }
+  });
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
@@ -1723,6 +1750,8 @@ __global__ __launch_bounds__(256) void flce_few_rows_kernel(const bf16* __restri
 }
 
 // ---------------------------------------------------------------- launches
+int tile_log(int columns) { return __builtin_ctz((unsigned)columns / 8); }
+
 unsigned row_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, 4096); }
 
 void launch_logits(LogitsArgs& lg, hipStream_t stream) {
@@ -1749,11 +1778,11 @@ void launch_dh(DhArgs& dh, hipStream_t stream) {
 }
 
 void launch_logits_few(LogitsArgs& lg, hipStream_t stream) {
-  const dim3 grid((unsigned)((lg.V + kVT - 1) / kVT));
+  const dim3 grid((unsigned)((lg.V + kFewBI - 1) / kFewBI));
   if (lg.nc <= 64)
-    hipLaunchKernelGGL(flce_logits_few_kernel<2>, grid, dim3(NT), 0, stream, lg);
+    hipLaunchKernelGGL(flce_logits_few_kernel<2>, grid, dim3(kFewThreads), 0, stream, lg);
   else
-    hipLaunchKernelGGL(flce_logits_few_kernel<4>, grid, dim3(NT), 0, stream, lg);
+    hipLaunchKernelGGL(flce_logits_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, lg);
 }
 
 void launch_dh_few(FewSumArgs& a, hipStream_t stream) {
@@ -1874,6 +1903,7 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     rw.c0 = c0;
     rw.nc = nc;
     rw.nvt = L.nvt;
+    rw.vlog = tile_log(kVT);
     rw.V = V;
     rw.hdim = Hd;
     rw.ldp = L.chunk;
@@ -1973,7 +2003,7 @@ FlpSaved flp_saved(int64_t n, int64_t V) {
 struct FlpLayout {
   size_t scal, spart, mpart, zy, ref, hc, saved, part, f, wt, acc32, keys, slot, next, lsum, total;
   int64_t chunk, nchunks, nvt;
-  int splits, prow, run, nsort;
+  int splits, prow, run, nsort, vt;
   bool few;
 };
 // logits: the logits product and its row pass run (not: E comes from the
@@ -1983,7 +2013,9 @@ FlpLayout flp_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool log
   FlpLayout L{};
   L.chunk = std::max<int64_t>(std::min(chunk, n), 1);
   L.nchunks = (n + L.chunk - 1) / L.chunk;
-  L.nvt = (V + kVT - 1) / kVT;
+  L.few = L.chunk <= kFewRows;
+  L.vt = L.few ? kFewBI : kVT;
+  L.nvt = (V + L.vt - 1) / L.vt;
   const size_t npad = (size_t)((std::max<int64_t>(n, 1) + 255) / 256 * 256);
   size_t off = 256;  // scal: an unused divisor, the count and the bad labels of a backward
   auto take = [&](bool on, size_t bytes) {
@@ -1998,7 +2030,6 @@ FlpLayout flp_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool log
   L.hc = take(logits || need_dw, sizeof(bf16) * npad * (size_t)hdim);
   // a state of its own, with one chunk's E (the backward's) or none (a forward that keeps nothing)
   L.saved = take(!have_saved, flp_saved(n, 0).total + (grads ? sizeof(bf16) * (size_t)(L.chunk * V) : 0));
-  L.few = L.chunk <= kFewRows;
   L.splits = L.few ? few_splits(hdim, V) : dh_splits(hdim, L.chunk);
   L.prow = (int)std::min<int64_t>(L.chunk, BJ);
   L.run = dh_run(V);
@@ -2087,6 +2118,7 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   rw.c0 = c0;
   rw.nc = nc;
   rw.nvt = L.nvt;
+  rw.vlog = tile_log(L.vt);
   rw.V = a.vocab;
   rw.hdim = a.hdim;
   rw.ldp = L.chunk;
