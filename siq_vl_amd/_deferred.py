@@ -6,7 +6,8 @@ count at once would synchronise the host with the GPU on every call, so each
 call copies its counts to pinned host memory without blocking, records an
 event, and the counts are judged once the copy has landed: at the operator's
 next call, or when the caller asks (``check(block=True)``, e.g. at the end
-of a training or evaluation loop).  Inside HIP graph capture neither the copy
+of a training or evaluation loop).  An operator may also write them there itself
+(``landing`` and ``landed_on``): a copy takes 8 us of the stream.  Inside HIP graph capture neither the copy
 nor an event query of earlier work is allowed, so captured calls are not
 tracked.
 """
@@ -40,6 +41,23 @@ class DeferredChecks:
         ev.record(stream)
         with self._lock:
             self._pending.append((ev, (counts.device, stream.cuda_stream), host, judge))
+
+    def landing(self, n: int) -> torch.Tensor | None:
+        """Pinned memory for ``n`` counts of a call that writes them by itself
+        (None while a graph is captured); ``landed_on`` follows the call."""
+        return None if torch.cuda.is_current_stream_capturing() else torch.empty(n, dtype=torch.int64, pin_memory=True)
+
+    def landed_on(self, device: torch.device, host: torch.Tensor, judge: Callable[[list], None]) -> None:
+        """Tracks the counts that the work now on ``device``'s current stream
+        leaves in ``host``, which is held until it has."""
+        ev = torch.cuda.Event()
+        stream = torch.cuda.current_stream(device)
+        ev.record(stream)
+        try:
+            self.check()
+        finally:
+            with self._lock:
+                self._pending.append((ev, (device, stream.cuda_stream), host, judge))
 
     def check(self, block: bool = False) -> None:
         """Judges every tracked call whose counts have landed (all of them when

@@ -168,11 +168,17 @@ def _track_bad(bad: torch.Tensor, vocab: int, ignore_index: int, validate) -> No
             _raise_bad(nbad, vocab, ignore_index)
         return
 
-    def judge(vals):
-        if vals[0] > 0:
-            _raise_bad(int(vals[0]), vocab, ignore_index)
+    _LABEL_CHECKS.add(bad, _judge(vocab, ignore_index))
 
-    _LABEL_CHECKS.add(bad, judge)
+
+def _judge(vocab: int, ignore_index: int):
+    """Raises LabelError for counts whose last is that of bad labels."""
+
+    def judge(vals):
+        if vals[-1] > 0:
+            _raise_bad(int(vals[-1]), vocab, ignore_index)
+
+    return judge
 
 
 def _keeps_graph() -> bool:

@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .cross_entropy import IGNORE_INDEX, _track_bad, default_chunk_tokens
+from .cross_entropy import _LABEL_CHECKS, IGNORE_INDEX, _judge, _track_bad, default_chunk_tokens
 
 # What the forward may keep for its backward: rows x vocab bf16.  The head's
 # backward is a step's first, so this is held beside all other activations, but
@@ -69,9 +69,13 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
     if chunk_tokens is None:
         chunk_tokens = default_chunk_tokens(w.shape[0])
     ignore_index = int(ignore_index)
+    host = _LABEL_CHECKS.landing(2) if h.is_cuda and validate not in (None, False, "sync") else None
     logp, counts = _lib.native().linear_log_probs(h, w, labels, ignore_index, float(temperature), int(chunk_tokens),
-                                                  int(keep_bytes))
-    _track_bad(counts[1], w.shape[0], ignore_index, validate)
+                                                  int(keep_bytes), host)
+    if host is not None:
+        _LABEL_CHECKS.landed_on(h.device, host, _judge(w.shape[0], ignore_index))
+    else:
+        _track_bad(counts[1], w.shape[0], ignore_index, validate)
     return logp
 
 

@@ -436,22 +436,21 @@ void check_head(const Tensor& hidden, const Tensor& weight, const Tensor& labels
   on_device(labels, "labels", hidden);
 }
 
-// (logp of that shape, [count, bad labels] int64, what is kept or undefined)
-std::tuple<Tensor, Tensor, Tensor> flp_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels,
-                                           int64_t ignore_index, double temperature, bool keep, at::IntArrayRef shape) {
+// (logp of that shape, what is kept or undefined); counts: the valid and the bad labels
+std::pair<Tensor, Tensor> flp_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels, int64_t ignore_index,
+                                  double temperature, bool keep, at::IntArrayRef shape, int64_t* counts) {
   check_head(hidden, weight, labels);
   const c10::DeviceGuard guard(hidden.device());
   const Tensor h = hidden.contiguous(), w = weight.contiguous(), y = labels.contiguous();
   const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0);
-  const Tensor logp = floats(shape, h), counts = at::empty({2}, y.options());
+  const Tensor logp = floats(shape, h);
   const Tensor saved = keep ? bytes(api.siq_flp_saved_bytes(n, vocab), h) : Tensor();
   const Tensor ws = bytes(api.siq_flp_fwd_workspace_bytes(n, hdim, vocab, keep), h);
-  int64_t* const c = counts.data_ptr<int64_t>();
   check(api.siq_flp_fwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), n, hdim, vocab, ignore_index,
-                        temperature, fptr(logp), c, c + 1, ptr(saved), keep ? saved.numel() : 0, ptr(ws), ws.numel(),
+                        temperature, fptr(logp), counts, counts + 1, ptr(saved), keep ? saved.numel() : 0, ptr(ws), ws.numel(),
                         stream_of(h)),
         "siq_flp_fwd");
-  return {logp, counts, saved};
+  return {logp, saved};
 }
 
 std::pair<Tensor, Tensor> flp_bwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const Tensor& dlogp,
@@ -485,22 +484,21 @@ Tensor rows_2d(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.siz
 Tensor rows_1d(const Tensor& t) { return t.dim() == 1 ? t : t.reshape({-1}); }
 
 struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
-                               int64_t ignore_index, double temperature, int64_t chunk, int64_t keep_bytes) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
+                        int64_t ignore_index, double temperature, int64_t chunk, int64_t keep_bytes, int64_t* counts) {
     const Tensor h = rows_2d(hidden), y = rows_1d(labels);
     const bool keep = weight.dim() == 2 && (int64_t)api.siq_flp_saved_bytes(h.size(0), weight.size(0)) <= keep_bytes;
-    auto [logp, counts, saved] = flp_fwd(h, weight, y, ignore_index, temperature, keep, labels.sizes());
+    auto [logp, saved] = flp_fwd(h, weight, y, ignore_index, temperature, keep, labels.sizes(), counts);
     ctx->save_for_backward({hidden, weight, labels, saved});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["chunk"] = chunk;
-    ctx->mark_non_differentiable({counts});
     ctx->set_materialize_grads(false);
-    return {logp, counts};
+    return logp;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     no_second_derivative("fused_linear_log_probs");
-    variable_list out(7);
+    variable_list out(8);
     if (!grads[0].defined()) return out;
     const variable_list s = ctx->get_saved_variables();
     auto [dh, dw] = flp_bwd(rows_2d(s[0]), s[1], rows_1d(s[2]), rows_1d(grads[0]), ctx->saved_data["ignore"].toInt(),
@@ -512,23 +510,28 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
   }
 };
 
-// (logp, [count, bad labels]); nothing is kept where no gradient can flow.
+// (logp, [count, bad labels]); nothing is kept where no gradient can flow.  `host`: pinned memory that the kernel
+// writes the counts to, so that no copy follows it; the caller keeps it until the call has run.
 std::pair<Tensor, Tensor> linear_log_probs(const Tensor& hidden, const Tensor& weight, const Tensor& labels,
-                                           int64_t ignore_index, double temperature, int64_t chunk, int64_t keep_bytes) {
+                                           int64_t ignore_index, double temperature, int64_t chunk, int64_t keep_bytes,
+                                           const optional<Tensor>& host) {
   TORCH_CHECK_VALUE(chunk > 0, "chunk_tokens must be positive");
-  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
-    const variable_list o = LinearLogProbs::apply(hidden, weight, labels, ignore_index, temperature, chunk, keep_bytes);
-    return {o[0], o[1]};
-  }
-  auto [logp, counts, saved] =
-      flp_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, false, labels.sizes());
-  return {logp, counts};
+  const Tensor counts = host.has_value() ? *host : at::empty({2}, hidden.options().dtype(at::kLong));
+  int64_t* const c = counts.data_ptr<int64_t>();
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
+    return {LinearLogProbs::apply(hidden, weight, labels, ignore_index, temperature, chunk, keep_bytes, c), counts};
+  return {flp_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, false, labels.sizes(), c).first,
+          counts};
 }
 
 // The raw forms.
 std::tuple<Tensor, Tensor, Tensor> raw_flp_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels,
                                                int64_t ignore_index, double temperature, bool keep) {
-  return flp_fwd(hidden, weight, labels, ignore_index, temperature, keep, labels.sizes());
+  check_head(hidden, weight, labels);
+  const Tensor counts = at::empty({2}, labels.options());
+  auto [logp, saved] =
+      flp_fwd(hidden, weight, labels, ignore_index, temperature, keep, labels.sizes(), counts.data_ptr<int64_t>());
+  return {logp, counts, saved};
 }
 
 std::pair<Tensor, Tensor> raw_flp_bwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const Tensor& dlogp,

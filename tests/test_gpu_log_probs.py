@@ -395,3 +395,25 @@ def test_a_label_of_no_probability_beside_columns_of_little(n, keep):
     up = 0.5 + torch.rand(n, generator=torch.Generator().manual_seed(1))
     _, _, dw = check(h.to(torch.bfloat16), w.to(torch.bfloat16), y, up, 1.0, keep, rounds=2.0)
     assert bool((dw[300:400, 0] < 0).all())
+
+
+@pytest.mark.parametrize("n", [50, 300])
+def test_every_call_with_bad_labels_is_judged_once(n):
+    h, w, y, _ = (t.to(DEV) for t in make(n, 64, 1000, seed=2))
+    bad = y.clone()
+    bad[3] = 1000
+    C.check_pending_labels(block=True)
+    for _ in range(3):
+        LP.fused_linear_log_probs(h, w, y)
+    C.check_pending_labels(block=True)
+    LP.fused_linear_log_probs(h, w, bad)
+    torch.cuda.synchronize()
+    with pytest.raises(C.LabelError, match="1 label"):  # the first call's; the second is tracked all the same
+        LP.fused_linear_log_probs(h.clone().requires_grad_(), w, bad)
+    with pytest.raises(C.LabelError, match="1 label"):
+        C.check_pending_labels(block=True)
+    C.check_pending_labels(block=True)
+    LP.fused_linear_log_probs(h, w, bad, validate=False)
+    C.check_pending_labels(block=True)
+    with pytest.raises(C.LabelError):
+        LP.fused_linear_log_probs(h, w, bad, validate="sync")
