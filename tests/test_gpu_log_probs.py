@@ -417,3 +417,18 @@ def test_every_call_with_bad_labels_is_judged_once(n):
     C.check_pending_labels(block=True)
     with pytest.raises(C.LabelError):
         LP.fused_linear_log_probs(h, w, bad, validate="sync")
+
+
+def test_a_freed_graph_is_refused_and_a_kept_one_repeats():
+    h, w, y, up = (t.to(DEV) for t in make(40, 64, 1000, seed=4))
+    cu = torch.tensor([0, 25, 40], dtype=torch.int32, device=DEV)
+    old = torch.randn(40, device=DEV)
+    h.requires_grad_()
+    for last in (lambda lp: (lp * up).sum(), lambda lp: P.preference_loss(lp, old, cu).loss,
+                 lambda lp: P.policy_loss(lp, old, torch.ones(2, device=DEV), cu).loss):
+        loss = last(LP.fused_linear_log_probs(h, w, y))
+        first, = torch.autograd.grad(loss, [h], retain_graph=True)
+        again, = torch.autograd.grad(loss, [h])
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(loss, [h])
