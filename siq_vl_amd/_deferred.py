@@ -36,28 +36,39 @@ class DeferredChecks:
         self.check()
         host = torch.empty(counts.shape, dtype=counts.dtype, pin_memory=True)
         host.copy_(counts, non_blocking=True)
-        ev = torch.cuda.Event()
-        stream = torch.cuda.current_stream(counts.device)
-        ev.record(stream)
+        call = self._call(counts.device, host, judge)
         with self._lock:
-            self._pending.append((ev, (counts.device, stream.cuda_stream), host, judge))
+            self._pending.append(call)
 
     def landing(self, n: int) -> torch.Tensor | None:
         """Pinned memory for ``n`` counts of a call that writes them by itself
         (None while a graph is captured); ``landed_on`` follows the call."""
-        return None if torch.cuda.is_current_stream_capturing() else torch.empty(n, dtype=torch.int64, pin_memory=True)
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        return torch.empty(n, dtype=torch.int64, device="cpu", pin_memory=True)
 
     def landed_on(self, device: torch.device, host: torch.Tensor, judge: Callable[[list], None]) -> None:
         """Tracks the counts that the work now on ``device``'s current stream
         leaves in ``host``, which is held until it has."""
-        ev = torch.cuda.Event()
-        stream = torch.cuda.current_stream(device)
-        ev.record(stream)
+        call = self._call(device, host, judge)
         try:
             self.check()
         finally:
             with self._lock:
-                self._pending.append((ev, (device, stream.cuda_stream), host, judge))
+                self._pending.append(call)
+
+    def hold(self, device: torch.device, host: torch.Tensor) -> None:
+        """Keeps ``host`` as ``landed_on`` does, for a call that failed: it may
+        have been launched, and what it leaves there is not judged."""
+        with self._lock:
+            self._pending.append(self._call(device, host, lambda counts: None))
+
+    @staticmethod
+    def _call(device: torch.device, host: torch.Tensor, judge: Callable[[list], None]) -> tuple:
+        ev = torch.cuda.Event()
+        stream = torch.cuda.current_stream(device)
+        ev.record(stream)
+        return ev, (device, stream.cuda_stream), host, judge
 
     def check(self, block: bool = False) -> None:
         """Judges every tracked call whose counts have landed (all of them when

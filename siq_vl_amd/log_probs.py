@@ -70,8 +70,13 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
         chunk_tokens = default_chunk_tokens(w.shape[0])
     ignore_index = int(ignore_index)
     host = _LABEL_CHECKS.landing(2) if h.is_cuda and validate not in (None, False, "sync") else None
-    logp, counts = _lib.native().linear_log_probs(h, w, labels, ignore_index, float(temperature), int(chunk_tokens),
-                                                  int(keep_bytes), host)
+    try:
+        logp, counts = _lib.native().linear_log_probs(h, w, labels, ignore_index, float(temperature), int(chunk_tokens),
+                                                      int(keep_bytes), host)
+    except BaseException:  # (a checkpoint's recomputation ends in one, behind the launch)
+        if host is not None:
+            _LABEL_CHECKS.hold(h.device, host)
+        raise
     if host is not None:
         _LABEL_CHECKS.landed_on(h.device, host, _judge(w.shape[0], ignore_index))
     else:

@@ -169,8 +169,9 @@ Tensor rows_of(const Tensor& t) {
   const int64_t step = r.scalar_type() == at::kFloat ? 4 : 8;
   const bool in_place = r.is_contiguous() || (r.stride(1) == 1 && r.stride(0) >= r.size(1) && r.stride(0) % step == 0 &&
                                               r.size(1) % 8 == 0);
-  if (!in_place) return r.contiguous();
-  return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 ? r.contiguous().clone() : r;
+  const bool aligned = reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
+  if (in_place && aligned) return r;
+  return r.is_contiguous() ? r.clone() : r.contiguous();
 }
 int64_t ld_of(const Tensor& r) { return r.size(0) > 1 && !r.is_contiguous() ? r.stride(0) : r.size(1); }
 

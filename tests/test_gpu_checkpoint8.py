@@ -10,6 +10,8 @@ import torch
 
 from oracle import pack8 as op
 from siq_vl_amd import checkpoint8 as K
+from siq_vl_amd.log_probs import fused_linear_log_probs
+from siq_vl_amd.policy import policy_loss, preference_loss
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -342,3 +344,51 @@ def test_a_second_derivative_is_refused():
     for y in (K.swiglu8(g, g), K.swiglu8(g), K.swiglu8_linear(g, g, w)):
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(y.sum(), [g], create_graph=True)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("last", ["fused", "two", "linear", "log_probs", "preference", "policy"])
+def test_operators_inside_torchs_checkpoints(last, reentrant):
+    """The recomputation stops inside the last operator's saving of its tensors, and gradients are the direct ones."""
+    torch.manual_seed(3)
+    x = torch.randn(48, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(128, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    y = torch.randint(0, 128, (48,), device=DEV)
+    cu = torch.tensor([0, 20, 48], dtype=torch.int32, device=DEV)
+    old = torch.randn(48, device=DEV)
+
+    def run(x, w):
+        z = x @ w.T
+        if last == "fused":
+            return K.swiglu8(z)
+        if last == "two":
+            return K.swiglu8(z[:, :64], z[:, 64:])
+        if last == "linear":
+            return K.swiglu8_linear(z[:, :64], z[:, 64:], w)
+        logp = fused_linear_log_probs(x * 0.1, w, y)
+        if last == "log_probs":
+            return logp
+        if last == "preference":
+            return preference_loss(logp, old, cu).loss
+        return policy_loss(logp, old, torch.ones(2, device=DEV), cu).loss
+
+    direct = run(x, w)
+    up = torch.randn_like(direct)
+    want = torch.autograd.grad(direct, [x, w], up)
+    out = torch.utils.checkpoint.checkpoint(run, x, w, use_reentrant=reentrant)
+    assert torch.equal(out, direct)
+    out.backward(up)
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+
+
+def test_layers_and_mlps_together():
+    model = tiny_qwen2()
+    ids = torch.randint(0, 256, (2, 65), device=DEV)
+    _, grads0 = _loss_and_grads(model, ids)
+    assert K.enable_8bit_mlp(model) == 2 and K.enable_8bit_checkpoints(model) >= 2
+    model.zero_grad()
+    model(input_ids=ids, labels=ids, use_cache=False).loss.backward()
+    for n, p in model.named_parameters():
+        if p.requires_grad:
+            # both kinds of storage: twice the noise that either is held to
+            assert float((p.grad.double() - grads0[n]).norm() / grads0[n].norm()) <= 0.2, n

@@ -432,3 +432,25 @@ def test_a_freed_graph_is_refused_and_a_kept_one_repeats():
         assert torch.equal(first, again)
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(loss, [h])
+
+
+def test_a_call_that_fails_behind_its_launch_keeps_its_counts_memory(monkeypatch):
+    h, w, y, _ = (t.to(DEV) for t in make(40, 64, 1000, seed=6))
+    C.check_pending_labels(block=True)
+    native = LP._lib.native()
+    hosts = []
+
+    class Failing:
+        def linear_log_probs(self, *args):
+            hosts.append(args[-1])
+            native.linear_log_probs(*args)
+            raise KeyboardInterrupt
+
+    monkeypatch.setattr(LP._lib, "_NATIVE", Failing())
+    y[0] = 1000  # (a failed call's labels are not judged)
+    with pytest.raises(KeyboardInterrupt):
+        LP.fused_linear_log_probs(h, w, y)
+    held = [call[2] for call in C._LABEL_CHECKS._pending]
+    assert len(held) == 1 and held[0] is hosts[0] and held[0].is_pinned()
+    C.check_pending_labels(block=True)
+    assert len(C._LABEL_CHECKS) == 0 and hosts[0].tolist() == [int((y >= 0).sum()) - 1, 1]
