@@ -257,7 +257,12 @@ struct RowArgs {
 // tiles and its E one after the other: 512 x 1536 over 151936 columns 1.87 ->
 // 0.58 ms, 2048 x 896 2.48 -> 1.17 ms, 16384 x 1536 13.5 -> 10.6 ms; no row
 // redone: 0.52, 0.92 and 9.4 ms either way.
+//
+// ROWS: 64, or 16 for calls of few rows (label_apart alone), where one workgroup's
+// reads of all tile sums were what the pass took: SUB = 64 / ROWS lanes then share
+// a row, each with tiles of its own.  48 rows, 1187 tiles: 11.6 -> 6.8 us.
 constexpr int kRowThreads = 1024, kRowRows = 64, kRowGroups = 256, kRowSeg = 64;
+constexpr int kFewRowRows = 16;
 // One sorted run: the labels of rows [base, base + kIdChunk) below nv (1024 threads).
 __device__ __forceinline__ void sort_labels(uint64_t* sk, const int64_t* y, int64_t base, int64_t nv, uint64_t* keys) {
   const int len = (int)max((int64_t)0, min((int64_t)kIdChunk, nv - base));
@@ -269,17 +274,19 @@ __device__ __forceinline__ void sort_labels(uint64_t* sk, const int64_t* y, int6
   sort_keys(sk, np2);
   for (int i = threadIdx.x; i < kIdChunk; i += kRowThreads) keys[base + i] = i < np2 ? sk[i] : kNoKey;
 }
+template <int ROWS>
 __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) {
-  constexpr int NWR = kRowThreads / 64, U = 8;
+  constexpr int NWR = kRowThreads / 64, U = 8, SUB = 64 / ROWS, NT0 = NWR * SUB;  // tiles read at once
   __shared__ union {
     uint64_t sk[kIdChunk];
     struct {
-      float sum[NWR][kRowRows], mx[NWR][kRowRows], redone[NWR][kRowRows], f[kRowRows], lse[kRowRows];
-      int list[kRowRows], n;  // the rows with redone tiles
-      float fac[kRowSeg][kRowRows];
+      float sum[NWR][ROWS], mx[NWR][ROWS], redone[NWR][ROWS], f[ROWS], lse[ROWS];
+      int list[ROWS], n;  // the rows with redone tiles
+      float fac[kRowSeg][ROWS];
     } r;
   } sh;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & (ROWS - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int sub = (tid & 63) / ROWS, t1 = w * SUB + sub;  // this lane's first tile
   const int64_t nv = min(p.nc, *p.nvalid - p.c0);  // valid rows of the chunk
   if ((int)blockIdx.x < p.nsort) {
     sort_labels(sh.sk, p.y, (int64_t)blockIdx.x * kIdChunk, nv, p.keys);
@@ -290,45 +297,53 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
   if (p.nsort > 0)
     for (int64_t v = (int64_t)blk * kRowThreads + tid; v < p.V; v += (int64_t)groups * p.parts * kRowThreads)
       p.slot[v] = 0;
-  const int64_t r0 = (int64_t)(blk - part * groups) * kRowRows;
+  const int64_t r0 = (int64_t)(blk - part * groups) * ROWS;
   if (r0 >= nv) return;
   const int64_t row = min(r0 + lane, nv - 1);
   const float rf = p.ref[row];
   float sum = 0.f;  // of the tiles relative to ref
   bool redone = false;
-  for (int64_t t0 = w; t0 < p.nvt; t0 += NWR * U) {
+  for (int64_t t0 = t1; t0 < p.nvt; t0 += NT0 * U) {
     float s[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) s[u] = t0 + NWR * u < p.nvt ? p.spart[(t0 + NWR * u) * p.ldp + row] : 0.f;
+    for (int u = 0; u < U; ++u) s[u] = t0 + NT0 * u < p.nvt ? p.spart[(t0 + NT0 * u) * p.ldp + row] : 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       redone |= s[u] < 0.f;
       sum += s[u] < 0.f ? 0.f : s[u];  // (a NaN too)
     }
   }
+#pragma unroll
+  for (int o = ROWS; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
   sh.r.sum[w][lane] = sum;
   float top = rf;  // the reference of the sum
   if (__syncthreads_or(redone)) {
     // redone tiles: this wave's relative to their largest reference, then everything relative to the row's
     float mx = -INFINITY, s2 = 0.f;
-    for (int64_t t0 = w; t0 < p.nvt; t0 += NWR * U) {
+    for (int64_t t0 = t1; t0 < p.nvt; t0 += NT0 * U) {
       float s[U], m[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t at = min(t0 + NWR * u, p.nvt - 1) * p.ldp + row;
+        const int64_t at = min(t0 + NT0 * u, p.nvt - 1) * p.ldp + row;
         s[u] = p.spart[at];
         m[u] = p.mpart[at];
       }
       float top2 = mx;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        s[u] = t0 + NWR * u < p.nvt && s[u] < 0.f ? s[u] : 0.f;
+        s[u] = t0 + NT0 * u < p.nvt && s[u] < 0.f ? s[u] : 0.f;
         top2 = s[u] < 0.f ? fmaxf(top2, m[u]) : top2;
       }
       s2 = s2 > 0.f ? s2 * exp2f_fast(mx - top2) : 0.f;
       mx = top2;
 #pragma unroll
       for (int u = 0; u < U; ++u) s2 -= s[u] < 0.f ? s[u] * exp2f_fast(m[u] - mx) : 0.f;
+    }
+#pragma unroll
+    for (int o = ROWS; o < 64; o <<= 1) {
+      const float mo = __shfl_xor(mx, o), so = __shfl_xor(s2, o), both = fmaxf(mx, mo);
+      s2 = (s2 > 0.f ? s2 * exp2f_fast(mx - both) : 0.f) + (so > 0.f ? so * exp2f_fast(mo - both) : 0.f);
+      mx = both;
     }
     sh.r.mx[w][lane] = mx;
     sh.r.redone[w][lane] = s2;
@@ -346,7 +361,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       for (int i = 0; i < NWR; ++i)
         if (sh.r.redone[i][lane] > 0.f) sum += sh.r.redone[i][lane] * exp2f_fast(sh.r.mx[i][lane] - top);
     }
-    const bool mine = r0 + lane < nv && part == 0;
+    const bool mine = sub == 0 && r0 + lane < nv && part == 0;
     float lse2, w0, f0;  // log2 sum, (probability of the label) - 1, what E times it is a probability
     if (p.label_apart) {
       // `sum` is that of the other columns: with t its ratio to the label's term the label's probability is 1 / (1 + t),
@@ -375,9 +390,9 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       }
       sh.r.f[lane] = f;
       sh.r.lse[lane] = lse2;
-      const uint64_t m = __ballot(redone && r0 + lane < nv);
+      const uint64_t m = __ballot(sub == 0 && redone && r0 + lane < nv);
       if ((m >> lane) & 1) sh.r.list[__popcll(m & ((1ull << lane) - 1))] = lane;
-      if (lane == 0) sh.r.n = __popcll(m);
+      if (tid == 0) sh.r.n = __popcll(m);
     }
   }
   if (!p.grads) return;
@@ -389,21 +404,21 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
   const int64_t tper = (p.nvt + p.parts - 1) / p.parts, te = min(p.nvt, (part + 1) * tper);
   for (int64_t tb = part * tper; sh.r.n > 0 && tb < te; tb += kRowSeg) {
     const int nt = (int)min((int64_t)kRowSeg, te - tb);
-    float m[kRowSeg / NWR];
+    float m[kRowSeg / NT0];
 #pragma unroll
-    for (int u = 0; u < kRowSeg / NWR; ++u) {
-      const int64_t at = (tb + min(w + NWR * u, nt - 1)) * p.ldp + row;
+    for (int u = 0; u < kRowSeg / NT0; ++u) {
+      const int64_t at = (tb + min(t1 + NT0 * u, nt - 1)) * p.ldp + row;
       m[u] = p.mpart[at];
       m[u] = p.spart[at] < 0.f ? m[u] : rf;
     }
 #pragma unroll
-    for (int u = 0; u < kRowSeg / NWR; ++u) {
+    for (int u = 0; u < kRowSeg / NT0; ++u) {
       // (a label of next to no probability: the factor of a tile relative to it may leave fp32's range where its
       // products with E, up to kRefLimit, do not: 2^100 times it then, marked by its sign)
       const float d = m[u] - lse2;
       const bool far = p.label_apart && d < -100.f;
       const float k = exp2f_fast(far ? d + 100.f : d) * gm;
-      sh.r.fac[w + NWR * u][lane] = far ? -k : k;
+      sh.r.fac[t1 + NT0 * u][lane] = far ? -k : k;
     }
     __syncthreads();
     const int64_t c0 = tb << p.vlog;
@@ -431,7 +446,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
     __syncthreads();
   }
   if (p.nsort == 0) return;
-  const int rows = (int)min((int64_t)kRowRows, nv - r0), gpr = (int)(p.hdim / 8);
+  const int rows = (int)min((int64_t)ROWS, nv - r0), gpr = (int)(p.hdim / 8);
   for (int i = part * kRowThreads + tid; i < rows * gpr; i += p.parts * kRowThreads) {
     const float f = sh.r.f[i / gpr];
     bf16* hp = p.H + r0 * p.hdim + 8 * (int64_t)i;
@@ -1253,8 +1268,8 @@ __device__ __forceinline__ void few_steps(int n, I issue, C step) {
 }
 
 // Rows of a call (NB = 2: 64) that take these kernels.  Forward and dH with a
-// frozen head over 151936 columns of 896: 48 rows 61 and 51 us, 128 rows 86 and
-// 69 us, 129 rows (the general kernels, which take as long for fewer) 112 and 102.
+// frozen head over 151936 columns of 896: 48 rows 56 and 51 us, 128 rows 81 and
+// 70 us, 129 rows (the general kernels, which take as long for fewer) 113 and 103.
 constexpr int kFewRows = 128;
 
 // The logits kernel over 128 vocabulary rows x 32 NB rows of the call: four
@@ -1761,10 +1776,15 @@ void launch_logits(LogitsArgs& lg, hipStream_t stream) {
   hipLaunchKernelGGL(flce_logits_kernel, dim3(grid), dim3(NT), 0, stream, lg);
 }
 
-void launch_row(RowArgs& rw, hipStream_t stream) {
-  const int64_t groups = (rw.nc + kRowRows - 1) / kRowRows;
+void launch_row(RowArgs& rw, hipStream_t stream, bool few = false) {
+  const int rows = few ? kFewRowRows : kRowRows;
+  const int64_t groups = (rw.nc + rows - 1) / rows;
   rw.parts = rw.grads ? (int)std::max<int64_t>(kRowGroups / groups, 1) : 1;
-  hipLaunchKernelGGL(flce_row_kernel, dim3((unsigned)(rw.nsort + groups * rw.parts)), dim3(kRowThreads), 0, stream, rw);
+  const dim3 grid((unsigned)(rw.nsort + groups * rw.parts));
+  if (few)
+    hipLaunchKernelGGL(flce_row_kernel<kFewRowRows>, grid, dim3(kRowThreads), 0, stream, rw);
+  else
+    hipLaunchKernelGGL(flce_row_kernel<kRowRows>, grid, dim3(kRowThreads), 0, stream, rw);
 }
 
 void launch_dh(DhArgs& dh, hipStream_t stream) {
@@ -2124,7 +2144,7 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   rw.ldp = L.chunk;
   rw.grads = lg.store_e;
   rw.label_apart = 1;
-  launch_row(rw, stream);
+  launch_row(rw, stream, L.few);
 }
 
 }  // namespace
