@@ -259,8 +259,8 @@ int siq_flce_loss(const void* hidden, const void* weight, const int64_t* labels,
  * of them):
  *   logp[i] = z_iy - log sum_j exp(z_ij),  z = hidden weight^T / temperature,
  * fp32 [n]; 0 where the label is ignore_index or, counted in *bad_labels,
- * outside [0, vocab).  *count = rows that count.  Operands as for
- * siq_flce_fwd_bwd.
+ * outside [0, vocab).  *count = rows that count.  Both are only written, and may
+ * lie in pinned host memory.  Operands as for siq_flce_fwd_bwd.
  * siq_flp_bwd: with dlogp [n] the upstream gradients (those of rows that do not
  * count are not read),
  *   dhidden = dZ weight,  dweight = dZ^T hidden,

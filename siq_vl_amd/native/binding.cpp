@@ -464,8 +464,9 @@ std::pair<Tensor, Tensor> flp_bwd(const Tensor& hidden, const Tensor& weight, co
   on_device(dlogp, "dlogp", hidden);
   if (saved.defined()) {
     on_device(saved, "saved", hidden);
-    TORCH_CHECK_VALUE(saved.scalar_type() == at::kByte && saved.dim() == 1 && saved.is_contiguous(),
-                      "saved must be what the forward kept, got ", shape_name(saved), " ", type_name(saved));
+    const int64_t size = api.siq_flp_saved_bytes(n, vocab);
+    TORCH_CHECK_VALUE(saved.scalar_type() == at::kByte && saved.dim() == 1 && saved.numel() == size && saved.is_contiguous(),
+                      "saved must be what the forward kept (", size, " bytes), got ", shape_name(saved), " ", type_name(saved));
   }
   TORCH_CHECK_VALUE(chunk > 0, "chunk_tokens must be positive");
   const c10::DeviceGuard guard(hidden.device());

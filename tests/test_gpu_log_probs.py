@@ -454,3 +454,10 @@ def test_a_call_that_fails_behind_its_launch_keeps_its_counts_memory(monkeypatch
     assert len(held) == 1 and held[0] is hosts[0] and held[0].is_pinned()
     C.check_pending_labels(block=True)
     assert len(C._LABEL_CHECKS) == 0 and hosts[0].tolist() == [int((y >= 0).sum()) - 1, 1]
+
+
+def test_what_another_shape_kept_is_refused():
+    h, w, y, up = (t.to(DEV) for t in make(40, 64, 1000, seed=1))
+    more = LP.flp_fwd(h.repeat(2, 1), w, y.repeat(2), keep=True)[3]
+    with pytest.raises(ValueError, match="what the forward kept"):
+        LP.flp_bwd(h, w, y, up, saved=more)
