@@ -174,14 +174,16 @@ def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs
     if not torch.is_grad_enabled():
         return function(x, *args)
     packed, first, trained = pack8(x, format), [x], x.requires_grad
+    # torch keeps the random state of the GPUs that its arguments' tensors are on: an empty one stands for x there
+    there = x.new_empty(0)
     del x
 
-    def run(*rest):
+    def run(there, *rest):
         # the forward takes x from the list, so that nothing here keeps it
         value = first.pop() if first else unpack8(packed).requires_grad_(trained)
         return function(value, *rest)
 
-    return torch.utils.checkpoint.checkpoint(run, *args, use_reentrant=False, **kwargs)
+    return torch.utils.checkpoint.checkpoint(run, there, *args, use_reentrant=False, **kwargs)
 
 
 def _layer_checkpoint(format: str, function, *args):

@@ -392,3 +392,55 @@ def test_layers_and_mlps_together():
         if p.requires_grad:
             # both kinds of storage: twice the noise that either is held to
             assert float((p.grad.double() - grads0[n]).norm() / grads0[n].norm()) <= 0.2, n
+
+
+def test_checkpoint_draws_the_same_numbers_again_whatever_the_other_arguments():
+    """Dropout in a function of x alone, or of x and a CPU tensor: the recomputation takes the forward's mask, and the
+    backward leaves the generators as they were."""
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(96, 96, device=DEV, dtype=torch.bfloat16)
+    drop = torch.nn.Dropout(0.5)
+    x = torch.randn(33, 96, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(33, 96, device=DEV, dtype=torch.bfloat16)
+
+    def alone(t):
+        return drop(torch.tanh(lin(t))) + t
+
+    def with_cpu(t, s):
+        return drop(torch.tanh(lin(t))) * float(s) + t
+
+    for block, rest in ((alone, ()), (with_cpu, (torch.tensor(0.75),))):
+        torch.manual_seed(5)
+        y = K.checkpoint8(block, x, *rest)
+        states = torch.get_rng_state(), torch.cuda.get_rng_state()
+        got = torch.autograd.grad(y, [x, lin.weight], dy, retain_graph=True)
+        again = torch.autograd.grad(y, [x, lin.weight], dy)
+        assert torch.equal(torch.get_rng_state(), states[0]) and torch.equal(torch.cuda.get_rng_state(), states[1])
+        xq = K.unpack8(K.pack8(x)).requires_grad_()
+        torch.manual_seed(5)
+        want = torch.autograd.grad(block(xq, *rest), [xq, lin.weight], dy)
+        for a, b, c in zip(got, want, again):
+            assert torch.equal(a, b) and torch.equal(a, c)
+    # as in torch's own, the caller may give the numbers up
+    y = K.checkpoint8(alone, x, preserve_rng_state=False)
+    assert torch.autograd.grad(y, [x], dy)[0].shape == x.shape
+
+
+def test_layers_with_dropout_on_a_qwen2_model():
+    """Dropout behind every MLP: the same seed gives the gradients of the stock step but for what 8 bits cost."""
+    model = tiny_qwen2()
+    for layer in model.model.layers:
+        layer.mlp = torch.nn.Sequential(layer.mlp, torch.nn.Dropout(0.4))
+    ids = torch.randint(0, 256, (2, 65), device=DEV)
+    torch.manual_seed(7)
+    loss0, grads0 = _loss_and_grads(model, ids)
+    K.enable_8bit_checkpoints(model)
+    model.zero_grad()
+    torch.manual_seed(7)
+    loss = model(input_ids=ids, labels=ids, use_cache=False).loss
+    state = torch.cuda.get_rng_state()
+    loss.backward()
+    assert float(loss.detach()) == loss0 and torch.equal(torch.cuda.get_rng_state(), state)
+    for n, p in model.named_parameters():
+        # as without dropout (above); another mask in the recomputation is off by the gradient's own size
+        assert float((p.grad.double() - grads0[n]).norm() / grads0[n].norm()) <= 0.1, n
