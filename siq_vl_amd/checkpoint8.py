@@ -163,6 +163,19 @@ def enable_8bit_mlp(model: torch.nn.Module, format: str = "int8") -> int:
 
 
 # --------------------------------------------------------------------------- checkpoints of whole functions
+class _Unpacked(torch.autograd.Function):
+    """The unpacked input as no leaf (``source`` requires grad), so that the function may change it in place where it
+    may change the forward's.  Gradients flow through the forward's input, not through this one."""
+
+    @staticmethod
+    def forward(ctx, source, packed):
+        return unpack8(packed)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, None
+
+
 def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs):
     """``function(x, *args)``, run again in the backward as
     ``torch.utils.checkpoint.checkpoint(..., use_reentrant=False)`` does
@@ -180,7 +193,12 @@ def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs
 
     def run(there, *rest):
         # the forward takes x from the list, so that nothing here keeps it
-        value = first.pop() if first else unpack8(packed).requires_grad_(trained)
+        if first:
+            value = first.pop()
+        elif trained:
+            value = _Unpacked.apply(there.detach().requires_grad_(), packed)
+        else:
+            value = unpack8(packed)
         return function(value, *rest)
 
     return torch.utils.checkpoint.checkpoint(run, there, *args, use_reentrant=False, **kwargs)

@@ -444,3 +444,27 @@ def test_layers_with_dropout_on_a_qwen2_model():
     for n, p in model.named_parameters():
         # as without dropout (above); another mask in the recomputation is off by the gradient's own size
         assert float((p.grad.double() - grads0[n]).norm() / grads0[n].norm()) <= 0.1, n
+
+
+def test_checkpoint_of_a_function_that_changes_its_input():
+    """In place on an input that is no leaf: the forward allows it, and so does the recomputation."""
+    torch.manual_seed(2)
+    w, s = torch.randn(64, 64, device=DEV).requires_grad_(), torch.randn(64, device=DEV).requires_grad_()
+    leaf = torch.randn(40, 64, device=DEV).requires_grad_()
+    dy = torch.randn(40, 64, device=DEV)
+
+    def block(t):
+        t += s
+        t.mul_(0.5)
+        return torch.tanh(t @ w) + t
+
+    y = K.checkpoint8(block, leaf * 2)
+    got = torch.autograd.grad(y, [leaf, s, w], dy)
+    xq = K.unpack8(K.pack8(leaf.detach() * 2)).requires_grad_()
+    dx, ds, dw = torch.autograd.grad(block(xq * 1), [xq, s, w], dy)
+    assert torch.equal(got[0], 2 * dx) and torch.equal(got[1], ds) and torch.equal(got[2], dw)
+    x = leaf.detach().clone()  # nor is an input without gradient one that must not be changed
+    y = K.checkpoint8(block, x)
+    got = torch.autograd.grad(y, [s, w], dy)
+    want = torch.autograd.grad(block(K.unpack8(K.pack8(leaf.detach()))), [s, w], dy)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
