@@ -168,12 +168,18 @@ class _Unpacked(torch.autograd.Function):
     may change the forward's.  Gradients flow through the forward's input, not through this one."""
 
     @staticmethod
-    def forward(ctx, source, packed):
-        return unpack8(packed)
+    def forward(ctx, source, packed, strides):
+        return _unpacked(packed, strides)
 
     @staticmethod
     def backward(ctx, grad):
-        return None, None
+        return None, None, None
+
+
+def _unpacked(packed: Packed8, strides) -> torch.Tensor:
+    """``unpack8(packed)`` with its dimensions in the order of ``strides`` in memory (None: as they are)."""
+    x = unpack8(packed)
+    return x if strides is None else torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device).copy_(x)
 
 
 def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs):
@@ -187,6 +193,8 @@ def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs
     if not torch.is_grad_enabled():
         return function(x, *args)
     packed, first, trained = pack8(x, format), [x], x.requires_grad
+    # (a transposed input is recomputed as one: the function may view it as its strides allow)
+    strides = None if x.is_contiguous() else torch.empty_like(x, device="meta").stride()
     # torch keeps the random state of the GPUs that its arguments' tensors are on: an empty one stands for x there
     there = x.new_empty(0)
     del x
@@ -196,9 +204,9 @@ def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs
         if first:
             value = first.pop()
         elif trained:
-            value = _Unpacked.apply(there.detach().requires_grad_(), packed)
+            value = _Unpacked.apply(there.detach().requires_grad_(), packed, strides)
         else:
-            value = unpack8(packed)
+            value = _unpacked(packed, strides)
         return function(value, *rest)
 
     return torch.utils.checkpoint.checkpoint(run, there, *args, use_reentrant=False, **kwargs)

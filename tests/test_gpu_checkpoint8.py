@@ -468,3 +468,35 @@ def test_checkpoint_of_a_function_that_changes_its_input():
     got = torch.autograd.grad(y, [s, w], dy)
     want = torch.autograd.grad(block(K.unpack8(K.pack8(leaf.detach()))), [s, w], dy)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("form", ["transposed", "channels last", "slice of transposed", "rows of a wider tensor", "expanded"])
+def test_checkpoint_recomputes_on_an_input_of_the_same_order(form):
+    """A function may view its input as its strides allow: the recomputation's input allows the same."""
+    torch.manual_seed(4)
+    base = torch.randn(6, 10, 64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    w = torch.randn(64, 32, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    if form == "transposed":
+        make, flat = (lambda t: t.transpose(0, 1)), (lambda t: t.transpose(0, 1).view(-1, 64))
+    elif form == "channels last":
+        make = lambda t: t.view(6, 2, 5, 64).permute(0, 3, 1, 2)  # noqa: E731
+        flat = lambda t: t.permute(0, 2, 3, 1).view(-1, 64)  # noqa: E731
+    elif form == "slice of transposed":
+        make, flat = (lambda t: t.transpose(0, 1)[2:, :, :]), (lambda t: t.transpose(0, 1).flatten(1).view(6, 8, 64).reshape(-1, 64))
+    elif form == "rows of a wider tensor":
+        make, flat = (lambda t: t.view(60, 64)[:, :32]), (lambda t: torch.cat([t.view(6, 10, 32).reshape(60, 32)] * 2, 1))
+    else:
+        make, flat = (lambda t: t[:1].expand(6, 10, 64)), (lambda t: t.reshape(-1, 64))
+
+    def block(t):
+        return torch.tanh(flat(t) @ w)
+
+    x = make(base)
+    assert form == "expanded" or not x.is_contiguous()
+    y = K.checkpoint8(block, x)
+    dy = torch.randn_like(y)
+    dx, dw = torch.autograd.grad(y, [base, w], dy)
+    # at the unpacked input, in an order that the function can view
+    xq = torch.empty_like(x.detach()).copy_(K.unpack8(K.pack8(x))).requires_grad_()
+    dxq, dwq = torch.autograd.grad(block(xq), [xq, w], dy)
+    assert torch.equal(dw, dwq) and torch.equal(dx, torch.autograd.grad(x, [base], dxq)[0])
