@@ -134,15 +134,25 @@ def swiglu8_linear(gate: torch.Tensor, up: torch.Tensor, weight: torch.Tensor, f
         return torch.nn.functional.linear(swiglu8_fwd(gate, up, format, keep=False)[0], weight)
 
 
+def _only_forward(mod: torch.nn.Module) -> bool:
+    """Whether a call of ``mod`` is its class's forward and nothing else (no
+    hooks, no forward of its own), so that what computes the same may take its place."""
+    every = torch.nn.modules.module
+    return not (mod._forward_pre_hooks or mod._forward_hooks or mod._backward_pre_hooks or mod._backward_hooks
+                or every._global_forward_pre_hooks or every._global_forward_hooks
+                or every._global_backward_pre_hooks or every._global_backward_hooks or "forward" in vars(mod))
+
+
 def checkpointed_qwen2_mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
     """``Qwen2MLP.forward`` (``down_proj(act_fn(gate_proj(x)) * up_proj(x))``) on
-    ``swiglu8``.  Projections that are not bf16 or fp32 on the GPU take the
-    stock forward."""
+    ``swiglu8``.  Projections that are not bf16 or fp32 on the GPU, and an
+    activation with hooks or a forward of its own, take the stock forward; a
+    down projection that is more than a Linear's product is called as it is."""
     gate, up = self.gate_proj(x), self.up_proj(x)
-    if not (gate.is_cuda and gate.dtype in _DTYPES and gate.dtype == up.dtype):
+    if not (gate.is_cuda and gate.dtype in _DTYPES and gate.dtype == up.dtype and _only_forward(self.act_fn)):
         return self.down_proj(self.act_fn(gate) * up)
     down = self.down_proj
-    if type(down) is torch.nn.Linear and down.bias is None and down.weight.requires_grad:
+    if type(down) is torch.nn.Linear and _only_forward(down) and down.bias is None and down.weight.requires_grad:
         return swiglu8_linear(gate, up, down.weight, self.siq_mlp_format)
     return down(swiglu8(gate, up, self.siq_mlp_format))
 

@@ -500,3 +500,57 @@ def test_checkpoint_recomputes_on_an_input_of_the_same_order(form):
     xq = torch.empty_like(x.detach()).copy_(K.unpack8(K.pack8(x))).requires_grad_()
     dxq, dwq = torch.autograd.grad(block(xq), [xq, w], dy)
     assert torch.equal(dw, dwq) and torch.equal(dx, torch.autograd.grad(x, [base], dxq)[0])
+
+
+def _mlp_and_input():
+    mlp = tiny_qwen2().model.layers[0].mlp
+    return mlp, torch.randn(2, 9, 256, device=DEV, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("where", ["pre", "post", "backward", "backward pre", "global", "forward"])
+def test_hooks_of_the_down_projection_are_called(where):
+    """Hooks on the projection, or a forward of its own, count as they do in the stock MLP."""
+    mlp, x = _mlp_and_input()
+    stock = mlp(x)
+    K.enable_8bit_mlp(mlp)
+    down, calls = mlp.down_proj, []
+    plain = mlp(x)
+    handle = None
+    if where == "pre":
+        handle = down.register_forward_pre_hook(lambda m, a: (calls.append(m), (a[0] * 2,))[1])
+    elif where == "post":
+        handle = down.register_forward_hook(lambda m, a, out: (calls.append(m), out * 2)[1])
+    elif where == "backward":
+        handle = down.register_full_backward_hook(lambda m, gi, go: calls.append(m))
+    elif where == "backward pre":
+        handle = down.register_full_backward_pre_hook(lambda m, go: calls.append(m))
+    elif where == "global":
+        handle = torch.nn.modules.module.register_module_forward_hook(
+            lambda m, a, out: (calls.append(m), out * 2)[1] if m is down else None)
+    else:
+        own = down.forward
+        down.forward = lambda h: (calls.append(down), 2 * own(h))[1]
+    try:
+        y = mlp(x.requires_grad_())
+        y.sum().backward()
+    finally:
+        if handle is not None:
+            handle.remove()
+    assert calls == [down]
+    # (a power of two passes every rounding; a hook on all modules is one on the activation too)
+    assert torch.equal(y, plain if "backward" in where else 2 * (stock if where == "global" else plain))
+    assert down.weight.grad is not None and x.grad is not None
+
+
+@pytest.mark.parametrize("where", ["post", "forward"])
+def test_hooks_of_the_activation_are_called(where):
+    mlp, x = _mlp_and_input()
+    stock = mlp(x)
+    K.enable_8bit_mlp(mlp)
+    act, seen = mlp.act_fn, []
+    if where == "post":
+        act.register_forward_hook(lambda m, a, out: seen.append(out.shape))
+    else:
+        own = act.forward
+        act.forward = lambda t: (seen.append(t.shape), own(t))[1]
+    assert torch.equal(mlp(x), stock) and seen == [(2, 9, 512)]
