@@ -307,8 +307,10 @@ __device__ __forceinline__ void policy_slice(const PolicyArgs& p, const Slice& c
       if (KL != kKlNone) {
         float kl, dkl;
         kl_term<KL>((float)((double)ref[i] - (double)lp[i]), kl, dkl);
-        loss = __builtin_fmaf(p.kl_coef, kl, loss);
-        g = __builtin_fmaf(p.kl_coef, dkl, g);
+        if (p.kl_coef != 0.f) {  // (an estimate that is only reported may be infinite)
+          loss = __builtin_fmaf(p.kl_coef, kl, loss);
+          g = __builtin_fmaf(p.kl_coef, dkl, g);
+        }
         x[1] += (double)(m ? kl : 0.f);
       }
       x[0] += (double)(m ? loss : 0.f);

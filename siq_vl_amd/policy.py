@@ -107,7 +107,8 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor, advantages: torch.
 
     (``clip_high`` None: ``clip_low``; ``dual_clip`` c > 1: for ``A < 0`` the
     objective is not below ``c A``), with ``x = reference_logps - logps`` and
-    ``kl`` = ``-x`` (``"k1"``), ``x^2 / 2`` (``"k2"``) or ``e^x - 1 - x`` (``"k3"``).
+    ``kl`` = ``-x`` (``"k1"``), ``x^2 / 2`` (``"k2"``) or ``e^x - 1 - x`` (``"k3"``);
+    at ``kl_coef`` 0 the estimate is reported alone.
     ``aggregation="token"`` averages over the counted tokens, ``"sequence"`` each
     sequence's counted tokens and then the sequences; ``num_items_in_batch``
     replaces the number of counted tokens, or of sequences, divided by.  A batch

@@ -422,3 +422,19 @@ def test_two_threads_on_streams_of_their_own():
     for i in range(2):
         assert len(got[i]) == 20
         assert all(torch.equal(a, b) for step in got[i] for a, b in zip(step, want[i]))
+
+
+@pytest.mark.parametrize("kl_type,far", [("k3", 100.0), ("k3", -np.inf), ("k2", 1e30), ("k1", np.inf)])
+@pytest.mark.parametrize("tokens", [300, 5000])
+def test_a_kl_estimate_that_is_only_reported_leaves_the_loss_alone(tokens, kl_type, far):
+    """Coefficient 0: an infinite estimate shows in ``kl`` and nowhere else."""
+    cu, mask, lp, old, ref = batch([tokens - 100, 100], seed=11)
+    mask[:] = True
+    ref[7] = lp[7] + np.float32(far)
+    adv = np.float32([1.0, -0.5])
+    for aggregation in ("token", "sequence"):
+        kw = dict(kl_coef=0.0, kl_type=kl_type, aggregation=aggregation)
+        out, grad = run_policy(cu, mask, lp, old, adv, ref, kw)
+        lone, want = run_policy(cu, mask, lp, old, adv, None, kw)
+        assert not np.isfinite(float(out.kl))
+        assert float(out.loss) == float(lone.loss) and torch.equal(grad, want)
