@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArg
     if (tid % lanes != 0) continue;
     const double w = 1. / (div * fmax(n, 1.));
     if (p.by_sequence) p.weight[s] = (float)w;
-    x[0] += p.by_sequence ? l * w : l;
+    x[0] += !p.by_sequence ? l : n > 0. ? l * w : 0.;  // (divided by 0 items, w is infinite)
     x[2] += n;
   }
   block_sum<kSumThreads, 4>(x);
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const PolicyArg
   const double per = 1. / fmax(x[2], 1.);
   if (!p.by_sequence) {
     const double w = p.divisor != nullptr ? 1. / div : per;
-    x[0] *= w;
+    x[0] = x[2] > 0. ? x[0] * w : 0.;
     p.weight[0] = (float)w;
   }
   *p.loss = (float)x[0];

@@ -438,3 +438,15 @@ def test_a_kl_estimate_that_is_only_reported_leaves_the_loss_alone(tokens, kl_ty
         lone, want = run_policy(cu, mask, lp, old, adv, None, kw)
         assert not np.isfinite(float(out.kl))
         assert float(out.loss) == float(lone.loss) and torch.equal(grad, want)
+
+
+@pytest.mark.parametrize("aggregation", ["token", "sequence"])
+@pytest.mark.parametrize("tokens", [300, 50_000])
+def test_a_batch_that_counts_nothing_is_zero_whatever_is_divided_by(tokens, aggregation):
+    """The number of items of a step in which nothing counts is 0."""
+    cu, mask, lp, old, ref = batch([tokens - 100, 100])
+    mask[:] = False
+    for items in (0, torch.zeros((), device=DEV), 3):
+        kw = dict(kl_coef=0.1, aggregation=aggregation, num_items_in_batch=items)
+        out, grad = run_policy(cu, mask, lp, old, np.float32([1, 2]), ref, kw)
+        assert float(out.loss) == 0 and float(out.kl) == 0 and bool((grad == 0).all())
