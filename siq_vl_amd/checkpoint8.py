@@ -128,6 +128,7 @@ def swiglu8_linear(gate: torch.Tensor, up: torch.Tensor, weight: torch.Tensor, f
     if weight.dim() != 2 or weight.shape[1] != gate.shape[-1]:
         raise ValueError(f"weight must be [out, {gate.shape[-1]}], got {tuple(weight.shape)}")
     weight = weight.to(gate.dtype)
+    _lib.native().no_tangent("swiglu8_linear", [gate, up, weight])
     with torch.autocast(gate.device.type, enabled=False):
         if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad or weight.requires_grad):
             return _Swiglu8Linear.apply(gate, up, weight, format)

@@ -261,6 +261,7 @@ def fused_linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, label
             divisor = torch.tensor(float(num_items_in_batch), dtype=torch.float32, device=hidden.device)
     h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
     w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
+    _lib.native().no_tangent("fused_linear_cross_entropy", [h, w])
     if not torch.is_grad_enabled() or not (h.requires_grad or w.requires_grad):
         loss, _, bad = flce_loss(h.reshape(-1, h.shape[-1]), w, labels.reshape(-1), int(ignore_index), divisor)
         _track_bad(bad, w.shape[0], int(ignore_index), validate)

@@ -103,6 +103,14 @@ void no_second_derivative(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
 
+// Where no gradient is recorded the kernels are called without their node, which would refuse a forward-mode tangent:
+// a result without one would say that the derivative is zero.
+void no_tangent(const char* what, std::initializer_list<Tensor> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 // Contiguous and 16-byte aligned.
 Tensor flat(const Tensor& t) {
   Tensor c = t.contiguous();
@@ -271,6 +279,7 @@ struct Swiglu8Fused : torch::autograd::Function<Swiglu8Fused> {
 };
 
 Tensor swiglu8(const Tensor& gate, const optional<Tensor>& up, int format) {
+  no_tangent("swiglu8", {gate, defined(up)});
   const bool grad = at::GradMode::is_enabled();
   if (!up.has_value()) {
     TORCH_CHECK_VALUE(gate.dim() > 0 && gate.size(-1) % 2 == 0,
@@ -518,6 +527,7 @@ std::pair<Tensor, Tensor> linear_log_probs(const Tensor& hidden, const Tensor& w
                                            int64_t ignore_index, double temperature, int64_t chunk, int64_t keep_bytes,
                                            const optional<Tensor>& host) {
   TORCH_CHECK_VALUE(chunk > 0, "chunk_tokens must be positive");
+  no_tangent("fused_linear_log_probs", {hidden, weight});
   const Tensor counts = host.has_value() ? *host : at::empty({2}, hidden.options().dtype(at::kLong));
   int64_t* const c = counts.data_ptr<int64_t>();
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
@@ -560,5 +570,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   SIQ_DEF("flp_fwd", raw_flp_fwd);
   SIQ_DEF("flp_bwd", raw_flp_bwd);
   SIQ_DEF("linear_log_probs", linear_log_probs);
+  m.def("no_tangent", [](const char* what, const std::vector<Tensor>& inputs) {
+    for (const Tensor& t : inputs) no_tangent(what, {t});
+  });
 #undef SIQ_DEF
 }

@@ -554,3 +554,29 @@ def test_hooks_of_the_activation_are_called(where):
         own = act.forward
         act.forward = lambda t: (seen.append(t.shape), own(t))[1]
     assert torch.equal(mlp(x), stock) and seen == [(2, 9, 512)]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("call", ["two", "up", "one", "linear", "weight"])
+def test_a_forward_mode_derivative_is_refused(call, grad):
+    """No call gives a result that has lost its tangent, whether or not gradients are recorded."""
+    fw = torch.autograd.forward_ad
+    g, u, t = torch.randn(3, 4, 64, device=DEV)
+    w = torch.randn(8, 64, device=DEV)
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        d = fw.make_dual(g, t)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            if call == "two":
+                K.swiglu8(d, u)
+            elif call == "up":
+                K.swiglu8(u, d)
+            elif call == "one":
+                K.swiglu8(d)
+            elif call == "linear":
+                K.swiglu8_linear(u, d, w)
+            else:
+                K.swiglu8_linear(g, u, fw.make_dual(w, torch.ones_like(w)))
+        assert K.swiglu8(g, u).shape == g.shape  # (primals alone)
+    leaf = torch.randn(4, 64, device=DEV, requires_grad=True)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        K.swiglu8(fw.make_dual(leaf, t), u)

@@ -461,3 +461,20 @@ def test_what_another_shape_kept_is_refused():
     more = LP.flp_fwd(h.repeat(2, 1), w, y.repeat(2), keep=True)[3]
     with pytest.raises(ValueError, match="what the forward kept"):
         LP.flp_bwd(h, w, y, up, saved=more)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", ["hidden", "weight"])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_a_forward_mode_derivative_is_refused(fp32, which, grad):
+    """The log-probabilities and the cross-entropy give no result that has lost its tangent."""
+    fw = torch.autograd.forward_ad
+    h, w, y, _ = (t.to(DEV) for t in make(20, 64, 264))
+    if fp32:
+        h, w = h.float(), w.float()
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        args = [fw.make_dual(h, h), w, y] if which == "hidden" else [h, fw.make_dual(w, w), y]
+        for call in (LP.fused_linear_log_probs, C.fused_linear_cross_entropy):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*args)
+            call(h, w, y)
