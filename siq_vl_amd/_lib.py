@@ -248,6 +248,17 @@ def on_device(device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def scalar_on(device, value) -> torch.Tensor:
+    """A number, or a tensor of one, as an fp32 scalar on ``device``.  One that
+    the host holds goes there in a fill kernel's arguments: a copy would wait for
+    the GPU, and could not be captured in a graph."""
+    if torch.is_tensor(value):
+        if value.is_cuda:
+            return value.detach().to(device=device, dtype=torch.float32).reshape(())
+        value = value.item()
+    return torch.full((), float(value), dtype=torch.float32, device=device)
+
+
 def int64_array(values) -> ctypes.Array:
     arr = (_i64 * len(values))(*[int(v) for v in values])
     return arr

@@ -253,12 +253,7 @@ def fused_linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, label
     reference's stage 1, and stage 2's LoRA, which leaves ``lm_head`` out of
     its targets) gives the dH-only call: no dW GEMM and no dW buffer.
     """
-    divisor = None
-    if num_items_in_batch is not None:
-        if torch.is_tensor(num_items_in_batch):
-            divisor = num_items_in_batch.to(device=hidden.device, dtype=torch.float32)
-        else:
-            divisor = torch.tensor(float(num_items_in_batch), dtype=torch.float32, device=hidden.device)
+    divisor = None if num_items_in_batch is None else _lib.scalar_on(hidden.device, num_items_in_batch)
     h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
     w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
     _lib.native().no_tangent("fused_linear_cross_entropy", [h, w])

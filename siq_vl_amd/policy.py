@@ -54,11 +54,9 @@ def _choice(name: str, value: str, of: dict) -> int:
 def _divisor(items, device: torch.device) -> torch.Tensor | None:
     if items is None:
         return None
-    if torch.is_tensor(items):
-        if items.numel() != 1:
-            raise ValueError(f"num_items_in_batch must be one number, got {tuple(items.shape)}")
-        return items.detach().to(device=device, dtype=torch.float32).reshape(())
-    return torch.tensor(float(items), dtype=torch.float32, device=device)
+    if torch.is_tensor(items) and items.numel() != 1:
+        raise ValueError(f"num_items_in_batch must be one number, got {tuple(items.shape)}")
+    return _lib.scalar_on(device, items)
 
 
 def preference_loss(policy_logps: torch.Tensor, reference_logps: torch.Tensor | None, cu_seqlens: torch.Tensor,

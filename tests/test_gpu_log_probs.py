@@ -478,3 +478,17 @@ def test_a_forward_mode_derivative_is_refused(fp32, which, grad):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call(*args)
             call(h, w, y)
+
+
+@pytest.mark.parametrize("items", [300, torch.tensor(300)])
+def test_a_number_of_items_on_the_host_costs_the_cross_entropy_no_synchronisation(items):
+    h, w, y, _ = make(400, 64, 264, seed=3)
+    hd, wd, yd = h.to(DEV), w.to(DEV), y.to(DEV)
+    want = C.fused_linear_cross_entropy(hd, wd, yd, num_items_in_batch=torch.tensor(300.0, device=DEV))
+    C.check_pending_labels(block=True)
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = C.fused_linear_cross_entropy(hd, wd, yd, num_items_in_batch=items)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(got, want)

@@ -450,3 +450,46 @@ def test_a_batch_that_counts_nothing_is_zero_whatever_is_divided_by(tokens, aggr
         kw = dict(kl_coef=0.1, aggregation=aggregation, num_items_in_batch=items)
         out, grad = run_policy(cu, mask, lp, old, np.float32([1, 2]), ref, kw)
         assert float(out.loss) == 0 and float(out.kl) == 0 and bool((grad == 0).all())
+
+
+@pytest.mark.parametrize("items", [7, 7.0, torch.tensor(7), torch.tensor([7.0])])
+def test_a_number_of_items_on_the_host_costs_no_synchronisation(items):
+    cu, mask, lp, old, ref = batch([500, 2100, 40, 900], seed=9)
+    lp_t, old_t, ref_t, mask_t, cu_t = gpu(lp, old, ref, mask, cu)
+    lp_t.requires_grad_()
+    adv = torch.randn(4, device=DEV)
+    on_device = torch.tensor(7.0, device=DEV)
+
+    def calls(n):
+        a = P.policy_loss(lp_t, old_t, adv, cu_t, mask=mask_t, num_items_in_batch=n).loss
+        b = P.preference_loss(lp_t, ref_t, cu_t, mask=mask_t, num_items_in_batch=n).loss
+        return a.detach(), b.detach()
+
+    want = calls(on_device)
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = calls(items)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_captured_call_with_a_number_of_items_replays():
+    cu, mask, lp, old, ref = batch([500, 2100, 0, 900], seed=10)
+    lp_t, old_t, mask_t, cu_t = gpu(lp, old, mask, cu)
+    adv = torch.randn(4, device=DEV)
+
+    def call():
+        return P.policy_loss(lp_t, old_t, adv, cu_t, mask=mask_t, num_items_in_batch=7).loss
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        lp_t.copy_(old_t + 0.3 * torch.randn_like(old_t))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, call())
