@@ -9,7 +9,6 @@ operators; it calls this library through the same ABI.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import importlib
 import os
@@ -23,7 +22,6 @@ from . import build as _build
 _LOCK = threading.Lock()
 _LIB: ctypes.CDLL | None = None
 _NATIVE = None
-_HERE = contextlib.nullcontext()
 
 SIQ_OK = 0
 SIQ_ERR_INVALID_ARGUMENT = -1
@@ -240,12 +238,6 @@ def first_order(what: str) -> None:
     as if they were constants."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no second derivative (create_graph=True)")
-
-
-def on_device(device):
-    """A context in which ``device`` is the current GPU (none is entered when it
-    is already): kernels go to the current one, whatever their stream."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def scalar_on(device, value) -> torch.Tensor:
