@@ -492,3 +492,54 @@ def test_a_number_of_items_on_the_host_costs_the_cross_entropy_no_synchronisatio
     finally:
         torch.cuda.set_sync_debug_mode("default")
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n,hdim,need_dw", [(48, 896, False), (48, 896, True), (128, 896, True), (128, 1536, True),
+                                            (129, 896, True), (1, 1536, True)])
+@pytest.mark.parametrize("keep", [True, False])
+def test_few_rows_of_a_real_vocabulary(n, hdim, need_dw, keep):
+    """151,936 columns, against the definition in 64 bits on the GPU; bounds as the oracle's."""
+    vocab, half, t = 151_936, 2.0 ** -8, 0.8
+    print(f"few rows n={n} h={hdim} dw={need_dw} keep={keep}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(n + hdim)
+    w = (0.05 * torch.randn(vocab, hdim, generator=g, device=DEV)).to(torch.bfloat16)
+    y = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    lean = 20 * torch.rand(n, 1, generator=g, device=DEV) / (0.05 ** 2 * hdim)
+    h = (torch.randn(n, hdim, generator=g, device=DEV) + lean * w[y].float()).to(torch.bfloat16)
+    up = torch.randn(n, generator=g, device=DEV)
+    if n > 1:
+        y[::5], y[1], y[n - 1] = -100, vocab - 1, 0
+        up[::5] = float("nan")  # of rows that do not count
+    logp, count, bad, saved = LP.flp_fwd(h, w, y, temperature=t, keep=keep)
+    dh, dw = LP.flp_bwd(h, w, y, up, temperature=t, saved=saved, need_dweight=need_dw)
+    del saved
+    at = (y >= 0).nonzero()[:, 0]
+    assert int(count) == at.numel() and int(bad) == 0
+    out = y < 0
+    assert bool((logp[out] == 0).all()) and bool((dh[out] == 0).all())
+    hk, wd, yk = h[at].double(), w.double(), y[at]
+    rows = torch.arange(at.numel(), device=DEV)
+    z = hk @ wd.T.contiguous() / t
+    want = z[rows, yk] - torch.logsumexp(z, 1)
+    depth = hdim / 8 + 4
+    wabs = wd.abs()
+    off = 2 * depth * 2.0 ** -24 * (hk.abs() @ wabs.T.contiguous()).amax(1) / t + 1e-6 + 4 * 2.0 ** -24 * want.abs()
+    assert bool(((logp[at].double() - want).abs() <= off).all())
+    p = torch.softmax(z, 1)
+    gk = up[at].double()[:, None] / t
+    dz = -gk * p
+    soft = dz.abs()
+    soft[rows, yk] = 0.0
+    dz[rows, yk] += gk[:, 0]
+    label = gk.abs() * (8 * 2.0 ** -24 + off[:, None])
+    dh_want, spread = dz @ wd, soft @ wabs
+    bound = 1.05 * ((half + off[:, None]) * spread + label * wabs[yk] + half * dh_want.abs()) + 1e-30
+    assert bool(((dh[at].double() - dh_want).abs() <= bound).all())
+    if not need_dw:
+        assert dw is None
+        return
+    dw_want = dz.T.contiguous() @ hk
+    bound = 2 * half * (soft.T.contiguous() @ hk.abs()) + half * dw_want.abs()
+    bound += (off[:, None] * soft).T.contiguous() @ hk.abs()
+    bound.index_add_(0, yk, label * hk.abs())
+    assert bool(((dw.double() - dw_want).abs() <= 1.05 * bound + 1e-30).all())
