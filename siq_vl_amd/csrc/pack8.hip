@@ -242,9 +242,23 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(const uint8_t* __rest
   }
 }
 
-// silu(g) = g s and the rest of what the products need: s = 1 / (1 + e^-g).
-__device__ __forceinline__ float sigmoid(float g) {
-  return __builtin_amdgcn_rcpf(1.f + exp2f_fast(-g * kLog2e));
+// sigmoid(g) = r k with k = 1.  LOW: 2^-64 where g < -64, so that silu(g) = (g k) r and its slope are normal numbers
+// down to g = -91.9; 1 / (1 + e^-g) is none from -87.3 on, and its reciprocal would be taken as zero.  (A path of its
+// own, that vectors with such a gate alone take: in all of them it cost the backward 6%.)
+template <bool LOW>
+__device__ __forceinline__ void sigmoid(float g, float& r, float& k) {
+  const bool low = LOW && g < -64.f;
+  k = low ? 0x1p-64f : 1.f;
+  r = __builtin_amdgcn_rcpf(k + exp2f_fast(__builtin_fmaf(-g, kLog2e, low ? -64.f : 0.f)));
+}
+// f(LOW) for eight gates.
+template <class F>
+__device__ __forceinline__ void with_gates(const float (&g)[8], F f) {
+  const float m = fminf(fminf(fminf(g[0], g[1]), fminf(g[2], g[3])), fminf(fminf(g[4], g[5]), fminf(g[6], g[7])));
+  if (m < -64.f)
+    f(std::true_type());
+  else
+    f(std::false_type());
 }
 
 // Offset of vector v in a [rows, cols] tensor whose rows are ld elements apart
@@ -275,8 +289,14 @@ __global__ __launch_bounds__(kThreads) void swiglu8_fwd_kernel(const SwigluArgs 
     const int64_t v = v0 + u * kThreads;
     const int have = have_of(v, numel);
     float o[8];
+    with_gates(g[u], [&](auto low) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = g[u][i] * sigmoid(g[u][i]) * w[u][i];
+      for (int i = 0; i < 8; ++i) {
+        float r, k;
+        sigmoid<decltype(low)::value>(g[u][i], r, k);
+        o[i] = g[u][i] * k * r * w[u][i];
+      }
+    });
     store8(h + 8 * v, have, o);
     if (KEEP) {
       int gb, ub;
@@ -318,13 +338,17 @@ __global__ __launch_bounds__(kThreads) void swiglu8_bwd_kernel(const SwigluArgs 
     float g[8], w[8], dg[8], du[8], o[8];
     decode8<E4M3>(gc[u], gb[u], g);
     decode8<E4M3>(uc[u], ub[u], w);
+    with_gates(g, [&](auto low) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float s = sigmoid(g[i]), gs = g[i] * s;
-      du[i] = d[u][i] * gs;
-      dg[i] = d[u][i] * w[i] * s * __builtin_fmaf(g[i], 1.f - s, 1.f);
-      o[i] = gs * w[i];
-    }
+      for (int i = 0; i < 8; ++i) {
+        float r, k;
+        sigmoid<decltype(low)::value>(g[i], r, k);
+        const float gs = g[i] * k * r;
+        du[i] = d[u][i] * gs;
+        dg[i] = d[u][i] * w[i] * r * (k * __builtin_fmaf(g[i], 1.f - r * k, 1.f));
+        o[i] = gs * w[i];
+      }
+    });
     if (have > 0) {
       store8<true>(dgate + at<STRIDED>(v, p.cols, p.ld0), have, dg);
       store8<true>(dup + at<STRIDED>(v, p.cols, p.ld1), have, du);

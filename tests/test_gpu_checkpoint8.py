@@ -580,3 +580,25 @@ def test_a_forward_mode_derivative_is_refused(call, grad):
     leaf = torch.randn(4, 64, device=DEV, requires_grad=True)
     with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         K.swiglu8(fw.make_dual(leaf, t), u)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_swiglu_of_very_negative_gates(dtype, fmt):
+    """e^g leaves fp32's normal numbers at g = -87.3, g e^g and its slope only at -91.9."""
+    dt = DTYPES[dtype]
+    g = -torch.arange(60, 108, dtype=torch.float32).repeat(2, 4)  # whole numbers: int8 holds them, groups of 32 differ
+    gen = torch.Generator().manual_seed(8)
+    u = (1 + torch.rand(g.shape, generator=gen)).to(dt)
+    dh = torch.randn(g.shape, generator=gen).to(dt)
+    gd, ud = g.to(dt).to(DEV).requires_grad_(), u.to(DEV).requires_grad_()
+    h = K.swiglu8(gd, ud, fmt)
+    dgate, dup = torch.autograd.grad(h, [gd, ud], dh.to(DEV))
+    g64, u64, d64 = np64(g), np64(u), np64(dh)
+    close("h", h, op.swiglu(g64, u64), np.abs(op.swiglu(g64, u64)), dt, g64)
+    assert float(h[0, 88 - 60].abs()) > 4e-37  # g = -88
+    gq, uq = op.rounded(g64, fmt), op.rounded(u64, fmt)
+    dg, du = op.swiglu_bwd(d64, gq, uq)
+    s = 1 / (1 + np.exp(-gq))
+    close("dgate", dgate, dg, np.abs(d64 * uq * s) * (1 + np.abs(gq) * (1 + s)), dt, gq)
+    close("dup", dup, du, np.abs(du), dt, gq)
