@@ -602,3 +602,37 @@ def test_swiglu_of_very_negative_gates(dtype, fmt):
     s = 1 / (1 + np.exp(-gq))
     close("dgate", dgate, dg, np.abs(d64 * uq * s) * (1 + np.abs(gq) * (1 + s)), dt, gq)
     close("dup", dup, du, np.abs(du), dt, gq)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_a_captured_checkpoint_replays_with_dropout(fmt):
+    """Every replay draws new numbers, and its backward takes the same ones."""
+    x = torch.randn(64, 96, device=DEV)
+    w = torch.rand(96, device=DEV) + 1
+    leaf = x.clone().requires_grad_()
+
+    def step():
+        y = K.checkpoint8(lambda t: torch.nn.functional.dropout(torch.tanh(t) * w, 0.5), leaf, format=fmt)
+        return y.detach(), torch.autograd.grad(y, [leaf], torch.ones_like(y))[0]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, g = step()
+    masks = []
+    for i in range(3):
+        with torch.no_grad():
+            leaf.copy_((i + 1) * 0.5 * torch.randn_like(x) + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        xq = K.unpack8(K.pack8(leaf, fmt)).requires_grad_()
+        masks.append(y != 0)
+        want, = torch.autograd.grad(torch.tanh(xq) * w * 2 * masks[-1], [xq], torch.ones_like(xq))
+        # the same products in another order: a few roundings of fp32, of terms of up to 4
+        assert float((g - want).abs().max()) <= 16 * 2.0 ** -24 * 4
+    assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
