@@ -121,3 +121,43 @@ def test_python_refusals():
     assert K.enable_8bit_mlp(torch.nn.Linear(2, 2)) == 0
     with pytest.raises(ValueError, match="format"):
         K.enable_8bit_mlp(torch.nn.Linear(2, 2), "int4")
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_seen_where_they_are(grad):
+    fw, native = torch.autograd.forward_ad, _lib.native()
+    x, y = torch.ones(2, 3), torch.ones(3)
+    with torch.set_grad_enabled(grad):
+        native.no_tangent("an operator", [x, y])
+        with fw.dual_level():
+            native.no_tangent("an operator", [x, y])
+            d = fw.make_dual(y, y)
+            for args in ([x, d], [d], [d * 2, x]):
+                with pytest.raises(NotImplementedError, match="an operator has no forward-mode derivative"):
+                    native.no_tangent("an operator", args)
+            native.no_tangent("an operator", [fw.unpack_dual(d).primal, x])
+        native.no_tangent("an operator", [y])
+
+
+def test_modules_that_are_more_than_their_forward():
+    def plain():
+        return torch.nn.Linear(2, 2)
+
+    assert K._only_forward(plain())
+    for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                     "register_full_backward_pre_hook"):
+        mod = plain()
+        handle = getattr(mod, register)(lambda *a: None)
+        assert not K._only_forward(mod)
+        handle.remove()
+        assert K._only_forward(mod)
+    for register in ("register_module_forward_hook", "register_module_forward_pre_hook",
+                     "register_module_full_backward_hook", "register_module_full_backward_pre_hook"):
+        handle = getattr(torch.nn.modules.module, register)(lambda *a: None)
+        try:
+            assert not K._only_forward(plain())
+        finally:
+            handle.remove()
+    mod = plain()
+    mod.forward = lambda x: x
+    assert not K._only_forward(mod)

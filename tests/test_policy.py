@@ -1,5 +1,7 @@
 """Preference and policy losses on the CPU: the oracle against differences, and every refusal."""
 
+import warnings
+
 import numpy as np
 import pytest
 import torch
@@ -142,3 +144,13 @@ def test_errors_come_from_the_extension_as_python_errors():
         P.preference_loss(x.half(), None, x)
     with pytest.raises(TypeError):
         P.policy_loss(x, None, x)
+
+
+@pytest.mark.parametrize("value", [7, 7.0, 0, torch.tensor(7), torch.tensor([7.0]), torch.tensor(7.0, requires_grad=True),
+                                   2 ** 24 + 1, torch.tensor(2 ** 24 + 1)])
+def test_numbers_become_fp32_scalars(value):
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        t = _lib.scalar_on(torch.device("cpu"), value)
+    assert t.shape == () and t.dtype == torch.float32 and not t.requires_grad
+    assert t.item() == np.float32(value.item() if torch.is_tensor(value) else value)
