@@ -198,7 +198,8 @@ def checkpoint8(function, x: torch.Tensor, *args, format: str = "int8", **kwargs
     ``torch.utils.checkpoint.checkpoint(..., use_reentrant=False)`` does
     (``kwargs`` go there), with ``x`` kept in 8 bits instead of as it is.  The
     forward runs on ``x`` itself; what the backward recomputes, and so the
-    gradients, are those at the unpacked ``x``."""
+    gradients, are those at the unpacked ``x``, with the forward's random numbers.
+    ``function`` may change ``x`` in place, and view it as its strides allow."""
     _format(format)
     _check(x, "x")
     if not torch.is_grad_enabled():

@@ -57,8 +57,9 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
     ``temperature``: what sampled answers were drawn with.
 
     ``keep_bytes`` bounds what the forward may keep for the backward (2 * rows *
-    vocab bytes); a batch above it keeps nothing, and the backward forms the
-    logits again, ``chunk_tokens`` rows at a time (None: 2 GiB of them).
+    vocab bytes, ignored rows counted: how many there are is known on the device
+    alone); a batch above it keeps nothing, and the backward forms the logits
+    again, ``chunk_tokens`` rows at a time (None: 2 GiB of them).
     Without gradients nothing is kept.  A frozen ``weight`` gives the dH-only
     backward.
     """

@@ -110,7 +110,7 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor, advantages: torch.
     ``aggregation="token"`` averages over the counted tokens, ``"sequence"`` each
     sequence's counted tokens and then the sequences; ``num_items_in_batch``
     replaces the number of counted tokens, or of sequences, divided by.  A batch
-    that counts nothing has loss 0 and gradient 0.
+    that counts nothing has loss 0 and gradient 0, divided by 0 too.
     """
     agg, kind = _choice("aggregation", aggregation, _AGGREGATIONS), _choice("kl_type", kl_type, _KL_TYPES)
     high = clip_low if clip_high is None else clip_high
