@@ -508,11 +508,12 @@ int siq_swiglu8_bwd(const void* dh, const void* gate_codes, const void* gate_sca
  * not below dual_clip * A (dual_clip 0: no such bound); its loss is -objective +
  * kl_coef * kl with x = reference - logp and kl = -x (SIQ_KL_K1), x^2 / 2 (_K2)
  * or e^x - 1 - x (_K3), left out at kl_coef 0 (it may be infinite) but for
- * *mean_kl.  advantages A: [tokens] (advantage_per_token) or [seqs].  SIQ_AGG_TOKEN: the mean over counted tokens; SIQ_AGG_SEQUENCE: the
- * mean over sequences of their counted tokens' mean (0 where none counts);
- * with divisor its value replaces the number of counted tokens, or of
- * sequences.  cu_seqlens NULL: one sequence.  A token exactly at a border is
- * not cut.  *loss, *mean_kl and *clip_fraction (the share of cut tokens), the
+ * *mean_kl.  advantages A: [tokens] (advantage_per_token) or [seqs].
+ * SIQ_AGG_TOKEN: the mean over counted tokens; SIQ_AGG_SEQUENCE: the mean over
+ * sequences of their counted tokens' mean (0 where none counts); with divisor
+ * its value replaces the number of counted tokens, or of sequences.
+ * cu_seqlens NULL: one sequence.  A token exactly at a border is not cut.
+ * *loss, *mean_kl and *clip_fraction (the share of cut tokens), the
  * latter two over counted tokens, are 0 where none counts; dtoken [tokens]
  * (16-byte aligned) and weight [seqs] (SIQ_AGG_TOKEN: [1]) are what
  * siq_policy_bwd multiplies: dlogps = grad_loss weight dtoken (dlogps 16-byte
