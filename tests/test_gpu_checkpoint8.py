@@ -636,3 +636,34 @@ def test_a_captured_checkpoint_replays_with_dropout(fmt):
         # the same products in another order: a few roundings of fp32, of terms of up to 4
         assert float((g - want).abs().max()) <= 16 * 2.0 ** -24 * 4
     assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
+
+
+def test_more_elements_than_32_bits_count():
+    """Codes, scales and gradients behind 2^32 stored elements, and behind 2^31 of an activation in strided rows, are
+    those of the same rows alone."""
+    n = (1 << 32) + 5 * 4096 + 77
+    x = torch.empty(n, dtype=torch.bfloat16, device=DEV)
+    for a in range(0, n, 1 << 28):
+        x[a:a + (1 << 28)].normal_()
+    p = K.pack8(x)
+    y = K.unpack8(p)
+    for a in (0, (1 << 31) - 4096, (1 << 32) - 4096, (1 << 32) + 4 * 4096):
+        seg = x[a:a + 8192].clone()
+        q = K.pack8(seg)
+        assert torch.equal(q.codes, p.codes[a:a + seg.numel()])
+        assert torch.equal(q.scales, p.scales[a // 32:a // 32 + q.scales.numel()])
+        assert torch.equal(K.unpack8(q), y[a:a + seg.numel()])
+    del p, y
+    rows, cols = 349_527, 6144
+    both = x[:rows * 2 * cols].view(rows, 2 * cols)
+    gate, up = both[:, :cols], both[:, cols:]
+    h, s = K.swiglu8_fwd(gate, up)
+    dgate, dup, _ = K.swiglu8_bwd(h, s)
+    side, _, h2 = K.swiglu8_bwd(h, s, need_h=True, fused=True)
+    assert h.numel() > 1 << 31 and h2.shape == h.shape
+    for r in (0, 174_763, 349_520, rows - 3):
+        at = slice(r, r + 3)
+        hh, ss = K.swiglu8_fwd(gate[at], up[at])
+        a, b, c = K.swiglu8_bwd(h[at].clone(), ss, need_h=True)
+        assert torch.equal(hh, h[at]) and torch.equal(a, dgate[at]) and torch.equal(b, dup[at]) and torch.equal(c, h2[at])
+        assert torch.equal(torch.cat([a, b], 1), side[at])

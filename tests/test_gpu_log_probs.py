@@ -543,3 +543,47 @@ def test_few_rows_of_a_real_vocabulary(n, hdim, need_dw, keep):
     bound += (off[:, None] * soft).T.contiguous() @ hk.abs()
     bound.index_add_(0, yk, label * hk.abs())
     assert bool(((dw.double() - dw_want).abs() <= 1.05 * bound + 1e-30).all())
+
+
+def test_more_kept_numerators_than_32_bits_count():
+    """16,390 rows of 151,936 columns: 2.5e9 numerators, and offsets of 5e9 bytes, in the weight's gradient and the rows'."""
+    n, hdim, vocab, half = 16_390, 64, 151_936, 2.0 ** -8
+    g = torch.Generator(device=DEV).manual_seed(6)
+    h = torch.randn(n, hdim, generator=g, device=DEV).to(torch.bfloat16)
+    w = (0.3 * torch.randn(vocab, hdim, generator=g, device=DEV)).to(torch.bfloat16)
+    y = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    y[100:130], y[n - 1] = -100, vocab - 1
+    up = torch.randn(n, generator=g, device=DEV)
+    logp, count, _, saved = LP.flp_fwd(h, w, y, keep=True)
+    assert int(count) == n - 30 and saved.numel() > 2 * (1 << 31)
+    got = [LP.flp_bwd(h, w, y, up, saved=saved), LP.flp_bwd(h, w, y, up)]
+    del saved
+    wd, wabs = w.double(), w.double().abs()
+    wt, wt_abs = wd.T.contiguous(), wabs.T.contiguous()
+    dw, dw_off = torch.zeros(2, vocab, hdim, dtype=torch.float64, device=DEV)
+    for c in range(0, n, 1024):  # bounds as the oracle's
+        at = c + (y[c:c + 1024] >= 0).nonzero()[:, 0]
+        rows, hk, yk = torch.arange(at.numel(), device=DEV), h[at].double(), y[at]
+        z = hk @ wt
+        want = z[rows, yk] - torch.logsumexp(z, 1)
+        off = 2 * (hdim / 8 + 4) * 2.0 ** -24 * (hk.abs() @ wt_abs).amax(1) + 1e-6 + 4 * 2.0 ** -24 * want.abs()
+        assert bool(((logp[at].double() - want).abs() <= off).all())
+        gk = up[at].double()[:, None]
+        dz = torch.softmax(z, 1).mul_(-gk)
+        soft = dz.abs()
+        soft[rows, yk] = 0.0
+        dz[rows, yk] += gk[:, 0]
+        label = gk.abs() * (8 * 2.0 ** -24 + off[:, None])
+        dh_want = dz @ wd
+        bound = 1.05 * ((half + off[:, None]) * (soft @ wabs) + label * wabs[yk] + half * dh_want.abs()) + 1e-30
+        for dh, _ in got:
+            assert bool(((dh[at].double() - dh_want).abs() <= bound).all())
+        dw += dz.T.contiguous() @ hk
+        dw_off += (soft * (2 * half + off[:, None])).T.contiguous() @ hk.abs()
+        dw_off.index_add_(0, yk, label * hk.abs())
+        del z, dz, soft
+    # sums of n products in fp32, eight at once, beside the oracle's terms
+    dw_off += half * dw.abs() + n / 8 * 2.0 ** -24 * dw_off / half
+    for dh, grad in got:
+        assert bool((dh[100:130] == 0).all())
+        assert bool(((grad.double() - dw).abs() <= 1.05 * dw_off + 1e-30).all())
