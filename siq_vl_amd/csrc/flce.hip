@@ -57,7 +57,9 @@
 // stops at the loss, and neither gradient GEMM runs.
 #include <algorithm>
 
+#include "few.h"
 #include "flce.h"
+#include "flce_launch.h"
 #include "gemm.h"
 #include "ids.h"
 
@@ -67,29 +69,18 @@ namespace {
 
 using namespace gemm;
 
-constexpr int kVT = BI;  // vocab columns per logits tile
-
 // ---------------------------------------------------------------- logits
 // A tile sum at or above this (or not a number) means the row's reference is
 // too low for the tile.
 constexpr float kRefLimit = 0x1p60f;
 
-struct LogitsArgs {
-  GOp W, H;               // W [V, hdim], H = hidden rows of the chunk [nc, hdim]
-  const int64_t* y;       // chunk labels
-  const float* ref;       // [nc] row references (log2 units)
-  bf16* E;                // [nc, V]
-  float* spart;           // [nvt, ldp] tile sum of exp2(z2 - ref); negated for a redone tile
-  float* mpart;           // [nvt, ldp] a redone tile's own reference
-  float* zy;              // [nc] label logit (natural units); label_apart: log2 units, relative to ref
-  const int64_t* nvalid;  // valid (compacted) rows in all chunks
-  int64_t V, nc, c0, ldp;
-  int nI, nJ;
-  int store_e;            // 0: loss only, E is not needed
-  int label_apart;        // the label is left out of E and of the sums
-  float zscale;           // log2(e) / temperature
-};
-
+// LISTS: instead of the label, every token of a row's list is left out of E and
+// of the sums, and its logit goes to zk.  A row has a few tokens a hundred tiles,
+// a wave's 32 rows together one or two of this tile's: they are taken one after
+// the other, each from the one accumulator that holds it, which a uniform branch
+// selects.  (A compare and two selects for each of the 64 accumulators, as for
+// the label, would be made for nearly every tile.)
+template <bool LISTS>
 __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
   int ti, tj;
@@ -108,8 +99,13 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
   for (int b = 0; b < 2; ++b) {
     const int64_t tok = min(j0 + wave_col(b, wj) + l32, p.nc - 1);
     ref[b] = p.ref[tok];
-    const int64_t d = p.y[tok] - vbase;
-    rel[b] = d >= 0 && d < 256 ? (int)d : -1;
+    if constexpr (LISTS) {  // the list's entries of this tile
+      const uint8_t* first = p.first + tok * p.ldt + ti;
+      rel[b] = first[0] | first[1] << 8;
+    } else {
+      const int64_t d = p.y[tok] - vbase;
+      rel[b] = d >= 0 && d < 256 ? (int)d : -1;
+    }
   }
   f32x16 acc[4][2];
   gemm_core<true, true, false>(smem, p.W, p.H, i0, j0, 0, p.W.cols, acc);
@@ -151,21 +147,50 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
     const int col = wave_col(b, wj) + l32;
     const int64_t tok = j0 + col;
     const bool tv = tok < p.nc;
-    // the label logit: held by at most one lane of the workgroup, for one
-    // vocab tile in ~600 -- located with one range test per token
-    const bool hit = tv && rel[b] >= 0 && ((rel[b] >> 6) & 1) == wi && ((rel[b] >> 3) & 1) == 0;
-    if (__any(hit)) {
-      const int r0 = rel[b] - 64 * wi;
-      float zsel = 0.f;
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (hit && r0 == wave_row(a, 0) + 16 * (r >> 3) + (r & 7)) {
-            zsel = acc[a][b][r];
-            if (p.label_apart) acc[a][b][r] = -INFINITY;
+    if constexpr (LISTS) {
+      for (int at = rel[b] & 255; __any(tv && at < rel[b] >> 8); ++at) {
+        const bool mine = tv && at < rel[b] >> 8;
+        const int v = mine ? (int)((p.ids[tok * p.ldk + at] & kIdMask) - i0) : -1;  // 0 .. 255
+        // (both halves of the wave look at the same entry; one of them, of one of two waves, holds its logit)
+        const bool hit = mine && ((v >> 6) & 1) == wi && ((v >> 3) & 1) == h;
+        const int reg = ((v >> 7) << 5) | ((v >> 5 & 1) << 4) | ((v >> 4 & 1) << 3) | (v & 7);  // 16 a + r
+        float zsel = 0.f;
+        for (uint64_t todo = __ballot(hit); todo != 0; todo &= todo - 1) {
+          const int l = (int)__builtin_ctzll(todo);
+          const bool me = lane == l;
+          switch (__builtin_amdgcn_readlane(reg, l)) {
+#define SIQ_TAKE(a, r)                                  \
+  case 16 * a + r:                                      \
+    zsel = me ? acc[a][b][r] : zsel;                    \
+    acc[a][b][r] = me ? -INFINITY : acc[a][b][r];       \
+    break;
+#define SIQ_TAKE4(a, r) SIQ_TAKE(a, r) SIQ_TAKE(a, r + 1) SIQ_TAKE(a, r + 2) SIQ_TAKE(a, r + 3)
+#define SIQ_TAKE16(a) SIQ_TAKE4(a, 0) SIQ_TAKE4(a, 4) SIQ_TAKE4(a, 8) SIQ_TAKE4(a, 12)
+            SIQ_TAKE16(0) SIQ_TAKE16(1) SIQ_TAKE16(2) SIQ_TAKE16(3)
+#undef SIQ_TAKE16
+#undef SIQ_TAKE4
+#undef SIQ_TAKE
           }
-      if (hit) p.zy[tok] = p.label_apart ? __builtin_fmaf(zsel, p.zscale, -ref[b]) : zsel;
+        }
+        if (hit) p.zk[tok * p.ldk + at] = __builtin_fmaf(zsel, p.zscale, -ref[b]);
+      }
+    } else {
+      // the label logit: held by at most one lane of the workgroup, for one
+      // vocab tile in ~600 -- located with one range test per token
+      const bool hit = tv && rel[b] >= 0 && ((rel[b] >> 6) & 1) == wi && ((rel[b] >> 3) & 1) == 0;
+      if (__any(hit)) {
+        const int r0 = rel[b] - 64 * wi;
+        float zsel = 0.f;
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (hit && r0 == wave_row(a, 0) + 16 * (r >> 3) + (r & 7)) {
+              zsel = acc[a][b][r];
+              if (p.label_apart) acc[a][b][r] = -INFINITY;
+            }
+        if (hit) p.zy[tok] = p.label_apart ? __builtin_fmaf(zsel, p.zscale, -ref[b]) : zsel;
+      }
     }
     const float sum = numerators(b, ref[b], p.store_e && tv);
     if (h == 0) red[wi * 256 + col] = sum;
@@ -221,30 +246,6 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
 }
 
 // ---------------------------------------------------------------- row pass
-struct RowArgs {
-  const float* spart;    // [nvt, ldp] tile sums (negative: redone, relative to mpart)
-  const float* mpart;
-  const float* ref;      // [nc] row references (log2 units)
-  const float* zy;       // [nc] as the logits kernel left it
-  const int64_t* y;      // chunk labels
-  bf16* E;               // [nc, V]
-  bf16* H;               // [nc, hdim] compacted rows: scaled by f (need_dw)
-  float* f;              // [nc] factors of E
-  float* wt;             // [nc] weights of the label terms
-  float* loss_row;       // [nc] (chunk slice; not with label_apart)
-  float* logp;           // [n] log-probabilities of the labels by original row (label_apart), or nullptr
-  const int32_t* rows;   // compacted row -> original row (chunk slice; label_apart)
-  const float* invden;   // nullptr: 1
-  const int64_t* nvalid;
-  uint64_t* keys;        // [nsort, kIdChunk] rows sorted by label
-  int32_t* slot;         // [V] cleared
-  int64_t nc, nvt, V, hdim, c0, ldp;
-  int vlog;              // log2 of the eight-column groups of a tile
-  int nsort;             // sorting workgroups (0 without dW)
-  int parts;             // workgroups per 64 rows
-  int grads;             // 0: loss only (E was never stored)
-  int label_apart;
-};
 
 // Workgroups [0, nsort) sort the chunk's labels; the others take 64 rows each,
 // `parts` workgroups the same ones.  Sixteen waves read the rows' tile sums
@@ -274,7 +275,11 @@ __device__ __forceinline__ void sort_labels(uint64_t* sk, const int64_t* y, int6
   sort_keys(sk, np2);
   for (int i = threadIdx.x; i < kIdChunk; i += kRowThreads) keys[base + i] = i < np2 ? sk[i] : kNoKey;
 }
-template <int ROWS>
+//
+// LISTS: rows with a list of tokens apart.  What they add is not known here: a
+// row's sum over the others is left as it is, and E of rows with redone tiles is
+// brought to the sum's own reference.
+template <int ROWS, bool LISTS>
 __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) {
   constexpr int NWR = kRowThreads / 64, U = 8, SUB = 64 / ROWS, NT0 = NWR * SUB;  // tiles read at once
   __shared__ union {
@@ -363,7 +368,14 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
     }
     const bool mine = sub == 0 && r0 + lane < nv && part == 0;
     float lse2, w0, f0;  // log2 sum, (probability of the label) - 1, what E times it is a probability
-    if (p.label_apart) {
+    if constexpr (LISTS) {
+      lse2 = top;
+      w0 = f0 = 0.f;
+      if (mine) {
+        p.rsum[row] = sum;
+        p.rtop[row] = top;
+      }
+    } else if (p.label_apart) {
       // `sum` is that of the other columns: with t its ratio to the label's term the label's probability is 1 / (1 + t),
       // and both its logarithm and its distance from 1 keep their digits where t is small.  Redone tiles are 2^60 above
       // the label: there only the sum counts.
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       // (a power of two in rows whose E is rounded once more below: then f H is exact)
       const float g = p.invden != nullptr ? *p.invden : 1.f;
       const float f = redone ? __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(g)) : f0 * g;
-      if (mine) {
+      if (mine && !LISTS) {
         p.f[row] = f;
         p.wt[row] = w0 * g;
         if (!redone && !p.label_apart) p.E[row * p.V + p.y[row]] = (bf16)0.f;
@@ -400,7 +412,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
   // rows with redone tiles: E of every tile times what makes it the gradient over f (8 columns never straddle a
   // tile); this part's tiles, kRowSeg of them at a time, four rows at once
   constexpr int CT = 256, UE = 4;
-  const float lse2 = sh.r.lse[lane], gm = __builtin_amdgcn_frexp_mantf(p.invden != nullptr ? *p.invden : 1.f);
+  const float lse2 = sh.r.lse[lane], gm = LISTS ? 1.f : __builtin_amdgcn_frexp_mantf(p.invden != nullptr ? *p.invden : 1.f);
   const int64_t tper = (p.nvt + p.parts - 1) / p.parts, te = min(p.nvt, (part + 1) * tper);
   for (int64_t tb = part * tper; sh.r.n > 0 && tb < te; tb += kRowSeg) {
     const int nt = (int)min((int64_t)kRowSeg, te - tb);
@@ -416,7 +428,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
       // (a label of next to no probability: the factor of a tile relative to it may leave fp32's range where its
       // products with E, up to kRefLimit, do not: 2^100 times it then, marked by its sign)
       const float d = m[u] - lse2;
-      const bool far = p.label_apart && d < -100.f;
+      const bool far = (LISTS || p.label_apart) && d < -100.f;
       const float k = exp2f_fast(far ? d + 100.f : d) * gm;
       sh.r.fac[t1 + NT0 * u][lane] = far ? -k : k;
     }
@@ -469,17 +481,6 @@ __global__ __launch_bounds__(kRowThreads) void flce_row_kernel(const RowArgs p) 
 // one per thread; wave k adds rows k, k + 4, ..., eight in flight, and the
 // waves' sums are added in order at the end.
 constexpr int kLabelRound = 256;
-struct LabelArgs {
-  const uint64_t* keys;  // [nsort, kIdChunk]
-  const bf16* H;         // [n, hdim] all rows, unscaled
-  const int32_t* rows;   // chunk's compacted row -> row of H
-  const float* wt;       // [nc]
-  float* lsum;           // [nsort * kIdChunk (rows that exist), hdim]
-  int32_t* slot;         // [V]
-  int32_t* next;         // [nsort * kIdChunk]
-  int64_t hdim;
-  int nsort;
-};
 __global__ __launch_bounds__(256) void flce_label_kernel(const LabelArgs p) {
   constexpr int U = 3, R = 8, NWL = 4;
   static_assert(kLabelRound == 64 * NWL, "a thread per listed row");
@@ -587,19 +588,6 @@ __global__ __launch_bounds__(256) void flce_label_kernel(const LabelArgs p) {
 }
 
 // ---------------------------------------------------------------- dH
-struct DhArgs {
-  GOp Wt;        // W [V, hdim] read as A[i = h][k = v]
-  GOp E;         // [nc, V] read as B[j = tok][k = v]
-  bf16* dh;      // dhidden [n, hdim]
-  float* part;   // [slots][prow][hdim] partial sums (DhTiles; none when splits == 1)
-  const float* f;         // [nc] row factors, label weights, labels
-  const float* wt;
-  const int64_t* y;
-  const int32_t* rows;    // compacted row -> original row (whole batch)
-  const int64_t* nvalid;
-  int64_t hdim, nc, c0;
-  int nI, splits, prow, run;  // hdim tiles; vocab ranges; rows of a slot; dh_run
-};
 
 // dH work: a unit is one (token tile, vocab range); its nI hdim tiles share
 // the unit's E slab, so they run as consecutive blocks on one XCD (block b
@@ -620,6 +608,8 @@ struct DhArgs {
 // or not by its place in its run and by the batch's valid-row count, on the
 // device.
 constexpr int kDhSub = 4, kXcdSlots = 32;
+}  // namespace
+
 // Splits of the dH vocab reduction: enough WGs to fill the chip several
 // rounds over, bounded by the size of the fp32 partial sums.
 int dh_splits(int64_t hdim, int64_t chunk) {
@@ -631,6 +621,8 @@ int dh_splits(int64_t hdim, int64_t chunk) {
 }
 // Token tiles whose E takes 2 GiB (the Python entry's default chunk).
 int dh_run(int64_t V) { return (int)std::max<int64_t>((int64_t(1) << 31) / (2 * BJ * V), 1); }
+
+namespace {
 
 // The token tiles of the rows [c0, c0 + nv), and where their partial sums lie:
 // splits slots for a tile with whole ranges, kDhSub times 8 for one with cut
@@ -660,6 +652,8 @@ __device__ __forceinline__ DhTiles dh_tiles(int64_t nvalid, int64_t c0, int64_t 
   T.last = cut(T.nj % run);
   return T;
 }
+}  // namespace
+
 // Slots, also units, that the rows [c0, c0 + nc) can need.
 int64_t dh_slots(int64_t c0, int64_t nc, int nI, int splits, int run) {
   const int64_t t0 = c0 / BJ, t1 = (c0 + nc + BJ - 1) / BJ, tiles = t1 - t0;
@@ -667,6 +661,8 @@ int64_t dh_slots(int64_t c0, int64_t nc, int nI, int splits, int run) {
   const int64_t cut = std::min<int64_t>(run, (kXcdSlots - 1 + nI - 1) / nI) * ((t1 - 1) / run - t0 / run + 1);
   return kXcds * (tiles + (kDhSub - 1) * std::min(tiles, cut));
 }
+
+namespace {
 
 __global__ __launch_bounds__(NT) void flce_dh_kernel(const DhArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
@@ -787,19 +783,6 @@ __global__ __launch_bounds__(256) void flce_dh_sum_kernel(const DhArgs p) {
 }
 
 // ---------------------------------------------------------------- dW
-struct DwArgs {
-  GOp Ht;        // hidden rows of the chunk [nc, hdim], scaled by f, read as A[i = h][k = tok]
-  GOp Et;        // E [nc, V] read as B[j = v][k = tok]
-  const int32_t* slot;   // [V] label terms: row of lsum + 1, or 0
-  const int32_t* next;   // [rows] the label's next row of lsum + 1, or 0
-  const float* lsum;     // [rows, hdim]
-  bf16* dw;      // [V, hdim]
-  float* acc32;  // [V, hdim] fp32 accumulator across chunks
-  const int64_t* nvalid;
-  int64_t hdim, V, c0, chunk;
-  int nI, nJ;
-  int two_in_bf16;  // over two chunks the first one's sum waits in dw
-};
 
 __global__ __launch_bounds__(NT) void flce_dw_kernel(const DwArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
@@ -1060,8 +1043,6 @@ struct Layout {
   int nsort;  // sorted runs of a chunk's labels (dW only)
 };
 
-size_t al(size_t x) { return (x + 255) & ~size_t(255); }
-
 // need_dh false: loss only (no E, no gradient buffers); its chunks only bound
 // the per-(row, vocab tile) sum buffers, so they are large.
 constexpr int64_t kLossChunk = 32768;
@@ -1138,25 +1119,6 @@ Layout layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool need_dh, b
 // sorted, as the row pass does.  Rows are read from the caller's hidden states
 // in their original order and written compacted; zero rows follow the valid
 // ones up to the k-step in which dW ends.
-struct WeighArgs {
-  const bf16* H;          // [n, hdim] all rows
-  const int32_t* rows;    // chunk's compacted row -> row of H
-  const int64_t* y;       // chunk labels
-  const float* f0;        // [nc]
-  const float* w0;
-  const float* g;         // [n] upstream gradients, by original row
-  const int64_t* nvalid;
-  const int64_t* labels;  // [n] all labels, with dh: rows that do not count are zeroed
-  bf16* dh;               // or nullptr
-  bf16* Hs;               // [nc, hdim] (nsort > 0)
-  float* f;               // [nc]
-  float* wt;
-  uint64_t* keys;         // [nsort, kIdChunk]
-  int32_t* slot;          // [V] cleared
-  int64_t n, nc, c0, V, hdim, ignore_index;
-  float scale;            // -1 / temperature
-  int nsort;              // sorting workgroups (0 without dW)
-};
 __global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs p) {
   constexpr int NWR = kRowThreads / 64;
   __shared__ uint64_t sk[kIdChunk];
@@ -1174,7 +1136,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs
     for (int64_t k = blk * NWR + w; k < end; k += nblk * NWR) {
       const bool real = k < nv;
       const int64_t src = real ? p.rows[k] : 0;
-      const float f = real ? p.f0[k] * (p.scale * p.g[src]) : 0.f;
+      const float f = real ? p.f0[k] * (p.g != nullptr ? p.scale * p.g[src] : p.scale) : 0.f;
       for (int64_t c = lane; c < nvec; c += 64) {
         bf16x8 x = zero_bf16x8();
         if (real) {
@@ -1187,7 +1149,7 @@ __global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs
     }
   }
   for (int64_t k = blk * kRowThreads + tid; k < nv; k += nblk * kRowThreads) {
-    const float g = p.scale * p.g[p.rows[k]];
+    const float g = p.g != nullptr ? p.scale * p.g[p.rows[k]] : p.scale;
     p.f[k] = p.f0[k] * g;
     p.wt[k] = p.w0[k] * g;
   }
@@ -1206,78 +1168,18 @@ __global__ __launch_bounds__(kRowThreads) void flce_weigh_kernel(const WeighArgs
 // would be padding.  Smaller stages let two workgroups share a CU, so loads are
 // in flight while the other one waits at a barrier, and the last round of tiles,
 // which leaves CUs idle, is short.
-constexpr int kFewBI = 128, kFewThreads = 256;  // weight rows or features of a tile; threads of its workgroup
-
-// One k-step's loads of an operand with k contiguous: ROWS rows x 64 k (swizzled
-// as gemm.h's KC halves), 8 rows an instruction, dealt over NWV waves.
-template <int ROWS, int NWV>
-struct FewRows {
-  static constexpr int PER = ROWS / 8 / NWV;
-  uint32_t off[PER];
-  __device__ __forceinline__ void init(int64_t ld, int64_t last, int lane, int w) {
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int r = 8 * (PER * w + q) + lane / 8;
-      off[q] = 2 * (uint32_t)(min((int64_t)r, last) * ld + 8 * ((lane % 8) ^ swz_kc(r)));
-    }
-  }
-  __device__ __forceinline__ void issue(const bf16* base, bf16* lds, int wu) const {
-#pragma unroll
-    for (int q = 0; q < PER; ++q) dma16(base, off[q], lds + (PER * wu + q) * 512);
-  }
-};
-
-// The k-steps s of n of a few-rows product through STAGES buffers: issue(s, b)
-// asks for step s into buffer b (PER loads a wave), step(s, b) multiplies it.
-// With three buffers two steps are loading at any time, and one barrier a step
-// does: behind it every wave has read the buffer that the next loads go to.
-template <int STAGES, int PER, class I, class C>
-__device__ __forceinline__ void few_steps(int n, I issue, C step) {
-  static_assert(STAGES == 2 || STAGES == 3, "two or three buffers");
-  if (n <= 0) return;
-  issue(0, 0);
-  if constexpr (STAGES == 2) {
-    for (int s = 0; s < n; ++s) {
-      if (s + 1 < n) {
-        issue(s + 1, (s + 1) & 1);
-        wait_vmcnt<PER>();
-      } else {
-        wait_vmcnt<0>();
-      }
-      phase_barrier();
-      step(s, s & 1);
-      wait_lds();
-      phase_barrier();
-    }
-  } else {
-    if (n > 1) issue(1, 1);
-    int b = 0;
-    for (int s = 0; s < n; ++s) {
-      if (s + 1 < n)
-        wait_vmcnt<PER>();
-      else
-        wait_vmcnt<0>();
-      phase_barrier();
-      if (s + 2 < n) issue(s + 2, b == 0 ? 2 : b - 1);
-      step(s, b);
-      wait_lds();
-      b = b == 2 ? 0 : b + 1;
-    }
-    phase_barrier();
-  }
-}
-
 // Rows of a call (NB = 2: 64) that take these kernels.  Forward and dH with a
 // frozen head over 151936 columns of 896: 48 rows 56 and 51 us, 128 rows 81 and
 // 70 us, 129 rows (the general kernels, which take as long for fewer) 113 and 103.
-constexpr int kFewRows = 128;
+static_assert(kFewRows == 128, "64 G rows of launch_compact's few-rows kernel");
 
 // The logits kernel over 128 vocabulary rows x 32 NB rows of the call: four
 // waves, 32 vocabulary rows each.  Same outputs; always with the label apart.
 // Bound by reading the weight: 48 rows over 151936 x 896 44.6 us, 6.1 TB/s; 52.6
 // with tiles of 256 rows in two buffers, whose last 82 tiles ran by themselves.
 // (128 rows of the call: two buffers, for two workgroups a CU; 60 us.)
-template <int NB>
+// LISTS: as flce_logits_kernel's.
+template <int NB, bool LISTS>
 __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const LogitsArgs p) {
   constexpr int TOK = 32 * NB, STAGE = (kFewBI + TOK) * BK, NWV = kFewThreads / 64, STAGES = NB <= 2 ? 3 : 2;
   __shared__ __align__(16) bf16 smem[STAGES * STAGE];
@@ -1299,13 +1201,19 @@ __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const Logi
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = zero16();
   float ref[NB];
-  int rel[NB];  // the token's label, counted from vbase (-1: not in this wave's rows)
+  int rel[NB], end[NB];  // the token's label, counted from vbase (-1: not in this wave's rows)
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = min((int64_t)(32 * b + l32), p.nc - 1);
     ref[b] = p.ref[tok];
-    const int64_t d = p.y[tok] - vbase;
-    rel[b] = d >= 0 && d < 32 && (d & 8) == 0 ? (int)d : -1;
+    if constexpr (LISTS) {
+      const uint8_t* first = p.first + tok * p.ldt + blockIdx.x;
+      rel[b] = first[0];
+      end[b] = first[1];
+    } else {
+      const int64_t d = p.y[tok] - vbase;
+      rel[b] = d >= 0 && d < 32 && (d & 8) == 0 ? (int)d : -1;
+    }
   }
   few_steps<STAGES, la.PER + lb.PER>(
       (int)(p.W.cols / BK),
@@ -1352,16 +1260,25 @@ __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const Logi
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
-    const bool tv = tok < p.nc, hit = tv && rel[b] >= 0;
-    if (__any(hit)) {
-      float zsel = 0.f;
+    const bool tv = tok < p.nc;
+    for (int at = LISTS ? rel[b] : 0; LISTS ? __any(tv && at < end[b]) : at == 0; ++at) {
+      bool hit = tv && rel[b] >= 0;
+      int d = rel[b];
+      if constexpr (LISTS) {
+        hit = tv && at < end[b];
+        d = hit ? (int)((p.ids[tok * p.ldk + at] & kIdMask) - vbase) : 0;
+        hit = hit && d >= 0 && d < 32 && (d & 8) == 0;
+      }
+      if (__any(hit)) {
+        float zsel = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (hit && rel[b] == 16 * (r >> 3) + (r & 7)) {
-          zsel = acc[b][r];
-          acc[b][r] = -INFINITY;
-        }
-      if (hit) p.zy[tok] = __builtin_fmaf(zsel, p.zscale, -ref[b]);
+        for (int r = 0; r < 16; ++r)
+          if (hit && d == 16 * (r >> 3) + (r & 7)) {
+            zsel = acc[b][r];
+            acc[b][r] = -INFINITY;
+          }
+        if (hit) (LISTS ? p.zk[tok * p.ldk + at] : p.zy[tok]) = __builtin_fmaf(zsel, p.zscale, -ref[b]);
+      }
     }
     const float sum = numerators(b, ref[b], p.store_e && tv);
     if (h == 0) red[w * TOK + 32 * b + l32] = sum;
@@ -1417,10 +1334,12 @@ __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const Logi
 // columns of E, follow one another there.  Bound by reading the weight: 48 rows
 // over 151936 x 896 45.4 us, 6.0 TB/s; three buffers take as long as two.
 constexpr int kFewPerXcd = 64;
+}  // namespace
 int few_splits(int64_t hdim, int64_t V) {
   const int64_t nI = (hdim + kFewBI - 1) / kFewBI, steps = (V + BK - 1) / BK;
   return (int)(kXcds * std::min(std::max<int64_t>(kFewPerXcd / nI, 1), (steps + kXcds - 1) / kXcds));
 }
+namespace {
 template <int NB>
 __global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p) {
   constexpr int TOK = 32 * NB, STAGE = (kFewBI + TOK) * BK, NWV = kFewThreads / 64, QA = 16 / NWV;
@@ -1508,15 +1427,6 @@ __global__ __launch_bounds__(kFewThreads) void flce_dh_few_kernel(const DhArgs p
 // The sum over the ranges, with the row's factor and label term: a workgroup a
 // row and 256 features, thirty-two lanes of 8 features x eight that share the
 // ranges.  Row r of the call is cleared where it does not count.
-struct FewSumArgs {
-  DhArgs dh;
-  const float* f0;        // as WeighArgs: dH alone needs no pass of its own for them
-  const float* w0;
-  const float* g;
-  const int64_t* labels;  // of all rows, or nullptr: nothing is cleared
-  int64_t ignore_index;
-  float scale;
-};
 __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const FewSumArgs a) {
   __shared__ __align__(16) float sh[8][32][8];
   const DhArgs& p = a.dh;
@@ -1543,7 +1453,7 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const FewSumArgs a
   if (q != 0 || col >= p.hdim) return;
   const int64_t row = p.rows[p.c0 + r];
   const bf16x8 l = ld_bf16x8(p.Wt.base + p.y[r] * p.hdim + col);
-  const float gr = a.scale * a.g[row], f = a.f0[r] * gr, wt = a.w0[r] * gr;
+  const float gr = a.g != nullptr ? a.scale * a.g[row] : a.scale, f = a.f0[r] * gr, wt = a.w0[r] * gr;
   bf16x8 o;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -1764,27 +1674,63 @@ __global__ __launch_bounds__(256) void flce_few_rows_kernel(const bf16* __restri
     for (int64_t c = lane; c < nvec; c += 64) st_bf16x8(dh + (int64_t)k * hdim + 8 * c, zero_bf16x8());
 }
 
-// ---------------------------------------------------------------- launches
-int tile_log(int columns) { return __builtin_ctz((unsigned)columns / 8); }
-
 unsigned row_blocks(int64_t n) { return (unsigned)std::min<int64_t>((n + 3) / 4, 4096); }
 
-void launch_logits(LogitsArgs& lg, hipStream_t stream) {
+}  // namespace
+
+// ---------------------------------------------------------------- launches
+void launch_compact(const CompactArgs& a, hipStream_t stream) {
+  if (a.n > 0 && a.n <= kFewRows) {
+    hipLaunchKernelGGL(flce_few_rows_kernel, dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, stream, a.hidden, a.weight,
+                       a.labels, (int)a.n, a.hdim, a.vocab, a.ignore_index, a.zscale, a.rows, a.nvalid, a.count, a.bad,
+                       a.hc, a.yc, a.ref, a.dh, a.logp);
+    return;
+  }
+  hipLaunchKernelGGL(flce_compact_kernel, dim3(1), dim3(1024), 0, stream, a.labels, a.n, a.vocab, a.ignore_index,
+                     a.reduction, a.divisor, a.rows, a.nvalid, a.count, a.bad, a.invden);
+  if (a.n > 0)
+    hipLaunchKernelGGL(flce_gather_kernel, dim3(row_blocks(a.n)), dim3(256), 0, stream, a.hidden, a.weight, a.labels,
+                       a.rows, a.nvalid, a.n, a.hdim, a.vocab, a.ignore_index, a.zscale, a.hc, a.yc, a.ref, a.dh, a.logp);
+}
+
+void launch_logits(LogitsArgs& lg, bool few, bool lists, hipStream_t stream) {
+  if (few) {
+    const dim3 grid((unsigned)((lg.V + kFewBI - 1) / kFewBI));
+    const bool two = lg.nc <= 64;
+    if (lists)
+      hipLaunchKernelGGL((two ? flce_logits_few_kernel<2, true> : flce_logits_few_kernel<4, true>), grid, dim3(kFewThreads), 0,
+                         stream, lg);
+    else
+      hipLaunchKernelGGL((two ? flce_logits_few_kernel<2, false> : flce_logits_few_kernel<4, false>), grid, dim3(kFewThreads),
+                         0, stream, lg);
+    return;
+  }
   lg.nI = (int)((lg.V + kVT - 1) / kVT);
   lg.nJ = (int)((lg.nc + BJ - 1) / BJ);
   const int grid = ((lg.nI * lg.nJ + kXcds - 1) / kXcds) * kXcds;
-  hipLaunchKernelGGL(flce_logits_kernel, dim3(grid), dim3(NT), 0, stream, lg);
+  hipLaunchKernelGGL((lists ? flce_logits_kernel<true> : flce_logits_kernel<false>), dim3(grid), dim3(NT), 0, stream, lg);
 }
 
-void launch_row(RowArgs& rw, hipStream_t stream, bool few = false) {
+void launch_row(RowArgs& rw, bool few, bool lists, hipStream_t stream) {
   const int rows = few ? kFewRowRows : kRowRows;
   const int64_t groups = (rw.nc + rows - 1) / rows;
   rw.parts = rw.grads ? (int)std::max<int64_t>(kRowGroups / groups, 1) : 1;
   const dim3 grid((unsigned)(rw.nsort + groups * rw.parts));
   if (few)
-    hipLaunchKernelGGL(flce_row_kernel<kFewRowRows>, grid, dim3(kRowThreads), 0, stream, rw);
+    hipLaunchKernelGGL((lists ? flce_row_kernel<kFewRowRows, true> : flce_row_kernel<kFewRowRows, false>), grid,
+                       dim3(kRowThreads), 0, stream, rw);
   else
-    hipLaunchKernelGGL(flce_row_kernel<kRowRows>, grid, dim3(kRowThreads), 0, stream, rw);
+    hipLaunchKernelGGL((lists ? flce_row_kernel<kRowRows, true> : flce_row_kernel<kRowRows, false>), grid,
+                       dim3(kRowThreads), 0, stream, rw);
+}
+
+void launch_weigh(const WeighArgs& wg, hipStream_t stream) {
+  const int64_t blocks = std::min<int64_t>((wg.nc + kRowThreads / 64 - 1) / (kRowThreads / 64), 1024);
+  hipLaunchKernelGGL(flce_weigh_kernel, dim3((unsigned)(wg.nsort + blocks)), dim3(kRowThreads), 0, stream, wg);
+}
+
+void launch_labels(const LabelArgs& la, int64_t nc, hipStream_t stream) {
+  hipLaunchKernelGGL(flce_label_kernel, dim3((unsigned)nc), dim3(256), 0, stream, la);
 }
 
 void launch_dh(DhArgs& dh, hipStream_t stream) {
@@ -1795,14 +1741,6 @@ void launch_dh(DhArgs& dh, hipStream_t stream) {
   if (dh.splits == 1) return;
   const int64_t blocks = std::min<int64_t>((dh.nc * dh.hdim / 8 + 255) / 256, 4096);
   hipLaunchKernelGGL(flce_dh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, dh);
-}
-
-void launch_logits_few(LogitsArgs& lg, hipStream_t stream) {
-  const dim3 grid((unsigned)((lg.V + kFewBI - 1) / kFewBI));
-  if (lg.nc <= 64)
-    hipLaunchKernelGGL(flce_logits_few_kernel<2>, grid, dim3(kFewThreads), 0, stream, lg);
-  else
-    hipLaunchKernelGGL(flce_logits_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, lg);
 }
 
 void launch_dh_few(FewSumArgs& a, hipStream_t stream) {
@@ -1817,17 +1755,17 @@ void launch_dh_few(FewSumArgs& a, hipStream_t stream) {
                      a);
 }
 
-void launch_dw_few(DwArgs& dw, hipStream_t stream) {
-  dw.nI = (int)((dw.hdim + 127) / 128);
-  dw.nJ = (int)((dw.V + 127) / 128);
-  const int parts = (dw.nI + kDwTiles - 1) / kDwTiles, grid = ((parts * dw.nJ + kXcds - 1) / kXcds) * kXcds;
-  if (dw.Ht.rows <= BK)
-    hipLaunchKernelGGL(flce_dw_few_kernel<1>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
-  else
-    hipLaunchKernelGGL(flce_dw_few_kernel<2>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
-}
-
-void launch_dw(DwArgs& dw, hipStream_t stream) {
+void launch_dw(DwArgs& dw, bool few, hipStream_t stream) {
+  if (few) {
+    dw.nI = (int)((dw.hdim + 127) / 128);
+    dw.nJ = (int)((dw.V + 127) / 128);
+    const int parts = (dw.nI + kDwTiles - 1) / kDwTiles, grid = ((parts * dw.nJ + kXcds - 1) / kXcds) * kXcds;
+    if (dw.Ht.rows <= BK)
+      hipLaunchKernelGGL(flce_dw_few_kernel<1>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
+    else
+      hipLaunchKernelGGL(flce_dw_few_kernel<2>, dim3(grid), dim3(kFewThreads), 0, stream, dw);
+    return;
+  }
   dw.nI = (int)((dw.hdim + BI - 1) / BI);
   dw.nJ = (int)((dw.V + kVT - 1) / kVT);
   const int grid = ((dw.nI * dw.nJ + kXcds - 1) / kXcds) * kXcds;
@@ -1839,8 +1777,6 @@ void launch_zero(bf16* x, int64_t numel, hipStream_t stream) {
   const int64_t nvec = numel / 8, blocks = std::min<int64_t>((nvec + 255) / 256, 4096);
   hipLaunchKernelGGL(zero_bf16_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, x, nvec);
 }
-
-}  // namespace
 
 size_t flce_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dh, bool need_dw) {
   if (chunk <= 0) return 0;
@@ -1903,7 +1839,7 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     lg.ldp = L.chunk;
     lg.store_e = grads ? 1 : 0;
     lg.zscale = kLog2e;
-    launch_logits(lg, stream);
+    launch_logits(lg, false, false, stream);
 
     RowArgs rw{};
     rw.mpart = mpart;
@@ -1929,7 +1865,7 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
     rw.ldp = L.chunk;
     rw.nsort = L.nsort;
     rw.grads = grads ? 1 : 0;
-    launch_row(rw, stream);
+    launch_row(rw, false, false, stream);
     if (!grads) continue;
     auto label_sums = [&]() {
       LabelArgs la{};
@@ -1942,7 +1878,7 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
       la.next = next;
       la.hdim = Hd;
       la.nsort = L.nsort;
-      hipLaunchKernelGGL(flce_label_kernel, dim3((unsigned)nc), dim3(256), 0, stream, la);
+      launch_labels(la, nc, stream);
     };
     // dH may take the place of the hidden states: then they are read before it is written (otherwise right before
     // dW, which finds the sums in the caches: 300 x 4096 over 128256 columns 1134 us, 1153 in the other order)
@@ -1983,7 +1919,7 @@ hipError_t flce_run(const FlceArgs& a, hipStream_t stream) {
       dw.V = V;
       dw.chunk = L.chunk;
       dw.two_in_bf16 = 1;
-      launch_dw(dw, stream);
+      launch_dw(dw, false, stream);
     }
   }
   if (grads && a.n == 0 && a.dweight != nullptr) launch_zero(a.dweight, V * Hd, stream);
@@ -2070,31 +2006,31 @@ FlpLayout flp_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool log
   return L;
 }
 
-template <class T>
-T* at(void* base, size_t off) {
-  return reinterpret_cast<T*>(static_cast<char*>(base) + off);
-}
-
 float zscale_of(const FlpArgs& a) { return (float)(1.4426950408889634 / a.temperature); }
 
 // The valid rows' list and their compacted hidden states, labels and references.
 void flp_compact(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSaved& S, float* logp, int64_t* count,
                  int64_t* bad, bf16* dh, hipStream_t stream) {
-  if (a.n > 0 && a.n <= kFewRows) {
-    hipLaunchKernelGGL(flce_few_rows_kernel, dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, stream, a.hidden, a.weight,
-                       a.labels, (int)a.n, a.hdim, a.vocab, a.ignore_index, zscale_of(a), at<int32_t>(saved, S.rows),
-                       at<int64_t>(saved, S.nvalid), count, bad, at<bf16>(a.ws, L.hc), at<int64_t>(saved, S.yc),
-                       at<float>(a.ws, L.ref), dh, logp);
-    return;
-  }
-  hipLaunchKernelGGL(flce_compact_kernel, dim3(1), dim3(1024), 0, stream, a.labels, a.n, a.vocab, a.ignore_index, 0,
-                     nullptr, at<int32_t>(saved, S.rows), at<int64_t>(saved, S.nvalid), count, bad,
-                     at<float>(a.ws, L.scal));
-  if (a.n > 0)
-    hipLaunchKernelGGL(flce_gather_kernel, dim3(row_blocks(a.n)), dim3(256), 0, stream, a.hidden, a.weight, a.labels,
-                       at<int32_t>(saved, S.rows), at<int64_t>(saved, S.nvalid), a.n, a.hdim, a.vocab, a.ignore_index,
-                       zscale_of(a), at<bf16>(a.ws, L.hc), at<int64_t>(saved, S.yc),
-                       at<float>(a.ws, L.ref), dh, logp);
+  CompactArgs c{};
+  c.hidden = a.hidden;
+  c.weight = a.weight;
+  c.labels = a.labels;
+  c.n = a.n;
+  c.hdim = a.hdim;
+  c.vocab = a.vocab;
+  c.ignore_index = a.ignore_index;
+  c.zscale = zscale_of(a);
+  c.rows = at<int32_t>(saved, S.rows);
+  c.nvalid = at<int64_t>(saved, S.nvalid);
+  c.count = count;
+  c.bad = bad;
+  c.invden = at<float>(a.ws, L.scal);
+  c.hc = at<bf16>(a.ws, L.hc);
+  c.yc = at<int64_t>(saved, S.yc);
+  c.ref = at<float>(a.ws, L.ref);
+  c.dh = dh;
+  c.logp = logp;
+  launch_compact(c, stream);
 }
 
 // Logits and row pass of the chunk at c0: E (unless nullptr) with f0 and w0, logp (unless nullptr).
@@ -2118,10 +2054,7 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   lg.store_e = E != nullptr ? 1 : 0;
   lg.zscale = zscale_of(a);
   lg.label_apart = 1;
-  if (L.few)
-    launch_logits_few(lg, stream);
-  else
-    launch_logits(lg, stream);
+  launch_logits(lg, L.few, false, stream);
 
   RowArgs rw{};
   rw.mpart = lg.mpart;
@@ -2144,7 +2077,7 @@ void flp_logits(const FlpArgs& a, const FlpLayout& L, char* saved, const FlpSave
   rw.ldp = L.chunk;
   rw.grads = lg.store_e;
   rw.label_apart = 1;
-  launch_row(rw, stream, L.few);
+  launch_row(rw, L.few, false, stream);
 }
 
 }  // namespace
@@ -2212,10 +2145,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
     wg.scale = (float)(-1. / a.temperature);
     wg.nsort = L.nsort;
     const bool few_dh = L.few && L.nchunks == 1 && !need_dw;
-    if (!few_dh) {
-      const int64_t blocks = std::min<int64_t>((nc + kRowThreads / 64 - 1) / (kRowThreads / 64), 1024);
-      hipLaunchKernelGGL(flce_weigh_kernel, dim3((unsigned)(L.nsort + blocks)), dim3(kRowThreads), 0, stream, wg);
-    }
+    if (!few_dh) launch_weigh(wg, stream);
 
     if (a.dhidden != nullptr) {
       DhArgs dh{};
@@ -2259,7 +2189,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       la.next = at<int32_t>(a.ws, L.next);
       la.hdim = a.hdim;
       la.nsort = L.nsort;
-      hipLaunchKernelGGL(flce_label_kernel, dim3((unsigned)nc), dim3(256), 0, stream, la);
+      launch_labels(la, nc, stream);
       DwArgs dw{};
       dw.Ht = GOp{Hs, a.hdim, nc, a.hdim};
       dw.Et = GOp{E, a.vocab, nc, a.vocab};
@@ -2273,10 +2203,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream) {
       dw.hdim = a.hdim;
       dw.V = a.vocab;
       dw.chunk = L.chunk;
-      if (L.few && L.nchunks == 1)
-        launch_dw_few(dw, stream);
-      else
-        launch_dw(dw, stream);
+      launch_dw(dw, L.few && L.nchunks == 1, stream);
     }
   }
   return hipGetLastError();
