@@ -552,6 +552,70 @@ int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* wei
                    int64_t seqs, int64_t tokens, int aggregation, float* dlogps, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Token statistics and distillation (no reference counterpart): what a model
+ * thinks of its tokens, and the loss of a student against what a teacher thinks.
+ * Operands, rows that count, count and bad_labels as for siq_flp_fwd; logits
+ * z = hidden weight^T / temperature exist only as one chunk's.
+ *
+ * siq_stats_fwd: for each counted row logp = ln softmax(z) at the label,
+ * entropy = -sum p ln p, and with top_k > 0 (at most 128 and vocab; vocab at most
+ * 2^19) the largest logits' ids in order, equal ones by lower id first
+ * (top_ids [n, top_k]), with their log-probabilities (top_logp).  Rows that do not
+ * count have 0, and ids of -1.  A row with a NaN logit has NaN log-probabilities
+ * and ids in [0, vocab).  logp, entropy, lse [n]; lse is what siq_stats_bwd takes
+ * besides them.  top_logp and top_ids may be NULL with top_k 0.
+ * siq_stats_bwd: dhidden and / or dweight (NULL: not computed) from the upstream
+ * gradients dlogp and dentropy [n] (NULL: zero),
+ *   dz_j = dlogp ([j = label] - p_j) - dentropy p_j (ln p_j + entropy).
+ * They may not overlap hidden.  The logits are formed again, chunk_tokens rows at a
+ * time.
+ *
+ * siq_distill: ids [n, top_k] (ids_bytes 8: int64, 4: int32) name a teacher's
+ * tokens and teacher [n, top_k] their log-probabilities ln t; top_k in [1, 128].  An
+ * id of -1, or a log-probability of -infinity, names none.  An id outside the
+ * vocabulary, or named twice in a row that counts, is left out (twice: but for its
+ * first place) and counted in counts[2].  With m = sum t, r = max(1 - m, 0), s =
+ * softmax(z) at the named tokens and q its sum over all others:
+ *   SIQ_DIVERGENCE_FORWARD: D = sum t (ln t - ln s), with tail != 0 also
+ *     + r (ln r - ln q);
+ *   SIQ_DIVERGENCE_REVERSE: D = sum s (ln s - ln t) + q (ln q - ln r), r at least
+ *     2^-24; it needs a tail.
+ * (Where every token is named there is no tail.)  *loss = sum over counted rows of
+ * (1 - ce_weight) D + ce_weight CE, CE = -ln softmax(z) at the label, over the number
+ * of them, or over *divisor (a device scalar) if not NULL; *divergence and
+ * *cross_entropy its two parts, divided likewise.  ce_weight in [0, 1], and 0 where
+ * temperature is not 1.  dhidden and dweight (NULL: not computed) are the gradients
+ * of *loss; dhidden may not overlap hidden.  counts[0] = rows that count, counts[1] =
+ * bad labels.
+ * Everything in fixed orders: bitwise reproducible.
+ * ------------------------------------------------------------------------- */
+#define SIQ_DIVERGENCE_FORWARD 0
+#define SIQ_DIVERGENCE_REVERSE 1
+
+size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k);
+
+int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
+                  int64_t vocab, int64_t ignore_index, double temperature, int top_k, float* logp, float* entropy,
+                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight);
+
+int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* logp,
+                  const float* entropy, const float* lse, const float* dlogp, const float* dentropy, int64_t n,
+                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, void* dhidden, void* dweight,
+                  int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t siq_distill_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t chunk_tokens,
+                                   int need_grads, int need_dweight);
+
+int siq_distill(const void* hidden, const void* weight, const int64_t* labels, const void* ids, int ids_bytes,
+                const float* teacher, int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t ignore_index,
+                double temperature, double ce_weight, int divergence, int tail, const float* divisor, float* loss,
+                float* mean_divergence, float* mean_cross_entropy, int64_t* counts, void* dhidden, void* dweight,
+                int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement support (no reference counterpart).
  *
  * siq_probe_clock: one wave per CU spins for about spin_ticks ticks of the

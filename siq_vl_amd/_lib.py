@@ -109,6 +109,25 @@ _PROTOS = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _f64, _c_void_p, _size, _c_void_p,
          _c_void_p, _i64, _c_void_p, _size, _c_void_p],
     ),
+    "siq_stats_fwd_workspace_bytes": (_size, [_i64, _i64, _i64, _i32]),
+    "siq_stats_fwd": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _f64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
+    ),
+    "siq_stats_bwd_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i32]),
+    "siq_stats_bwd": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64,
+         _f64, _c_void_p, _c_void_p, _i64, _c_void_p, _size, _c_void_p],
+    ),
+    "siq_distill_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64, _i32, _i32]),
+    "siq_distill": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _i64, _i64, _i64, _i32, _i64, _f64, _f64, _i32,
+         _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _size,
+         _c_void_p],
+    ),
     "siq_scale_bf16": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p]),
     "siq_scale_bf16_inplace": (_i32, [_c_void_p, _i64, _c_void_p, _c_void_p]),
     "siq_proj_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64]),

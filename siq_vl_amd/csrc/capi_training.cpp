@@ -7,9 +7,11 @@
 
 #include "../../include/siq_kernels.h"
 #include "capi_internal.h"
+#include "distill.h"
 #include "flce.h"
 #include "pack8.h"
 #include "policy.h"
+#include "token_stats.h"
 
 using namespace siq_capi;
 
@@ -115,6 +117,29 @@ siq::FlpArgs flp_args(const void* hidden, const void* weight, const int64_t* lab
   a.saved = saved;
   a.ws = ws;
   return a;
+}
+
+// hidden [n, hdim] and a gradient of its shape (or NULL).
+int check_apart(const void* hidden, const void* dhidden, int64_t n, int64_t hdim) {
+  const char *h0 = static_cast<const char*>(hidden), *d0 = static_cast<const char*>(dhidden);
+  const size_t bytes = sizeof(siq::bf16) * (size_t)n * (size_t)hdim;
+  if (n > 0 && dhidden != nullptr && d0 < h0 + bytes && h0 < d0 + bytes)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "dhidden must not overlap hidden");
+  return SIQ_OK;
+}
+
+int check_grads(const void* hidden, const void* dhidden, const void* dweight, int64_t n, int64_t hdim) {
+  if (dhidden != nullptr && !aligned16(dhidden)) return fail(SIQ_ERR_ALIGNMENT, "dhidden is not 16-byte aligned");
+  if (dweight != nullptr && !aligned16(dweight)) return fail(SIQ_ERR_ALIGNMENT, "dweight is not 16-byte aligned");
+  return check_apart(hidden, dhidden, n, hdim);
+}
+
+// Alternatives of a row: at least `least`.
+int check_top_k(int top_k, int least, int64_t vocab) {
+  if (top_k < least || top_k > siq::kMaxTopK || top_k > vocab)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "top_k must be in [%d, %d] and at most the vocabulary's %lld (got %d)", least,
+                siq::kMaxTopK, (long long)vocab, top_k);
+  return SIQ_OK;
 }
 
 int launched(hipError_t e, const char* what) {
@@ -391,10 +416,7 @@ int siq_flp_bwd(const void* hidden, const void* weight, const int64_t* labels, c
   if (dhidden != nullptr && !aligned16(dhidden)) return fail(SIQ_ERR_ALIGNMENT, "dhidden is not 16-byte aligned");
   if (dweight != nullptr && !aligned16(dweight)) return fail(SIQ_ERR_ALIGNMENT, "dweight is not 16-byte aligned");
   if (dhidden == nullptr && dweight == nullptr) return ok();
-  const char *h0 = static_cast<const char*>(hidden), *d0 = static_cast<const char*>(dhidden);
-  const size_t bytes = sizeof(siq::bf16) * (size_t)n * (size_t)hdim;
-  if (n > 0 && dhidden != nullptr && d0 < h0 + bytes && h0 < d0 + bytes)
-    return fail(SIQ_ERR_INVALID_ARGUMENT, "dhidden must not overlap hidden");
+  if ((rc = check_apart(hidden, dhidden, n, hdim))) return rc;
   const size_t need = siq::flp_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, dweight != nullptr, saved != nullptr);
   if ((rc = check_ws(workspace, workspace_bytes, need))) return rc;
   siq::FlpArgs a = flp_args(hidden, weight, labels, n, hdim, vocab, ignore_index, temperature, const_cast<void*>(saved),
@@ -404,6 +426,153 @@ int siq_flp_bwd(const void* hidden, const void* weight, const int64_t* labels, c
   a.dweight = static_cast<siq::bf16*>(dweight);
   a.chunk = chunk_tokens;
   return launched(siq::flp_bwd(a, static_cast<hipStream_t>(stream)), "log-probabilities backward");
+}
+
+size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k) {
+  if (n < 0 || hdim <= 0 || vocab <= 0 || top_k < 0 || top_k > siq::kMaxTopK) return 0;
+  return siq::stats_fwd_workspace_bytes(n, hdim, vocab, top_k);
+}
+
+size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight) {
+  if (n < 0 || hdim <= 0 || vocab <= 0 || chunk_tokens <= 0) return 0;
+  return siq::stats_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, need_dweight != 0);
+}
+
+int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
+                  int64_t vocab, int64_t ignore_index, double temperature, int top_k, float* logp, float* entropy,
+                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
+      (rc = check_top_k(top_k, 0, vocab)) || (rc = check_not_null(count, "count")) ||
+      (rc = check_not_null(bad_labels, "bad_labels")))
+    return rc;
+  if (top_k > 0 && vocab > siq::kMaxTopVocab)
+    return fail(SIQ_ERR_UNSUPPORTED, "top_k needs a vocabulary of at most 2^19 (got %lld)", (long long)vocab);
+  if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
+                (rc = check_not_null(lse, "lse"))))
+    return rc;
+  if (n > 0 && top_k > 0 && ((rc = check_not_null(top_logp, "top_logp")) || (rc = check_not_null(top_ids, "top_ids"))))
+    return rc;
+  if ((rc = check_ws(workspace, workspace_bytes, siq::stats_fwd_workspace_bytes(n, hdim, vocab, top_k)))) return rc;
+  siq::StatsArgs a{};
+  a.hidden = static_cast<const siq::bf16*>(hidden);
+  a.weight = static_cast<const siq::bf16*>(weight);
+  a.labels = labels;
+  a.n = n;
+  a.hdim = hdim;
+  a.vocab = vocab;
+  a.ignore_index = ignore_index;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.logp = logp;
+  a.entropy = entropy;
+  a.lse = lse;
+  a.top_logp = top_logp;
+  a.top_ids = top_ids;
+  a.count = count;
+  a.bad_labels = bad_labels;
+  a.ws = workspace;
+  return launched(siq::stats_fwd(a, static_cast<hipStream_t>(stream)), "token statistics");
+}
+
+int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* logp,
+                  const float* entropy, const float* lse, const float* dlogp, const float* dentropy, int64_t n,
+                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, void* dhidden, void* dweight,
+                  int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0))) return rc;
+  if (chunk_tokens <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "chunk_tokens must be positive");
+  if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
+                (rc = check_not_null(lse, "lse"))))
+    return rc;
+  if ((rc = check_grads(hidden, dhidden, dweight, n, hdim))) return rc;
+  if (dhidden == nullptr && dweight == nullptr) return ok();
+  if ((rc = check_ws(workspace, workspace_bytes,
+                     siq::stats_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, dweight != nullptr))))
+    return rc;
+  siq::StatsArgs a{};
+  a.hidden = static_cast<const siq::bf16*>(hidden);
+  a.weight = static_cast<const siq::bf16*>(weight);
+  a.labels = labels;
+  a.n = n;
+  a.hdim = hdim;
+  a.vocab = vocab;
+  a.ignore_index = ignore_index;
+  a.temperature = temperature;
+  a.logp = const_cast<float*>(logp);
+  a.entropy = const_cast<float*>(entropy);
+  a.lse = const_cast<float*>(lse);
+  a.dlogp = dlogp;
+  a.dentropy = dentropy;
+  a.dhidden = static_cast<siq::bf16*>(dhidden);
+  a.dweight = static_cast<siq::bf16*>(dweight);
+  a.chunk = chunk_tokens;
+  a.ws = workspace;
+  return launched(siq::stats_bwd(a, static_cast<hipStream_t>(stream)), "token statistics backward");
+}
+
+size_t siq_distill_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t chunk_tokens,
+                                   int need_grads, int need_dweight) {
+  if (n < 0 || hdim <= 0 || vocab <= 0 || chunk_tokens <= 0 || top_k < 1 || top_k > siq::kMaxTeacher) return 0;
+  return siq::distill_workspace_bytes(n, hdim, vocab, top_k, chunk_tokens, need_grads != 0, need_dweight != 0);
+}
+
+int siq_distill(const void* hidden, const void* weight, const int64_t* labels, const void* ids, int ids_bytes,
+                const float* teacher, int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t ignore_index,
+                double temperature, double ce_weight, int divergence, int tail, const float* divisor, float* loss,
+                float* mean_divergence, float* mean_cross_entropy, int64_t* counts, void* dhidden, void* dweight,
+                int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
+      (rc = check_top_k(top_k, 1, vocab)))
+    return rc;
+  if (ids_bytes != 4 && ids_bytes != 8)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "ids_bytes must be 8 (int64) or 4 (int32), got %d", ids_bytes);
+  if (divergence != SIQ_DIVERGENCE_FORWARD && divergence != SIQ_DIVERGENCE_REVERSE)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "divergence must be SIQ_DIVERGENCE_FORWARD or _REVERSE");
+  if (divergence == SIQ_DIVERGENCE_REVERSE && !tail)
+    return fail(SIQ_ERR_UNSUPPORTED, "the reverse divergence needs the tail: without it, it has no least value");
+  if (!(ce_weight >= 0. && ce_weight <= 1.)) return fail(SIQ_ERR_INVALID_ARGUMENT, "ce_weight must be in [0, 1]");
+  if (ce_weight != 0. && temperature != 1.)
+    return fail(SIQ_ERR_UNSUPPORTED, "ce_weight goes with temperature 1 only: labels are not softened");
+  if (n > 0 && ((rc = check_not_null(ids, "ids")) || (rc = check_not_null(teacher, "teacher")))) return rc;
+  if ((rc = check_not_null(loss, "loss")) || (rc = check_not_null(mean_divergence, "mean_divergence")) ||
+      (rc = check_not_null(mean_cross_entropy, "mean_cross_entropy")) || (rc = check_not_null(counts, "counts")))
+    return rc;
+  if (chunk_tokens <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "chunk_tokens must be positive");
+  if ((rc = check_grads(hidden, dhidden, dweight, n, hdim))) return rc;
+  siq::DistillArgs a{};
+  a.grads = dhidden != nullptr || dweight != nullptr;
+  if ((rc = check_ws(workspace, workspace_bytes,
+                     siq::distill_workspace_bytes(n, hdim, vocab, top_k, chunk_tokens, a.grads, dweight != nullptr))))
+    return rc;
+  a.hidden = static_cast<const siq::bf16*>(hidden);
+  a.weight = static_cast<const siq::bf16*>(weight);
+  a.labels = labels;
+  a.ids = ids;
+  a.teacher = teacher;
+  a.n = n;
+  a.hdim = hdim;
+  a.vocab = vocab;
+  a.ignore_index = ignore_index;
+  a.top_k = top_k;
+  a.ids32 = ids_bytes == 4;
+  a.reverse = divergence == SIQ_DIVERGENCE_REVERSE;
+  a.tail = tail != 0;
+  a.temperature = temperature;
+  a.ce_weight = ce_weight;
+  a.reduction = divisor != nullptr;
+  a.divisor = divisor;
+  a.loss = loss;
+  a.divergence = mean_divergence;
+  a.cross_entropy = mean_cross_entropy;
+  a.counts = counts;
+  a.dhidden = static_cast<siq::bf16*>(dhidden);
+  a.dweight = static_cast<siq::bf16*>(dweight);
+  a.chunk = chunk_tokens;
+  a.ws = workspace;
+  return launched(siq::distill_run(a, static_cast<hipStream_t>(stream)), "distillation");
 }
 
 }  // extern "C"

@@ -1,0 +1,649 @@
+// Distillation from a teacher's most probable tokens, from the student's hidden
+// states and without logits, forward and backward, for gfx950.
+//
+// A row's teacher names K tokens with log-probabilities ln t_k; m = sum t_k, and
+// r = max(1 - m, 0) is what it leaves to all others, its tail.  The student's
+// p = softmax(h W^T / temperature) is s_k at those tokens and q elsewhere.
+//   forward:  D = sum t_k (ln t_k - ln s_k) + r (ln r - ln q)   (the second term with a tail)
+//   reverse:  D = sum s_k (ln s_k - ln t_k) + q (ln q - ln r),  r at least 2^-24
+//   loss = sum over rows of ((1 - c) D + c CE) / den,  CE = -ln p_y.
+// All tokens outside the list have the same dD/dz_j / p_j = O, so the gradient is a
+// row factor times the softmax numerators, but for a few tokens a row:
+//   forward:  O = m + r - r / q (tail) or m,  inside: p_k (m + r) - t_k or p_k m - t_k
+//   reverse:  O = ln q - ln r - D,            inside: p_k (ln p_k - ln t_k - D),
+// and with the label  dz = (1 - c) dD/dz + c (p - [y]).
+//
+// The products are the fused cross-entropy's, over chunks of compacted rows:
+//  1. lists: a row's tokens (the label among them) sorted by id, and how many of
+//     them lie before each tile of the vocabulary;
+//  2. logits GEMM: softmax numerators E in bf16 and their sums per tile without the
+//     listed tokens, whose logits it leaves in fp32: what is outside the list is
+//     never a difference from 1;
+//  3. sums over the tiles; then, a wave a row, the losses and gradients of the row in
+//     64 bits.  The gradient of the listed token with the largest one is kept in
+//     fp32 and added by the products' kernels as a label's is; the others' are put
+//     in their places in E, divided by the row's factor;
+//  4. dH = f (E W) + w W[y'],  dW = (f H)^T E + the sums of w H by token.
+// (All listed tokens in fp32 would take gathers of rows x K rows of W and of H.)
+#include <algorithm>
+
+#include "distill.h"
+#include "flce_launch.h"
+#include "gemm.h"
+#include "ids.h"
+
+namespace siq {
+
+namespace {
+
+using namespace gemm;
+
+// What a list's entry is: a token of the teacher, the label where the teacher does
+// not name it, or one that repeats another.
+enum Kind { kTeacher = 0, kLabelOnly = 1, kDead = 2 };
+constexpr int kKindShift = 24;
+constexpr int kListLanes = 3, kListMost = 64 * kListLanes;  // entries a lane; of a row
+static_assert(kMaxTeacher + 1 <= kListMost, "the label behind the teacher's tokens");
+
+// ---------------------------------------------------------------- lists
+struct ListArgs {
+  const void* ids;        // [n, K]
+  const float* teacher;   // [n, K]
+  const int32_t* rows;    // [nc]
+  const int64_t* y;       // [nc]
+  const int64_t* nvalid;
+  int32_t* out;           // [nc, ldk] ids with kinds, in order of ids
+  float* lt;              // [nc, ldk] the teacher's log-probabilities
+  uint8_t* first;         // [nc, ldt] entries before each tile
+  int32_t* len;           // [nc]
+  int32_t* bad;           // [nc] tokens outside the vocabulary, or named twice
+  int64_t nc, c0, V, nvt;
+  int K, ldk, ldt, vt;    // vt: columns of a tile
+};
+
+// A wave a row.  Keys are id * 256 + place (the label's place is 255: behind a
+// teacher's same token), unique, and their ranks are counted.  Tokens of
+// probability zero and ids of -1 are not there.
+template <class ID>
+__global__ __launch_bounds__(256) void distill_list_kernel(const ListArgs p) {
+  constexpr uint32_t kNone = ~0u;
+  __shared__ uint32_t key_sh[4][kListMost], sorted_sh[4][kListMost];
+  __shared__ float lt_sh[4][kListMost];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t k = (int64_t)blockIdx.x * 4 + w, nv = min(p.nc, *p.nvalid - p.c0);
+  const bool real = k < nv;
+  uint32_t* key = key_sh[w];
+  uint32_t mine[kListLanes];
+  float lt[kListLanes];
+  int nbad = 0;
+  if (real) {
+    const int64_t src = (int64_t)p.rows[k] * p.K;
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i) {
+      const int e = lane + 64 * i;
+      mine[i] = kNone;
+      lt[i] = -INFINITY;
+      bool wrong = false;
+      if (e < p.K) {
+        const int64_t id = static_cast<const ID*>(p.ids)[src + e];
+        lt[i] = p.teacher[src + e];
+        wrong = id != -1 && (id < 0 || id >= p.V);
+        if (id >= 0 && id < p.V && lt[i] != -INFINITY) mine[i] = (uint32_t)id << 8 | (uint32_t)e;
+      } else if (e == p.K) {
+        mine[i] = (uint32_t)p.y[k] << 8 | 255u;
+      }
+      nbad += __popcll(__ballot(wrong));
+      key[e] = mine[i];
+    }
+  }
+  __syncthreads();
+  int n = 0;
+  if (real) {
+    int rank[kListLanes] = {};
+    for (int j = 0; j <= p.K; ++j) {
+      const uint32_t x = key[j];
+#pragma unroll
+      for (int i = 0; i < kListLanes; ++i) rank[i] += x < mine[i] ? 1 : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i) {
+      n += __popcll(__ballot(mine[i] != kNone));
+      if (mine[i] == kNone) continue;
+      sorted_sh[w][rank[i]] = mine[i];
+      lt_sh[w][rank[i]] = lt[i];
+    }
+  }
+  __syncthreads();
+  if (k >= p.nc) return;
+  if (real) {
+    int32_t* out = p.out + k * p.ldk;
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i) {
+      const int e = lane + 64 * i;
+      bool twice = false;
+      if (e < n) {
+        const uint32_t x = sorted_sh[w][e], id = x >> 8;
+        const bool label = (x & 255u) == 255u, same = e > 0 && (sorted_sh[w][e - 1] >> 8) == id;
+        twice = same && !label;
+        out[e] = (int32_t)(id | (uint32_t)(same ? kDead : label ? kLabelOnly : kTeacher) << kKindShift);
+        p.lt[k * p.ldk + e] = lt_sh[w][e];
+      }
+      nbad += __popcll(__ballot(twice));
+    }
+    if (lane == 0) {
+      p.len[k] = n;
+      p.bad[k] = nbad;
+    }
+  }
+  // (rows that fill up a tile have no entries)
+  for (int64_t t = lane; t <= p.nvt; t += 64) {
+    const uint32_t bound = (uint32_t)(t * p.vt) << 8;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (sorted_sh[w][mid] < bound)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    p.first[k * p.ldt + t] = (uint8_t)lo;
+  }
+}
+
+// ---------------------------------------------------------------- rows
+struct RowMathArgs {
+  const int32_t* ids;     // [nc, ldk] with kinds
+  const float* lt;        // [nc, ldk]
+  const float* zk;        // [nc, ldk] log2 units, relative to ref
+  const int32_t* len;     // [nc]
+  const float* ref;       // [nc]
+  const float* rsum;      // [nc] sum over the tokens that are not listed, relative to rtop
+  const float* rtop;
+  const int64_t* y;       // [nc]
+  const int64_t* nvalid;
+  const float* divisor;   // nullptr: the rows that count
+  bf16* E;                // [nc, V] or nullptr: losses alone
+  float* f;               // [nc] factor of E
+  float* w;               // [nc] the largest gradient of a listed token, and
+  int64_t* at;            // [nc] whose it is
+  double* loss;           // [3, n] by compacted row: loss, divergence, cross-entropy
+  int64_t nc, c0, n, V;
+  int ldk;
+  bool reverse, tail;
+  double c, inv_t;
+};
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ double wave_max(double x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x = fmax(x, __shfl_xor(x, o));
+  return x;
+}
+
+__global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
+  constexpr double kLn2d = 0.6931471805599453;
+  const int lane = threadIdx.x & 63;
+  const int64_t counted = *p.nvalid, nv = min(p.nc, counted - p.c0);
+  const int64_t k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (k >= nv) return;
+  const int n = p.len[k];
+  const int64_t y = p.y[k];
+  const double ref = p.ref[k], rtop = p.rtop[k], rsum = p.rsum[k];
+  int id[kListLanes], kind[kListLanes];
+  double l2[kListLanes], lt[kListLanes];  // ln p in log2 units, ln t
+  double top = rtop;
+#pragma unroll
+  for (int i = 0; i < kListLanes; ++i) {
+    const int e = lane + 64 * i;
+    id[i] = -1;
+    kind[i] = kDead;
+    l2[i] = lt[i] = -INFINITY;
+    if (e >= n) continue;
+    const int32_t x = p.ids[k * p.ldk + e];
+    id[i] = x & kIdMask;
+    kind[i] = x >> kKindShift;
+    if (kind[i] == kDead) continue;
+    l2[i] = ref + (double)p.zk[k * p.ldk + e];
+    lt[i] = p.lt[k * p.ldk + e];
+    top = fmax(top, l2[i]);
+  }
+  top = wave_max(top);
+  // sums of 2^(z2 - top): the teacher's tokens, and all others (the label may be among them)
+  double inside = 0., extra = 0., ly = 0., mass = 0.;
+  int named = 0;
+  double ex[kListLanes], t[kListLanes];
+#pragma unroll
+  for (int i = 0; i < kListLanes; ++i) {
+    ex[i] = t[i] = 0.;
+    if (kind[i] == kDead) continue;
+    ex[i] = exp2(l2[i] - top);
+    if (kind[i] == kTeacher) {
+      t[i] = exp(lt[i]);
+      inside += ex[i];
+      mass += t[i];
+      ++named;
+    } else {
+      extra += ex[i];
+    }
+    if (id[i] == y) ly = l2[i] - top;
+  }
+  inside = wave_sum(inside);
+  extra = wave_sum(extra);
+  ly = wave_sum(ly);  // (one lane's, and zeros)
+  mass = wave_sum(mass);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) named += __shfl_xor(named, o);
+  const double shift = exp2(rtop - top), outside = rsum * shift + extra, all = inside + outside;
+  const double lall = log(all), q = outside / all;
+  // (all others together below 2^-126 of the row's reference are taken for that)
+  const double lq = log(fmax(outside, 0x1p-126)) - lall;
+  const bool tail = p.tail && named < p.V;  // a teacher that names every token has no tail
+  double r = 1. - mass;
+  r = r < 0. ? 0. : r;
+  if (p.reverse) r = r < 0x1p-24 ? 0x1p-24 : r;
+  const double lr = log(r);
+  double div = 0.;
+#pragma unroll
+  for (int i = 0; i < kListLanes; ++i) {
+    if (kind[i] != kTeacher) continue;
+    const double ls = (l2[i] - top) * kLn2d - lall, s = ex[i] / all;
+    div += p.reverse ? (s == 0. ? 0. : s * (ls - lt[i])) : t[i] * (lt[i] - ls);
+  }
+  div = wave_sum(div);
+  if (tail) div += p.reverse ? q * (lq - lr) : r > 0. ? r * (lr - lq) : 0.;
+  const double ce = lall - ly * kLn2d, c = p.c;
+  if (lane == 0) {
+    const int64_t o = p.c0 + k;
+    p.loss[o] = (1. - c) * div + c * ce;
+    p.loss[p.n + o] = div;
+    p.loss[2 * p.n + o] = ce;
+  }
+  if (p.E == nullptr) return;
+  const double whole = tail ? mass + r : mass;
+  double outer = p.reverse ? (tail ? lq - lr - div : 0.) : whole;
+  if (!p.reverse && tail) outer -= outside > 0. ? r / q : 0.;
+  outer = (1. - c) * outer + c;
+  const double inv = p.inv_t / (p.divisor != nullptr ? (double)*p.divisor : (double)counted);
+  // gradients of the listed tokens, and the largest of them (of equal ones the lowest id)
+  double dz[kListLanes], big = -1.;
+  int place = 1 << 30;
+#pragma unroll
+  for (int i = 0; i < kListLanes; ++i) {
+    dz[i] = 0.;
+    if (kind[i] == kDead) continue;
+    const double s = ex[i] / all;
+    if (kind[i] == kLabelOnly) {
+      dz[i] = s * outer;
+    } else {
+      const double ls = (l2[i] - top) * kLn2d - lall;
+      dz[i] = (1. - c) * (p.reverse ? (s == 0. ? 0. : s * (ls - lt[i] - div)) : s * whole - t[i]) + c * s;
+    }
+    if (id[i] == y) dz[i] -= c;
+    dz[i] *= inv;
+    const double a = dz[i] != dz[i] ? INFINITY : fabs(dz[i]);
+    if (a > big) {
+      big = a;
+      place = lane + 64 * i;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const double b = __shfl_xor(big, o);
+    const int q2 = __shfl_xor(place, o);
+    if (b > big || (b == big && q2 < place)) {
+      big = b;
+      place = q2;
+    }
+  }
+  // The factor of the others.  What is listed is divided by it, so it is kept from vanishing beside them: then the
+  // others are off by at most 2^-20 of the largest together, far below the rounding of the listed ones to bf16.
+  double f = outer * inv * shift / all;
+  const double least = fmax(0x1p-20 * big / fmax(rsum, 1.), 0x1p-110);
+  if (fabs(f) < least) f = big > 0. ? copysign(least, f) : 0.;
+  if (fabs(f) > 0x1p100) f = copysign(0x1p100, f);
+#pragma unroll
+  for (int i = 0; i < kListLanes; ++i) {
+    if (kind[i] == kDead) continue;
+    const bool apart = lane + 64 * i == place;
+    p.E[k * p.V + id[i]] = (bf16)(apart || f == 0. ? 0.f : (float)(dz[i] / f));
+    if (apart) {
+      p.w[k] = (float)dz[i];
+      p.at[k] = id[i];
+    }
+  }
+  if (lane == 0) p.f[k] = (float)f;
+}
+
+// Sums of the rows' losses, in a fixed order and 64 bits; one workgroup.
+struct LossArgs {
+  const double* loss;     // [3, n]
+  const int32_t* bad;     // [n] by compacted row
+  const int64_t* nvalid;
+  const float* divisor;
+  float* out[3];
+  int64_t* total_bad;
+  int64_t n;
+};
+__global__ __launch_bounds__(1024) void distill_loss_kernel(const LossArgs p) {
+  __shared__ double sm[3][16];
+  __shared__ long long bad_sh[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t nv = min(p.n, *p.nvalid);
+  double s[3] = {0., 0., 0.};
+  long long bad = 0;
+  for (int64_t i = tid; i < nv; i += 1024) {
+#pragma unroll
+    for (int j = 0; j < 3; ++j) s[j] += p.loss[j * p.n + i];
+    bad += p.bad[i];
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) bad += __shfl_xor(bad, o);
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    s[j] = wave_sum(s[j]);
+    if (lane == 0) sm[j][w] = s[j];
+  }
+  if (lane == 0) bad_sh[w] = bad;
+  __syncthreads();
+  if (tid >= 4) return;
+  if (tid == 3) {
+    bad = 0;
+    for (int i = 0; i < 16; ++i) bad += bad_sh[i];
+    *p.total_bad = bad;
+    return;
+  }
+  double x = 0.;
+  for (int i = 0; i < 16; ++i) x += sm[tid][i];
+  *p.out[tid] = (float)(x / (p.divisor != nullptr ? (double)*p.divisor : (double)nv));
+}
+
+// ---------------------------------------------------------------- host
+struct Layout {
+  size_t scal, loss, bad, spart, mpart, ids, lt, zk, first, len, rsum, rtop, f0, w0, at, f, wt, E, part, acc32, rows, hc, yc,
+      ref, keys, slot, next, lsum, total;
+  int64_t chunk, nchunks, nvt;
+  int ldk, ldt, vt, splits, prow, run, nsort;
+  bool few;
+};
+
+// Loss alone: chunks bound what is held for a row besides (tile sums, lists).
+constexpr int64_t kLossChunk = 16384;
+
+Layout layout(int64_t n, int64_t hdim, int64_t V, int top_k, int64_t chunk, bool grads, bool need_dw) {
+  Layout L{};
+  need_dw = need_dw && grads;
+  L.chunk = std::max<int64_t>(std::min(grads ? chunk : kLossChunk, n), 1);
+  L.nchunks = (n + L.chunk - 1) / L.chunk;
+  L.few = L.chunk <= kFewRows;
+  L.vt = L.few ? kFewBI : kVT;
+  L.nvt = (V + L.vt - 1) / L.vt;
+  L.ldk = top_k + 1;
+  L.ldt = (int)((L.nvt + 1 + 15) / 16 * 16);
+  const size_t rows = (size_t)std::max<int64_t>(n, 1), npad = (rows + 255) / 256 * 256, nc = (size_t)L.chunk;
+  size_t off = 512;  // scal: nvalid; an unused factor
+  auto take = [&](bool on, size_t bytes) {
+    const size_t at = off;
+    if (on) off += al(bytes);
+    return at;
+  };
+  L.loss = take(true, 3 * sizeof(double) * rows);
+  L.bad = take(true, sizeof(int32_t) * rows);
+  L.spart = take(true, sizeof(float) * nc * L.nvt);
+  L.mpart = take(true, sizeof(float) * nc * L.nvt);
+  L.ids = take(true, sizeof(int32_t) * nc * L.ldk);
+  L.lt = take(true, sizeof(float) * nc * L.ldk);
+  L.zk = take(true, sizeof(float) * nc * L.ldk);
+  L.first = take(true, nc * L.ldt);
+  L.len = take(true, sizeof(int32_t) * nc);
+  L.rsum = take(true, sizeof(float) * nc);
+  L.rtop = take(true, sizeof(float) * nc);
+  L.f0 = take(grads, sizeof(float) * nc);
+  L.w0 = take(grads, sizeof(float) * nc);
+  L.at = take(grads, sizeof(int64_t) * nc);
+  L.f = take(need_dw, sizeof(float) * nc);
+  L.wt = take(need_dw, sizeof(float) * nc);
+  L.E = take(grads, sizeof(bf16) * nc * (size_t)V);
+  L.splits = L.few ? few_splits(hdim, V) : dh_splits(hdim, L.chunk);
+  L.prow = (int)std::min<int64_t>(L.chunk, BJ);
+  L.run = dh_run(V);
+  int64_t slots = grads && L.few ? L.splits : 0;
+  if (grads && !L.few && L.splits > 1)
+    for (int64_t c0 = 0; c0 < n; c0 += L.chunk)
+      slots = std::max(slots, dh_slots(c0, std::min(L.chunk, n - c0), (int)((hdim + BI - 1) / BI), L.splits, L.run));
+  L.part = take(slots > 0, sizeof(float) * (size_t)(slots * L.prow * hdim));
+  L.acc32 = take(need_dw && L.nchunks > 1, sizeof(float) * (size_t)(V * hdim));
+  L.rows = take(true, sizeof(int32_t) * npad);
+  L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
+  L.yc = take(true, sizeof(int64_t) * npad);
+  L.ref = take(true, sizeof(float) * npad);
+  L.nsort = need_dw ? (int)((L.chunk + kIdChunk - 1) / kIdChunk) : 0;
+  L.keys = take(need_dw, sizeof(uint64_t) * (size_t)L.nsort * kIdChunk);
+  L.slot = take(need_dw, sizeof(int32_t) * (size_t)V);
+  L.next = take(need_dw, sizeof(int32_t) * (size_t)L.nsort * kIdChunk);
+  L.lsum = take(need_dw, sizeof(float) * nc * (size_t)hdim);
+  L.total = off;
+  return L;
+}
+
+}  // namespace
+
+size_t distill_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t chunk, bool grads, bool need_dw) {
+  return layout(n, hdim, vocab, top_k, chunk, grads, need_dw).total;
+}
+
+hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
+  const bool need_dw = a.grads && a.dweight != nullptr;
+  const Layout L = layout(a.n, a.hdim, a.vocab, a.top_k, a.chunk, a.grads, need_dw);
+  int64_t* nvalid = at<int64_t>(a.ws, 0);
+  int32_t* rows = at<int32_t>(a.ws, L.rows);
+  const float* divisor = a.reduction == 0 ? nullptr : a.divisor;
+  CompactArgs c{};
+  c.hidden = a.hidden;
+  c.weight = a.weight;
+  c.labels = a.labels;
+  c.n = a.n;
+  c.hdim = a.hdim;
+  c.vocab = a.vocab;
+  c.ignore_index = a.ignore_index;
+  c.zscale = (float)(1.4426950408889634 / a.temperature);
+  c.rows = rows;
+  c.nvalid = nvalid;
+  c.count = a.counts;
+  c.bad = a.counts + 1;
+  c.invden = at<float>(a.ws, 256);
+  c.hc = at<bf16>(a.ws, L.hc);
+  c.yc = at<int64_t>(a.ws, L.yc);
+  c.ref = at<float>(a.ws, L.ref);
+  c.dh = a.grads ? a.dhidden : nullptr;
+  launch_compact(c, stream);
+  for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
+    const int64_t nc = std::min(L.chunk, a.n - c0);
+    bf16 *Hc = c.hc + c0 * a.hdim, *E = a.grads ? at<bf16>(a.ws, L.E) : nullptr;
+    ListArgs ls{};
+    ls.ids = a.ids;
+    ls.teacher = a.teacher;
+    ls.rows = rows + c0;
+    ls.y = c.yc + c0;
+    ls.nvalid = nvalid;
+    ls.out = at<int32_t>(a.ws, L.ids);
+    ls.lt = at<float>(a.ws, L.lt);
+    ls.first = at<uint8_t>(a.ws, L.first);
+    ls.len = at<int32_t>(a.ws, L.len);
+    ls.bad = at<int32_t>(a.ws, L.bad) + c0;
+    ls.nc = nc;
+    ls.c0 = c0;
+    ls.V = a.vocab;
+    ls.nvt = L.nvt;
+    ls.K = a.top_k;
+    ls.ldk = L.ldk;
+    ls.ldt = L.ldt;
+    ls.vt = L.vt;
+    const dim3 waves((unsigned)((nc + 3) / 4));
+    hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t> : distill_list_kernel<int64_t>), waves, dim3(256), 0, stream,
+                       ls);
+
+    LogitsArgs lg{};
+    lg.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
+    lg.H = GOp{Hc, a.hdim, nc, a.hdim};
+    lg.y = ls.y;
+    lg.ref = c.ref + c0;
+    lg.E = E;
+    lg.mpart = at<float>(a.ws, L.mpart);
+    lg.spart = at<float>(a.ws, L.spart);
+    lg.nvalid = nvalid;
+    lg.c0 = c0;
+    lg.V = a.vocab;
+    lg.nc = nc;
+    lg.ldp = L.chunk;
+    lg.store_e = a.grads ? 1 : 0;
+    lg.zscale = c.zscale;
+    lg.ids = ls.out;
+    lg.first = ls.first;
+    lg.zk = at<float>(a.ws, L.zk);
+    lg.ldk = L.ldk;
+    lg.ldt = L.ldt;
+    launch_logits(lg, L.few, true, stream);
+
+    RowArgs rw{};
+    rw.mpart = lg.mpart;
+    rw.spart = lg.spart;
+    rw.ref = lg.ref;
+    rw.y = ls.y;
+    rw.E = E;
+    rw.nvalid = nvalid;
+    rw.c0 = c0;
+    rw.nc = nc;
+    rw.nvt = L.nvt;
+    rw.vlog = tile_log(L.vt);
+    rw.V = a.vocab;
+    rw.hdim = a.hdim;
+    rw.ldp = L.chunk;
+    rw.grads = lg.store_e;
+    rw.rsum = at<float>(a.ws, L.rsum);
+    rw.rtop = at<float>(a.ws, L.rtop);
+    launch_row(rw, L.few, true, stream);
+
+    RowMathArgs rm{};
+    rm.ids = ls.out;
+    rm.lt = ls.lt;
+    rm.zk = lg.zk;
+    rm.len = ls.len;
+    rm.ref = lg.ref;
+    rm.rsum = rw.rsum;
+    rm.rtop = rw.rtop;
+    rm.y = ls.y;
+    rm.nvalid = nvalid;
+    rm.divisor = divisor;
+    rm.E = E;
+    rm.f = at<float>(a.ws, L.f0);
+    rm.w = at<float>(a.ws, L.w0);
+    rm.at = at<int64_t>(a.ws, L.at);
+    rm.loss = at<double>(a.ws, L.loss);
+    rm.nc = nc;
+    rm.c0 = c0;
+    rm.n = a.n;
+    rm.V = a.vocab;
+    rm.ldk = L.ldk;
+    rm.reverse = a.reverse;
+    rm.tail = a.tail;
+    rm.c = a.ce_weight;
+    rm.inv_t = 1. / a.temperature;
+    hipLaunchKernelGGL(distill_row_kernel, waves, dim3(256), 0, stream, rm);
+    if (!a.grads) continue;
+
+    if (a.dhidden != nullptr) {
+      DhArgs dh{};
+      dh.Wt = lg.W;
+      dh.E = GOp{E, a.vocab, nc, a.vocab};
+      dh.dh = a.dhidden;
+      dh.part = at<float>(a.ws, L.part);
+      dh.f = rm.f;
+      dh.wt = rm.w;
+      dh.y = rm.at;
+      dh.rows = rows;
+      dh.nvalid = nvalid;
+      dh.c0 = c0;
+      dh.hdim = a.hdim;
+      dh.nc = nc;
+      dh.splits = L.splits;
+      dh.prow = L.prow;
+      dh.run = L.run;
+      if (L.few) {
+        FewSumArgs fs{};
+        fs.dh = dh;
+        fs.f0 = rm.f;
+        fs.w0 = rm.w;
+        fs.scale = 1.f;
+        launch_dh_few(fs, stream);
+      } else {
+        launch_dh(dh, stream);
+      }
+    }
+    if (!need_dw) continue;
+    WeighArgs wg{};
+    wg.H = a.hidden;
+    wg.rows = rows + c0;
+    wg.y = rm.at;
+    wg.f0 = rm.f;
+    wg.w0 = rm.w;
+    wg.nvalid = nvalid;
+    wg.Hs = Hc;
+    wg.f = at<float>(a.ws, L.f);
+    wg.wt = at<float>(a.ws, L.wt);
+    wg.keys = at<uint64_t>(a.ws, L.keys);
+    wg.slot = at<int32_t>(a.ws, L.slot);
+    wg.n = a.n;
+    wg.nc = nc;
+    wg.c0 = c0;
+    wg.V = a.vocab;
+    wg.hdim = a.hdim;
+    wg.ignore_index = a.ignore_index;
+    wg.scale = 1.f;
+    wg.nsort = L.nsort;
+    launch_weigh(wg, stream);
+    LabelArgs la{};
+    la.keys = wg.keys;
+    la.H = a.hidden;
+    la.rows = wg.rows;
+    la.wt = wg.wt;
+    la.lsum = at<float>(a.ws, L.lsum);
+    la.slot = wg.slot;
+    la.next = at<int32_t>(a.ws, L.next);
+    la.hdim = a.hdim;
+    la.nsort = L.nsort;
+    launch_labels(la, nc, stream);
+    DwArgs dw{};
+    dw.Ht = GOp{Hc, a.hdim, nc, a.hdim};
+    dw.Et = GOp{E, a.vocab, nc, a.vocab};
+    dw.slot = la.slot;
+    dw.next = la.next;
+    dw.lsum = la.lsum;
+    dw.dw = a.dweight;
+    dw.acc32 = at<float>(a.ws, L.acc32);
+    dw.nvalid = nvalid;
+    dw.c0 = c0;
+    dw.hdim = a.hdim;
+    dw.V = a.vocab;
+    dw.chunk = L.chunk;
+    launch_dw(dw, L.few && L.nchunks == 1, stream);
+  }
+  if (need_dw && a.n == 0) launch_zero(a.dweight, a.vocab * a.hdim, stream);
+  LossArgs lo{};
+  lo.loss = at<double>(a.ws, L.loss);
+  lo.bad = at<int32_t>(a.ws, L.bad);
+  lo.nvalid = nvalid;
+  lo.divisor = divisor;
+  lo.out[0] = a.loss;
+  lo.out[1] = a.divergence;
+  lo.out[2] = a.cross_entropy;
+  lo.total_bad = a.counts + 2;
+  lo.n = a.n;
+  hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(1024), 0, stream, lo);
+  return hipGetLastError();
+}
+
+}  // namespace siq

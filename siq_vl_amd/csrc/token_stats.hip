@@ -1,0 +1,917 @@
+// Token statistics from hidden states, without logits, for gfx950: the
+// log-probabilities of given tokens, the entropy of each row's distribution and
+// its most probable tokens.
+//
+// With z = h W^T / temperature and p = softmax(z), by row:
+//   logp = ln p_y,   H = -sum_j p_j ln p_j,
+//   top  = the K largest z (of equal ones the lower ids), with their ln p;
+// and with upstream gradients g of logp and e of H
+//   dz_j = g ([j = y] - p_j) - e p_j (ln p_j + H)   (over temperature),
+//   dH = dZ W,  dW = dZ^T h.
+//
+// Forward, per chunk of compacted rows (rows whose label counts):
+//  1. logits GEMM (MFMA, 256 x 256 tiles; few rows: 128 columns of W).  The
+//     epilogue leaves, per (row, half tile), the maximum m, the sum of
+//     2^(z2 - m) and the sum of 2^(z2 - m) (z2 - m), in log2 units: what both
+//     the logsumexp and the entropy are merged from, without any reference that
+//     a row could exceed.  The given token is kept out of them, so that what is
+//     next to certain keeps its digits, and added in the row pass.  With
+//     alternatives wanted it also writes z itself in fp32 and the maximum of
+//     each segment of 64 columns (few rows: 32).
+//  2. row pass: merges in 64 bits; logp, H, lse.
+//  3. selection, a workgroup a row: the K segments of largest maxima hold the K
+//     largest z (each of K segments ranked before a segment has an element
+//     ranked before all of that one's), so K segments are read instead of the
+//     row.
+//
+// Backward: lse and H are known, so the logits GEMM, made again, writes dZ
+// itself in bf16 (but for the given token, whose term is added in fp32 by the
+// products' kernels), and the two gradient products follow.
+#include <algorithm>
+
+#include "few.h"
+#include "flce_launch.h"
+#include "gemm.h"
+#include "ids.h"
+#include "token_stats.h"
+
+namespace siq {
+
+namespace {
+
+using namespace gemm;
+
+// ---------------------------------------------------------------- logits
+struct StatLogitsArgs {
+  GOp W, H;               // W [V, hdim], H = compacted rows of the chunk [nc, hdim]
+  const int64_t* y;       // [nc]
+  float* Z;               // [nc, V] z before the temperature, or nullptr
+  float* smax;            // [nc, nseg] maxima of segments of columns (Z alone)
+  f32x4* part;            // [parts, ldp] {m, sum, sum of products, -} of (half) tiles
+  float* zy;              // [nc] z of the given token
+  const int64_t* nvalid;
+  int64_t V, nc, c0, ldp, nseg;
+  int nI, nJ;
+  float zscale;           // log2(e) / temperature
+};
+
+// {m, s, t} of NA x 16 accumulators of a lane and of its other half: the maximum of
+// z2 = z zscale, and the sums of 2^(z2 - m) and of 2^(z2 - m) (z2 - m).
+template <int NA, class Get>
+__device__ __forceinline__ f32x4 stat_part(float zscale, Get z) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int a = 0; a < NA; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = fmaxf(m, z(a, r));
+  m = half_max(m) * zscale;
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int a = 0; a < NA; ++a)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float x = __builtin_fmaf(z(a, r), zscale, -base), e = exp2f_fast(x);
+      s += e;
+      // (2^-1e4 is 0: masked columns, and those at minus infinity, add nothing)
+      t = __builtin_fmaf(e, fmaxf(x, -1e4f), t);
+    }
+  return f32x4{m, half_sum(s), half_sum(t), 0.f};
+}
+
+__global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p) {
+  __shared__ __align__(16) bf16 smem[SMEM];
+  int ti, tj;
+  if (!tile_of(p.nI, p.nJ, 4, ti, tj)) return;
+  const int64_t i0 = (int64_t)ti * BI, j0 = (int64_t)tj * BJ;
+  if (j0 >= *p.nvalid - p.c0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int wi = w & 1, wj = w >> 1;
+  // accumulator (a, b, r) holds z of column vbase + wave_row(a, wi) + 16 (r / 8) + (r % 8), row j0 + wave_col(b, wj) + l32
+  const int64_t vbase = i0 + 8 * h;
+  int rel[2];  // the given tokens' offsets from the tile (-1: elsewhere)
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int64_t d = p.y[min(j0 + wave_col(b, wj) + l32, p.nc - 1)] - vbase;
+    rel[b] = d >= 0 && d < 256 ? (int)d : -1;
+  }
+  f32x16 acc[4][2];
+  gemm_core<true, true, false>(smem, p.W, p.H, i0, j0, 0, p.W.cols, acc);
+  if (i0 + BI > p.V) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (vbase + wave_row(a, wi) + 16 * (r >> 3) + (r & 7) >= p.V) acc[a][b][r] = -INFINITY;
+  }
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int64_t tok = j0 + wave_col(b, wj) + l32;
+    const bool tv = tok < p.nc;
+    if (p.Z != nullptr) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {  // a wave's segment of each half of the tile
+        float m = -INFINITY;
+#pragma unroll
+        for (int a = 2 * q; a < 2 * q + 2; ++a)
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const int64_t v0 = vbase + wave_row(a, wi) + 16 * jj;
+            f32x4 lo, hi;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              lo[i] = acc[a][b][8 * jj + i];
+              hi[i] = acc[a][b][8 * jj + 4 + i];
+              m = fmaxf(m, fmaxf(lo[i], hi[i]));
+            }
+            if (tv && v0 < p.V) {
+              float* z = p.Z + tok * p.V + v0;
+              *reinterpret_cast<f32x4*>(z) = lo;
+              *reinterpret_cast<f32x4*>(z + 4) = hi;
+            }
+          }
+        m = half_max(m);
+        if (tv && h == 0) p.smax[tok * p.nseg + 4 * ti + 2 * q + wi] = m;
+      }
+    }
+    // the given token: in at most one lane of the workgroup, for one tile in ~600
+    const bool hit = tv && rel[b] >= 0 && ((rel[b] >> 6) & 1) == wi && ((rel[b] >> 3) & 1) == 0;
+    if (__any(hit)) {
+      const int r0 = rel[b] - 64 * wi;
+      float zsel = 0.f;
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (hit && r0 == wave_row(a, 0) + 16 * (r >> 3) + (r & 7)) {
+            zsel = acc[a][b][r];
+            acc[a][b][r] = -INFINITY;
+          }
+      if (hit) p.zy[tok] = zsel;
+    }
+    const f32x4 st = stat_part<4>(p.zscale, [&](int a, int r) { return acc[a][b][r]; });
+    if (tv && h == 0) p.part[(int64_t)(2 * ti + wi) * p.ldp + tok] = st;
+  }
+}
+
+// The main loop of a few-rows product: 128 rows of W (32 a wave) x 32 NB rows of the
+// call; accumulator r of block b: column i0 + 32 w + 8 h + 16 (r / 8) + r % 8, row
+// 32 b + l32.
+template <int NB, int STAGES>
+__device__ __forceinline__ void few_logits(bf16* smem, const GOp& W, const GOp& H, int64_t i0, f32x16 (&acc)[NB]) {
+  constexpr int TOK = 32 * NB, STAGE = (kFewBI + TOK) * BK, NWV = kFewThreads / 64;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wu = __builtin_amdgcn_readfirstlane(w);
+  FewRows<kFewBI, NWV> la;
+  FewRows<TOK, NWV> lb;
+  la.init(W.ld, W.rows - 1 - i0, lane, w);
+  lb.init(H.ld, H.rows - 1, lane, w);
+  const bf16 *wb = W.base + i0 * W.ld, *hb = H.base;
+  HalfRead<true, true, 1> ra;
+  HalfRead<true, false, NB> rb;
+  ra.init(lane, 32 * w);
+  rb.init(lane, 0);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = zero16();
+  few_steps<STAGES, la.PER + lb.PER>(
+      (int)(W.cols / BK),
+      [&](int s, int buf) {
+        bf16* st = smem + buf * STAGE;
+        lb.issue(hb + (int64_t)s * BK, st + kFewBI * BK, wu);
+        la.issue(wb + (int64_t)s * BK, st, wu);
+      },
+      [&](int, int buf) {
+        const bf16 *A = smem + buf * STAGE, *B = A + kFewBI * BK;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const bf16x8 a = ra.read(A, 0, ks);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, rb.read(B, b, ks), acc[b]);
+        }
+      });
+}
+
+template <int NB>
+constexpr int kFewStages = NB <= 2 ? 3 : 2;  // (64 rows: three buffers; 128: two, for two workgroups a CU)
+template <int NB>
+constexpr int kFewSmem = kFewStages<NB> * (kFewBI + 32 * NB) * BK;
+
+template <int NB>
+__global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const StatLogitsArgs p) {
+  constexpr int TOK = 32 * NB, NWV = kFewThreads / 64;
+  __shared__ __align__(16) bf16 smem[kFewSmem<NB>];
+  const int64_t i0 = (int64_t)blockIdx.x * kFewBI;
+  if (*p.nvalid <= p.c0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int64_t vbase = i0 + 32 * w + 8 * h;
+  int rel[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t d = p.y[min((int64_t)(32 * b + l32), p.nc - 1)] - vbase;
+    rel[b] = d >= 0 && d < 32 && (d & 8) == 0 ? (int)d : -1;
+  }
+  f32x16 acc[NB];
+  few_logits<NB, kFewStages<NB>>(smem, p.W, p.H, i0, acc);
+  if (i0 + kFewBI > p.V) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (vbase + 16 * (r >> 3) + (r & 7) >= p.V) acc[b][r] = -INFINITY;
+  }
+  f32x4* red = reinterpret_cast<f32x4*>(smem);  // [NWV][TOK] (behind the last step's barrier)
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t tok = 32 * b + l32;
+    const bool tv = tok < p.nc;
+    if (p.Z != nullptr) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const int64_t v0 = vbase + 16 * jj;
+        f32x4 lo, hi;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = acc[b][8 * jj + i];
+          hi[i] = acc[b][8 * jj + 4 + i];
+          m = fmaxf(m, fmaxf(lo[i], hi[i]));
+        }
+        if (tv && v0 < p.V) {
+          float* z = p.Z + tok * p.V + v0;
+          *reinterpret_cast<f32x4*>(z) = lo;
+          *reinterpret_cast<f32x4*>(z + 4) = hi;
+        }
+      }
+      m = half_max(m);
+      if (tv && h == 0) p.smax[tok * p.nseg + 4 * blockIdx.x + w] = m;
+    }
+    const bool hit = tv && rel[b] >= 0;
+    if (__any(hit)) {
+      float zsel = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (hit && rel[b] == 16 * (r >> 3) + (r & 7)) {
+          zsel = acc[b][r];
+          acc[b][r] = -INFINITY;
+        }
+      if (hit) p.zy[tok] = zsel;
+    }
+    const f32x4 st = stat_part<1>(p.zscale, [&](int, int r) { return acc[b][r]; });
+    if (h == 0) red[w * TOK + 32 * b + l32] = st;
+  }
+  __syncthreads();
+  // a thread a row of the call: the tile's, merged over its waves
+  if (tid >= TOK || tid >= p.nc) return;
+  f32x4 x[NWV];
+  float m = -INFINITY, s = 0.f, t = 0.f;
+#pragma unroll
+  for (int k = 0; k < NWV; ++k) {
+    x[k] = red[k * TOK + tid];
+    m = fmaxf(m, x[k][0]);
+  }
+#pragma unroll
+  for (int k = 0; k < NWV; ++k) {
+    const float d = fmaxf(x[k][0] - m, -1e4f), f = exp2f_fast(d);
+    s += x[k][1] * f;
+    t += (x[k][2] + x[k][1] * d) * f;
+  }
+  p.part[(int64_t)blockIdx.x * p.ldp + tid] = f32x4{m, s, t, 0.f};
+}
+
+// ---------------------------------------------------------------- row pass
+struct StatRowArgs {
+  const f32x4* part;      // [parts, ldp]
+  const float* zy;        // [nc]
+  const int32_t* rows;    // [nc] compacted row -> row
+  const int64_t* nvalid;
+  float *logp, *entropy, *lse;  // [n] by row
+  double* lse64;          // [nc] (compacted; alternatives alone)
+  int64_t nc, c0, ldp, parts;
+  float zscale;
+};
+
+// Merges a row's parts and its given token in 64 bits.  ROWS rows a workgroup of
+// 256 threads, 256 / ROWS threads that share a row: 16 rows where there are many (a
+// read is then 256 contiguous bytes), one where there are few.
+template <int ROWS>
+__global__ __launch_bounds__(256) void stats_row_kernel(const StatRowArgs p) {
+  constexpr int PER = 256 / ROWS, U = 4;
+  __shared__ double sh_s[256], sh_t[256];
+  __shared__ float sh_m[256];
+  const int64_t nv = min(p.nc, *p.nvalid - p.c0), r0 = (int64_t)blockIdx.x * ROWS;
+  if (r0 >= nv) return;
+  const int tid = threadIdx.x, lane = tid % ROWS, k = tid / ROWS;
+  const int64_t row = min(r0 + lane, nv - 1);
+  const float dy = p.zy[row] * p.zscale;
+  const f32x4* src = p.part + row;
+  float m = dy;
+  for (int64_t t0 = k; t0 < p.parts; t0 += PER * U) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = src[min(t0 + PER * u, p.parts - 1) * p.ldp][0];
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(m, x[u]);
+  }
+  sh_m[tid] = m;
+  __syncthreads();
+  for (int i = 0; i < PER; ++i) m = fmaxf(m, sh_m[i * ROWS + lane]);
+  double s = 0., t = 0.;
+  for (int64_t t0 = k; t0 < p.parts; t0 += PER * U) {
+    f32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = src[min(t0 + PER * u, p.parts - 1) * p.ldp];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float d = x[u][0] - m;
+      if (t0 + PER * u >= p.parts || x[u][1] == 0.f) continue;  // (nothing but minus infinities; a NaN counts)
+      // (a factor per 256 or more terms: its rounding is that of a sum of so many)
+      const float f = exp2f_fast(d);
+      s += (double)(x[u][1] * f);
+      t += ((double)x[u][2] + (double)x[u][1] * (double)d) * (double)f;
+    }
+  }
+  sh_s[tid] = s;
+  sh_t[tid] = t;
+  __syncthreads();
+  if (k != 0 || r0 + lane >= nv) return;
+  s = t = 0.;
+  for (int i = 0; i < PER; ++i) {
+    s += sh_s[i * ROWS + lane];
+    t += sh_t[i * ROWS + lane];
+  }
+  // the given token: all relative to m
+  constexpr double kLn2d = 0.6931471805599453;
+  const double d = (double)p.zy[row] * (double)p.zscale - (double)m, ey = exp2(d), all = s + ey, over = s * exp2(-d);
+  const double l2 = log2(all);
+  const double ent = kLn2d * (l2 - (t + (ey > 0. ? ey * d : 0.)) / all);
+  const int64_t at = p.rows[row];
+  // p_y = 1 / (1 + over): its logarithm keeps its digits where `over` is small
+  p.logp[at] = (float)(over <= 1e300 ? -log1p(over) : kLn2d * (d - l2));
+  p.entropy[at] = ent < 0. ? 0.f : (float)ent;
+  p.lse[at] = (float)((double)m + l2);
+  if (p.lse64 != nullptr) p.lse64[row] = (double)m + l2;
+}
+
+// ---------------------------------------------------------------- selection
+struct SelectArgs {
+  const float* Z;         // [nc, V]
+  const float* smax;      // [nc, nseg]
+  const double* lse64;    // [nc]
+  const int32_t* rows;    // [nc]
+  const int64_t* nvalid;
+  float* top_logp;        // [n, K]
+  int64_t* top_ids;
+  int64_t nc, c0, V;
+  int nseg, seg, K;       // segments of a row; columns of one (32 or 64)
+  float zscale;
+};
+
+// Larger numbers have larger keys, equal ones (both zeros) equal keys; NaN is above all.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return x != x ? 0xffffffffu : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float number_of(uint32_t k) {
+  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// One workgroup a row.  The K-th largest of the segments' maxima is found bit by
+// bit; the segments above it, and as many of those at it as K needs, lowest first,
+// are read, their columns that are not below it listed, and each listed column's
+// rank is how many of the others come before it.
+__global__ __launch_bounds__(256) void stats_select_kernel(const SelectArgs p) {
+  extern __shared__ uint64_t dyn[];  // the maxima's keys, then the listed columns (K * seg at most)
+  __shared__ int part_sh[2][4], list[kMaxTopK], n_sh;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn);
+  const int64_t k0 = blockIdx.x;
+  if (k0 >= min(p.nc, *p.nvalid - p.c0)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const float* sm = p.smax + k0 * p.nseg;
+  for (int i = tid; i < p.nseg; i += 256) keys[i] = order_of(sm[i]);
+  __syncthreads();
+  const int K = p.K, take = min(K, p.nseg);
+  uint32_t tau = 0;  // the take-th largest key
+  int turn = 0;
+  for (int bit = 31; bit >= 0; --bit, turn ^= 1) {
+    const uint32_t cand = tau | (1u << bit);
+    int c = 0;
+    for (int i = tid; i < p.nseg; i += 256) c += keys[i] >= cand ? 1 : 0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o);
+    if (lane == 0) part_sh[turn][w] = c;
+    __syncthreads();
+    if (part_sh[turn][0] + part_sh[turn][1] + part_sh[turn][2] + part_sh[turn][3] >= take) tau = cand;
+  }
+  if (w == 0) {
+    // the segments, those above tau first
+    const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
+    int n = 0;
+    for (int eq = 0; eq < 2; ++eq)
+      for (int i0 = 0; i0 < p.nseg && n < take; i0 += 64) {
+        const uint32_t x = i0 + lane < p.nseg ? keys[i0 + lane] : 0;
+        const bool in = i0 + lane < p.nseg && (eq ? x == tau : x > tau);
+        const uint64_t m = __ballot(in);
+        const int at = n + __popcll(m & below);
+        if (in && at < take) list[at] = i0 + lane;
+        n = min(take, n + __popcll(m));
+      }
+    if (lane == 0) n_sh = 0;
+  }
+  __syncthreads();
+  // a segment at a time for 64 or 32 lanes; with fewer segments than K there is no bound
+  const uint32_t least = p.nseg > K ? tau : 0u;
+  const float* z = p.Z + k0 * p.V;
+  const int groups = 256 / p.seg;
+  for (int s0 = 0; s0 < take; s0 += groups) {
+    const int s = s0 + tid / p.seg;
+    const int64_t v = s < take ? (int64_t)list[s] * p.seg + tid % p.seg : p.V;
+    if (v >= p.V) continue;
+    const uint32_t key = order_of(z[v]);
+    if (key >= least) dyn[atomicAdd(&n_sh, 1)] = (uint64_t)key << 32 | (uint32_t)~v;  // (in any order: ranks make one)
+  }
+  __syncthreads();
+  const int n = n_sh;
+  const double lse = p.lse64[k0];
+  const int64_t out = (int64_t)p.rows[k0] * K;
+  for (int i = tid; i < n; i += 256) {
+    const uint64_t mine = dyn[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += dyn[j] > mine ? 1 : 0;
+    if (rank >= K) continue;
+    const float zi = number_of((uint32_t)(mine >> 32));
+    p.top_logp[out + rank] = (float)(((double)zi * (double)p.zscale - lse) * 0.6931471805599453);
+    p.top_ids[out + rank] = (int64_t)(uint32_t)~(uint32_t)mine;
+  }
+}
+
+// Rows whose label does not count: 0, and -1 for ids.
+struct StatClearArgs {
+  const int64_t* labels;
+  float *logp, *entropy, *lse, *top_logp;
+  int64_t* top_ids;
+  int64_t n, V, ignore_index;
+  int K;
+};
+__global__ __launch_bounds__(256) void stats_clear_kernel(const StatClearArgs p) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < p.n; t += (int64_t)gridDim.x * 4) {
+    const int64_t v = p.labels[t];
+    if (v != p.ignore_index && v >= 0 && v < p.V) continue;
+    if (lane == 0) {
+      p.logp[t] = 0.f;
+      p.entropy[t] = 0.f;
+      p.lse[t] = 0.f;
+    }
+    for (int k = lane; k < p.K; k += 64) {
+      p.top_logp[t * p.K + k] = 0.f;
+      p.top_ids[t * p.K + k] = -1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- dZ
+struct StatGradArgs {
+  GOp W, H;
+  const int64_t* y;       // [nc]
+  const f32x4* coef;      // [nc] {lse, A, B, -}: dz_j = p_j (A + B log2 p_j)
+  bf16* G;                // [nc, V]
+  const int64_t* nvalid;
+  int64_t V, nc, c0;
+  int nI, nJ;
+  float zscale;
+};
+
+__device__ __forceinline__ float stat_dz(float z, float zscale, const f32x4& c) {
+  // (at most 0 but for the lse's own rounding; a probability of 0 times a finite logarithm is 0)
+  const float l = fmaxf(__builtin_fmaf(z, zscale, -c[0]), -1e4f);
+  return exp2f_fast(l) * __builtin_fmaf(c[2], l, c[1]);
+}
+
+__global__ __launch_bounds__(NT) void stats_grad_kernel(const StatGradArgs p) {
+  __shared__ __align__(16) bf16 smem[SMEM];
+  int ti, tj;
+  if (!tile_of(p.nI, p.nJ, 4, ti, tj)) return;
+  const int64_t i0 = (int64_t)ti * BI, j0 = (int64_t)tj * BJ;
+  if (j0 >= *p.nvalid - p.c0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int wi = w & 1, wj = w >> 1;
+  const int64_t vbase = i0 + 8 * h;
+  f32x16 acc[4][2];
+  gemm_core<true, true, false>(smem, p.W, p.H, i0, j0, 0, p.W.cols, acc);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int64_t tok = j0 + wave_col(b, wj) + l32;
+    if (tok >= p.nc) continue;
+    const f32x4 c = p.coef[tok];
+    const int64_t y = p.y[tok] - vbase;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const int v0 = wave_row(a, wi) + 16 * jj;
+        if (vbase + v0 >= p.V) continue;
+        bf16x8 g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = stat_dz(acc[a][b][8 * jj + i], p.zscale, c);
+          g[i] = (bf16)(y == v0 + i ? 0.f : x);
+        }
+        st_bf16x8(p.G + tok * p.V + vbase + v0, g);
+      }
+  }
+}
+
+template <int NB>
+__global__ __launch_bounds__(kFewThreads) void stats_grad_few_kernel(const StatGradArgs p) {
+  __shared__ __align__(16) bf16 smem[kFewSmem<NB>];
+  const int64_t i0 = (int64_t)blockIdx.x * kFewBI;
+  if (*p.nvalid <= p.c0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int64_t vbase = i0 + 32 * w + 8 * h;
+  f32x16 acc[NB];
+  few_logits<NB, kFewStages<NB>>(smem, p.W, p.H, i0, acc);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t tok = 32 * b + l32;
+    if (tok >= p.nc) continue;
+    const f32x4 c = p.coef[tok];
+    const int64_t y = p.y[tok] - vbase;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      if (vbase + 16 * jj >= p.V) continue;
+      bf16x8 g;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = stat_dz(acc[b][8 * jj + i], p.zscale, c);
+        g[i] = (bf16)(y == 16 * jj + i ? 0.f : x);
+      }
+      st_bf16x8(p.G + tok * p.V + vbase + 16 * jj, g);
+    }
+  }
+}
+
+// What a row's gradient needs of the forward's results and of the upstream
+// gradients: {lse, A, B} as above, and the given token's own dz (in 32 bits),
+//   A = -(g + e H) / T,  B = -e ln 2 / T,  dz_y = (g (1 - p_y) - e p_y (ln p_y + H)) / T.
+struct StatCoefArgs {
+  const int32_t* rows;    // [nc]
+  const int64_t* nvalid;
+  const float *logp, *entropy, *lse, *g, *e;  // by row; g and e may be nullptr
+  f32x4* coef;            // [nc]
+  float *f, *w;           // [nc]: 1, dz_y
+  int64_t nc, c0;
+  float inv_t;
+};
+__global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
+  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, nv = min(p.nc, *p.nvalid - p.c0);
+  if (k >= p.nc) return;
+  if (k >= nv) {  // dZ of the rows that fill up a tile is 0 (dW multiplies it with zeros, which a NaN would survive)
+    p.coef[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    return;
+  }
+  const int64_t row = p.rows[k];
+  const float lp = p.logp[row], hh = p.entropy[row];
+  const float g = (p.g != nullptr ? p.g[row] : 0.f) * p.inv_t, e = (p.e != nullptr ? p.e[row] : 0.f) * p.inv_t;
+  const float py = expf(lp);
+  p.coef[k] = f32x4{p.lse[row], -__builtin_fmaf(e, hh, g), -e * kLn2, 0.f};
+  p.f[k] = 1.f;
+  p.w[k] = -g * expm1f(lp) - (e != 0.f ? e * py * (fmaxf(lp, -1e4f) + hh) : 0.f);
+}
+
+// ---------------------------------------------------------------- host
+// Rows at a time: with alternatives, z of one chunk takes at most 2 GiB; without
+// them the tiles' sums alone bound it.
+int64_t stats_chunk(int64_t n, int64_t V, int top_k) {
+  const int64_t most = top_k > 0 ? std::max<int64_t>((int64_t(1) << 31) / (4 * V) / BJ * BJ, BJ) : 16384;
+  return std::max<int64_t>(std::min(n, most), 1);
+}
+
+struct FwdLayout {
+  size_t scal, rows, yc, ref, hc, zy, part, smax, lse64, Z, total;
+  int64_t chunk, parts, nseg;
+  bool few;
+};
+FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k) {
+  FwdLayout L{};
+  L.chunk = stats_chunk(n, V, top_k);
+  L.few = L.chunk <= kFewRows;
+  const int64_t tiles = (V + (L.few ? kFewBI : kVT) - 1) / (L.few ? kFewBI : kVT);
+  L.parts = L.few ? tiles : 2 * tiles;
+  L.nseg = 4 * tiles;
+  const size_t npad = (size_t)((std::max<int64_t>(n, 1) + 255) / 256 * 256);
+  size_t off = 256;  // scal: nvalid, an unused factor
+  auto take = [&](bool on, size_t bytes) {
+    const size_t at = off;
+    if (on) off += al(bytes);
+    return at;
+  };
+  L.rows = take(true, sizeof(int32_t) * npad);
+  L.yc = take(true, sizeof(int64_t) * npad);
+  L.ref = take(true, sizeof(float) * npad);
+  L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
+  L.zy = take(true, sizeof(float) * (size_t)L.chunk);
+  L.part = take(true, sizeof(f32x4) * (size_t)(L.chunk * L.parts));
+  L.smax = take(top_k > 0, sizeof(float) * (size_t)(L.chunk * L.nseg));
+  L.lse64 = take(top_k > 0, sizeof(double) * (size_t)L.chunk);
+  L.Z = take(top_k > 0, sizeof(float) * (size_t)(L.chunk * V));
+  L.total = off;
+  return L;
+}
+
+struct BwdLayout {
+  size_t scal, rows, yc, ref, hc, coef, f0, w0, f, wt, E, part, acc32, keys, slot, next, lsum, total;
+  int64_t chunk, nchunks;
+  int splits, prow, run, nsort;
+  bool few;
+};
+BwdLayout bwd_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool need_dw) {
+  BwdLayout L{};
+  L.chunk = std::max<int64_t>(std::min(chunk, n), 1);
+  L.nchunks = (n + L.chunk - 1) / L.chunk;
+  L.few = L.chunk <= kFewRows;
+  const size_t npad = (size_t)((std::max<int64_t>(n, 1) + 255) / 256 * 256);
+  size_t off = 256;  // scal: nvalid, count, bad labels, an unused factor
+  auto take = [&](bool on, size_t bytes) {
+    const size_t at = off;
+    if (on) off += al(bytes);
+    return at;
+  };
+  L.rows = take(true, sizeof(int32_t) * npad);
+  L.yc = take(true, sizeof(int64_t) * npad);
+  L.ref = take(true, sizeof(float) * npad);
+  L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
+  L.coef = take(true, sizeof(f32x4) * (size_t)L.chunk);
+  L.f0 = take(true, sizeof(float) * (size_t)L.chunk);
+  L.w0 = take(true, sizeof(float) * (size_t)L.chunk);
+  L.f = take(need_dw, sizeof(float) * (size_t)L.chunk);
+  L.wt = take(need_dw, sizeof(float) * (size_t)L.chunk);
+  L.E = take(true, sizeof(bf16) * (size_t)(L.chunk * V));
+  L.splits = L.few ? few_splits(hdim, V) : dh_splits(hdim, L.chunk);
+  L.prow = (int)std::min<int64_t>(L.chunk, BJ);
+  L.run = dh_run(V);
+  int64_t slots = L.few ? L.splits : 0;
+  if (!L.few && L.splits > 1)
+    for (int64_t c0 = 0; c0 < n; c0 += L.chunk)
+      slots = std::max(slots, dh_slots(c0, std::min(L.chunk, n - c0), (int)((hdim + BI - 1) / BI), L.splits, L.run));
+  L.part = take(slots > 0, sizeof(float) * (size_t)(slots * L.prow * hdim));
+  L.nsort = need_dw ? (int)((L.chunk + kIdChunk - 1) / kIdChunk) : 0;
+  L.acc32 = take(need_dw && L.nchunks > 1, sizeof(float) * (size_t)(V * hdim));
+  L.keys = take(need_dw, sizeof(uint64_t) * (size_t)L.nsort * kIdChunk);
+  L.slot = take(need_dw, sizeof(int32_t) * (size_t)V);
+  L.next = take(need_dw, sizeof(int32_t) * (size_t)L.nsort * kIdChunk);
+  L.lsum = take(need_dw, sizeof(float) * (size_t)(L.chunk * hdim));
+  L.total = off;
+  return L;
+}
+
+float zscale_of(const StatsArgs& a) { return (float)(1.4426950408889634 / a.temperature); }
+
+CompactArgs compact_of(const StatsArgs& a) {
+  CompactArgs c{};
+  c.hidden = a.hidden;
+  c.weight = a.weight;
+  c.labels = a.labels;
+  c.n = a.n;
+  c.hdim = a.hdim;
+  c.vocab = a.vocab;
+  c.ignore_index = a.ignore_index;
+  c.zscale = zscale_of(a);
+  return c;
+}
+
+}  // namespace
+
+size_t stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k) {
+  return fwd_layout(n, hdim, vocab, top_k).total;
+}
+size_t stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw) {
+  return bwd_layout(n, hdim, vocab, chunk, need_dw).total;
+}
+
+hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
+  const FwdLayout L = fwd_layout(a.n, a.hdim, a.vocab, a.top_k);
+  int64_t* nvalid = at<int64_t>(a.ws, L.scal);
+  int32_t* rows = at<int32_t>(a.ws, L.rows);
+  CompactArgs c = compact_of(a);
+  c.rows = rows;
+  c.nvalid = nvalid;
+  c.count = a.count;
+  c.bad = a.bad_labels;
+  c.invden = at<float>(a.ws, L.scal) + 32;
+  c.hc = at<bf16>(a.ws, L.hc);
+  c.yc = at<int64_t>(a.ws, L.yc);
+  c.ref = at<float>(a.ws, L.ref);
+  launch_compact(c, stream);
+  if (a.n == 0) return hipGetLastError();
+  StatClearArgs cl{a.labels, a.logp, a.entropy, a.lse, a.top_logp, a.top_ids, a.n, a.vocab, a.ignore_index, a.top_k};
+  hipLaunchKernelGGL(stats_clear_kernel, dim3((unsigned)std::min<int64_t>((a.n + 3) / 4, 1024)), dim3(256), 0, stream, cl);
+  for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
+    const int64_t nc = std::min(L.chunk, a.n - c0);
+    StatLogitsArgs lg{};
+    lg.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
+    lg.H = GOp{c.hc + c0 * a.hdim, a.hdim, nc, a.hdim};
+    lg.y = c.yc + c0;
+    lg.Z = a.top_k > 0 ? at<float>(a.ws, L.Z) : nullptr;
+    lg.smax = at<float>(a.ws, L.smax);
+    lg.part = at<f32x4>(a.ws, L.part);
+    lg.zy = at<float>(a.ws, L.zy);
+    lg.nvalid = nvalid;
+    lg.V = a.vocab;
+    lg.nc = nc;
+    lg.c0 = c0;
+    lg.ldp = L.chunk;
+    lg.nseg = L.nseg;
+    lg.zscale = c.zscale;
+    if (L.few) {
+      const dim3 grid((unsigned)((a.vocab + kFewBI - 1) / kFewBI));
+      hipLaunchKernelGGL((nc <= 64 ? stats_logits_few_kernel<2> : stats_logits_few_kernel<4>), grid, dim3(kFewThreads), 0,
+                         stream, lg);
+    } else {
+      lg.nI = (int)((a.vocab + kVT - 1) / kVT);
+      lg.nJ = (int)((nc + BJ - 1) / BJ);
+      const int grid = ((lg.nI * lg.nJ + kXcds - 1) / kXcds) * kXcds;
+      hipLaunchKernelGGL(stats_logits_kernel, dim3(grid), dim3(NT), 0, stream, lg);
+    }
+    StatRowArgs rw{};
+    rw.part = lg.part;
+    rw.zy = lg.zy;
+    rw.rows = rows + c0;
+    rw.nvalid = nvalid;
+    rw.logp = a.logp;
+    rw.entropy = a.entropy;
+    rw.lse = a.lse;
+    rw.lse64 = a.top_k > 0 ? at<double>(a.ws, L.lse64) : nullptr;
+    rw.nc = nc;
+    rw.c0 = c0;
+    rw.ldp = L.chunk;
+    rw.parts = L.parts;
+    rw.zscale = c.zscale;
+    if (L.few)
+      hipLaunchKernelGGL(stats_row_kernel<1>, dim3((unsigned)nc), dim3(256), 0, stream, rw);
+    else
+      hipLaunchKernelGGL(stats_row_kernel<16>, dim3((unsigned)((nc + 15) / 16)), dim3(256), 0, stream, rw);
+    if (a.top_k > 0) {
+      SelectArgs se{};
+      se.Z = lg.Z;
+      se.smax = lg.smax;
+      se.lse64 = rw.lse64;
+      se.rows = rows + c0;
+      se.nvalid = nvalid;
+      se.top_logp = a.top_logp;
+      se.top_ids = a.top_ids;
+      se.nc = nc;
+      se.c0 = c0;
+      se.V = a.vocab;
+      se.nseg = (int)L.nseg;
+      se.seg = L.few ? 32 : 64;
+      se.K = a.top_k;
+      se.zscale = c.zscale;
+      const size_t lds = std::max(sizeof(uint32_t) * (size_t)L.nseg, sizeof(uint64_t) * (size_t)a.top_k * se.seg);
+      hipLaunchKernelGGL(stats_select_kernel, dim3((unsigned)nc), dim3(256), lds, stream, se);
+    }
+  }
+  return hipGetLastError();
+}
+
+hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
+  const bool need_dw = a.dweight != nullptr;
+  const BwdLayout L = bwd_layout(a.n, a.hdim, a.vocab, a.chunk, need_dw);
+  if (a.n == 0) {
+    if (need_dw) launch_zero(a.dweight, a.vocab * a.hdim, stream);
+    return hipGetLastError();
+  }
+  int64_t* nvalid = at<int64_t>(a.ws, L.scal);
+  int32_t* rows = at<int32_t>(a.ws, L.rows);
+  CompactArgs c = compact_of(a);
+  c.rows = rows;
+  c.nvalid = nvalid;
+  c.count = nvalid + 1;
+  c.bad = nvalid + 2;
+  c.invden = at<float>(a.ws, L.scal) + 32;
+  c.hc = at<bf16>(a.ws, L.hc);
+  c.yc = at<int64_t>(a.ws, L.yc);
+  c.ref = at<float>(a.ws, L.ref);
+  c.dh = a.dhidden;
+  launch_compact(c, stream);
+  bf16* E = at<bf16>(a.ws, L.E);
+  float *f0 = at<float>(a.ws, L.f0), *w0 = at<float>(a.ws, L.w0);
+  for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
+    const int64_t nc = std::min(L.chunk, a.n - c0);
+    bf16* Hc = c.hc + c0 * a.hdim;
+    StatCoefArgs co{};
+    co.rows = rows + c0;
+    co.nvalid = nvalid;
+    co.logp = a.logp;
+    co.entropy = a.entropy;
+    co.lse = a.lse;
+    co.g = a.dlogp;
+    co.e = a.dentropy;
+    co.coef = at<f32x4>(a.ws, L.coef);
+    co.f = f0;
+    co.w = w0;
+    co.nc = nc;
+    co.c0 = c0;
+    co.inv_t = (float)(1. / a.temperature);
+    hipLaunchKernelGGL(stats_coef_kernel, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, stream, co);
+    StatGradArgs gr{};
+    gr.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
+    gr.H = GOp{Hc, a.hdim, nc, a.hdim};
+    gr.y = c.yc + c0;
+    gr.coef = co.coef;
+    gr.G = E;
+    gr.nvalid = nvalid;
+    gr.V = a.vocab;
+    gr.nc = nc;
+    gr.c0 = c0;
+    gr.zscale = c.zscale;
+    if (L.few) {
+      const dim3 grid((unsigned)((a.vocab + kFewBI - 1) / kFewBI));
+      hipLaunchKernelGGL((nc <= 64 ? stats_grad_few_kernel<2> : stats_grad_few_kernel<4>), grid, dim3(kFewThreads), 0, stream,
+                         gr);
+    } else {
+      gr.nI = (int)((a.vocab + kVT - 1) / kVT);
+      gr.nJ = (int)((nc + BJ - 1) / BJ);
+      const int grid = ((gr.nI * gr.nJ + kXcds - 1) / kXcds) * kXcds;
+      hipLaunchKernelGGL(stats_grad_kernel, dim3(grid), dim3(NT), 0, stream, gr);
+    }
+    if (a.dhidden != nullptr) {
+      DhArgs dh{};
+      dh.Wt = gr.W;
+      dh.E = GOp{E, a.vocab, nc, a.vocab};
+      dh.dh = a.dhidden;
+      dh.part = at<float>(a.ws, L.part);
+      dh.f = f0;
+      dh.wt = w0;
+      dh.y = gr.y;
+      dh.rows = rows;
+      dh.nvalid = nvalid;
+      dh.c0 = c0;
+      dh.hdim = a.hdim;
+      dh.nc = nc;
+      dh.splits = L.splits;
+      dh.prow = L.prow;
+      dh.run = L.run;
+      if (L.few) {
+        FewSumArgs fs{};
+        fs.dh = dh;
+        fs.f0 = f0;
+        fs.w0 = w0;
+        fs.scale = 1.f;
+        launch_dh_few(fs, stream);
+      } else {
+        launch_dh(dh, stream);
+      }
+    }
+    if (!need_dw) continue;
+    WeighArgs wg{};
+    wg.H = a.hidden;
+    wg.rows = rows + c0;
+    wg.y = gr.y;
+    wg.f0 = f0;
+    wg.w0 = w0;
+    wg.nvalid = nvalid;
+    wg.Hs = Hc;  // (read by the logits above; every factor is 1)
+    wg.f = at<float>(a.ws, L.f);
+    wg.wt = at<float>(a.ws, L.wt);
+    wg.keys = at<uint64_t>(a.ws, L.keys);
+    wg.slot = at<int32_t>(a.ws, L.slot);
+    wg.n = a.n;
+    wg.nc = nc;
+    wg.c0 = c0;
+    wg.V = a.vocab;
+    wg.hdim = a.hdim;
+    wg.ignore_index = a.ignore_index;
+    wg.scale = 1.f;
+    wg.nsort = L.nsort;
+    launch_weigh(wg, stream);
+    LabelArgs la{};
+    la.keys = wg.keys;
+    la.H = a.hidden;
+    la.rows = wg.rows;
+    la.wt = wg.wt;
+    la.lsum = at<float>(a.ws, L.lsum);
+    la.slot = wg.slot;
+    la.next = at<int32_t>(a.ws, L.next);
+    la.hdim = a.hdim;
+    la.nsort = L.nsort;
+    launch_labels(la, nc, stream);
+    DwArgs dw{};
+    dw.Ht = GOp{Hc, a.hdim, nc, a.hdim};
+    dw.Et = GOp{E, a.vocab, nc, a.vocab};
+    dw.slot = la.slot;
+    dw.next = la.next;
+    dw.lsum = la.lsum;
+    dw.dw = a.dweight;
+    dw.acc32 = at<float>(a.ws, L.acc32);
+    dw.nvalid = nvalid;
+    dw.c0 = c0;
+    dw.hdim = a.hdim;
+    dw.V = a.vocab;
+    dw.chunk = L.chunk;
+    launch_dw(dw, L.few && L.nchunks == 1, stream);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace siq

@@ -12,9 +12,15 @@ row.
 The backward starts from the numerators where the forward could keep them
 (``keep_bytes``), and forms the logits again, chunk by chunk, otherwise: a
 quarter of the work in full training, a third with a frozen ``lm_head``.
+
+``fused_linear_token_stats`` gives more of the same distributions: their
+entropies, with gradients (an entropy bonus), and their most probable tokens,
+which is what a teacher hands to a student (``siq_vl_amd.distillation``).
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -85,4 +91,66 @@ def fused_linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: t
     return logp
 
 
-__all__ = ["DEFAULT_KEEP_BYTES", "flp_bwd", "flp_fwd", "fused_linear_log_probs"]
+class TokenStats(NamedTuple):
+    """``fused_linear_token_stats``' results, fp32 (``top_ids`` int64) of the
+    labels' shape, the last two with ``top_k`` values behind it (None without)."""
+
+    log_probs: torch.Tensor | None
+    entropy: torch.Tensor
+    top_log_probs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def fused_linear_token_stats(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor | None = None, top_k: int = 0,
+                             ignore_index: int = IGNORE_INDEX, temperature: float = 1.0, chunk_tokens: int | None = None,
+                             validate="lazy") -> TokenStats:
+    """What ``p = softmax(hidden @ weight.T / temperature)`` says, without logits:
+    ``log p`` at ``labels``, the entropy ``-sum p log p`` of every row, and its
+    ``top_k`` (at most 128) most probable tokens in order, equal ones by lower id
+    first, with their log-probabilities.
+
+    ``labels`` as for ``fused_linear_log_probs``: rows with ``ignore_index`` take
+    no part and have 0 (``top_ids``: -1), bad labels raise ``LabelError``.  Without
+    labels every row counts and ``log_probs`` is None.
+
+    ``log_probs`` and ``entropy`` have gradients, the alternatives none.  The
+    forward keeps a few numbers a row for them; the backward forms the logits
+    again, ``chunk_tokens`` rows at a time (None: 2 GiB of them).
+    """
+    given = labels is not None
+    if not given:  # any token will do
+        labels, ignore_index = torch.zeros(hidden.shape[:-1], dtype=torch.int64, device=hidden.device), IGNORE_INDEX
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels must be {tuple(hidden.shape[:-1])}, got {tuple(labels.shape)}")
+    h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
+    w = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
+    if chunk_tokens is None:
+        chunk_tokens = default_chunk_tokens(w.shape[0])
+    ignore_index = int(ignore_index)
+    logp, entropy, top_logp, top_ids = _validated(
+        2, h, validate, _judge(w.shape[0], ignore_index),
+        lambda host: _lib.native().token_stats(h, w, labels, ignore_index, float(temperature), int(top_k),
+                                               int(chunk_tokens), host))
+    return TokenStats(logp if given else None, entropy, top_logp, top_ids)
+
+
+def _validated(n: int, hidden: torch.Tensor, validate, judge, call):
+    """``call(host)``'s results but for the last, its ``n`` counts, which ``judge``
+    gets: lazily (``host`` is pinned memory that the call leaves them in), at once
+    (``validate="sync"``) or never.  Captured calls are not validated."""
+    lazy = hidden.is_cuda and validate not in (None, False, "sync")
+    host = _LABEL_CHECKS.landing(n) if lazy else None
+    try:
+        *out, counts = call(host)
+    except BaseException:  # (a checkpoint's recomputation ends in one, behind the launch)
+        if host is not None:
+            _LABEL_CHECKS.hold(hidden.device, host)
+        raise
+    if host is not None:
+        _LABEL_CHECKS.landed_on(hidden.device, host, judge)
+    elif validate == "sync" and not torch.cuda.is_current_stream_capturing():
+        judge(counts.tolist())
+    return out
+
+
+__all__ = ["DEFAULT_KEEP_BYTES", "TokenStats", "flp_bwd", "flp_fwd", "fused_linear_log_probs", "fused_linear_token_stats"]

@@ -1,5 +1,5 @@
-// Native host side of the operators of preference and policy training and of
-// 8-bit activations: argument checks, allocation, launches through the C ABI and
+// Native host side of the operators of preference and policy training, of
+// scoring and distillation, and of 8-bit activations: argument checks, allocation, launches through the C ABI and
 // the autograd nodes, as cross_entropy.py and attention.py have them in Python.
 //
 // These calls are short: a loss of one pair takes 8 us of kernels, and with the
@@ -13,6 +13,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include <map>
@@ -31,7 +32,9 @@ using torch::autograd::variable_list;
 #define SIQ_ENTRIES(X)                                                                                              \
   X(siq_last_error) X(siq_pack8) X(siq_unpack8) X(siq_swiglu8_fwd) X(siq_swiglu8_bwd) X(siq_pref_workspace_bytes)   \
   X(siq_pref_fwd) X(siq_pref_bwd) X(siq_policy_workspace_bytes) X(siq_policy_fwd) X(siq_policy_bwd)                 \
-  X(siq_flp_saved_bytes) X(siq_flp_fwd_workspace_bytes) X(siq_flp_fwd) X(siq_flp_bwd_workspace_bytes) X(siq_flp_bwd)
+  X(siq_flp_saved_bytes) X(siq_flp_fwd_workspace_bytes) X(siq_flp_fwd) X(siq_flp_bwd_workspace_bytes) X(siq_flp_bwd) \
+  X(siq_stats_fwd_workspace_bytes) X(siq_stats_fwd) X(siq_stats_bwd_workspace_bytes) X(siq_stats_bwd)               \
+  X(siq_distill_workspace_bytes) X(siq_distill) X(siq_scale_bf16)
 
 struct Api {
 #define SIQ_MEMBER(name) decltype(&::name) name = nullptr;
@@ -553,6 +556,195 @@ std::pair<Tensor, Tensor> raw_flp_bwd(const Tensor& hidden, const Tensor& weight
                  chunk);
 }
 
+// ---------------------------------------------------------------- token statistics
+// What a call returns, and what its backward takes besides: by row of the labels' shape.
+struct Stats {
+  Tensor logp, entropy, lse, top_logp, top_ids;
+};
+
+Stats stats_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels, int64_t ignore_index, double temperature,
+                int64_t top_k, at::IntArrayRef shape, int64_t* counts) {
+  check_head(hidden, weight, labels);
+  // (as int for the library)
+  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= (1 << 20), "top_k must not be negative, or that large: ", top_k);
+  const c10::DeviceGuard guard(hidden.device());
+  const Tensor h = hidden.contiguous(), w = weight.contiguous(), y = labels.contiguous();
+  const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0);
+  std::vector<int64_t> top = shape.vec();
+  top.push_back(top_k);
+  Stats s{floats(shape, h), floats(shape, h), floats({n}, h), Tensor(), Tensor()};
+  if (top_k > 0) {
+    s.top_logp = floats(top, h);
+    s.top_ids = at::empty(top, h.options().dtype(at::kLong));
+  }
+  const Tensor ws = bytes(api.siq_stats_fwd_workspace_bytes(n, hdim, vocab, (int)top_k), h);
+  check(api.siq_stats_fwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), n, hdim, vocab, ignore_index,
+                          temperature, (int)top_k, fptr(s.logp), fptr(s.entropy), fptr(s.lse), fptr(s.top_logp),
+                          static_cast<int64_t*>(ptr(s.top_ids)), counts, counts + 1, ptr(ws), ws.numel(), stream_of(h)),
+        "siq_stats_fwd");
+  return s;
+}
+
+struct TokenStats : torch::autograd::Function<TokenStats> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
+                               int64_t ignore_index, double temperature, int64_t top_k, int64_t chunk, int64_t* counts) {
+    Stats s = stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, labels.sizes(), counts);
+    ctx->save_for_backward({hidden, weight, labels, s.logp, s.entropy, s.lse});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["chunk"] = chunk;
+    ctx->set_materialize_grads(false);
+    variable_list out = {s.logp, s.entropy};
+    if (top_k > 0) {
+      ctx->mark_non_differentiable({s.top_logp, s.top_ids});
+      out.push_back(s.top_logp);
+      out.push_back(s.top_ids);
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    no_second_derivative("fused_linear_token_stats");
+    variable_list out(8);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor h = rows_2d(s[0]).contiguous(), w = s[1].contiguous(), y = rows_1d(s[2]).contiguous();
+    const c10::DeviceGuard guard(h.device());
+    auto up = [](const Tensor& g) { return g.defined() ? rows_1d(upstream(g)).contiguous() : g; };
+    const Tensor g = up(grads[0]), e = up(grads[1]);
+    const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0), chunk = ctx->saved_data["chunk"].toInt();
+    const Tensor dh = ctx->needs_input_grad(0) ? at::empty(h.sizes(), h.options()) : Tensor();
+    const Tensor dw = ctx->needs_input_grad(1) ? at::empty(w.sizes(), w.options()) : Tensor();
+    const Tensor ws = bytes(api.siq_stats_bwd_workspace_bytes(n, hdim, vocab, chunk, dw.defined()), h);
+    check(api.siq_stats_bwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), fptr(s[3]), fptr(s[4]),
+                            fptr(s[5]), fptr(g), fptr(e), n, hdim, vocab, ctx->saved_data["ignore"].toInt(),
+                            ctx->saved_data["temperature"].toDouble(), ptr(dh), ptr(dw), chunk, ptr(ws), ws.numel(),
+                            stream_of(h)),
+          "siq_stats_bwd");
+    if (dh.defined()) out[0] = dh.view(s[0].sizes());
+    out[1] = dw;
+    return out;
+  }
+};
+
+Tensor counts_of(const optional<Tensor>& host, int64_t n, const Tensor& like) {
+  return host.has_value() ? *host : at::empty({n}, like.options().dtype(at::kLong));
+}
+
+// (logp, entropy, top_logp | None, top_ids | None, [count, bad labels])
+std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>, Tensor> token_stats(const Tensor& hidden, const Tensor& weight,
+                                                                                   const Tensor& labels, int64_t ignore_index,
+                                                                                   double temperature, int64_t top_k,
+                                                                                   int64_t chunk, const optional<Tensor>& host) {
+  TORCH_CHECK_VALUE(chunk > 0, "chunk_tokens must be positive");
+  no_tangent("fused_linear_token_stats", {hidden, weight});
+  const Tensor counts = counts_of(host, 2, hidden);
+  int64_t* const c = counts.data_ptr<int64_t>();
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
+    const variable_list o = TokenStats::apply(hidden, weight, labels, ignore_index, temperature, top_k, chunk, c);
+    if (top_k == 0) return {o[0], o[1], std::nullopt, std::nullopt, counts};
+    return {o[0], o[1], o[2], o[3], counts};
+  }
+  const Stats s = stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, labels.sizes(), c);
+  if (top_k == 0) return {s.logp, s.entropy, std::nullopt, std::nullopt, counts};
+  return {s.logp, s.entropy, s.top_logp, s.top_ids, counts};
+}
+
+// ---------------------------------------------------------------- distillation
+struct DistillOptions {
+  int64_t ignore_index;
+  double temperature, ce_weight;
+  bool reverse, tail;
+  int64_t chunk;
+};
+
+// {loss, divergence, cross_entropy, dh, dw}; gradients undefined unless wanted
+variable_list distill(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const Tensor& ids,
+                      const Tensor& teacher, const DistillOptions& o, const optional<Tensor>& divisor, bool need_dh, bool need_dw,
+                      int64_t* counts) {
+  check_head(hidden, weight, labels);
+  const int64_t n = hidden.size(0), hdim = hidden.size(1), vocab = weight.size(0);
+  TORCH_CHECK_VALUE(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "top_ids must be int64 or int32, got ",
+                    type_name(ids));
+  TORCH_CHECK_VALUE(ids.dim() == 2 && ids.size(0) == n && teacher.sizes() == ids.sizes(),
+                    "top_ids and top_log_probs must be [", n, ", top_k], got ", shape_name(ids), " and ", shape_name(teacher));
+  TORCH_CHECK_VALUE(ids.size(1) <= (1 << 20), "top_k is too large: ", ids.size(1));
+  TORCH_CHECK_VALUE(teacher.scalar_type() == at::kFloat, "top_log_probs must be float32, got ", type_name(teacher));
+  on_device(ids, "top_ids", hidden);
+  on_device(teacher, "top_log_probs", hidden);
+  const c10::DeviceGuard guard(hidden.device());
+  const Tensor h = hidden.contiguous(), w = weight.contiguous(), y = labels.contiguous(), i = ids.contiguous(),
+               t = teacher.contiguous();
+  const Tensor loss = floats({}, h), div = floats({}, h), ce = floats({}, h);
+  const Tensor dh = need_dh ? at::empty(h.sizes(), h.options()) : Tensor();
+  const Tensor dw = need_dw ? at::empty(w.sizes(), w.options()) : Tensor();
+  const int k = (int)i.size(1);
+  const Tensor ws = bytes(api.siq_distill_workspace_bytes(n, hdim, vocab, k, o.chunk, need_dh || need_dw, need_dw), h);
+  check(api.siq_distill(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), ptr(i), (int)i.element_size(), fptr(t),
+                        n, hdim, vocab, k, o.ignore_index, o.temperature, o.ce_weight,
+                        o.reverse ? SIQ_DIVERGENCE_REVERSE : SIQ_DIVERGENCE_FORWARD, o.tail, fptr(divisor), fptr(loss),
+                        fptr(div), fptr(ce), counts, ptr(dh), ptr(dw), o.chunk, ptr(ws), ws.numel(), stream_of(h)),
+        "siq_distill");
+  return {loss, div, ce, dh, dw};
+}
+
+// t times a device scalar: in place, unless the graph is kept and a second backward wants t as it is.
+Tensor scaled(const Tensor& t, const Tensor& g, bool in_place) {
+  const Tensor out = in_place ? t : at::empty(t.sizes(), t.options());
+  check(api.siq_scale_bf16(t.data_ptr(), out.data_ptr(), t.numel(), fptr(g), stream_of(t)), "siq_scale_bf16");
+  return out;
+}
+
+// The gradients are known in the forward up to the upstream one, a scalar.
+struct Distillation : torch::autograd::Function<Distillation> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
+                               const Tensor& ids, const Tensor& teacher, int64_t ignore_index, double temperature,
+                               double ce_weight, bool reverse, bool tail, int64_t chunk, const optional<Tensor>& divisor,
+                               int64_t* counts) {
+    const DistillOptions o{ignore_index, temperature, ce_weight, reverse, tail, chunk};
+    const variable_list r = distill(rows_2d(hidden), weight, rows_1d(labels), rows_2d(ids), rows_2d(teacher), o, divisor,
+                                    hidden.requires_grad(), weight.requires_grad(), counts);
+    ctx->save_for_backward({r[3], r[4]});
+    ctx->saved_data["shape"] = hidden.sizes().vec();
+    ctx->mark_non_differentiable({r[1], r[2]});
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1], r[2]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    no_second_derivative("fused_linear_distillation");
+    variable_list out(13);
+    if (!grads[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor g = upstream(grads[0]);
+    const c10::DeviceGuard guard(g.device());
+    const bool in_place = !torch::autograd::get_current_graph_task_keep_graph();
+    if (ctx->needs_input_grad(0)) out[0] = scaled(s[0], g, in_place).view(ctx->saved_data["shape"].toIntVector());
+    if (ctx->needs_input_grad(1)) out[1] = scaled(s[1], g, in_place);
+    return out;
+  }
+};
+
+// (loss, divergence, cross_entropy, [count, bad labels, bad tokens])
+std::tuple<Tensor, Tensor, Tensor, Tensor> distillation(const Tensor& hidden, const Tensor& weight, const Tensor& labels,
+                                                        const Tensor& ids, const Tensor& teacher, int64_t ignore_index,
+                                                        double temperature, double ce_weight, bool reverse, bool tail,
+                                                        int64_t chunk, const optional<Tensor>& divisor,
+                                                        const optional<Tensor>& host) {
+  TORCH_CHECK_VALUE(chunk > 0, "chunk_tokens must be positive");
+  TORCH_CHECK_VALUE(!teacher.requires_grad() || !at::GradMode::is_enabled(),
+                    "gradients with respect to top_log_probs are not supported (detach it)");
+  no_tangent("fused_linear_distillation", {hidden, weight, teacher});
+  const Tensor counts = counts_of(host, 3, hidden);
+  int64_t* const c = counts.data_ptr<int64_t>();
+  variable_list r;
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
+    r = Distillation::apply(hidden, weight, labels, ids, teacher, ignore_index, temperature, ce_weight, reverse, tail, chunk,
+                            divisor, c);
+  else
+    r = distill(rows_2d(hidden), weight, rows_1d(labels), rows_2d(ids), rows_2d(teacher),
+                {ignore_index, temperature, ce_weight, reverse, tail, chunk}, divisor, false, false, c);
+  return {r[0], r[1], r[2], counts};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -570,6 +762,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   SIQ_DEF("flp_fwd", raw_flp_fwd);
   SIQ_DEF("flp_bwd", raw_flp_bwd);
   SIQ_DEF("linear_log_probs", linear_log_probs);
+  SIQ_DEF("token_stats", token_stats);
+  SIQ_DEF("distillation", distillation);
   m.def("no_tangent", [](const char* what, const std::vector<Tensor>& inputs) {
     for (const Tensor& t : inputs) no_tangent(what, {t});
   });
