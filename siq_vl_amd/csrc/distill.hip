@@ -14,8 +14,8 @@
 // and with the label  dz = (1 - c) dD/dz + c (p - [y]).
 //
 // The products are the fused cross-entropy's, over chunks of compacted rows:
-//  1. lists: a row's tokens (the label among them) sorted by id, and how many of
-//     them lie before each tile of the vocabulary;
+//  1. lists: a row's tokens (the label among them), a bit of the vocabulary for
+//     each, and where a tile's begin;
 //  2. logits GEMM: softmax numerators E in bf16 and their sums per tile without the
 //     listed tokens, whose logits it leaves in fp32: what is outside the list is
 //     never a difference from 1;
@@ -38,10 +38,9 @@ namespace {
 
 using namespace gemm;
 
-// What a list's entry is: a token of the teacher, the label where the teacher does
-// not name it, or one that repeats another.
-enum Kind { kTeacher = 0, kLabelOnly = 1, kDead = 2 };
-constexpr int kKindShift = 24;
+// An entry of a list: the token's id, and whether it is the label where the teacher
+// does not name it.
+constexpr int32_t kIdMask = (1 << 24) - 1, kLabelOnly = 1 << 24;
 constexpr int kListLanes = 3, kListMost = 64 * kListLanes;  // entries a lane; of a row
 static_assert(kMaxTeacher + 1 <= kListMost, "the label behind the teacher's tokens");
 
@@ -52,30 +51,32 @@ struct ListArgs {
   const int32_t* rows;    // [nc]
   const int64_t* y;       // [nc]
   const int64_t* nvalid;
-  int32_t* out;           // [nc, ldk] ids with kinds, in order of ids
+  int32_t* out;           // [nc, ldk] the list, in the order of list_place
   float* lt;              // [nc, ldk] the teacher's log-probabilities
-  uint8_t* first;         // [nc, ldt] entries before each tile
+  uint8_t* mask;          // [nc, ldm] as the logits kernels want it
+  uint8_t* base;          // [nc, ldb]
   int32_t* len;           // [nc]
   int32_t* bad;           // [nc] tokens outside the vocabulary, or named twice
-  int64_t nc, c0, V, nvt;
-  int K, ldk, ldt, vt;    // vt: columns of a tile
+  int64_t nc, c0, V, nvt, ldm, ldb;
+  int K, ldk;
 };
 
-// A wave a row.  Keys are id * 256 + place (the label's place is 255: behind a
-// teacher's same token), unique, and their ranks are counted.  Tokens of
-// probability zero and ids of -1 are not there.
-template <class ID>
+// A wave a row.  Keys are (tile, place in it) * 256 + (place among the teacher's
+// tokens; 255: the label, behind a teacher's same token), unique, and their ranks
+// are counted.  Tokens of probability zero and ids of -1 are not there; of equal ids
+// the first stays.  Then a lane a tile writes its bits.
+template <class ID, bool FEW>
 __global__ __launch_bounds__(256) void distill_list_kernel(const ListArgs p) {
+  constexpr int VT = FEW ? kFewBI : kVT, LANE = list_lane_bits(FEW), NL = VT / LANE;
   constexpr uint32_t kNone = ~0u;
   __shared__ uint32_t key_sh[4][kListMost], sorted_sh[4][kListMost];
   __shared__ float lt_sh[4][kListMost];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t k = (int64_t)blockIdx.x * 4 + w, nv = min(p.nc, *p.nvalid - p.c0);
   const bool real = k < nv;
-  uint32_t* key = key_sh[w];
   uint32_t mine[kListLanes];
+  int id[kListLanes], nbad = 0;
   float lt[kListLanes];
-  int nbad = 0;
   if (real) {
     const int64_t src = (int64_t)p.rows[k] * p.K;
 #pragma unroll
@@ -83,76 +84,124 @@ __global__ __launch_bounds__(256) void distill_list_kernel(const ListArgs p) {
       const int e = lane + 64 * i;
       mine[i] = kNone;
       lt[i] = -INFINITY;
+      int64_t v = -1;
       bool wrong = false;
       if (e < p.K) {
-        const int64_t id = static_cast<const ID*>(p.ids)[src + e];
+        v = static_cast<const ID*>(p.ids)[src + e];
         lt[i] = p.teacher[src + e];
-        wrong = id != -1 && (id < 0 || id >= p.V);
-        if (id >= 0 && id < p.V && lt[i] != -INFINITY) mine[i] = (uint32_t)id << 8 | (uint32_t)e;
+        wrong = v != -1 && (v < 0 || v >= p.V);
+        if (wrong || lt[i] == -INFINITY) v = -1;
       } else if (e == p.K) {
-        mine[i] = (uint32_t)p.y[k] << 8 | 255u;
+        v = p.y[k];
       }
+      id[i] = (int)v;
+      if (v >= 0) mine[i] = (uint32_t)(id[i] / VT * VT + list_place(id[i] % VT, FEW)) << 8 | (e < p.K ? (uint32_t)e : 255u);
       nbad += __popcll(__ballot(wrong));
-      key[e] = mine[i];
+      key_sh[w][e] = mine[i];
     }
   }
   __syncthreads();
-  int n = 0;
+  int rank[kListLanes] = {};
   if (real) {
-    int rank[kListLanes] = {};
     for (int j = 0; j <= p.K; ++j) {
-      const uint32_t x = key[j];
+      const uint32_t x = key_sh[w][j];
 #pragma unroll
       for (int i = 0; i < kListLanes; ++i) rank[i] += x < mine[i] ? 1 : 0;
     }
 #pragma unroll
-    for (int i = 0; i < kListLanes; ++i) {
-      n += __popcll(__ballot(mine[i] != kNone));
-      if (mine[i] == kNone) continue;
-      sorted_sh[w][rank[i]] = mine[i];
-      lt_sh[w][rank[i]] = lt[i];
-    }
+    for (int i = 0; i < kListLanes; ++i)
+      if (mine[i] != kNone) sorted_sh[w][rank[i]] = mine[i];
   }
   __syncthreads();
-  if (k >= p.nc) return;
+  // those that repeat the one before them are left out: the others' ranks among themselves
+  int n = 0;
+  uint32_t kept[kListLanes];
   if (real) {
-    int32_t* out = p.out + k * p.ldk;
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i) all += __popcll(__ballot(mine[i] != kNone));
 #pragma unroll
     for (int i = 0; i < kListLanes; ++i) {
       const int e = lane + 64 * i;
-      bool twice = false;
-      if (e < n) {
-        const uint32_t x = sorted_sh[w][e], id = x >> 8;
-        const bool label = (x & 255u) == 255u, same = e > 0 && (sorted_sh[w][e - 1] >> 8) == id;
-        twice = same && !label;
-        out[e] = (int32_t)(id | (uint32_t)(same ? kDead : label ? kLabelOnly : kTeacher) << kKindShift);
-        p.lt[k * p.ldk + e] = lt_sh[w][e];
-      }
-      nbad += __popcll(__ballot(twice));
+      const uint32_t x = e < all ? sorted_sh[w][e] : kNone;
+      const bool same = e < all && e > 0 && sorted_sh[w][e - 1] >> 8 == x >> 8;
+      nbad += __popcll(__ballot(same && (x & 255u) != 255u));
+      const uint64_t m = __ballot(e < all && !same);
+      kept[i] = m >> lane & 1 ? x : kNone;
+      key_sh[w][e] = (uint32_t)(n + __popcll(m & (lane ? ~0ull >> (64 - lane) : 0ull)));  // where rank e goes
+      n += __popcll(m);
     }
+  }
+  __syncthreads();
+  uint32_t* list = sorted_sh[w];
+  if (real) {
+    bool stays[kListLanes];
+    int at[kListLanes];
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i) {
+      at[i] = mine[i] != kNone ? (int)key_sh[w][rank[i]] : 0;
+      stays[i] = mine[i] != kNone && (rank[i] == 0 || list[rank[i] - 1] >> 8 != mine[i] >> 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i)
+      if (stays[i]) {
+        p.out[k * p.ldk + at[i]] = id[i] | ((mine[i] & 255u) == 255u ? kLabelOnly : 0);
+        p.lt[k * p.ldk + at[i]] = lt[i];
+      }
     if (lane == 0) {
       p.len[k] = n;
       p.bad[k] = nbad;
     }
   }
+  __syncthreads();
+  if (real) {
+#pragma unroll
+    for (int i = 0; i < kListLanes; ++i)
+      if (kept[i] != kNone) list[key_sh[w][lane + 64 * i]] = kept[i] >> 8;
+  }
+  __syncthreads();
+  if (k >= p.nc) return;
   // (rows that fill up a tile have no entries)
-  for (int64_t t = lane; t <= p.nvt; t += 64) {
-    const uint32_t bound = (uint32_t)(t * p.vt) << 8;
+  for (int64_t t = lane; t < p.nvt; t += 64) {
+    const uint32_t t0 = (uint32_t)(t * VT);
     int lo = 0, hi = n;
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
-      if (sorted_sh[w][mid] < bound)
+      if (list[mid] < t0)
         lo = mid + 1;
       else
         hi = mid;
     }
-    p.first[k * p.ldt + t] = (uint8_t)lo;
+    uint32_t bits[VT / 32] = {};
+    uint64_t base = 0;  // a byte for each lane's bits
+#pragma unroll
+    for (int q = 0; q < NL; ++q) {
+      base |= (uint64_t)lo << (8 * q);
+      const uint32_t end = t0 + LANE * (q + 1);
+      while (lo < n && list[lo] < end) {
+        const uint32_t b = list[lo++] - t0;
+        const uint32_t bit = 1u << (b & 31);
+        if (LANE == 64) {
+          bits[2 * q] |= b & 32 ? 0u : bit;
+          bits[2 * q + 1] |= b & 32 ? bit : 0u;
+        } else {
+          bits[q / 2] |= bit;
+        }
+      }
+    }
+    u32x4* dst = reinterpret_cast<u32x4*>(p.mask + k * p.ldm + t * (VT / 8));
+#pragma unroll
+    for (int q = 0; q < VT / 128; ++q) dst[q] = u32x4{bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]};
+    if (NL == 8)
+      *reinterpret_cast<uint64_t*>(p.base + k * p.ldb + 8 * t) = base;
+    else
+      *reinterpret_cast<uint32_t*>(p.base + k * p.ldb + 4 * t) = (uint32_t)base;
   }
 }
 
 // ---------------------------------------------------------------- rows
 struct RowMathArgs {
-  const int32_t* ids;     // [nc, ldk] with kinds
+  const int32_t* ids;     // [nc, ldk] the lists
   const float* lt;        // [nc, ldk]
   const float* zk;        // [nc, ldk] log2 units, relative to ref
   const int32_t* len;     // [nc]
@@ -193,20 +242,20 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
   const int n = p.len[k];
   const int64_t y = p.y[k];
   const double ref = p.ref[k], rtop = p.rtop[k], rsum = p.rsum[k];
-  int id[kListLanes], kind[kListLanes];
+  int id[kListLanes];  // -1: no entry
+  bool teachers[kListLanes];
   double l2[kListLanes], lt[kListLanes];  // ln p in log2 units, ln t
   double top = rtop;
 #pragma unroll
   for (int i = 0; i < kListLanes; ++i) {
     const int e = lane + 64 * i;
     id[i] = -1;
-    kind[i] = kDead;
+    teachers[i] = false;
     l2[i] = lt[i] = -INFINITY;
     if (e >= n) continue;
     const int32_t x = p.ids[k * p.ldk + e];
     id[i] = x & kIdMask;
-    kind[i] = x >> kKindShift;
-    if (kind[i] == kDead) continue;
+    teachers[i] = (x & kLabelOnly) == 0;
     l2[i] = ref + (double)p.zk[k * p.ldk + e];
     lt[i] = p.lt[k * p.ldk + e];
     top = fmax(top, l2[i]);
@@ -219,9 +268,9 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
 #pragma unroll
   for (int i = 0; i < kListLanes; ++i) {
     ex[i] = t[i] = 0.;
-    if (kind[i] == kDead) continue;
+    if (id[i] < 0) continue;
     ex[i] = exp2(l2[i] - top);
-    if (kind[i] == kTeacher) {
+    if (teachers[i]) {
       t[i] = exp(lt[i]);
       inside += ex[i];
       mass += t[i];
@@ -249,7 +298,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
   double div = 0.;
 #pragma unroll
   for (int i = 0; i < kListLanes; ++i) {
-    if (kind[i] != kTeacher) continue;
+    if (!teachers[i]) continue;
     const double ls = (l2[i] - top) * kLn2d - lall, s = ex[i] / all;
     div += p.reverse ? (s == 0. ? 0. : s * (ls - lt[i])) : t[i] * (lt[i] - ls);
   }
@@ -274,9 +323,9 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
 #pragma unroll
   for (int i = 0; i < kListLanes; ++i) {
     dz[i] = 0.;
-    if (kind[i] == kDead) continue;
+    if (id[i] < 0) continue;
     const double s = ex[i] / all;
-    if (kind[i] == kLabelOnly) {
+    if (!teachers[i]) {
       dz[i] = s * outer;
     } else {
       const double ls = (l2[i] - top) * kLn2d - lall;
@@ -307,7 +356,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
   if (fabs(f) > 0x1p100) f = copysign(0x1p100, f);
 #pragma unroll
   for (int i = 0; i < kListLanes; ++i) {
-    if (kind[i] == kDead) continue;
+    if (id[i] < 0) continue;
     const bool apart = lane + 64 * i == place;
     p.E[k * p.V + id[i]] = (bf16)(apart || f == 0. ? 0.f : (float)(dz[i] / f));
     if (apart) {
@@ -363,10 +412,10 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const LossArgs p) {
 
 // ---------------------------------------------------------------- host
 struct Layout {
-  size_t scal, loss, bad, spart, mpart, ids, lt, zk, first, len, rsum, rtop, f0, w0, at, f, wt, E, part, acc32, rows, hc, yc,
+  size_t scal, loss, bad, spart, mpart, ids, lt, zk, mask, base, len, rsum, rtop, f0, w0, at, f, wt, E, part, acc32, rows, hc, yc,
       ref, keys, slot, next, lsum, total;
-  int64_t chunk, nchunks, nvt;
-  int ldk, ldt, vt, splits, prow, run, nsort;
+  int64_t chunk, nchunks, nvt, ldm, ldb;
+  int ldk, vt, splits, prow, run, nsort;
   bool few;
 };
 
@@ -382,7 +431,8 @@ Layout layout(int64_t n, int64_t hdim, int64_t V, int top_k, int64_t chunk, bool
   L.vt = L.few ? kFewBI : kVT;
   L.nvt = (V + L.vt - 1) / L.vt;
   L.ldk = top_k + 1;
-  L.ldt = (int)((L.nvt + 1 + 15) / 16 * 16);
+  L.ldm = L.nvt * L.vt / 8;
+  L.ldb = L.nvt * (L.vt / list_lane_bits(L.few));
   const size_t rows = (size_t)std::max<int64_t>(n, 1), npad = (rows + 255) / 256 * 256, nc = (size_t)L.chunk;
   size_t off = 512;  // scal: nvalid; an unused factor
   auto take = [&](bool on, size_t bytes) {
@@ -397,7 +447,8 @@ Layout layout(int64_t n, int64_t hdim, int64_t V, int top_k, int64_t chunk, bool
   L.ids = take(true, sizeof(int32_t) * nc * L.ldk);
   L.lt = take(true, sizeof(float) * nc * L.ldk);
   L.zk = take(true, sizeof(float) * nc * L.ldk);
-  L.first = take(true, nc * L.ldt);
+  L.mask = take(true, nc * L.ldm);
+  L.base = take(true, nc * L.ldb);
   L.len = take(true, sizeof(int32_t) * nc);
   L.rsum = take(true, sizeof(float) * nc);
   L.rtop = take(true, sizeof(float) * nc);
@@ -471,7 +522,8 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     ls.nvalid = nvalid;
     ls.out = at<int32_t>(a.ws, L.ids);
     ls.lt = at<float>(a.ws, L.lt);
-    ls.first = at<uint8_t>(a.ws, L.first);
+    ls.mask = at<uint8_t>(a.ws, L.mask);
+    ls.base = at<uint8_t>(a.ws, L.base);
     ls.len = at<int32_t>(a.ws, L.len);
     ls.bad = at<int32_t>(a.ws, L.bad) + c0;
     ls.nc = nc;
@@ -480,11 +532,15 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     ls.nvt = L.nvt;
     ls.K = a.top_k;
     ls.ldk = L.ldk;
-    ls.ldt = L.ldt;
-    ls.vt = L.vt;
+    ls.ldm = L.ldm;
+    ls.ldb = L.ldb;
     const dim3 waves((unsigned)((nc + 3) / 4));
-    hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t> : distill_list_kernel<int64_t>), waves, dim3(256), 0, stream,
-                       ls);
+    if (L.few)
+      hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, true> : distill_list_kernel<int64_t, true>), waves, dim3(256),
+                         0, stream, ls);
+    else
+      hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, false> : distill_list_kernel<int64_t, false>), waves,
+                         dim3(256), 0, stream, ls);
 
     LogitsArgs lg{};
     lg.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
@@ -501,11 +557,12 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     lg.ldp = L.chunk;
     lg.store_e = a.grads ? 1 : 0;
     lg.zscale = c.zscale;
-    lg.ids = ls.out;
-    lg.first = ls.first;
+    lg.mask = ls.mask;
+    lg.base = ls.base;
     lg.zk = at<float>(a.ws, L.zk);
     lg.ldk = L.ldk;
-    lg.ldt = L.ldt;
+    lg.ldm = L.ldm;
+    lg.ldb = L.ldb;
     launch_logits(lg, L.few, true, stream);
 
     RowArgs rw{};

@@ -75,11 +75,11 @@ using namespace gemm;
 constexpr float kRefLimit = 0x1p60f;
 
 // LISTS: instead of the label, every token of a row's list is left out of E and
-// of the sums, and its logit goes to zk.  A row has a few tokens a hundred tiles,
-// a wave's 32 rows together one or two of this tile's: they are taken one after
-// the other, each from the one accumulator that holds it, which a uniform branch
-// selects.  (A compare and two selects for each of the 64 accumulators, as for
-// the label, would be made for nearly every tile.)
+// of the sums, and its logit goes to zk.  A list of 64 has a token in one tile of
+// ten, so a wave finds one or two in its 32 rows: each lane has the bits of its own
+// columns, in the order of its accumulators, and only groups of eight in which some
+// lane has one are looked at.  Tokens of a lane lie in a row in zk, so nothing is
+// looked up.
 template <bool LISTS>
 __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
@@ -94,14 +94,15 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
   const int64_t vbase = i0 + 8 * h;
   // the tokens' references, and their labels' offsets from the tile (-1: elsewhere)
   float ref[2];
-  int rel[2];
+  int rel[2];          // LISTS: the list's tokens before this lane's
+  uint64_t listed[2];  // (LISTS alone) this lane's columns, accumulator 16 a + r
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     const int64_t tok = min(j0 + wave_col(b, wj) + l32, p.nc - 1);
     ref[b] = p.ref[tok];
-    if constexpr (LISTS) {  // the list's entries of this tile
-      const uint8_t* first = p.first + tok * p.ldt + ti;
-      rel[b] = first[0] | first[1] << 8;
+    if constexpr (LISTS) {
+      listed[b] = *reinterpret_cast<const uint64_t*>(p.mask + tok * p.ldm + 32 * ti + 8 * (2 * wi + h));
+      rel[b] = p.base[tok * p.ldb + 4 * ti + 2 * wi + h];
     } else {
       const int64_t d = p.y[tok] - vbase;
       rel[b] = d >= 0 && d < 256 ? (int)d : -1;
@@ -148,32 +149,20 @@ __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
     const int64_t tok = j0 + col;
     const bool tv = tok < p.nc;
     if constexpr (LISTS) {
-      for (int at = rel[b] & 255; __any(tv && at < rel[b] >> 8); ++at) {
-        const bool mine = tv && at < rel[b] >> 8;
-        const int v = mine ? (int)((p.ids[tok * p.ldk + at] & kIdMask) - i0) : -1;  // 0 .. 255
-        // (both halves of the wave look at the same entry; one of them, of one of two waves, holds its logit)
-        const bool hit = mine && ((v >> 6) & 1) == wi && ((v >> 3) & 1) == h;
-        const int reg = ((v >> 7) << 5) | ((v >> 5 & 1) << 4) | ((v >> 4 & 1) << 3) | (v & 7);  // 16 a + r
-        float zsel = 0.f;
-        for (uint64_t todo = __ballot(hit); todo != 0; todo &= todo - 1) {
-          const int l = (int)__builtin_ctzll(todo);
-          const bool me = lane == l;
-          switch (__builtin_amdgcn_readlane(reg, l)) {
-#define SIQ_TAKE(a, r)                                  \
-  case 16 * a + r:                                      \
-    zsel = me ? acc[a][b][r] : zsel;                    \
-    acc[a][b][r] = me ? -INFINITY : acc[a][b][r];       \
-    break;
-#define SIQ_TAKE4(a, r) SIQ_TAKE(a, r) SIQ_TAKE(a, r + 1) SIQ_TAKE(a, r + 2) SIQ_TAKE(a, r + 3)
-#define SIQ_TAKE16(a) SIQ_TAKE4(a, 0) SIQ_TAKE4(a, 4) SIQ_TAKE4(a, 8) SIQ_TAKE4(a, 12)
-            SIQ_TAKE16(0) SIQ_TAKE16(1) SIQ_TAKE16(2) SIQ_TAKE16(3)
-#undef SIQ_TAKE16
-#undef SIQ_TAKE4
-#undef SIQ_TAKE
-          }
+      float* zk = p.zk + tok * p.ldk + rel[b];
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const uint32_t bits = tv ? (uint32_t)(listed[b] >> (16 * a + 8 * jj)) & 255u : 0u;
+          if (!__any(bits != 0)) continue;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (bits >> i & 1) {
+              *zk++ = __builtin_fmaf(acc[a][b][8 * jj + i], p.zscale, -ref[b]);
+              acc[a][b][8 * jj + i] = -INFINITY;
+            }
         }
-        if (hit) p.zk[tok * p.ldk + at] = __builtin_fmaf(zsel, p.zscale, -ref[b]);
-      }
     } else {
       // the label logit: held by at most one lane of the workgroup, for one
       // vocab tile in ~600 -- located with one range test per token
@@ -1201,15 +1190,15 @@ __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const Logi
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = zero16();
   float ref[NB];
-  int rel[NB], end[NB];  // the token's label, counted from vbase (-1: not in this wave's rows)
+  int rel[NB];          // the token's label, counted from vbase (-1: not in this wave's rows); LISTS: as above
+  uint32_t listed[NB];  // (LISTS alone) this lane's columns, accumulator r
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = min((int64_t)(32 * b + l32), p.nc - 1);
     ref[b] = p.ref[tok];
     if constexpr (LISTS) {
-      const uint8_t* first = p.first + tok * p.ldt + blockIdx.x;
-      rel[b] = first[0];
-      end[b] = first[1];
+      listed[b] = *reinterpret_cast<const uint16_t*>(p.mask + tok * p.ldm + 16 * blockIdx.x + 2 * (2 * w + h));
+      rel[b] = p.base[tok * p.ldb + 8 * blockIdx.x + 2 * w + h];
     } else {
       const int64_t d = p.y[tok] - vbase;
       rel[b] = d >= 0 && d < 32 && (d & 8) == 0 ? (int)d : -1;
@@ -1261,23 +1250,28 @@ __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const Logi
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
     const bool tv = tok < p.nc;
-    for (int at = LISTS ? rel[b] : 0; LISTS ? __any(tv && at < end[b]) : at == 0; ++at) {
-      bool hit = tv && rel[b] >= 0;
-      int d = rel[b];
-      if constexpr (LISTS) {
-        hit = tv && at < end[b];
-        d = hit ? (int)((p.ids[tok * p.ldk + at] & kIdMask) - vbase) : 0;
-        hit = hit && d >= 0 && d < 32 && (d & 8) == 0;
+    if constexpr (LISTS) {
+      float* zk = p.zk + tok * p.ldk + rel[b];
+      const uint32_t bits = tv ? listed[b] : 0u;
+      if (__any(bits != 0)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (bits >> r & 1) {
+            *zk++ = __builtin_fmaf(acc[b][r], p.zscale, -ref[b]);
+            acc[b][r] = -INFINITY;
+          }
       }
+    } else {
+      const bool hit = tv && rel[b] >= 0;
       if (__any(hit)) {
         float zsel = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (hit && d == 16 * (r >> 3) + (r & 7)) {
+          if (hit && rel[b] == 16 * (r >> 3) + (r & 7)) {
             zsel = acc[b][r];
             acc[b][r] = -INFINITY;
           }
-        if (hit) (LISTS ? p.zk[tok * p.ldk + at] : p.zy[tok]) = __builtin_fmaf(zsel, p.zscale, -ref[b]);
+        if (hit) p.zy[tok] = __builtin_fmaf(zsel, p.zscale, -ref[b]);
       }
     }
     const float sum = numerators(b, ref[b], p.store_e && tv);

@@ -15,9 +15,15 @@ constexpr int kVT = gemm::BI;  // vocab columns per logits tile
 // features of a tile; threads of its workgroup.
 constexpr int kFewRows = 128, kFewBI = 128, kFewThreads = 256;
 
-// A token of a row's list, in order of ids: the id in the lower bits, what it is
-// above them.
-constexpr int32_t kIdMask = (1 << 24) - 1;
+// Rows with a list of tokens: a tile of columns has a bit for each, in the order in
+// which the logits kernels' lanes hold them, so that a lane's columns are 64 (few rows:
+// 16) bits in a row, and a list in that order has each lane's tokens in a row, too.
+// The place of column v of a tile:
+__host__ __device__ constexpr int list_place(int v, bool few) {
+  return few ? (v & 0x60) | (v & 8) << 1 | (v & 16) >> 1 | (v & 7)
+             : (v & 64) << 1 | (v & 8) << 3 | (v & 128) >> 2 | (v & 32) >> 1 | (v & 16) >> 1 | (v & 7);
+}
+constexpr int list_lane_bits(bool few) { return few ? 16 : 64; }
 
 struct LogitsArgs {
   gemm::GOp W, H;               // W [V, hdim], H = hidden rows of the chunk [nc, hdim]
@@ -34,10 +40,11 @@ struct LogitsArgs {
   int label_apart;        // the label is left out of E and of the sums
   float zscale;           // log2(e) / temperature
   // rows with a list of tokens apart (launch_logits' `lists`; zy is not written)
-  const int32_t* ids;     // [nc, ldk] a row's tokens in order, with kinds (kIdMask)
-  const uint8_t* first;   // [nc, ldt] how many of them lie before each tile of columns
-  float* zk;              // [nc, ldk] their logits in log2 units, relative to ref
-  int ldk, ldt;
+  const uint8_t* mask;    // [nc, ldm] a bit for each column: listed (list_place)
+  const uint8_t* base;    // [nc, ldb] for each lane's bits of a tile: how many tokens of the list come before them
+  float* zk;              // [nc, ldk] the listed tokens' logits in log2 units, relative to ref, in the list's order
+  int64_t ldm, ldb;
+  int ldk;
 };
 
 struct RowArgs {
