@@ -558,8 +558,8 @@ int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* wei
  * z = hidden weight^T / temperature exist only as one chunk's.
  *
  * siq_stats_fwd: for each counted row logp = ln softmax(z) at the label,
- * entropy = -sum p ln p, and with top_k > 0 (at most 128 and vocab; vocab at most
- * 2^19) the largest logits' ids in order, equal ones by lower id first
+ * entropy = -sum p ln p, and with top_k > 0 (at most 128 and vocab)
+ * the largest logits' ids in order, equal ones by lower id first
  * (top_ids [n, top_k]), with their log-probabilities (top_logp).  Rows that do not
  * count have 0, and ids of -1.  A row with a NaN logit has NaN log-probabilities
  * and ids in [0, vocab).  logp, entropy, lse [n]; lse is what siq_stats_bwd takes

@@ -447,8 +447,6 @@ int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels,
       (rc = check_top_k(top_k, 0, vocab)) || (rc = check_not_null(count, "count")) ||
       (rc = check_not_null(bad_labels, "bad_labels")))
     return rc;
-  if (top_k > 0 && vocab > siq::kMaxTopVocab)
-    return fail(SIQ_ERR_UNSUPPORTED, "top_k needs a vocabulary of at most 2^19 (got %lld)", (long long)vocab);
   if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
                 (rc = check_not_null(lse, "lse"))))
     return rc;

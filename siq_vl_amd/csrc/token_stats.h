@@ -9,7 +9,6 @@
 namespace siq {
 
 constexpr int kMaxTopK = 128;
-constexpr int64_t kMaxTopVocab = int64_t(1) << 19;  // with alternatives: what one workgroup selects from
 
 struct StatsArgs {
   const bf16* hidden;   // [n, hdim]

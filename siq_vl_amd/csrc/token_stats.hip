@@ -11,18 +11,15 @@
 //
 // Forward, per chunk of compacted rows (rows whose label counts):
 //  1. logits GEMM (MFMA, 256 x 256 tiles; few rows: 128 columns of W).  The
-//     epilogue leaves, per (row, half tile), the maximum m, the sum of
+//     epilogue leaves, per row and part of 128 columns, the maximum m, the sum of
 //     2^(z2 - m) and the sum of 2^(z2 - m) (z2 - m), in log2 units: what both
 //     the logsumexp and the entropy are merged from, without any reference that
 //     a row could exceed.  The given token is kept out of them, so that what is
 //     next to certain keeps its digits, and added in the row pass.  With
-//     alternatives wanted it also writes z itself in fp32 and the maximum of
-//     each segment of 64 columns (few rows: 32).
-//  2. row pass: merges in 64 bits; logp, H, lse.
-//  3. selection, a workgroup a row: the K segments of largest maxima hold the K
-//     largest z (each of K segments ranked before a segment has an element
-//     ranked before all of that one's), so K segments are read instead of the
-//     row.
+//     alternatives wanted it also writes z itself in fp32 and the part's largest z.
+//  2. row pass, a workgroup a row: merges in 64 bits; logp, H, lse.  The K-th
+//     largest of the maxima of 256 groups of parts is a bound that the K largest z
+//     do not lie below, so of z only the parts that reach it are read.
 //
 // Backward: lse and H are known, so the logits GEMM, made again, writes dZ
 // itself in bf16 (but for the given token, whose term is added in fp32 by the
@@ -46,26 +43,30 @@ struct StatLogitsArgs {
   GOp W, H;               // W [V, hdim], H = compacted rows of the chunk [nc, hdim]
   const int64_t* y;       // [nc]
   float* Z;               // [nc, V] z before the temperature, or nullptr
-  float* smax;            // [nc, nseg] maxima of segments of columns (Z alone)
-  f32x4* part;            // [parts, ldp] {m, sum, sum of products, -} of (half) tiles
+  f32x4* part;            // [nc, parts] {m, sum, sum of products, largest z (before the temperature)}
   float* zy;              // [nc] z of the given token
   const int64_t* nvalid;
-  int64_t V, nc, c0, ldp, nseg;
+  int64_t V, nc, c0, parts;
   int nI, nJ;
   float zscale;           // log2(e) / temperature
 };
 
-// {m, s, t} of NA x 16 accumulators of a lane and of its other half: the maximum of
-// z2 = z zscale, and the sums of 2^(z2 - m) and of 2^(z2 - m) (z2 - m).
+// The largest of NA x 16 accumulators of a lane and of its other half.
 template <int NA, class Get>
-__device__ __forceinline__ f32x4 stat_part(float zscale, Get z) {
+__device__ __forceinline__ float stat_max(Get z) {
   float m = -INFINITY;
 #pragma unroll
   for (int a = 0; a < NA; ++a)
 #pragma unroll
     for (int r = 0; r < 16; ++r) m = fmaxf(m, z(a, r));
-  m = half_max(m) * zscale;
-  const float base = m == -INFINITY ? 0.f : m;
+  return half_max(m);
+}
+
+// {m, s, t, top} of them: m = largest zscale, and the sums of 2^(z2 - m) and of
+// 2^(z2 - m) (z2 - m) with z2 = z zscale.
+template <int NA, class Get>
+__device__ __forceinline__ f32x4 stat_part(float zscale, float largest, float top, Get z) {
+  const float m = largest * zscale, base = m == -INFINITY ? 0.f : m;
   float s = 0.f, t = 0.f;
 #pragma unroll
   for (int a = 0; a < NA; ++a)
@@ -76,7 +77,7 @@ __device__ __forceinline__ f32x4 stat_part(float zscale, Get z) {
       // (2^-1e4 is 0: masked columns, and those at minus infinity, add nothing)
       t = __builtin_fmaf(e, fmaxf(x, -1e4f), t);
     }
-  return f32x4{m, half_sum(s), half_sum(t), 0.f};
+  return f32x4{m, half_sum(s), half_sum(t), top};
 }
 
 __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p) {
@@ -110,32 +111,27 @@ __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p
   for (int b = 0; b < 2; ++b) {
     const int64_t tok = j0 + wave_col(b, wj) + l32;
     const bool tv = tok < p.nc;
-    if (p.Z != nullptr) {
+    if (p.Z != nullptr && tv) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {  // a wave's segment of each half of the tile
-        float m = -INFINITY;
+      for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int a = 2 * q; a < 2 * q + 2; ++a)
+        for (int jj = 0; jj < 2; ++jj) {
+          const int64_t v0 = vbase + wave_row(a, wi) + 16 * jj;
+          if (v0 >= p.V) continue;
+          f32x4 lo, hi;
 #pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int64_t v0 = vbase + wave_row(a, wi) + 16 * jj;
-            f32x4 lo, hi;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              lo[i] = acc[a][b][8 * jj + i];
-              hi[i] = acc[a][b][8 * jj + 4 + i];
-              m = fmaxf(m, fmaxf(lo[i], hi[i]));
-            }
-            if (tv && v0 < p.V) {
-              float* z = p.Z + tok * p.V + v0;
-              *reinterpret_cast<f32x4*>(z) = lo;
-              *reinterpret_cast<f32x4*>(z + 4) = hi;
-            }
+          for (int i = 0; i < 4; ++i) {
+            lo[i] = acc[a][b][8 * jj + i];
+            hi[i] = acc[a][b][8 * jj + 4 + i];
           }
-        m = half_max(m);
-        if (tv && h == 0) p.smax[tok * p.nseg + 4 * ti + 2 * q + wi] = m;
-      }
+          float* z = p.Z + tok * p.V + v0;
+          *reinterpret_cast<f32x4*>(z) = lo;
+          *reinterpret_cast<f32x4*>(z + 4) = hi;
+        }
     }
+    auto get = [&](int a, int r) { return acc[a][b][r]; };
+    const float top = stat_max<4>(get);
+    float largest = top;
     // the given token: in at most one lane of the workgroup, for one tile in ~600
     const bool hit = tv && rel[b] >= 0 && ((rel[b] >> 6) & 1) == wi && ((rel[b] >> 3) & 1) == 0;
     if (__any(hit)) {
@@ -150,9 +146,10 @@ __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p
             acc[a][b][r] = -INFINITY;
           }
       if (hit) p.zy[tok] = zsel;
+      largest = stat_max<4>(get);
     }
-    const f32x4 st = stat_part<4>(p.zscale, [&](int a, int r) { return acc[a][b][r]; });
-    if (tv && h == 0) p.part[(int64_t)(2 * ti + wi) * p.ldp + tok] = st;
+    const f32x4 st = stat_part<4>(p.zscale, largest, top, get);
+    if (tv && h == 0) p.part[tok * p.parts + 2 * ti + wi] = st;
   }
 }
 
@@ -225,27 +222,25 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
     const bool tv = tok < p.nc;
-    if (p.Z != nullptr) {
-      float m = -INFINITY;
+    if (p.Z != nullptr && tv) {
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
         const int64_t v0 = vbase + 16 * jj;
+        if (v0 >= p.V) continue;
         f32x4 lo, hi;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           lo[i] = acc[b][8 * jj + i];
           hi[i] = acc[b][8 * jj + 4 + i];
-          m = fmaxf(m, fmaxf(lo[i], hi[i]));
         }
-        if (tv && v0 < p.V) {
-          float* z = p.Z + tok * p.V + v0;
-          *reinterpret_cast<f32x4*>(z) = lo;
-          *reinterpret_cast<f32x4*>(z + 4) = hi;
-        }
+        float* z = p.Z + tok * p.V + v0;
+        *reinterpret_cast<f32x4*>(z) = lo;
+        *reinterpret_cast<f32x4*>(z + 4) = hi;
       }
-      m = half_max(m);
-      if (tv && h == 0) p.smax[tok * p.nseg + 4 * blockIdx.x + w] = m;
     }
+    auto get = [&](int, int r) { return acc[b][r]; };
+    const float top = stat_max<1>(get);
+    float largest = top;
     const bool hit = tv && rel[b] >= 0;
     if (__any(hit)) {
       float zsel = 0.f;
@@ -256,19 +251,21 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
           acc[b][r] = -INFINITY;
         }
       if (hit) p.zy[tok] = zsel;
+      largest = stat_max<1>(get);
     }
-    const f32x4 st = stat_part<1>(p.zscale, [&](int, int r) { return acc[b][r]; });
+    const f32x4 st = stat_part<1>(p.zscale, largest, top, get);
     if (h == 0) red[w * TOK + 32 * b + l32] = st;
   }
   __syncthreads();
   // a thread a row of the call: the tile's, merged over its waves
   if (tid >= TOK || tid >= p.nc) return;
   f32x4 x[NWV];
-  float m = -INFINITY, s = 0.f, t = 0.f;
+  float m = -INFINITY, s = 0.f, t = 0.f, top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < NWV; ++k) {
     x[k] = red[k * TOK + tid];
     m = fmaxf(m, x[k][0]);
+    top = fmaxf(top, x[k][3]);
   }
 #pragma unroll
   for (int k = 0; k < NWV; ++k) {
@@ -276,94 +273,23 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
     s += x[k][1] * f;
     t += (x[k][2] + x[k][1] * d) * f;
   }
-  p.part[(int64_t)blockIdx.x * p.ldp + tid] = f32x4{m, s, t, 0.f};
+  p.part[tid * p.parts + blockIdx.x] = f32x4{m, s, t, top};
 }
 
 // ---------------------------------------------------------------- row pass
 struct StatRowArgs {
-  const f32x4* part;      // [parts, ldp]
+  const f32x4* part;      // [nc, parts]
   const float* zy;        // [nc]
+  const float* Z;         // [nc, V]
   const int32_t* rows;    // [nc] compacted row -> row
   const int64_t* nvalid;
+  const int64_t* labels;  // [n]
   float *logp, *entropy, *lse;  // [n] by row
-  double* lse64;          // [nc] (compacted; alternatives alone)
-  int64_t nc, c0, ldp, parts;
-  float zscale;
-};
-
-// Merges a row's parts and its given token in 64 bits.  ROWS rows a workgroup of
-// 256 threads, 256 / ROWS threads that share a row: 16 rows where there are many (a
-// read is then 256 contiguous bytes), one where there are few.
-template <int ROWS>
-__global__ __launch_bounds__(256) void stats_row_kernel(const StatRowArgs p) {
-  constexpr int PER = 256 / ROWS, U = 4;
-  __shared__ double sh_s[256], sh_t[256];
-  __shared__ float sh_m[256];
-  const int64_t nv = min(p.nc, *p.nvalid - p.c0), r0 = (int64_t)blockIdx.x * ROWS;
-  if (r0 >= nv) return;
-  const int tid = threadIdx.x, lane = tid % ROWS, k = tid / ROWS;
-  const int64_t row = min(r0 + lane, nv - 1);
-  const float dy = p.zy[row] * p.zscale;
-  const f32x4* src = p.part + row;
-  float m = dy;
-  for (int64_t t0 = k; t0 < p.parts; t0 += PER * U) {
-    float x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = src[min(t0 + PER * u, p.parts - 1) * p.ldp][0];
-#pragma unroll
-    for (int u = 0; u < U; ++u) m = fmaxf(m, x[u]);
-  }
-  sh_m[tid] = m;
-  __syncthreads();
-  for (int i = 0; i < PER; ++i) m = fmaxf(m, sh_m[i * ROWS + lane]);
-  double s = 0., t = 0.;
-  for (int64_t t0 = k; t0 < p.parts; t0 += PER * U) {
-    f32x4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = src[min(t0 + PER * u, p.parts - 1) * p.ldp];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float d = x[u][0] - m;
-      if (t0 + PER * u >= p.parts || x[u][1] == 0.f) continue;  // (nothing but minus infinities; a NaN counts)
-      // (a factor per 256 or more terms: its rounding is that of a sum of so many)
-      const float f = exp2f_fast(d);
-      s += (double)(x[u][1] * f);
-      t += ((double)x[u][2] + (double)x[u][1] * (double)d) * (double)f;
-    }
-  }
-  sh_s[tid] = s;
-  sh_t[tid] = t;
-  __syncthreads();
-  if (k != 0 || r0 + lane >= nv) return;
-  s = t = 0.;
-  for (int i = 0; i < PER; ++i) {
-    s += sh_s[i * ROWS + lane];
-    t += sh_t[i * ROWS + lane];
-  }
-  // the given token: all relative to m
-  constexpr double kLn2d = 0.6931471805599453;
-  const double d = (double)p.zy[row] * (double)p.zscale - (double)m, ey = exp2(d), all = s + ey, over = s * exp2(-d);
-  const double l2 = log2(all);
-  const double ent = kLn2d * (l2 - (t + (ey > 0. ? ey * d : 0.)) / all);
-  const int64_t at = p.rows[row];
-  // p_y = 1 / (1 + over): its logarithm keeps its digits where `over` is small
-  p.logp[at] = (float)(over <= 1e300 ? -log1p(over) : kLn2d * (d - l2));
-  p.entropy[at] = ent < 0. ? 0.f : (float)ent;
-  p.lse[at] = (float)((double)m + l2);
-  if (p.lse64 != nullptr) p.lse64[row] = (double)m + l2;
-}
-
-// ---------------------------------------------------------------- selection
-struct SelectArgs {
-  const float* Z;         // [nc, V]
-  const float* smax;      // [nc, nseg]
-  const double* lse64;    // [nc]
-  const int32_t* rows;    // [nc]
-  const int64_t* nvalid;
   float* top_logp;        // [n, K]
   int64_t* top_ids;
-  int64_t nc, c0, V;
-  int nseg, seg, K;       // segments of a row; columns of one (32 or 64)
+  int64_t c0, V, ignore_index;
+  int parts, K;
+  bool few;               // parts of 128 columns in a row, or twice 64 of a tile
   float zscale;
 };
 
@@ -375,98 +301,168 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float number_of(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
+// ... of a column: of equal numbers the lower column is larger.
+__device__ __forceinline__ uint64_t order_of(float x, int64_t v) { return (uint64_t)order_of(x) << 32 | (uint32_t)~v; }
 
-// One workgroup a row.  The K-th largest of the segments' maxima is found bit by
-// bit; the segments above it, and as many of those at it as K needs, lowest first,
-// are read, their columns that are not below it listed, and each listed column's
-// rank is how many of the others come before it.
-__global__ __launch_bounds__(256) void stats_select_kernel(const SelectArgs p) {
-  extern __shared__ uint64_t dyn[];  // the maxima's keys, then the listed columns (K * seg at most)
-  __shared__ int part_sh[2][4], list[kMaxTopK], n_sh;
-  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn);
-  const int64_t k0 = blockIdx.x;
-  if (k0 >= min(p.nc, *p.nvalid - p.c0)) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const float* sm = p.smax + k0 * p.nseg;
-  for (int i = tid; i < p.nseg; i += 256) keys[i] = order_of(sm[i]);
-  __syncthreads();
-  const int K = p.K, take = min(K, p.nseg);
-  uint32_t tau = 0;  // the take-th largest key
-  int turn = 0;
-  for (int bit = 31; bit >= 0; --bit, turn ^= 1) {
-    const uint32_t cand = tau | (1u << bit);
-    int c = 0;
-    for (int i = tid; i < p.nseg; i += 256) c += keys[i] >= cand ? 1 : 0;
+__device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o);
-    if (lane == 0) part_sh[turn][w] = c;
-    __syncthreads();
-    if (part_sh[turn][0] + part_sh[turn][1] + part_sh[turn][2] + part_sh[turn][3] >= take) tau = cand;
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+constexpr int kRowGroups = 256;               // threads of a workgroup, and groups of parts
+constexpr int kMostParts = 1024, kMostListed = 1024;
+static_assert(kMaxTopK <= kRowGroups, "a bound is the K-th largest group's");
+
+// One workgroup a row.  Columns that reach the bound are listed, usually K or
+// somewhat more, and each one's rank is how many of the others come before it.
+// Where they are too many (long ties, or a vocabulary of few parts) the K largest
+// are taken one after the other instead.
+__global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs p) {
+  constexpr int T = kRowGroups, NWV = T / 64;
+  __shared__ float m_sh[NWV];
+  __shared__ double s_sh[NWV], t_sh[NWV];
+  __shared__ uint32_t best_sh[T];
+  __shared__ int part_sh[kMostParts], nparts_sh, n_sh;
+  __shared__ uint64_t listed_sh[kMostListed], top_sh[NWV];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t k = blockIdx.x, own = p.c0 + k, y = p.labels[own];
+  if (y == p.ignore_index || y < 0 || y >= p.V) {  // a row whose label does not count
+    if (tid == 0) p.logp[own] = p.entropy[own] = p.lse[own] = 0.f;
+    if (tid < p.K) {
+      p.top_logp[own * p.K + tid] = 0.f;
+      p.top_ids[own * p.K + tid] = -1;
+    }
   }
-  if (w == 0) {
-    // the segments, those above tau first
-    const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
-    int n = 0;
-    for (int eq = 0; eq < 2; ++eq)
-      for (int i0 = 0; i0 < p.nseg && n < take; i0 += 64) {
-        const uint32_t x = i0 + lane < p.nseg ? keys[i0 + lane] : 0;
-        const bool in = i0 + lane < p.nseg && (eq ? x == tau : x > tau);
-        const uint64_t m = __ballot(in);
-        const int at = n + __popcll(m & below);
-        if (in && at < take) list[at] = i0 + lane;
-        n = min(take, n + __popcll(m));
-      }
-    if (lane == 0) n_sh = 0;
+  if (p.c0 + k >= *p.nvalid) return;
+  const f32x4* src = p.part + k * p.parts;
+  const double dy = (double)p.zy[k] * (double)p.zscale;
+  float m = (float)dy;
+  uint32_t best = 0;
+  for (int i = tid; i < p.parts; i += T) {
+    const f32x4 x = src[i];
+    m = fmaxf(m, x[0]);
+    best = max(best, order_of(x[3]));
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) m_sh[w] = m;
+  best_sh[tid] = best;
+  if (tid == 0) nparts_sh = n_sh = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NWV; ++i) m = fmaxf(m, m_sh[i]);
+  double s = 0., t = 0.;
+  for (int i = tid; i < p.parts; i += T) {
+    const f32x4 x = src[i];
+    if (x[1] == 0.f) continue;  // (nothing but minus infinities; a NaN counts)
+    // (a factor for the sums of 128 terms: its rounding is that of a sum of so many)
+    const float d = x[0] - m, f = exp2f_fast(d);
+    s += (double)(x[1] * f);
+    t += ((double)x[2] + (double)x[1] * (double)d) * (double)f;
+  }
+  s = wave_sum(s);
+  t = wave_sum(t);
+  if (lane == 0) {
+    s_sh[w] = s;
+    t_sh[w] = t;
+  }
+  // the bound, by each wave for itself: the K-th largest of the groups', bit by bit
+  uint32_t tau = 0;
+  if (p.K > 0) {
+    uint32_t b[NWV];
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) b[i] = best_sh[64 * i + lane];
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = tau | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < NWV; ++i) c += __popcll(__ballot(b[i] >= cand));
+      if (c >= p.K) tau = cand;
+    }
   }
   __syncthreads();
-  // a segment at a time for 64 or 32 lanes; with fewer segments than K there is no bound
-  const uint32_t least = p.nseg > K ? tau : 0u;
-  const float* z = p.Z + k0 * p.V;
-  const int groups = 256 / p.seg;
-  for (int s0 = 0; s0 < take; s0 += groups) {
-    const int s = s0 + tid / p.seg;
-    const int64_t v = s < take ? (int64_t)list[s] * p.seg + tid % p.seg : p.V;
-    if (v >= p.V) continue;
-    const uint32_t key = order_of(z[v]);
-    if (key >= least) dyn[atomicAdd(&n_sh, 1)] = (uint64_t)key << 32 | (uint32_t)~v;  // (in any order: ranks make one)
+  s = t = 0.;
+#pragma unroll
+  for (int i = 0; i < NWV; ++i) {
+    s += s_sh[i];
+    t += t_sh[i];
+  }
+  // the given token: all relative to m
+  constexpr double kLn2d = 0.6931471805599453;
+  const double d = dy - (double)m, ey = exp2(d), all = s + ey, l2 = log2(all), lse = (double)m + l2;
+  const int64_t row = p.rows[k];
+  if (tid == 0) {
+    const double over = s * exp2(-d), ent = kLn2d * (l2 - (t + (ey > 0. ? ey * d : 0.)) / all);
+    // p_y = 1 / (1 + over): its logarithm keeps its digits where `over` is small
+    p.logp[row] = (float)(over <= 1e300 ? -log1p(over) : kLn2d * (d - l2));
+    p.entropy[row] = ent < 0. ? 0.f : (float)ent;
+    p.lse[row] = (float)lse;
+  }
+  if (p.K == 0) return;
+  const float* z = p.Z + k * p.V;
+  auto result = [&](int rank, uint64_t key) {
+    const float zi = number_of((uint32_t)(key >> 32));
+    p.top_logp[row * p.K + rank] = (float)(((double)zi * (double)p.zscale - lse) * kLn2d);
+    p.top_ids[row * p.K + rank] = (int64_t)(uint32_t)~(uint32_t)key;
+  };
+  for (int i = tid; i < p.parts; i += T)
+    if (order_of(src[i][3]) >= tau) {
+      const int at = atomicAdd(&nparts_sh, 1);  // (in any order: ranks make one)
+      if (at < kMostParts) part_sh[at] = i;
+    }
+  __syncthreads();
+  const int np = nparts_sh, c = tid & 127, off = p.few ? c : (c & 63) + 128 * (c >> 6);
+  if (np <= kMostParts) {
+    constexpr int U = 4, STEP = T / 128;
+    for (int q0 = tid / 128; q0 < np; q0 += STEP * U) {
+      float x[U];
+      int64_t v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = q0 + STEP * u, part = part_sh[min(q, np - 1)];
+        v[u] = (p.few ? 128 * (int64_t)part : 256 * (int64_t)(part >> 1) + 64 * (part & 1)) + off;
+        if (q >= np || v[u] >= p.V) v[u] = -1;
+        x[u] = v[u] >= 0 ? z[v[u]] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v[u] >= 0 && order_of(x[u]) >= tau) {
+          const int at = atomicAdd(&n_sh, 1);
+          if (at < kMostListed) listed_sh[at] = order_of(x[u], v[u]);
+        }
+    }
   }
   __syncthreads();
   const int n = n_sh;
-  const double lse = p.lse64[k0];
-  const int64_t out = (int64_t)p.rows[k0] * K;
-  for (int i = tid; i < n; i += 256) {
-    const uint64_t mine = dyn[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += dyn[j] > mine ? 1 : 0;
-    if (rank >= K) continue;
-    const float zi = number_of((uint32_t)(mine >> 32));
-    p.top_logp[out + rank] = (float)(((double)zi * (double)p.zscale - lse) * 0.6931471805599453);
-    p.top_ids[out + rank] = (int64_t)(uint32_t)~(uint32_t)mine;
+  if (np <= kMostParts && n <= kMostListed) {
+    for (int i = tid; i < n; i += T) {
+      const uint64_t mine = listed_sh[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += listed_sh[j] > mine ? 1 : 0;
+      if (rank < p.K) result(rank, mine);
+    }
+    return;
   }
-}
-
-// Rows whose label does not count: 0, and -1 for ids.
-struct StatClearArgs {
-  const int64_t* labels;
-  float *logp, *entropy, *lse, *top_logp;
-  int64_t* top_ids;
-  int64_t n, V, ignore_index;
-  int K;
-};
-__global__ __launch_bounds__(256) void stats_clear_kernel(const StatClearArgs p) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < p.n; t += (int64_t)gridDim.x * 4) {
-    const int64_t v = p.labels[t];
-    if (v != p.ignore_index && v >= 0 && v < p.V) continue;
-    if (lane == 0) {
-      p.logp[t] = 0.f;
-      p.entropy[t] = 0.f;
-      p.lse[t] = 0.f;
+  uint64_t last = ~0ull;
+  for (int r = 0; r < p.K; ++r) {
+    uint64_t top = 0;
+    for (int64_t v = tid; v < p.V; v += T) {
+      const uint64_t key = order_of(z[v], v);
+      if (key < last && key > top) top = key;
     }
-    for (int k = lane; k < p.K; k += 64) {
-      p.top_logp[t * p.K + k] = 0.f;
-      p.top_ids[t * p.K + k] = -1;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const uint64_t other = __shfl_xor(top, o);
+      top = other > top ? other : top;
     }
+    if (lane == 0) top_sh[w] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) top = top_sh[i] > top ? top_sh[i] : top;
+    if (tid == 0) result(r, top);
+    last = top;
+    __syncthreads();
   }
 }
 
@@ -588,17 +584,15 @@ int64_t stats_chunk(int64_t n, int64_t V, int top_k) {
 }
 
 struct FwdLayout {
-  size_t scal, rows, yc, ref, hc, zy, part, smax, lse64, Z, total;
-  int64_t chunk, parts, nseg;
+  size_t scal, rows, yc, ref, hc, zy, part, Z, total;
+  int64_t chunk, parts;
   bool few;
 };
 FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k) {
   FwdLayout L{};
   L.chunk = stats_chunk(n, V, top_k);
   L.few = L.chunk <= kFewRows;
-  const int64_t tiles = (V + (L.few ? kFewBI : kVT) - 1) / (L.few ? kFewBI : kVT);
-  L.parts = L.few ? tiles : 2 * tiles;
-  L.nseg = 4 * tiles;
+  L.parts = L.few ? (V + kFewBI - 1) / kFewBI : 2 * ((V + kVT - 1) / kVT);
   const size_t npad = (size_t)((std::max<int64_t>(n, 1) + 255) / 256 * 256);
   size_t off = 256;  // scal: nvalid, an unused factor
   auto take = [&](bool on, size_t bytes) {
@@ -612,8 +606,6 @@ FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k) {
   L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
   L.zy = take(true, sizeof(float) * (size_t)L.chunk);
   L.part = take(true, sizeof(f32x4) * (size_t)(L.chunk * L.parts));
-  L.smax = take(top_k > 0, sizeof(float) * (size_t)(L.chunk * L.nseg));
-  L.lse64 = take(top_k > 0, sizeof(double) * (size_t)L.chunk);
   L.Z = take(top_k > 0, sizeof(float) * (size_t)(L.chunk * V));
   L.total = off;
   return L;
@@ -704,8 +696,6 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
   c.ref = at<float>(a.ws, L.ref);
   launch_compact(c, stream);
   if (a.n == 0) return hipGetLastError();
-  StatClearArgs cl{a.labels, a.logp, a.entropy, a.lse, a.top_logp, a.top_ids, a.n, a.vocab, a.ignore_index, a.top_k};
-  hipLaunchKernelGGL(stats_clear_kernel, dim3((unsigned)std::min<int64_t>((a.n + 3) / 4, 1024)), dim3(256), 0, stream, cl);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
     const int64_t nc = std::min(L.chunk, a.n - c0);
     StatLogitsArgs lg{};
@@ -713,15 +703,13 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
     lg.H = GOp{c.hc + c0 * a.hdim, a.hdim, nc, a.hdim};
     lg.y = c.yc + c0;
     lg.Z = a.top_k > 0 ? at<float>(a.ws, L.Z) : nullptr;
-    lg.smax = at<float>(a.ws, L.smax);
     lg.part = at<f32x4>(a.ws, L.part);
     lg.zy = at<float>(a.ws, L.zy);
     lg.nvalid = nvalid;
     lg.V = a.vocab;
     lg.nc = nc;
     lg.c0 = c0;
-    lg.ldp = L.chunk;
-    lg.nseg = L.nseg;
+    lg.parts = L.parts;
     lg.zscale = c.zscale;
     if (L.few) {
       const dim3 grid((unsigned)((a.vocab + kFewBI - 1) / kFewBI));
@@ -736,40 +724,23 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
     StatRowArgs rw{};
     rw.part = lg.part;
     rw.zy = lg.zy;
+    rw.Z = lg.Z;
     rw.rows = rows + c0;
     rw.nvalid = nvalid;
+    rw.labels = a.labels;
     rw.logp = a.logp;
     rw.entropy = a.entropy;
     rw.lse = a.lse;
-    rw.lse64 = a.top_k > 0 ? at<double>(a.ws, L.lse64) : nullptr;
-    rw.nc = nc;
+    rw.top_logp = a.top_logp;
+    rw.top_ids = a.top_ids;
     rw.c0 = c0;
-    rw.ldp = L.chunk;
-    rw.parts = L.parts;
+    rw.V = a.vocab;
+    rw.ignore_index = a.ignore_index;
+    rw.parts = (int)L.parts;
+    rw.K = a.top_k;
+    rw.few = L.few;
     rw.zscale = c.zscale;
-    if (L.few)
-      hipLaunchKernelGGL(stats_row_kernel<1>, dim3((unsigned)nc), dim3(256), 0, stream, rw);
-    else
-      hipLaunchKernelGGL(stats_row_kernel<16>, dim3((unsigned)((nc + 15) / 16)), dim3(256), 0, stream, rw);
-    if (a.top_k > 0) {
-      SelectArgs se{};
-      se.Z = lg.Z;
-      se.smax = lg.smax;
-      se.lse64 = rw.lse64;
-      se.rows = rows + c0;
-      se.nvalid = nvalid;
-      se.top_logp = a.top_logp;
-      se.top_ids = a.top_ids;
-      se.nc = nc;
-      se.c0 = c0;
-      se.V = a.vocab;
-      se.nseg = (int)L.nseg;
-      se.seg = L.few ? 32 : 64;
-      se.K = a.top_k;
-      se.zscale = c.zscale;
-      const size_t lds = std::max(sizeof(uint32_t) * (size_t)L.nseg, sizeof(uint64_t) * (size_t)a.top_k * se.seg);
-      hipLaunchKernelGGL(stats_select_kernel, dim3((unsigned)nc), dim3(256), lds, stream, se);
-    }
+    hipLaunchKernelGGL(stats_row_kernel, dim3((unsigned)nc), dim3(kRowGroups), 0, stream, rw);
   }
   return hipGetLastError();
 }
