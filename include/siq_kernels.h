@@ -563,12 +563,13 @@ int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* wei
  * (top_ids [n, top_k]), with their log-probabilities (top_logp).  Rows that do not
  * count have 0, and ids of -1.  A row with a NaN logit has NaN log-probabilities
  * and ids in [0, vocab).  logp, entropy, lse [n]; lse is what siq_stats_bwd takes
- * besides them.  top_logp and top_ids may be NULL with top_k 0.
+ * besides them.  top_logp and top_ids may be NULL with top_k 0.  saved (siq_stats_saved_bytes,
+ * or NULL): the softmax numerators in bf16, kept for the backward.
  * siq_stats_bwd: dhidden and / or dweight (NULL: not computed) from the upstream
  * gradients dlogp and dentropy [n] (NULL: zero),
  *   dz_j = dlogp ([j = label] - p_j) - dentropy p_j (ln p_j + entropy).
- * They may not overlap hidden.  The logits are formed again, chunk_tokens rows at a
- * time.
+ * They may not overlap hidden.  From what the forward kept on the same inputs, or
+ * (saved NULL) from logits that are formed again; chunk_tokens rows at a time.
  *
  * siq_distill: ids [n, top_k] (ids_bytes 8: int64, 4: int32) name a teacher's
  * tokens and teacher [n, top_k] their log-probabilities ln t; top_k in [1, 128].  An
@@ -592,19 +593,23 @@ int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* wei
 #define SIQ_DIVERGENCE_FORWARD 0
 #define SIQ_DIVERGENCE_REVERSE 1
 
-size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k);
+size_t siq_stats_saved_bytes(int64_t n, int64_t vocab);
+
+size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int keep);
 
 int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
                   int64_t vocab, int64_t ignore_index, double temperature, int top_k, float* logp, float* entropy,
-                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* workspace,
-                  size_t workspace_bytes, void* stream);
+                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* saved,
+                  size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
-size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight);
+size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight,
+                                     int have_saved);
 
 int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* logp,
                   const float* entropy, const float* lse, const float* dlogp, const float* dentropy, int64_t n,
-                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, void* dhidden, void* dweight,
-                  int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream);
+                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, const void* saved,
+                  size_t saved_bytes, void* dhidden, void* dweight, int64_t chunk_tokens, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 size_t siq_distill_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t chunk_tokens,
                                    int need_grads, int need_dweight);

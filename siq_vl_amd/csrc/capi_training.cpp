@@ -134,6 +134,12 @@ int check_grads(const void* hidden, const void* dhidden, const void* dweight, in
   return check_apart(hidden, dhidden, n, hdim);
 }
 
+int check_saved(const void* saved, size_t bytes, size_t need) {
+  if (saved != nullptr && (bytes < need || !aligned16(saved)))
+    return fail(SIQ_ERR_WORKSPACE, "saved needs %zu bytes (16-byte aligned), got %zu", need, bytes);
+  return SIQ_OK;
+}
+
 // Alternatives of a row: at least `least`.
 int check_top_k(int top_k, int least, int64_t vocab) {
   if (top_k < least || top_k > siq::kMaxTopK || top_k > vocab)
@@ -428,23 +434,29 @@ int siq_flp_bwd(const void* hidden, const void* weight, const int64_t* labels, c
   return launched(siq::flp_bwd(a, static_cast<hipStream_t>(stream)), "log-probabilities backward");
 }
 
-size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k) {
-  if (n < 0 || hdim <= 0 || vocab <= 0 || top_k < 0 || top_k > siq::kMaxTopK) return 0;
-  return siq::stats_fwd_workspace_bytes(n, hdim, vocab, top_k);
+size_t siq_stats_saved_bytes(int64_t n, int64_t vocab) {
+  if (n < 0 || vocab <= 0) return 0;
+  return siq::stats_saved_bytes(n, vocab);
 }
 
-size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight) {
+size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int keep) {
+  if (n < 0 || hdim <= 0 || vocab <= 0 || top_k < 0 || top_k > siq::kMaxTopK) return 0;
+  return siq::stats_fwd_workspace_bytes(n, hdim, vocab, top_k, keep != 0);
+}
+
+size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight,
+                                     int have_saved) {
   if (n < 0 || hdim <= 0 || vocab <= 0 || chunk_tokens <= 0) return 0;
-  return siq::stats_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, need_dweight != 0);
+  return siq::stats_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, need_dweight != 0, have_saved != 0);
 }
 
 int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
                   int64_t vocab, int64_t ignore_index, double temperature, int top_k, float* logp, float* entropy,
-                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* workspace,
-                  size_t workspace_bytes, void* stream) {
+                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* saved,
+                  size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
-      (rc = check_top_k(top_k, 0, vocab)) || (rc = check_not_null(count, "count")) ||
+      (rc = check_saved(saved, saved_bytes, siq::stats_saved_bytes(n, vocab))) || (rc = check_top_k(top_k, 0, vocab)) || (rc = check_not_null(count, "count")) ||
       (rc = check_not_null(bad_labels, "bad_labels")))
     return rc;
   if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
@@ -452,7 +464,9 @@ int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels,
     return rc;
   if (n > 0 && top_k > 0 && ((rc = check_not_null(top_logp, "top_logp")) || (rc = check_not_null(top_ids, "top_ids"))))
     return rc;
-  if ((rc = check_ws(workspace, workspace_bytes, siq::stats_fwd_workspace_bytes(n, hdim, vocab, top_k)))) return rc;
+  if ((rc = check_ws(workspace, workspace_bytes,
+                     siq::stats_fwd_workspace_bytes(n, hdim, vocab, top_k, saved != nullptr))))
+    return rc;
   siq::StatsArgs a{};
   a.hidden = static_cast<const siq::bf16*>(hidden);
   a.weight = static_cast<const siq::bf16*>(weight);
@@ -470,16 +484,20 @@ int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels,
   a.top_ids = top_ids;
   a.count = count;
   a.bad_labels = bad_labels;
+  a.saved = saved;
   a.ws = workspace;
   return launched(siq::stats_fwd(a, static_cast<hipStream_t>(stream)), "token statistics");
 }
 
 int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* logp,
                   const float* entropy, const float* lse, const float* dlogp, const float* dentropy, int64_t n,
-                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, void* dhidden, void* dweight,
-                  int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream) {
+                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, const void* saved,
+                  size_t saved_bytes, void* dhidden, void* dweight, int64_t chunk_tokens, void* workspace,
+                  size_t workspace_bytes, void* stream) {
   int rc;
-  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0))) return rc;
+  if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
+      (rc = check_saved(saved, saved_bytes, siq::stats_saved_bytes(n, vocab))))
+    return rc;
   if (chunk_tokens <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "chunk_tokens must be positive");
   if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
                 (rc = check_not_null(lse, "lse"))))
@@ -487,7 +505,7 @@ int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels,
   if ((rc = check_grads(hidden, dhidden, dweight, n, hdim))) return rc;
   if (dhidden == nullptr && dweight == nullptr) return ok();
   if ((rc = check_ws(workspace, workspace_bytes,
-                     siq::stats_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, dweight != nullptr))))
+                     siq::stats_bwd_workspace_bytes(n, hdim, vocab, chunk_tokens, dweight != nullptr, saved != nullptr))))
     return rc;
   siq::StatsArgs a{};
   a.hidden = static_cast<const siq::bf16*>(hidden);
@@ -503,6 +521,7 @@ int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels,
   a.lse = const_cast<float*>(lse);
   a.dlogp = dlogp;
   a.dentropy = dentropy;
+  a.saved = const_cast<void*>(saved);
   a.dhidden = static_cast<siq::bf16*>(dhidden);
   a.dweight = static_cast<siq::bf16*>(dweight);
   a.chunk = chunk_tokens;

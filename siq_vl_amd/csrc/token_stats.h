@@ -29,11 +29,13 @@ struct StatsArgs {
   bf16* dhidden;          // [n, hdim] or nullptr
   bf16* dweight;          // [vocab, hdim] or nullptr
   int64_t chunk;          // tokens per chunk of the backward
+  void* saved;            // forward: kept for the backward, or nullptr; backward: what was kept, or nullptr
   void* ws;
 };
 
-size_t stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k);
-size_t stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw);
+size_t stats_saved_bytes(int64_t n, int64_t vocab);
+size_t stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, bool keep);
+size_t stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw, bool have_saved);
 hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream);
 hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream);
 

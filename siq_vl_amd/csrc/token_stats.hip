@@ -21,9 +21,10 @@
 //     largest of the maxima of 256 groups of parts is a bound that the K largest z
 //     do not lie below, so of z only the parts that reach it are read.
 //
-// Backward: lse and H are known, so the logits GEMM, made again, writes dZ
-// itself in bf16 (but for the given token, whose term is added in fp32 by the
-// products' kernels), and the two gradient products follow.
+// Backward: lse and H are known.  Where the forward could keep 2^(z2 - m) in bf16,
+// one pass over that makes dZ; otherwise the logits GEMM, made again, writes it.
+// The given token is left out: its term is added in fp32 by the products' kernels.
+// The two gradient products follow.
 #include <algorithm>
 
 #include "few.h"
@@ -43,6 +44,7 @@ struct StatLogitsArgs {
   GOp W, H;               // W [V, hdim], H = compacted rows of the chunk [nc, hdim]
   const int64_t* y;       // [nc]
   float* Z;               // [nc, V] z before the temperature, or nullptr
+  bf16* E;                // [nc, V] 2^(z2 - m), 0 for the given token, or nullptr
   f32x4* part;            // [nc, parts] {m, sum, sum of products, largest z (before the temperature)}
   float* zy;              // [nc] z of the given token
   const int64_t* nvalid;
@@ -62,22 +64,28 @@ __device__ __forceinline__ float stat_max(Get z) {
   return half_max(m);
 }
 
-// {m, s, t, top} of them: m = largest zscale, and the sums of 2^(z2 - m) and of
-// 2^(z2 - m) (z2 - m) with z2 = z zscale.
-template <int NA, class Get>
-__device__ __forceinline__ f32x4 stat_part(float zscale, float largest, float top, Get z) {
-  const float m = largest * zscale, base = m == -INFINITY ? 0.f : m;
+// {m, s, t, -} of them: the sums of 2^(z2 - m) and of 2^(z2 - m) (z2 - m) with z2 =
+// z zscale; keep(a, j, e): the terms of accumulators 8 j .. of block a.
+template <int NA, class Get, class Keep>
+__device__ __forceinline__ f32x4 stat_part(float zscale, float m, Get z, Keep keep) {
+  const float base = m == -INFINITY ? 0.f : m;
   float s = 0.f, t = 0.f;
 #pragma unroll
   for (int a = 0; a < NA; ++a)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float x = __builtin_fmaf(z(a, r), zscale, -base), e = exp2f_fast(x);
-      s += e;
-      // (2^-1e4 is 0: masked columns, and those at minus infinity, add nothing)
-      t = __builtin_fmaf(e, fmaxf(x, -1e4f), t);
+    for (int j = 0; j < 2; ++j) {
+      bf16x8 e8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_fmaf(z(a, 8 * j + i), zscale, -base), e = exp2f_fast(x);
+        s += e;
+        // (2^-1e4 is 0: masked columns, and those at minus infinity, add nothing)
+        t = __builtin_fmaf(e, fmaxf(x, -1e4f), t);
+        e8[i] = (bf16)e;
+      }
+      keep(a, j, e8);
     }
-  return f32x4{m, half_sum(s), half_sum(t), top};
+  return f32x4{m, half_sum(s), half_sum(t), 0.f};
 }
 
 __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p) {
@@ -148,7 +156,11 @@ __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p
       if (hit) p.zy[tok] = zsel;
       largest = stat_max<4>(get);
     }
-    const f32x4 st = stat_part<4>(p.zscale, largest, top, get);
+    f32x4 st = stat_part<4>(p.zscale, largest * p.zscale, get, [&](int a, int j, const bf16x8& e) {
+      const int64_t v0 = vbase + wave_row(a, wi) + 16 * j;
+      if (p.E != nullptr && tv && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e);
+    });
+    st[3] = top;
     if (tv && h == 0) p.part[tok * p.parts + 2 * ti + wi] = st;
   }
 }
@@ -217,7 +229,9 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
       for (int r = 0; r < 16; ++r)
         if (vbase + 16 * (r >> 3) + (r & 7) >= p.V) acc[b][r] = -INFINITY;
   }
-  f32x4* red = reinterpret_cast<f32x4*>(smem);  // [NWV][TOK] (behind the last step's barrier)
+  // (behind the last step's barrier) the waves' maxima, then their sums
+  float *max_sh = reinterpret_cast<float*>(smem), *top_sh = max_sh + NWV * TOK;  // [NWV][TOK]
+  f32x4* red = reinterpret_cast<f32x4*>(smem) + 2 * NWV * TOK / 4;               // [NWV][TOK]
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
@@ -253,27 +267,37 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
       if (hit) p.zy[tok] = zsel;
       largest = stat_max<1>(get);
     }
-    const f32x4 st = stat_part<1>(p.zscale, largest, top, get);
-    if (h == 0) red[w * TOK + 32 * b + l32] = st;
+    if (h == 0) {
+      max_sh[w * TOK + 32 * b + l32] = largest;
+      top_sh[w * TOK + 32 * b + l32] = top;
+    }
   }
   __syncthreads();
-  // a thread a row of the call: the tile's, merged over its waves
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t tok = 32 * b + l32;
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NWV; ++k) m = fmaxf(m, max_sh[k * TOK + tok]);
+    const f32x4 st = stat_part<1>(p.zscale, m * p.zscale, [&](int, int r) { return acc[b][r]; },
+                                  [&](int, int j, const bf16x8& e) {
+                                    const int64_t v0 = vbase + 16 * j;
+                                    if (p.E != nullptr && tok < p.nc && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e);
+                                  });
+    if (h == 0) red[w * TOK + tok] = st;
+  }
+  __syncthreads();
+  // a thread a row of the call: the tile's
   if (tid >= TOK || tid >= p.nc) return;
-  f32x4 x[NWV];
-  float m = -INFINITY, s = 0.f, t = 0.f, top = -INFINITY;
+  f32x4 x = red[tid];
+  x[3] = top_sh[tid];
 #pragma unroll
-  for (int k = 0; k < NWV; ++k) {
-    x[k] = red[k * TOK + tid];
-    m = fmaxf(m, x[k][0]);
-    top = fmaxf(top, x[k][3]);
+  for (int k = 1; k < NWV; ++k) {
+    x[1] += red[k * TOK + tid][1];
+    x[2] += red[k * TOK + tid][2];
+    x[3] = fmaxf(x[3], top_sh[k * TOK + tid]);
   }
-#pragma unroll
-  for (int k = 0; k < NWV; ++k) {
-    const float d = fmaxf(x[k][0] - m, -1e4f), f = exp2f_fast(d);
-    s += x[k][1] * f;
-    t += (x[k][2] + x[k][1] * d) * f;
-  }
-  p.part[tid * p.parts + blockIdx.x] = f32x4{m, s, t, top};
+  p.part[tid * p.parts + blockIdx.x] = x;
 }
 
 // ---------------------------------------------------------------- row pass
@@ -547,6 +571,47 @@ __global__ __launch_bounds__(kFewThreads) void stats_grad_few_kernel(const StatG
   }
 }
 
+// dZ from the numerators that the forward kept, a workgroup 2048 columns of a row;
+// the rows that fill up a tile are zeroed, and dH of rows whose label does not
+// count.  It reads and writes 2 bytes an element where the logits take 2 hdim flops.
+struct UnpackArgs {
+  const bf16* E;          // [nc, V]
+  const f32x4* part;      // [nc, parts]
+  const f32x4* coef;      // [nc]
+  bf16* G;                // [nc, V]
+  const int64_t* nvalid;
+  const int64_t* labels;  // [n]
+  bf16* dh;               // or nullptr
+  int64_t nc, c0, V, hdim, ignore_index;
+  int parts;
+  bool few;
+};
+constexpr int kUnpackCols = 2048;
+__global__ __launch_bounds__(256) void stats_unpack_kernel(const UnpackArgs p) {
+  const int64_t nv = min(p.nc, *p.nvalid - p.c0), v = (int64_t)blockIdx.x * kUnpackCols + 8 * threadIdx.x;
+  for (int64_t k = blockIdx.y; k < p.nc; k += gridDim.y) {
+    if (blockIdx.x == 0 && p.dh != nullptr) {
+      const int64_t row = p.c0 + k, y = p.labels[row];
+      if (y == p.ignore_index || y < 0 || y >= p.V)
+        for (int64_t c = 8 * (int64_t)threadIdx.x; c < p.hdim; c += 8 * 256) st_bf16x8(p.dh + row * p.hdim + c, zero_bf16x8());
+    }
+    if (k >= nv + BJ || v >= p.V) continue;
+    bf16x8 g = zero_bf16x8();
+    if (k < nv) {
+      const bf16x8 e = ld_bf16x8(p.E + k * p.V + v);
+      const int64_t part = p.few ? v / kFewBI : 2 * (v / kVT) + (v >> 6 & 1);
+      const f32x4 c = p.coef[k];
+      const float d = p.part[k * p.parts + part][0] - c[0], f = exp2f_fast(d), a = __builtin_fmaf(c[2], d, c[1]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = (float)e[i];
+        g[i] = (bf16)(x * f * __builtin_fmaf(c[2], fmaxf(__log2f(x), -1e4f), a));
+      }
+    }
+    st_bf16x8(p.G + k * p.V + v, g);
+  }
+}
+
 // What a row's gradient needs of the forward's results and of the upstream
 // gradients: {lse, A, B} as above, and the given token's own dz (in 32 bits),
 //   A = -(g + e H) / T,  B = -e ln 2 / T,  dz_y = (g (1 - p_y) - e p_y (ln p_y + H)) / T.
@@ -583,12 +648,29 @@ int64_t stats_chunk(int64_t n, int64_t V, int top_k) {
   return std::max<int64_t>(std::min(n, most), 1);
 }
 
+// What the forward keeps for the backward.
+struct StatsSaved {
+  size_t nvalid, rows, yc, part, E, total;
+  int64_t parts;
+};
+StatsSaved saved_layout(int64_t n, int64_t V) {
+  StatsSaved S{};
+  const size_t npad = (size_t)((std::max<int64_t>(n, 1) + 255) / 256 * 256);
+  S.parts = n <= kFewRows ? (V + kFewBI - 1) / kFewBI : 2 * ((V + kVT - 1) / kVT);
+  S.rows = 256;
+  S.yc = S.rows + al(sizeof(int32_t) * npad);
+  S.part = S.yc + al(sizeof(int64_t) * npad);
+  S.E = S.part + al(sizeof(f32x4) * (size_t)(n * S.parts));
+  S.total = S.E + al(sizeof(bf16) * (size_t)(n * V));
+  return S;
+}
+
 struct FwdLayout {
   size_t scal, rows, yc, ref, hc, zy, part, Z, total;
   int64_t chunk, parts;
   bool few;
 };
-FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k) {
+FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k, bool keep) {
   FwdLayout L{};
   L.chunk = stats_chunk(n, V, top_k);
   L.few = L.chunk <= kFewRows;
@@ -600,12 +682,12 @@ FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k) {
     if (on) off += al(bytes);
     return at;
   };
-  L.rows = take(true, sizeof(int32_t) * npad);
-  L.yc = take(true, sizeof(int64_t) * npad);
+  L.rows = take(!keep, sizeof(int32_t) * npad);
+  L.yc = take(!keep, sizeof(int64_t) * npad);
   L.ref = take(true, sizeof(float) * npad);
   L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
   L.zy = take(true, sizeof(float) * (size_t)L.chunk);
-  L.part = take(true, sizeof(f32x4) * (size_t)(L.chunk * L.parts));
+  L.part = take(!keep, sizeof(f32x4) * (size_t)(L.chunk * L.parts));
   L.Z = take(top_k > 0, sizeof(float) * (size_t)(L.chunk * V));
   L.total = off;
   return L;
@@ -617,7 +699,7 @@ struct BwdLayout {
   int splits, prow, run, nsort;
   bool few;
 };
-BwdLayout bwd_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool need_dw) {
+BwdLayout bwd_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool need_dw, bool have) {
   BwdLayout L{};
   L.chunk = std::max<int64_t>(std::min(chunk, n), 1);
   L.nchunks = (n + L.chunk - 1) / L.chunk;
@@ -629,10 +711,10 @@ BwdLayout bwd_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool nee
     if (on) off += al(bytes);
     return at;
   };
-  L.rows = take(true, sizeof(int32_t) * npad);
-  L.yc = take(true, sizeof(int64_t) * npad);
-  L.ref = take(true, sizeof(float) * npad);
-  L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
+  L.rows = take(!have, sizeof(int32_t) * npad);
+  L.yc = take(!have, sizeof(int64_t) * npad);
+  L.ref = take(!have, sizeof(float) * npad);
+  L.hc = take(!have || need_dw, sizeof(bf16) * npad * (size_t)hdim);
   L.coef = take(true, sizeof(f32x4) * (size_t)L.chunk);
   L.f0 = take(true, sizeof(float) * (size_t)L.chunk);
   L.w0 = take(true, sizeof(float) * (size_t)L.chunk);
@@ -674,17 +756,20 @@ CompactArgs compact_of(const StatsArgs& a) {
 
 }  // namespace
 
-size_t stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k) {
-  return fwd_layout(n, hdim, vocab, top_k).total;
+size_t stats_saved_bytes(int64_t n, int64_t vocab) { return saved_layout(n, vocab).total; }
+size_t stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, bool keep) {
+  return fwd_layout(n, hdim, vocab, top_k, keep).total;
 }
-size_t stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw) {
-  return bwd_layout(n, hdim, vocab, chunk, need_dw).total;
+size_t stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dw, bool have_saved) {
+  return bwd_layout(n, hdim, vocab, chunk, need_dw, have_saved).total;
 }
 
 hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
-  const FwdLayout L = fwd_layout(a.n, a.hdim, a.vocab, a.top_k);
-  int64_t* nvalid = at<int64_t>(a.ws, L.scal);
-  int32_t* rows = at<int32_t>(a.ws, L.rows);
+  const bool keep = a.saved != nullptr;
+  const FwdLayout L = fwd_layout(a.n, a.hdim, a.vocab, a.top_k, keep);
+  const StatsSaved S = saved_layout(a.n, a.vocab);
+  int64_t* nvalid = keep ? at<int64_t>(a.saved, S.nvalid) : at<int64_t>(a.ws, L.scal);
+  int32_t* rows = keep ? at<int32_t>(a.saved, S.rows) : at<int32_t>(a.ws, L.rows);
   CompactArgs c = compact_of(a);
   c.rows = rows;
   c.nvalid = nvalid;
@@ -692,10 +777,9 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
   c.bad = a.bad_labels;
   c.invden = at<float>(a.ws, L.scal) + 32;
   c.hc = at<bf16>(a.ws, L.hc);
-  c.yc = at<int64_t>(a.ws, L.yc);
+  c.yc = keep ? at<int64_t>(a.saved, S.yc) : at<int64_t>(a.ws, L.yc);
   c.ref = at<float>(a.ws, L.ref);
   launch_compact(c, stream);
-  if (a.n == 0) return hipGetLastError();
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
     const int64_t nc = std::min(L.chunk, a.n - c0);
     StatLogitsArgs lg{};
@@ -703,7 +787,8 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
     lg.H = GOp{c.hc + c0 * a.hdim, a.hdim, nc, a.hdim};
     lg.y = c.yc + c0;
     lg.Z = a.top_k > 0 ? at<float>(a.ws, L.Z) : nullptr;
-    lg.part = at<f32x4>(a.ws, L.part);
+    lg.part = keep ? at<f32x4>(a.saved, S.part) + c0 * L.parts : at<f32x4>(a.ws, L.part);
+    lg.E = keep ? at<bf16>(a.saved, S.E) + c0 * a.vocab : nullptr;
     lg.zy = at<float>(a.ws, L.zy);
     lg.nvalid = nvalid;
     lg.V = a.vocab;
@@ -747,13 +832,15 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
 
 hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
   const bool need_dw = a.dweight != nullptr;
-  const BwdLayout L = bwd_layout(a.n, a.hdim, a.vocab, a.chunk, need_dw);
+  const bool have = a.saved != nullptr;
+  const BwdLayout L = bwd_layout(a.n, a.hdim, a.vocab, a.chunk, need_dw, have);
+  const StatsSaved S = saved_layout(a.n, a.vocab);
   if (a.n == 0) {
     if (need_dw) launch_zero(a.dweight, a.vocab * a.hdim, stream);
     return hipGetLastError();
   }
-  int64_t* nvalid = at<int64_t>(a.ws, L.scal);
-  int32_t* rows = at<int32_t>(a.ws, L.rows);
+  int64_t* nvalid = have ? at<int64_t>(a.saved, S.nvalid) : at<int64_t>(a.ws, L.scal);
+  int32_t* rows = have ? at<int32_t>(a.saved, S.rows) : at<int32_t>(a.ws, L.rows);
   CompactArgs c = compact_of(a);
   c.rows = rows;
   c.nvalid = nvalid;
@@ -761,10 +848,10 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
   c.bad = nvalid + 2;
   c.invden = at<float>(a.ws, L.scal) + 32;
   c.hc = at<bf16>(a.ws, L.hc);
-  c.yc = at<int64_t>(a.ws, L.yc);
+  c.yc = have ? at<int64_t>(a.saved, S.yc) : at<int64_t>(a.ws, L.yc);
   c.ref = at<float>(a.ws, L.ref);
   c.dh = a.dhidden;
-  launch_compact(c, stream);
+  if (!have) launch_compact(c, stream);
   bf16* E = at<bf16>(a.ws, L.E);
   float *f0 = at<float>(a.ws, L.f0), *w0 = at<float>(a.ws, L.w0);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
@@ -796,7 +883,25 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
     gr.nc = nc;
     gr.c0 = c0;
     gr.zscale = c.zscale;
-    if (L.few) {
+    if (have) {
+      UnpackArgs un{};
+      un.E = at<bf16>(a.saved, S.E) + c0 * a.vocab;
+      un.part = at<f32x4>(a.saved, S.part) + c0 * S.parts;
+      un.coef = co.coef;
+      un.G = E;
+      un.nvalid = nvalid;
+      un.labels = a.labels;
+      un.dh = a.dhidden;
+      un.nc = nc;
+      un.c0 = c0;
+      un.V = a.vocab;
+      un.hdim = a.hdim;
+      un.ignore_index = a.ignore_index;
+      un.parts = (int)S.parts;
+      un.few = a.n <= kFewRows;
+      const dim3 grid((unsigned)((a.vocab + kUnpackCols - 1) / kUnpackCols), (unsigned)std::min<int64_t>(nc, 32768));
+      hipLaunchKernelGGL(stats_unpack_kernel, grid, dim3(256), 0, stream, un);
+    } else if (L.few) {
       const dim3 grid((unsigned)((a.vocab + kFewBI - 1) / kFewBI));
       hipLaunchKernelGGL((nc <= 64 ? stats_grad_few_kernel<2> : stats_grad_few_kernel<4>), grid, dim3(kFewThreads), 0, stream,
                          gr);
@@ -842,7 +947,7 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
     wg.f0 = f0;
     wg.w0 = w0;
     wg.nvalid = nvalid;
-    wg.Hs = Hc;  // (read by the logits above; every factor is 1)
+    wg.Hs = Hc;  // (which the logits above have read; every factor is 1)
     wg.f = at<float>(a.ws, L.f);
     wg.wt = at<float>(a.ws, L.wt);
     wg.keys = at<uint64_t>(a.ws, L.keys);

@@ -103,7 +103,7 @@ class TokenStats(NamedTuple):
 
 def fused_linear_token_stats(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor | None = None, top_k: int = 0,
                              ignore_index: int = IGNORE_INDEX, temperature: float = 1.0, chunk_tokens: int | None = None,
-                             validate="lazy") -> TokenStats:
+                             keep_bytes: int = DEFAULT_KEEP_BYTES, validate="lazy") -> TokenStats:
     """What ``p = softmax(hidden @ weight.T / temperature)`` says, without logits:
     ``log p`` at ``labels``, the entropy ``-sum p log p`` of every row, and its
     ``top_k`` (at most 128) most probable tokens in order, equal ones by lower id
@@ -113,9 +113,10 @@ def fused_linear_token_stats(hidden: torch.Tensor, weight: torch.Tensor, labels:
     no part and have 0 (``top_ids``: -1), bad labels raise ``LabelError``.  Without
     labels every row counts and ``log_probs`` is None.
 
-    ``log_probs`` and ``entropy`` have gradients, the alternatives none.  The
-    forward keeps a few numbers a row for them; the backward forms the logits
-    again, ``chunk_tokens`` rows at a time (None: 2 GiB of them).
+    ``log_probs`` and ``entropy`` have gradients, the alternatives none.
+    ``keep_bytes`` bounds what the forward may keep for them (2.1 * rows * vocab
+    bytes, ignored rows counted); above it the backward forms the logits again.  It
+    works ``chunk_tokens`` rows at a time (None: 2 GiB of their gradients).
     """
     given = labels is not None
     if not given:  # any token will do
@@ -130,7 +131,7 @@ def fused_linear_token_stats(hidden: torch.Tensor, weight: torch.Tensor, labels:
     logp, entropy, top_logp, top_ids = _validated(
         2, h, validate, _judge(w.shape[0], ignore_index),
         lambda host: _lib.native().token_stats(h, w, labels, ignore_index, float(temperature), int(top_k),
-                                               int(chunk_tokens), host))
+                                               int(chunk_tokens), int(keep_bytes), host))
     return TokenStats(logp if given else None, entropy, top_logp, top_ids)
 
 

@@ -33,8 +33,8 @@ using torch::autograd::variable_list;
   X(siq_last_error) X(siq_pack8) X(siq_unpack8) X(siq_swiglu8_fwd) X(siq_swiglu8_bwd) X(siq_pref_workspace_bytes)   \
   X(siq_pref_fwd) X(siq_pref_bwd) X(siq_policy_workspace_bytes) X(siq_policy_fwd) X(siq_policy_bwd)                 \
   X(siq_flp_saved_bytes) X(siq_flp_fwd_workspace_bytes) X(siq_flp_fwd) X(siq_flp_bwd_workspace_bytes) X(siq_flp_bwd) \
-  X(siq_stats_fwd_workspace_bytes) X(siq_stats_fwd) X(siq_stats_bwd_workspace_bytes) X(siq_stats_bwd)               \
-  X(siq_distill_workspace_bytes) X(siq_distill) X(siq_scale_bf16)
+  X(siq_stats_saved_bytes) X(siq_stats_fwd_workspace_bytes) X(siq_stats_fwd) X(siq_stats_bwd_workspace_bytes)       \
+  X(siq_stats_bwd) X(siq_distill_workspace_bytes) X(siq_distill) X(siq_scale_bf16)
 
 struct Api {
 #define SIQ_MEMBER(name) decltype(&::name) name = nullptr;
@@ -559,11 +559,11 @@ std::pair<Tensor, Tensor> raw_flp_bwd(const Tensor& hidden, const Tensor& weight
 // ---------------------------------------------------------------- token statistics
 // What a call returns, and what its backward takes besides: by row of the labels' shape.
 struct Stats {
-  Tensor logp, entropy, lse, top_logp, top_ids;
+  Tensor logp, entropy, lse, top_logp, top_ids, saved;
 };
 
 Stats stats_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels, int64_t ignore_index, double temperature,
-                int64_t top_k, at::IntArrayRef shape, int64_t* counts) {
+                int64_t top_k, bool keep, at::IntArrayRef shape, int64_t* counts) {
   check_head(hidden, weight, labels);
   // (as int for the library)
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= (1 << 20), "top_k must not be negative, or that large: ", top_k);
@@ -572,24 +572,29 @@ Stats stats_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels
   const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0);
   std::vector<int64_t> top = shape.vec();
   top.push_back(top_k);
-  Stats s{floats(shape, h), floats(shape, h), floats({n}, h), Tensor(), Tensor()};
+  Stats s{floats(shape, h), floats(shape, h), floats({n}, h), Tensor(), Tensor(), Tensor()};
   if (top_k > 0) {
     s.top_logp = floats(top, h);
     s.top_ids = at::empty(top, h.options().dtype(at::kLong));
   }
-  const Tensor ws = bytes(api.siq_stats_fwd_workspace_bytes(n, hdim, vocab, (int)top_k), h);
+  if (keep) s.saved = bytes(api.siq_stats_saved_bytes(n, vocab), h);
+  const Tensor ws = bytes(api.siq_stats_fwd_workspace_bytes(n, hdim, vocab, (int)top_k, keep), h);
   check(api.siq_stats_fwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), n, hdim, vocab, ignore_index,
                           temperature, (int)top_k, fptr(s.logp), fptr(s.entropy), fptr(s.lse), fptr(s.top_logp),
-                          static_cast<int64_t*>(ptr(s.top_ids)), counts, counts + 1, ptr(ws), ws.numel(), stream_of(h)),
+                          static_cast<int64_t*>(ptr(s.top_ids)), counts, counts + 1, ptr(s.saved),
+                          keep ? s.saved.numel() : 0, ptr(ws), ws.numel(), stream_of(h)),
         "siq_stats_fwd");
   return s;
 }
 
 struct TokenStats : torch::autograd::Function<TokenStats> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
-                               int64_t ignore_index, double temperature, int64_t top_k, int64_t chunk, int64_t* counts) {
-    Stats s = stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, labels.sizes(), counts);
-    ctx->save_for_backward({hidden, weight, labels, s.logp, s.entropy, s.lse});
+                               int64_t ignore_index, double temperature, int64_t top_k, int64_t chunk, int64_t keep_bytes,
+                               int64_t* counts) {
+    const Tensor h = rows_2d(hidden);
+    const bool keep = weight.dim() == 2 && (int64_t)api.siq_stats_saved_bytes(h.size(0), weight.size(0)) <= keep_bytes;
+    Stats s = stats_fwd(h, weight, rows_1d(labels), ignore_index, temperature, top_k, keep, labels.sizes(), counts);
+    ctx->save_for_backward({hidden, weight, labels, s.logp, s.entropy, s.lse, s.saved});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["chunk"] = chunk;
@@ -604,7 +609,7 @@ struct TokenStats : torch::autograd::Function<TokenStats> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     no_second_derivative("fused_linear_token_stats");
-    variable_list out(8);
+    variable_list out(9);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     const variable_list s = ctx->get_saved_variables();
     const Tensor h = rows_2d(s[0]).contiguous(), w = s[1].contiguous(), y = rows_1d(s[2]).contiguous();
@@ -614,11 +619,13 @@ struct TokenStats : torch::autograd::Function<TokenStats> {
     const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0), chunk = ctx->saved_data["chunk"].toInt();
     const Tensor dh = ctx->needs_input_grad(0) ? at::empty(h.sizes(), h.options()) : Tensor();
     const Tensor dw = ctx->needs_input_grad(1) ? at::empty(w.sizes(), w.options()) : Tensor();
-    const Tensor ws = bytes(api.siq_stats_bwd_workspace_bytes(n, hdim, vocab, chunk, dw.defined()), h);
+    const Tensor& saved = s[6];
+    const bool have = saved.defined();
+    const Tensor ws = bytes(api.siq_stats_bwd_workspace_bytes(n, hdim, vocab, chunk, dw.defined(), have), h);
     check(api.siq_stats_bwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), fptr(s[3]), fptr(s[4]),
                             fptr(s[5]), fptr(g), fptr(e), n, hdim, vocab, ctx->saved_data["ignore"].toInt(),
-                            ctx->saved_data["temperature"].toDouble(), ptr(dh), ptr(dw), chunk, ptr(ws), ws.numel(),
-                            stream_of(h)),
+                            ctx->saved_data["temperature"].toDouble(), ptr(saved), have ? saved.numel() : 0, ptr(dh), ptr(dw),
+                            chunk, ptr(ws), ws.numel(), stream_of(h)),
           "siq_stats_bwd");
     if (dh.defined()) out[0] = dh.view(s[0].sizes());
     out[1] = dw;
@@ -634,17 +641,20 @@ Tensor counts_of(const optional<Tensor>& host, int64_t n, const Tensor& like) {
 std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>, Tensor> token_stats(const Tensor& hidden, const Tensor& weight,
                                                                                    const Tensor& labels, int64_t ignore_index,
                                                                                    double temperature, int64_t top_k,
-                                                                                   int64_t chunk, const optional<Tensor>& host) {
+                                                                                   int64_t chunk, int64_t keep_bytes,
+                                                                                   const optional<Tensor>& host) {
   TORCH_CHECK_VALUE(chunk > 0, "chunk_tokens must be positive");
   no_tangent("fused_linear_token_stats", {hidden, weight});
   const Tensor counts = counts_of(host, 2, hidden);
   int64_t* const c = counts.data_ptr<int64_t>();
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
-    const variable_list o = TokenStats::apply(hidden, weight, labels, ignore_index, temperature, top_k, chunk, c);
+    const variable_list o =
+        TokenStats::apply(hidden, weight, labels, ignore_index, temperature, top_k, chunk, keep_bytes, c);
     if (top_k == 0) return {o[0], o[1], std::nullopt, std::nullopt, counts};
     return {o[0], o[1], o[2], o[3], counts};
   }
-  const Stats s = stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, labels.sizes(), c);
+  const Stats s =
+      stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, false, labels.sizes(), c);
   if (top_k == 0) return {s.logp, s.entropy, std::nullopt, std::nullopt, counts};
   return {s.logp, s.entropy, s.top_logp, s.top_ids, counts};
 }
