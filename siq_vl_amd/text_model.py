@@ -14,7 +14,14 @@ of ``Qwen2ForCausalLM.forward`` (transformers models/qwen2/modeling_qwen2.py:
 * with ``labels`` and ``return_log_probs=True`` (preference and policy training,
   ``siq_vl_amd.policy``): instead of a loss, the log-probabilities of the shifted
   labels (``fused_linear_log_probs``, at ``temperature``) in the output's
-  ``log_probs``, [batch, seqlen], 0 where the shifted label is ignored;
+  ``log_probs``, [batch, seqlen], 0 where the shifted label is ignored; with
+  ``top_k`` besides (0: none of the last two) the distributions' ``entropy`` and
+  most probable tokens, ``top_ids`` and ``top_log_probs`` [batch, seqlen, top_k]
+  (``fused_linear_token_stats``): what a teacher hands to a student;
+* with ``labels`` and ``teacher=(top_ids, top_log_probs)``, those of a teacher's call
+  on the same batch: ``loss`` is ``fused_linear_distillation``'s, with the options
+  in ``distillation`` (a dict: ``ce_weight``, ``divergence``, ``tail``), its parts
+  ``divergence`` and ``cross_entropy`` beside it;
 * without ``labels`` (``generate``): the original logits path;
 * with ``labels`` but no gradient (evaluation under ``torch.no_grad``): the
   loss-only kernel, no logits and no gradient work.
@@ -33,7 +40,8 @@ from typing import Any
 import torch
 
 from .cross_entropy import IGNORE_INDEX, fused_linear_cross_entropy, shift_labels
-from .log_probs import fused_linear_log_probs
+from .distillation import fused_linear_distillation
+from .log_probs import fused_linear_log_probs, fused_linear_token_stats
 
 
 @functools.cache
@@ -43,17 +51,40 @@ def _output_with_log_probs():
     @dataclass
     class CausalLMOutputWithLogProbs(CausalLMOutputWithPast):
         log_probs: torch.Tensor | None = None
+        entropy: torch.Tensor | None = None
+        top_log_probs: torch.Tensor | None = None
+        top_ids: torch.Tensor | None = None
 
     return CausalLMOutputWithLogProbs
 
 
+@functools.cache
+def _output_with_distillation():
+    from transformers.modeling_outputs import CausalLMOutputWithPast
+
+    @dataclass
+    class CausalLMOutputWithDistillation(CausalLMOutputWithPast):
+        divergence: torch.Tensor | None = None
+        cross_entropy: torch.Tensor | None = None
+
+    return CausalLMOutputWithDistillation
+
+
 def fused_causal_lm_forward(self, input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
                             inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0,
-                            return_log_probs: bool = False, temperature: float = 1.0, **kwargs: Any):
+                            return_log_probs: bool = False, temperature: float = 1.0, top_k: int | None = None,
+                            teacher: tuple[torch.Tensor, torch.Tensor] | None = None,
+                            distillation: dict[str, Any] | None = None, **kwargs: Any):
     from transformers.modeling_outputs import CausalLMOutputWithPast
 
     if return_log_probs and labels is None and kwargs.get("shift_labels") is None:
         raise ValueError("return_log_probs needs labels: they say which tokens' log-probabilities are wanted")
+    if top_k is not None and not return_log_probs:
+        raise ValueError("top_k goes with return_log_probs")
+    if teacher is not None and return_log_probs:
+        raise ValueError("a call gives log-probabilities or a teacher's loss, not both")
+    if teacher is not None and labels is None and kwargs.get("shift_labels") is None:
+        raise ValueError("a teacher needs labels: they say which positions count")
     outputs = self.model(
         input_ids=input_ids,
         attention_mask=attention_mask,
@@ -73,22 +104,33 @@ def fused_causal_lm_forward(self, input_ids=None, attention_mask=None, position_
     targets = kwargs.get("shift_labels")
     if targets is None:
         targets = shift_labels(labels, IGNORE_INDEX)
+    chunk_tokens = getattr(self, "siq_ce_chunk_tokens", None)
+    targets = targets.to(hidden.device)
+    common = dict(logits=None, past_key_values=outputs.past_key_values, hidden_states=outputs.hidden_states,
+                  attentions=outputs.attentions)
+    if teacher is not None:
+        loss = fused_linear_distillation(hidden, self.lm_head.weight, targets, *(t.to(hidden.device) for t in teacher),
+                                         temperature=temperature, num_items_in_batch=kwargs.get("num_items_in_batch"),
+                                         chunk_tokens=chunk_tokens, **(distillation or {}))
+        return _output_with_distillation()(loss=loss.loss, divergence=loss.divergence, cross_entropy=loss.cross_entropy,
+                                           **common)
+    if return_log_probs and top_k is not None:
+        stats = fused_linear_token_stats(hidden, self.lm_head.weight, targets, top_k, temperature=temperature,
+                                         chunk_tokens=chunk_tokens)
+        return _output_with_log_probs()(loss=None, **stats._asdict(), **common)
     if return_log_probs:
-        logps = fused_linear_log_probs(hidden, self.lm_head.weight, targets.to(hidden.device), IGNORE_INDEX, temperature,
-                                       chunk_tokens=getattr(self, "siq_ce_chunk_tokens", None))
-        return _output_with_log_probs()(loss=None, logits=None, past_key_values=outputs.past_key_values,
-                                        hidden_states=outputs.hidden_states, attentions=outputs.attentions,
-                                        log_probs=logps)
+        logps = fused_linear_log_probs(hidden, self.lm_head.weight, targets, IGNORE_INDEX, temperature,
+                                       chunk_tokens=chunk_tokens)
+        return _output_with_log_probs()(loss=None, log_probs=logps, **common)
     loss = fused_linear_cross_entropy(
         hidden.reshape(-1, hidden.shape[-1]),
         self.lm_head.weight,
-        targets.reshape(-1).to(hidden.device),
+        targets.reshape(-1),
         ignore_index=IGNORE_INDEX,
         num_items_in_batch=kwargs.get("num_items_in_batch"),
-        chunk_tokens=getattr(self, "siq_ce_chunk_tokens", None),
+        chunk_tokens=chunk_tokens,
     )
-    return CausalLMOutputWithPast(loss=loss, logits=None, past_key_values=outputs.past_key_values,
-                                  hidden_states=outputs.hidden_states, attentions=outputs.attentions)
+    return CausalLMOutputWithPast(loss=loss, **common)
 
 
 def enable_fused_cross_entropy(model: torch.nn.Module, chunk_tokens: int | None = None) -> torch.nn.Module:
