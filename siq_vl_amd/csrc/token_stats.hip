@@ -16,7 +16,9 @@
 //     the logsumexp and the entropy are merged from, without any reference that
 //     a row could exceed.  The given token is kept out of them, so that what is
 //     next to certain keeps its digits, and added in the row pass.  With
-//     alternatives wanted it also writes z itself in fp32 and the part's largest z.
+//     alternatives wanted it also writes z itself in fp32 and the part's largest z:
+//     first for an eighth of the columns, whose K-th largest part bounds what can be
+//     among the K largest of all, then for the parts of the others that reach that.
 //  2. row pass, a workgroup a row: merges in 64 bits; logp, H, lse.  The K-th
 //     largest of the maxima of 256 groups of parts is a bound that the K largest z
 //     do not lie below, so of z only the parts that reach it are read.
@@ -47,9 +49,10 @@ struct StatLogitsArgs {
   bf16* E;                // [nc, V] 2^(z2 - m), 0 for the given token, or nullptr
   f32x4* part;            // [nc, parts] {m, sum, sum of products, largest z (before the temperature)}
   float* zy;              // [nc] z of the given token
+  const float* bound;     // [nc] parts whose largest z is below are not written to Z, or nullptr
   const int64_t* nvalid;
   int64_t V, nc, c0, parts;
-  int nI, nJ;
+  int nI, nJ, t0;         // tiles of columns of this launch, and the first one
   float zscale;           // log2(e) / temperature
 };
 
@@ -88,10 +91,13 @@ __device__ __forceinline__ f32x4 stat_part(float zscale, float m, Get z, Keep ke
   return f32x4{m, half_sum(s), half_sum(t), 0.f};
 }
 
+// TOP: Z is written; KEEP: E is.
+template <bool TOP, bool KEEP>
 __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
   int ti, tj;
   if (!tile_of(p.nI, p.nJ, 4, ti, tj)) return;
+  ti += p.t0;
   const int64_t i0 = (int64_t)ti * BI, j0 = (int64_t)tj * BJ;
   if (j0 >= *p.nvalid - p.c0) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
@@ -119,7 +125,10 @@ __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p
   for (int b = 0; b < 2; ++b) {
     const int64_t tok = j0 + wave_col(b, wj) + l32;
     const bool tv = tok < p.nc;
-    if (p.Z != nullptr && tv) {
+    auto get = [&](int a, int r) { return acc[a][b][r]; };
+    const float top = stat_max<4>(get);
+    float largest = top;
+    if (TOP && tv && (p.bound == nullptr || top >= p.bound[tok])) {
 #pragma unroll
       for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -137,9 +146,6 @@ __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p
           *reinterpret_cast<f32x4*>(z + 4) = hi;
         }
     }
-    auto get = [&](int a, int r) { return acc[a][b][r]; };
-    const float top = stat_max<4>(get);
-    float largest = top;
     // the given token: in at most one lane of the workgroup, for one tile in ~600
     const bool hit = tv && rel[b] >= 0 && ((rel[b] >> 6) & 1) == wi && ((rel[b] >> 3) & 1) == 0;
     if (__any(hit)) {
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p
     }
     f32x4 st = stat_part<4>(p.zscale, largest * p.zscale, get, [&](int a, int j, const bf16x8& e) {
       const int64_t v0 = vbase + wave_row(a, wi) + 16 * j;
-      if (p.E != nullptr && tv && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e);
+      if (KEEP && tv && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e);
     });
     st[3] = top;
     if (tv && h == 0) p.part[tok * p.parts + 2 * ti + wi] = st;
@@ -206,7 +212,7 @@ constexpr int kFewStages = NB <= 2 ? 3 : 2;  // (64 rows: three buffers; 128: tw
 template <int NB>
 constexpr int kFewSmem = kFewStages<NB> * (kFewBI + 32 * NB) * BK;
 
-template <int NB>
+template <int NB, bool TOP, bool KEEP>
 __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const StatLogitsArgs p) {
   constexpr int TOK = 32 * NB, NWV = kFewThreads / 64;
   __shared__ __align__(16) bf16 smem[kFewSmem<NB>];
@@ -236,7 +242,7 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
     const bool tv = tok < p.nc;
-    if (p.Z != nullptr && tv) {
+    if (TOP && tv) {
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
         const int64_t v0 = vbase + 16 * jj;
@@ -282,7 +288,7 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
     const f32x4 st = stat_part<1>(p.zscale, m * p.zscale, [&](int, int r) { return acc[b][r]; },
                                   [&](int, int j, const bf16x8& e) {
                                     const int64_t v0 = vbase + 16 * j;
-                                    if (p.E != nullptr && tok < p.nc && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e);
+                                    if (KEEP && tok < p.nc && v0 < p.V) st_bf16x8(p.E + tok * p.V + v0, e);
                                   });
     if (h == 0) red[w * TOK + tok] = st;
   }
@@ -304,7 +310,8 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
 struct StatRowArgs {
   const f32x4* part;      // [nc, parts]
   const float* zy;        // [nc]
-  const float* Z;         // [nc, V]
+  const float* Z;         // [nc, V], where a part's largest reaches the bound
+  const float* bound;     // [nc] or nullptr
   const int32_t* rows;    // [nc] compacted row -> row
   const int64_t* nvalid;
   const int64_t* labels;  // [n]
@@ -334,9 +341,47 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
+constexpr int kCus = 256;
 constexpr int kRowGroups = 256;               // threads of a workgroup, and groups of parts
 constexpr int kMostParts = 1024, kMostListed = 1024;
 static_assert(kMaxTopK <= kRowGroups, "a bound is the K-th largest group's");
+
+// The K-th largest of the keys of 256 groups (behind a barrier), bit by bit, by one wave.
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* best_sh, int K, int lane) {
+  constexpr int N = kRowGroups / 64;
+  uint32_t b[N], tau = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) b[i] = best_sh[64 * i + lane];
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cand = tau | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) c += __popcll(__ballot(b[i] >= cand));
+    if (c >= K) tau = cand;
+  }
+  return tau;
+}
+
+// The bound that the first `parts` parts of a row give.
+struct BoundArgs {
+  const f32x4* part;      // [nc, ld]
+  float* bound;           // [nc]
+  const int64_t* nvalid;
+  int64_t c0, ld;
+  int parts, K;
+};
+__global__ __launch_bounds__(kRowGroups) void stats_bound_kernel(const BoundArgs p) {
+  __shared__ uint32_t best_sh[kRowGroups];
+  const int64_t k = blockIdx.x;
+  if (p.c0 + k >= *p.nvalid) return;
+  uint32_t best = 0;
+  for (int i = threadIdx.x; i < p.parts; i += kRowGroups) best = max(best, order_of(p.part[k * p.ld + i][3]));
+  best_sh[threadIdx.x] = best;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const uint32_t tau = kth_largest(best_sh, p.K, threadIdx.x);
+  if (threadIdx.x == 0) p.bound[k] = tau == 0 ? -INFINITY : number_of(tau);
+}
 
 // One workgroup a row.  Columns that reach the bound are listed, usually K or
 // somewhat more, and each one's rank is how many of the others come before it.
@@ -345,8 +390,8 @@ static_assert(kMaxTopK <= kRowGroups, "a bound is the K-th largest group's");
 __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs p) {
   constexpr int T = kRowGroups, NWV = T / 64;
   __shared__ float m_sh[NWV];
-  __shared__ double s_sh[NWV], t_sh[NWV];
-  __shared__ uint32_t best_sh[T];
+  __shared__ double s_sh[NWV], t_sh[NWV], lse_sh;
+  __shared__ uint32_t best_sh[T], tau_sh;
   __shared__ int part_sh[kMostParts], nparts_sh, n_sh;
   __shared__ uint64_t listed_sh[kMostListed], top_sh[NWV];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -391,43 +436,36 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     s_sh[w] = s;
     t_sh[w] = t;
   }
-  // the bound, by each wave for itself: the K-th largest of the groups', bit by bit
-  uint32_t tau = 0;
-  if (p.K > 0) {
-    uint32_t b[NWV];
-#pragma unroll
-    for (int i = 0; i < NWV; ++i) b[i] = best_sh[64 * i + lane];
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t cand = tau | (1u << bit);
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < NWV; ++i) c += __popcll(__ballot(b[i] >= cand));
-      if (c >= p.K) tau = cand;
-    }
+  // the bound (parts below an earlier one were not written)
+  if (w == 0 && p.K > 0) {
+    const uint32_t own_bound = kth_largest(best_sh, p.K, lane);
+    if (tid == 0) tau_sh = p.bound != nullptr ? max(own_bound, order_of(p.bound[k])) : own_bound;
   }
   __syncthreads();
-  s = t = 0.;
-#pragma unroll
-  for (int i = 0; i < NWV; ++i) {
-    s += s_sh[i];
-    t += t_sh[i];
-  }
-  // the given token: all relative to m
   constexpr double kLn2d = 0.6931471805599453;
-  const double d = dy - (double)m, ey = exp2(d), all = s + ey, l2 = log2(all), lse = (double)m + l2;
   const int64_t row = p.rows[k];
-  if (tid == 0) {
+  if (tid == T - 1) {  // (in a wave that has no bound to find)
+    s = t = 0.;
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) {
+      s += s_sh[i];
+      t += t_sh[i];
+    }
+    // the given token: all relative to m
+    const double d = dy - (double)m, ey = exp2(d), all = s + ey, l2 = log2(all), lse = (double)m + l2;
     const double over = s * exp2(-d), ent = kLn2d * (l2 - (t + (ey > 0. ? ey * d : 0.)) / all);
+    lse_sh = lse;
     // p_y = 1 / (1 + over): its logarithm keeps its digits where `over` is small
     p.logp[row] = (float)(over <= 1e300 ? -log1p(over) : kLn2d * (d - l2));
     p.entropy[row] = ent < 0. ? 0.f : (float)ent;
     p.lse[row] = (float)lse;
   }
   if (p.K == 0) return;
+  const uint32_t tau = tau_sh;
   const float* z = p.Z + k * p.V;
   auto result = [&](int rank, uint64_t key) {
     const float zi = number_of((uint32_t)(key >> 32));
-    p.top_logp[row * p.K + rank] = (float)(((double)zi * (double)p.zscale - lse) * kLn2d);
+    p.top_logp[row * p.K + rank] = (float)(((double)zi * (double)p.zscale - lse_sh) * kLn2d);
     p.top_ids[row * p.K + rank] = (int64_t)(uint32_t)~(uint32_t)key;
   };
   for (int i = tid; i < p.parts; i += T)
@@ -437,15 +475,18 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     }
   __syncthreads();
   const int np = nparts_sh, c = tid & 127, off = p.few ? c : (c & 63) + 128 * (c >> 6);
+  auto column = [&](int part) {
+    return (p.few ? 128 * (int64_t)part : 256 * (int64_t)(part >> 1) + 64 * (part & 1)) + off;
+  };
   if (np <= kMostParts) {
-    constexpr int U = 4, STEP = T / 128;
+    constexpr int U = 8, STEP = T / 128;
     for (int q0 = tid / 128; q0 < np; q0 += STEP * U) {
       float x[U];
       int64_t v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int q = q0 + STEP * u, part = part_sh[min(q, np - 1)];
-        v[u] = (p.few ? 128 * (int64_t)part : 256 * (int64_t)(part >> 1) + 64 * (part & 1)) + off;
+        v[u] = column(part);
         if (q >= np || v[u] >= p.V) v[u] = -1;
         x[u] = v[u] >= 0 ? z[v[u]] : 0.f;
       }
@@ -471,7 +512,9 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
   uint64_t last = ~0ull;
   for (int r = 0; r < p.K; ++r) {
     uint64_t top = 0;
-    for (int64_t v = tid; v < p.V; v += T) {
+    for (int i = tid / 128; i < p.parts; i += T / 128) {
+      const int64_t v = column(i);
+      if (v >= p.V || order_of(src[i][3]) < tau) continue;
       const uint64_t key = order_of(z[v], v);
       if (key < last && key > top) top = key;
     }
@@ -666,7 +709,7 @@ StatsSaved saved_layout(int64_t n, int64_t V) {
 }
 
 struct FwdLayout {
-  size_t scal, rows, yc, ref, hc, zy, part, Z, total;
+  size_t scal, rows, yc, ref, hc, zy, part, bound, Z, total;
   int64_t chunk, parts;
   bool few;
 };
@@ -688,6 +731,7 @@ FwdLayout fwd_layout(int64_t n, int64_t hdim, int64_t V, int top_k, bool keep) {
   L.hc = take(true, sizeof(bf16) * npad * (size_t)hdim);
   L.zy = take(true, sizeof(float) * (size_t)L.chunk);
   L.part = take(!keep, sizeof(f32x4) * (size_t)(L.chunk * L.parts));
+  L.bound = take(top_k > 0, sizeof(float) * (size_t)L.chunk);
   L.Z = take(top_k > 0, sizeof(float) * (size_t)(L.chunk * V));
   L.total = off;
   return L;
@@ -737,6 +781,39 @@ BwdLayout bwd_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool nee
   L.lsum = take(need_dw, sizeof(float) * (size_t)(L.chunk * hdim));
   L.total = off;
   return L;
+}
+
+// Tiles whose parts bound the others': at least K of them, so that the K-th largest of
+// their 2 K parts says something, and three rounds of workgroups, so that the last round
+// of a launch of its own costs little; 0: all in one launch.
+int bound_tiles(int nI, int nJ, int K) {
+  const int tiles = std::max({nI / 8, K, (3 * kCus + nJ - 1) / nJ});
+  return 3 * tiles <= nI ? tiles : 0;
+}
+
+template <bool TOP, bool KEEP>
+void launch_stat_logits(StatLogitsArgs lg, bool few, int K, float* bound, hipStream_t stream) {
+  if (few) {
+    const dim3 grid((unsigned)((lg.V + kFewBI - 1) / kFewBI));
+    hipLaunchKernelGGL((lg.nc <= 64 ? stats_logits_few_kernel<2, TOP, KEEP> : stats_logits_few_kernel<4, TOP, KEEP>), grid,
+                       dim3(kFewThreads), 0, stream, lg);
+    return;
+  }
+  const int nI = (int)((lg.V + kVT - 1) / kVT), first = bound != nullptr ? bound_tiles(nI, (int)((lg.nc + BJ - 1) / BJ), K) : 0;
+  lg.nJ = (int)((lg.nc + BJ - 1) / BJ);
+  lg.nI = first > 0 ? first : nI;
+  auto launch = [&]() {
+    const int grid = ((lg.nI * lg.nJ + kXcds - 1) / kXcds) * kXcds;
+    hipLaunchKernelGGL((stats_logits_kernel<TOP, KEEP>), dim3(grid), dim3(NT), 0, stream, lg);
+  };
+  launch();
+  if (first == 0) return;
+  const BoundArgs bd{lg.part, bound, lg.nvalid, lg.c0, lg.parts, 2 * first, K};
+  hipLaunchKernelGGL(stats_bound_kernel, dim3((unsigned)lg.nc), dim3(kRowGroups), 0, stream, bd);
+  lg.t0 = first;
+  lg.nI = nI - first;
+  lg.bound = bound;
+  launch();
 }
 
 float zscale_of(const StatsArgs& a) { return (float)(1.4426950408889634 / a.temperature); }
@@ -796,20 +873,19 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
     lg.c0 = c0;
     lg.parts = L.parts;
     lg.zscale = c.zscale;
-    if (L.few) {
-      const dim3 grid((unsigned)((a.vocab + kFewBI - 1) / kFewBI));
-      hipLaunchKernelGGL((nc <= 64 ? stats_logits_few_kernel<2> : stats_logits_few_kernel<4>), grid, dim3(kFewThreads), 0,
-                         stream, lg);
-    } else {
-      lg.nI = (int)((a.vocab + kVT - 1) / kVT);
-      lg.nJ = (int)((nc + BJ - 1) / BJ);
-      const int grid = ((lg.nI * lg.nJ + kXcds - 1) / kXcds) * kXcds;
-      hipLaunchKernelGGL(stats_logits_kernel, dim3(grid), dim3(NT), 0, stream, lg);
-    }
+    const int nI = (int)((a.vocab + kVT - 1) / kVT), nJ = (int)((nc + BJ - 1) / BJ);
+    float* bound = !L.few && a.top_k > 0 && bound_tiles(nI, nJ, a.top_k) > 0 ? at<float>(a.ws, L.bound) : nullptr;
+    if (a.top_k > 0)
+      keep ? launch_stat_logits<true, true>(lg, L.few, a.top_k, bound, stream)
+           : launch_stat_logits<true, false>(lg, L.few, a.top_k, bound, stream);
+    else
+      keep ? launch_stat_logits<false, true>(lg, L.few, 0, nullptr, stream)
+           : launch_stat_logits<false, false>(lg, L.few, 0, nullptr, stream);
     StatRowArgs rw{};
     rw.part = lg.part;
     rw.zy = lg.zy;
     rw.Z = lg.Z;
+    rw.bound = bound;
     rw.rows = rows + c0;
     rw.nvalid = nvalid;
     rw.labels = a.labels;
