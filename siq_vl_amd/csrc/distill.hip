@@ -61,141 +61,90 @@ struct ListArgs {
   int K, ldk;
 };
 
-// A wave a row.  Keys are (tile, place in it) * 256 + (place among the teacher's
-// tokens; 255: the label, behind a teacher's same token), unique, and their ranks
-// are counted.  Tokens of probability zero and ids of -1 are not there; of equal ids
-// the first stays.  Then a lane a tile writes its bits.
+// A workgroup a row, a thread a token: its key is (tile, place in it) * 256 + (place
+// among the teacher's tokens; 255: the label, behind a teacher's same token), and its
+// place in the list how many other kept keys are less.  Tokens of probability zero and
+// ids of -1 are not there; of equal ids the first stays.  The bits are set in LDS,
+// kListSpan columns at a time.
+constexpr int kListThreads = 256, kListSpan = 1 << 17;
+static_assert(kMaxTeacher + 1 <= kListThreads, "a thread a token");
+// How many of the first n keys (in fours; the last ones none) are less than x.
+__device__ __forceinline__ int less_than(const uint32_t* keys, int n, uint32_t x) {
+  int c = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; j += 4) {
+    const u32x4 k = *reinterpret_cast<const u32x4*>(keys + j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c += k[i] < x ? 1 : 0;
+  }
+  return c;
+}
+
 template <class ID, bool FEW>
-__global__ __launch_bounds__(256) void distill_list_kernel(const ListArgs p) {
-  constexpr int VT = FEW ? kFewBI : kVT, LANE = list_lane_bits(FEW), NL = VT / LANE;
+__global__ __launch_bounds__(kListThreads) void distill_list_kernel(const ListArgs p) {
+  constexpr int VT = FEW ? kFewBI : kVT, LANE = list_lane_bits(FEW), NL = VT / LANE, T = kListThreads;
   constexpr uint32_t kNone = ~0u;
-  __shared__ uint32_t key_sh[4][kListMost], sorted_sh[4][kListMost];
-  __shared__ float lt_sh[4][kListMost];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t k = (int64_t)blockIdx.x * 4 + w, nv = min(p.nc, *p.nvalid - p.c0);
-  const bool real = k < nv;
-  uint32_t mine[kListLanes];
-  int id[kListLanes], nbad = 0;
-  float lt[kListLanes];
-  if (real) {
-    const int64_t src = (int64_t)p.rows[k] * p.K;
+  __shared__ __align__(16) uint32_t key_sh[kMaxTeacher + 4];
+  __shared__ __align__(16) uint32_t kept_sh[T];  // of each token, by its place among the teacher's: its key, or none
+  __shared__ __align__(16) uint32_t bits_sh[kListSpan / 32];
+  const int tid = threadIdx.x, K = p.K;
+  const int64_t k = blockIdx.x;
+  const bool real = k < min(p.nc, *p.nvalid - p.c0);
+  uint32_t mine = kNone;
+  int id = -1;
+  float lt = -INFINITY;
+  bool wrong = false;
+  if (real && tid < K) {
+    const int64_t src = (int64_t)p.rows[k] * K + tid, v = static_cast<const ID*>(p.ids)[src];
+    lt = p.teacher[src];
+    wrong = v != -1 && (v < 0 || v >= p.V);
+    id = wrong || lt == -INFINITY ? -1 : (int)v;
+  } else if (real && tid == K) {
+    id = (int)p.y[k];
+  }
+  if (id >= 0) mine = (uint32_t)(id / VT * VT + list_place(id % VT, FEW)) << 8 | (tid < K ? (uint32_t)tid : 255u);
+  if (tid < kMaxTeacher + 4) key_sh[tid] = mine;
+  __syncthreads();
+  // a token is kept unless the same one has a lower key: no key lies between (tile, place) * 256 and its own
+  const bool kept = mine != kNone && less_than(key_sh, K + 1, mine) == less_than(key_sh, K + 1, mine & ~255u);
+  const bool twice = mine != kNone && !kept && tid < K;
+  kept_sh[tid] = kept ? mine : kNone;
+  const int n = __syncthreads_count(kept), bad = __syncthreads_count(wrong || twice);
+  if (kept) {
+    const int at = less_than(kept_sh, K + 1, mine);
+    p.out[k * p.ldk + at] = id | (tid == K ? kLabelOnly : 0);
+    p.lt[k * p.ldk + at] = lt;
+  }
+  if (real && tid == 0) {
+    p.len[k] = n;
+    p.bad[k] = bad;
+  }
+  const uint32_t bit = mine >> 8;  // (none: past every column)
+  for (int64_t s0 = 0; s0 < p.nvt * VT; s0 += kListSpan) {
+    const int words = (int)(min((int64_t)kListSpan, p.nvt * VT - s0) / 32);
+    for (int i = tid; i < words / 4; i += T) reinterpret_cast<u32x4*>(bits_sh)[i] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+    if (kept && bit >= s0 && bit < s0 + kListSpan) atomicOr(&bits_sh[(bit - s0) / 32], 1u << (bit & 31));
+    __syncthreads();
+    u32x4* mask = reinterpret_cast<u32x4*>(p.mask + k * p.ldm + s0 / 8);
+    for (int i = tid; i < words / 4; i += T) mask[i] = reinterpret_cast<const u32x4*>(bits_sh)[i];
+    for (int t = tid; t < words / (VT / 32); t += T) {
+      uint64_t base = 0;  // a byte for each lane's bits
+      const uint32_t t0 = (uint32_t)(s0 + t * VT) << 8;
+      int before = n > 0 ? less_than(kept_sh, K + 1, t0) : 0;
 #pragma unroll
-    for (int i = 0; i < kListLanes; ++i) {
-      const int e = lane + 64 * i;
-      mine[i] = kNone;
-      lt[i] = -INFINITY;
-      int64_t v = -1;
-      bool wrong = false;
-      if (e < p.K) {
-        v = static_cast<const ID*>(p.ids)[src + e];
-        lt[i] = p.teacher[src + e];
-        wrong = v != -1 && (v < 0 || v >= p.V);
-        if (wrong || lt[i] == -INFINITY) v = -1;
-      } else if (e == p.K) {
-        v = p.y[k];
+      for (int q = 0; q < NL; ++q) {
+        base |= (uint64_t)before << (8 * q);
+        const uint32_t* w = bits_sh + (t * VT + q * LANE) / 32;
+        before += LANE == 64 ? __popc(w[0]) + __popc(w[1]) : __popc(w[0] >> (q % 2 * 16) & 0xffffu);
       }
-      id[i] = (int)v;
-      if (v >= 0) mine[i] = (uint32_t)(id[i] / VT * VT + list_place(id[i] % VT, FEW)) << 8 | (e < p.K ? (uint32_t)e : 255u);
-      nbad += __popcll(__ballot(wrong));
-      key_sh[w][e] = mine[i];
-    }
-  }
-  __syncthreads();
-  int rank[kListLanes] = {};
-  if (real) {
-    for (int j = 0; j <= p.K; ++j) {
-      const uint32_t x = key_sh[w][j];
-#pragma unroll
-      for (int i = 0; i < kListLanes; ++i) rank[i] += x < mine[i] ? 1 : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < kListLanes; ++i)
-      if (mine[i] != kNone) sorted_sh[w][rank[i]] = mine[i];
-  }
-  __syncthreads();
-  // those that repeat the one before them are left out: the others' ranks among themselves
-  int n = 0;
-  uint32_t kept[kListLanes];
-  if (real) {
-    int all = 0;
-#pragma unroll
-    for (int i = 0; i < kListLanes; ++i) all += __popcll(__ballot(mine[i] != kNone));
-#pragma unroll
-    for (int i = 0; i < kListLanes; ++i) {
-      const int e = lane + 64 * i;
-      const uint32_t x = e < all ? sorted_sh[w][e] : kNone;
-      const bool same = e < all && e > 0 && sorted_sh[w][e - 1] >> 8 == x >> 8;
-      nbad += __popcll(__ballot(same && (x & 255u) != 255u));
-      const uint64_t m = __ballot(e < all && !same);
-      kept[i] = m >> lane & 1 ? x : kNone;
-      key_sh[w][e] = (uint32_t)(n + __popcll(m & (lane ? ~0ull >> (64 - lane) : 0ull)));  // where rank e goes
-      n += __popcll(m);
-    }
-  }
-  __syncthreads();
-  uint32_t* list = sorted_sh[w];
-  if (real) {
-    bool stays[kListLanes];
-    int at[kListLanes];
-#pragma unroll
-    for (int i = 0; i < kListLanes; ++i) {
-      at[i] = mine[i] != kNone ? (int)key_sh[w][rank[i]] : 0;
-      stays[i] = mine[i] != kNone && (rank[i] == 0 || list[rank[i] - 1] >> 8 != mine[i] >> 8);
-    }
-#pragma unroll
-    for (int i = 0; i < kListLanes; ++i)
-      if (stays[i]) {
-        p.out[k * p.ldk + at[i]] = id[i] | ((mine[i] & 255u) == 255u ? kLabelOnly : 0);
-        p.lt[k * p.ldk + at[i]] = lt[i];
-      }
-    if (lane == 0) {
-      p.len[k] = n;
-      p.bad[k] = nbad;
-    }
-  }
-  __syncthreads();
-  if (real) {
-#pragma unroll
-    for (int i = 0; i < kListLanes; ++i)
-      if (kept[i] != kNone) list[key_sh[w][lane + 64 * i]] = kept[i] >> 8;
-  }
-  __syncthreads();
-  if (k >= p.nc) return;
-  // (rows that fill up a tile have no entries)
-  for (int64_t t = lane; t < p.nvt; t += 64) {
-    const uint32_t t0 = (uint32_t)(t * VT);
-    int lo = 0, hi = n;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (list[mid] < t0)
-        lo = mid + 1;
+      const int64_t at = s0 / VT + t;
+      if (NL == 8)
+        *reinterpret_cast<uint64_t*>(p.base + k * p.ldb + 8 * at) = base;
       else
-        hi = mid;
+        *reinterpret_cast<uint32_t*>(p.base + k * p.ldb + 4 * at) = (uint32_t)base;
     }
-    uint32_t bits[VT / 32] = {};
-    uint64_t base = 0;  // a byte for each lane's bits
-#pragma unroll
-    for (int q = 0; q < NL; ++q) {
-      base |= (uint64_t)lo << (8 * q);
-      const uint32_t end = t0 + LANE * (q + 1);
-      while (lo < n && list[lo] < end) {
-        const uint32_t b = list[lo++] - t0;
-        const uint32_t bit = 1u << (b & 31);
-        if (LANE == 64) {
-          bits[2 * q] |= b & 32 ? 0u : bit;
-          bits[2 * q + 1] |= b & 32 ? bit : 0u;
-        } else {
-          bits[q / 2] |= bit;
-        }
-      }
-    }
-    u32x4* dst = reinterpret_cast<u32x4*>(p.mask + k * p.ldm + t * (VT / 8));
-#pragma unroll
-    for (int q = 0; q < VT / 128; ++q) dst[q] = u32x4{bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]};
-    if (NL == 8)
-      *reinterpret_cast<uint64_t*>(p.base + k * p.ldb + 8 * t) = base;
-    else
-      *reinterpret_cast<uint32_t*>(p.base + k * p.ldb + 4 * t) = (uint32_t)base;
+    __syncthreads();
   }
 }
 
@@ -534,13 +483,13 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     ls.ldk = L.ldk;
     ls.ldm = L.ldm;
     ls.ldb = L.ldb;
-    const dim3 waves((unsigned)((nc + 3) / 4));
+    const dim3 each((unsigned)nc), waves((unsigned)((nc + 3) / 4));
     if (L.few)
-      hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, true> : distill_list_kernel<int64_t, true>), waves, dim3(256),
-                         0, stream, ls);
+      hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, true> : distill_list_kernel<int64_t, true>), each,
+                         dim3(kListThreads), 0, stream, ls);
     else
-      hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, false> : distill_list_kernel<int64_t, false>), waves,
-                         dim3(256), 0, stream, ls);
+      hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, false> : distill_list_kernel<int64_t, false>), each,
+                         dim3(kListThreads), 0, stream, ls);
 
     LogitsArgs lg{};
     lg.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
