@@ -45,6 +45,77 @@ constexpr int kListLanes = 3, kListMost = 64 * kListLanes;  // entries a lane; o
 static_assert(kMaxTeacher + 1 <= kListMost, "the label behind the teacher's tokens");
 
 // ---------------------------------------------------------------- lists
+// A call of at most kFewRows rows: the kernel of the lists compacts them, too, as
+// launch_compact does.
+struct FewPrep {
+  const int64_t* labels;  // [n]
+  const bf16* hidden;
+  const bf16* weight;
+  int32_t* rows;          // [n]
+  int64_t *y, *nvalid, *counts;  // [n]; ; [2]
+  bf16* hc;               // [n, hdim]
+  float* ref;             // [n]
+  bf16* dh;               // or nullptr
+  int64_t hdim, ignore_index;
+  int n;
+  float zscale;
+};
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// Workgroup k: the k-th counted row's operands, where there is one (its label, or -1),
+// and what belongs to row k where its label does not count.
+__device__ __forceinline__ int64_t few_compact(const FewPrep& p, int64_t V, int64_t& src) {
+  constexpr int G = kFewRows / 64;
+  __shared__ float dot_sh[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, k = blockIdx.x;
+  int nv = 0, nbad = 0, at = -1;
+  bool counts = false;  // row k
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int64_t v = 64 * g + lane < p.n ? p.labels[64 * g + lane] : p.ignore_index;
+    const bool ok = v >= 0 && v < V && v != p.ignore_index;
+    const uint64_t m = __ballot(ok);
+    nbad += __popcll(__ballot(v != p.ignore_index && !ok));
+    const int rank = nv + __popcll(m & (lane ? ~0ull >> (64 - lane) : 0ull));
+    const uint64_t mine = __ballot(ok && rank == k);
+    if (mine != 0) at = 64 * g + (int)__builtin_ctzll(mine);
+    counts = counts || (k / 64 == g && (m >> (k % 64) & 1));
+    nv += __popcll(m);
+  }
+  const int64_t y = at >= 0 ? p.labels[at] : -1;
+  float dot = 0.f;
+  for (int64_t c = 8 * (int64_t)tid; c < p.hdim; c += 8 * 256) {
+    bf16x8 x = zero_bf16x8();
+    if (at >= 0) {
+      x = ld_bf16x8(p.hidden + at * p.hdim + c);
+      const bf16x8 wy = ld_bf16x8(p.weight + y * p.hdim + c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = __builtin_fmaf((float)x[i], (float)wy[i], dot);
+    }
+    st_bf16x8(p.hc + k * p.hdim + c, x);
+    if (!counts && p.dh != nullptr) st_bf16x8(p.dh + k * p.hdim + c, zero_bf16x8());
+  }
+  dot = wave_sum(dot);
+  if (lane == 0) dot_sh[w] = dot;
+  __syncthreads();
+  if (tid == 0) {
+    p.ref[k] = (dot_sh[0] + dot_sh[1] + dot_sh[2] + dot_sh[3]) * p.zscale;
+    p.y[k] = y;
+    if (at >= 0) p.rows[k] = at;
+    if (k == 0) {
+      *p.nvalid = p.counts[0] = nv;
+      p.counts[1] = nbad;
+    }
+  }
+  src = at;
+  return y;
+}
+
 struct ListArgs {
   const void* ids;        // [n, K]
   const float* teacher;   // [n, K]
@@ -59,6 +130,7 @@ struct ListArgs {
   int32_t* bad;           // [nc] tokens outside the vocabulary, or named twice
   int64_t nc, c0, V, nvt, ldm, ldb;
   int K, ldk;
+  FewPrep few;            // few.labels != nullptr: a call of few rows, nothing above has been compacted yet
 };
 
 // A workgroup a row, a thread a token: its key is (tile, place in it) * 256 + (place
@@ -89,18 +161,25 @@ __global__ __launch_bounds__(kListThreads) void distill_list_kernel(const ListAr
   __shared__ __align__(16) uint32_t bits_sh[kListSpan / 32];
   const int tid = threadIdx.x, K = p.K;
   const int64_t k = blockIdx.x;
-  const bool real = k < min(p.nc, *p.nvalid - p.c0);
+  int64_t row = -1, y = -1;
+  if (FEW && p.few.labels != nullptr) {
+    y = few_compact(p.few, p.V, row);
+  } else if (k < min(p.nc, *p.nvalid - p.c0)) {
+    row = p.rows[k];
+    y = p.y[k];
+  }
+  const bool real = row >= 0;
   uint32_t mine = kNone;
   int id = -1;
   float lt = -INFINITY;
   bool wrong = false;
   if (real && tid < K) {
-    const int64_t src = (int64_t)p.rows[k] * K + tid, v = static_cast<const ID*>(p.ids)[src];
+    const int64_t src = row * K + tid, v = static_cast<const ID*>(p.ids)[src];
     lt = p.teacher[src];
     wrong = v != -1 && (v < 0 || v >= p.V);
     id = wrong || lt == -INFINITY ? -1 : (int)v;
   } else if (real && tid == K) {
-    id = (int)p.y[k];
+    id = (int)y;
   }
   if (id >= 0) mine = (uint32_t)(id / VT * VT + list_place(id % VT, FEW)) << 8 | (tid < K ? (uint32_t)tid : 255u);
   if (tid < kMaxTeacher + 4) key_sh[tid] = mine;
@@ -169,6 +248,11 @@ struct RowMathArgs {
   int ldk;
   bool reverse, tail;
   double c, inv_t;
+  // few rows: the sums over the tiles are made here, too
+  const float* spart;     // [nvt, ldp]
+  const float* mpart;
+  bf16* H;                // [nc, hdim] times f, or nullptr
+  int64_t nvt, ldp, hdim;
 };
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -182,15 +266,14 @@ __device__ __forceinline__ double wave_max(double x) {
   return x;
 }
 
-__global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
+// Row k by one wave, from its sum over the tokens that are not listed: losses, and with E
+// the row's factor (returned) and gradients of listed tokens.
+__device__ __forceinline__ float row_math(const RowMathArgs& p, int64_t k, int64_t counted, double rsum, double rtop) {
   constexpr double kLn2d = 0.6931471805599453;
   const int lane = threadIdx.x & 63;
-  const int64_t counted = *p.nvalid, nv = min(p.nc, counted - p.c0);
-  const int64_t k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (k >= nv) return;
   const int n = p.len[k];
   const int64_t y = p.y[k];
-  const double ref = p.ref[k], rtop = p.rtop[k], rsum = p.rsum[k];
+  const double ref = p.ref[k];
   int id[kListLanes];  // -1: no entry
   bool teachers[kListLanes];
   double l2[kListLanes], lt[kListLanes];  // ln p in log2 units, ln t
@@ -260,7 +343,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
     p.loss[p.n + o] = div;
     p.loss[2 * p.n + o] = ce;
   }
-  if (p.E == nullptr) return;
+  if (p.E == nullptr) return 0.f;
   const double whole = tail ? mass + r : mass;
   double outer = p.reverse ? (tail ? lq - lr - div : 0.) : whole;
   if (!p.reverse && tail) outer -= outside > 0. ? r / q : 0.;
@@ -314,6 +397,13 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
     }
   }
   if (lane == 0) p.f[k] = (float)f;
+  return (float)f;
+}
+
+// A wave a row, behind flce_row_kernel's sums.
+__global__ __launch_bounds__(256) void distill_row_kernel(const RowMathArgs p) {
+  const int64_t counted = *p.nvalid, k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (k < min(p.nc, counted - p.c0)) row_math(p, k, counted, p.rsum[k], p.rtop[k]);
 }
 
 // Sums of the rows' losses, in a fixed order and 64 bits; one workgroup.
@@ -327,13 +417,14 @@ struct LossArgs {
   int64_t n;
 };
 __global__ __launch_bounds__(1024) void distill_loss_kernel(const LossArgs p) {
-  __shared__ double sm[3][16];
-  __shared__ long long bad_sh[16];
+  constexpr int T = 1024, NWV = T / 64;
+  __shared__ double sm[3][NWV];
+  __shared__ long long bad_sh[NWV];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t nv = min(p.n, *p.nvalid);
   double s[3] = {0., 0., 0.};
   long long bad = 0;
-  for (int64_t i = tid; i < nv; i += 1024) {
+  for (int64_t i = tid; i < nv; i += T) {
 #pragma unroll
     for (int j = 0; j < 3; ++j) s[j] += p.loss[j * p.n + i];
     bad += p.bad[i];
@@ -350,18 +441,85 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const LossArgs p) {
   if (tid >= 4) return;
   if (tid == 3) {
     bad = 0;
-    for (int i = 0; i < 16; ++i) bad += bad_sh[i];
+    for (int i = 0; i < NWV; ++i) bad += bad_sh[i];
     *p.total_bad = bad;
     return;
   }
   double x = 0.;
-  for (int i = 0; i < 16; ++i) x += sm[tid][i];
+  for (int i = 0; i < NWV; ++i) x += sm[tid][i];
   *p.out[tid] = (float)(x / (p.divisor != nullptr ? (double)*p.divisor : (double)nv));
+}
+
+// Few rows: a workgroup a row adds its tiles' sums (E of rows with redone tiles is
+// brought to the largest of their references, as flce_row_kernel does), one wave of it does
+// the row's math, and all scale its hidden state for dW.
+__global__ __launch_bounds__(256) void distill_row_few_kernel(const RowMathArgs p) {
+  constexpr int T = 256, NWV = T / 64;
+  __shared__ double s_sh[NWV];
+  __shared__ float m_sh[NWV], f_sh;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t counted = *p.nvalid, nv = min(p.nc, counted - p.c0), k = blockIdx.x;
+  if (k >= nv) return;
+  const float rf = p.ref[k];
+  float m = rf;  // the reference of the sum: the row's, or a redone tile's above it
+  bool redone = false;
+  for (int64_t t = tid; t < p.nvt; t += T)
+    if (p.spart[t * p.ldp + k] < 0.f) {
+      redone = true;
+      m = fmaxf(m, p.mpart[t * p.ldp + k]);
+    }
+  redone = __syncthreads_or(redone);
+  if (redone) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (lane == 0) m_sh[w] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) m = fmaxf(m, m_sh[i]);
+  }
+  double sum = 0.;
+  for (int64_t t = tid; t < p.nvt; t += T) {
+    const float s = p.spart[t * p.ldp + k];
+    sum += redone ? (double)fabsf(s) * exp2((double)((s < 0.f ? p.mpart[t * p.ldp + k] : rf) - m)) : (double)s;
+  }
+  sum = wave_sum(sum);
+  if (lane == 0) s_sh[w] = sum;
+  if (redone && p.E != nullptr) {
+    bf16* e = p.E + k * p.V;
+    for (int64_t v = 8 * (int64_t)tid; v < p.V; v += 8 * T) {
+      const int64_t t = v / kFewBI;
+      const float s = p.spart[t * p.ldp + k], d = (s < 0.f ? p.mpart[t * p.ldp + k] : rf) - m;
+      // (in two factors: one alone may leave fp32's range where its products with E, up to 2^60, do not)
+      const float f = exp2f_fast(0.5f * d);
+      bf16x8 x = ld_bf16x8(e + v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (bf16)((float)x[i] * f * f);
+      st_bf16x8(e + v, x);
+    }
+  }
+  __syncthreads();  // (E is behind it, too: the listed tokens' gradients go there next)
+  if (w == 0) {
+    sum = 0.;
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) sum += s_sh[i];
+    const float f = row_math(p, k, counted, sum, m);
+    if (lane == 0) f_sh = f;
+  }
+  if (p.H != nullptr) {
+    __syncthreads();
+    const float f = f_sh;
+    for (int64_t c = 8 * (int64_t)tid; c < p.hdim; c += 8 * T) {
+      bf16x8 x = ld_bf16x8(p.H + k * p.hdim + c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (bf16)((float)x[i] * f);
+      st_bf16x8(p.H + k * p.hdim + c, x);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host
 struct Layout {
-  size_t scal, loss, bad, spart, mpart, ids, lt, zk, mask, base, len, rsum, rtop, f0, w0, at, f, wt, E, part, acc32, rows, hc, yc,
+  size_t loss, bad, spart, mpart, ids, lt, zk, mask, base, len, rsum, rtop, f0, w0, at, f, wt, E, part, acc32, rows, hc, yc,
       ref, keys, slot, next, lsum, total;
   int64_t chunk, nchunks, nvt, ldm, ldb;
   int ldk, vt, splits, prow, run, nsort;
@@ -383,7 +541,7 @@ Layout layout(int64_t n, int64_t hdim, int64_t V, int top_k, int64_t chunk, bool
   L.ldm = L.nvt * L.vt / 8;
   L.ldb = L.nvt * (L.vt / list_lane_bits(L.few));
   const size_t rows = (size_t)std::max<int64_t>(n, 1), npad = (rows + 255) / 256 * 256, nc = (size_t)L.chunk;
-  size_t off = 512;  // scal: nvalid; an unused factor
+  size_t off = 512;  // nvalid, an unused factor
   auto take = [&](bool on, size_t bytes) {
     const size_t at = off;
     if (on) off += al(bytes);
@@ -459,7 +617,8 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
   c.yc = at<int64_t>(a.ws, L.yc);
   c.ref = at<float>(a.ws, L.ref);
   c.dh = a.grads ? a.dhidden : nullptr;
-  launch_compact(c, stream);
+  const bool one_few = L.few && L.nchunks == 1;  // all rows in one chunk of the few-rows kernels
+  if (!one_few) launch_compact(c, stream);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
     const int64_t nc = std::min(L.chunk, a.n - c0);
     bf16 *Hc = c.hc + c0 * a.hdim, *E = a.grads ? at<bf16>(a.ws, L.E) : nullptr;
@@ -483,6 +642,22 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     ls.ldk = L.ldk;
     ls.ldm = L.ldm;
     ls.ldb = L.ldb;
+    if (one_few) {
+      ls.few.labels = a.labels;
+      ls.few.hidden = a.hidden;
+      ls.few.weight = a.weight;
+      ls.few.rows = rows;
+      ls.few.y = c.yc;
+      ls.few.nvalid = nvalid;
+      ls.few.counts = a.counts;
+      ls.few.hc = c.hc;
+      ls.few.ref = c.ref;
+      ls.few.dh = c.dh;
+      ls.few.hdim = a.hdim;
+      ls.few.ignore_index = a.ignore_index;
+      ls.few.n = (int)a.n;
+      ls.few.zscale = c.zscale;
+    }
     const dim3 each((unsigned)nc), waves((unsigned)((nc + 3) / 4));
     if (L.few)
       hipLaunchKernelGGL((a.ids32 ? distill_list_kernel<int32_t, true> : distill_list_kernel<int64_t, true>), each,
@@ -512,6 +687,7 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     lg.ldk = L.ldk;
     lg.ldm = L.ldm;
     lg.ldb = L.ldb;
+    lg.slot = one_few && need_dw ? at<int32_t>(a.ws, L.slot) : nullptr;
     launch_logits(lg, L.few, true, stream);
 
     RowArgs rw{};
@@ -531,7 +707,7 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     rw.grads = lg.store_e;
     rw.rsum = at<float>(a.ws, L.rsum);
     rw.rtop = at<float>(a.ws, L.rtop);
-    launch_row(rw, L.few, true, stream);
+    if (!L.few) launch_row(rw, false, true, stream);
 
     RowMathArgs rm{};
     rm.ids = ls.out;
@@ -558,10 +734,20 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     rm.tail = a.tail;
     rm.c = a.ce_weight;
     rm.inv_t = 1. / a.temperature;
-    hipLaunchKernelGGL(distill_row_kernel, waves, dim3(256), 0, stream, rm);
+    if (L.few) {
+      rm.spart = lg.spart;
+      rm.mpart = lg.mpart;
+      rm.H = one_few && need_dw ? Hc : nullptr;
+      rm.nvt = L.nvt;
+      rm.ldp = L.chunk;
+      rm.hdim = a.hdim;
+      hipLaunchKernelGGL(distill_row_few_kernel, each, dim3(256), 0, stream, rm);
+    } else {
+      hipLaunchKernelGGL(distill_row_kernel, waves, dim3(256), 0, stream, rm);
+    }
     if (!a.grads) continue;
 
-    if (a.dhidden != nullptr) {
+    if (a.dhidden != nullptr || one_few) {
       DhArgs dh{};
       dh.Wt = lg.W;
       dh.E = GOp{E, a.vocab, nc, a.vocab};
@@ -584,50 +770,58 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
         fs.f0 = rm.f;
         fs.w0 = rm.w;
         fs.scale = 1.f;
+        if (one_few && need_dw) {
+          fs.H = a.hidden;
+          fs.lsum = at<float>(a.ws, L.lsum);
+          fs.slot = at<int32_t>(a.ws, L.slot);
+          fs.next = at<int32_t>(a.ws, L.next);
+        }
         launch_dh_few(fs, stream);
       } else {
         launch_dh(dh, stream);
       }
     }
     if (!need_dw) continue;
-    WeighArgs wg{};
-    wg.H = a.hidden;
-    wg.rows = rows + c0;
-    wg.y = rm.at;
-    wg.f0 = rm.f;
-    wg.w0 = rm.w;
-    wg.nvalid = nvalid;
-    wg.Hs = Hc;
-    wg.f = at<float>(a.ws, L.f);
-    wg.wt = at<float>(a.ws, L.wt);
-    wg.keys = at<uint64_t>(a.ws, L.keys);
-    wg.slot = at<int32_t>(a.ws, L.slot);
-    wg.n = a.n;
-    wg.nc = nc;
-    wg.c0 = c0;
-    wg.V = a.vocab;
-    wg.hdim = a.hdim;
-    wg.ignore_index = a.ignore_index;
-    wg.scale = 1.f;
-    wg.nsort = L.nsort;
-    launch_weigh(wg, stream);
-    LabelArgs la{};
-    la.keys = wg.keys;
-    la.H = a.hidden;
-    la.rows = wg.rows;
-    la.wt = wg.wt;
-    la.lsum = at<float>(a.ws, L.lsum);
-    la.slot = wg.slot;
-    la.next = at<int32_t>(a.ws, L.next);
-    la.hdim = a.hdim;
-    la.nsort = L.nsort;
-    launch_labels(la, nc, stream);
+    if (!one_few) {
+      WeighArgs wg{};
+      wg.H = a.hidden;
+      wg.rows = rows + c0;
+      wg.y = rm.at;
+      wg.f0 = rm.f;
+      wg.w0 = rm.w;
+      wg.nvalid = nvalid;
+      wg.Hs = Hc;
+      wg.f = at<float>(a.ws, L.f);
+      wg.wt = at<float>(a.ws, L.wt);
+      wg.keys = at<uint64_t>(a.ws, L.keys);
+      wg.slot = at<int32_t>(a.ws, L.slot);
+      wg.n = a.n;
+      wg.nc = nc;
+      wg.c0 = c0;
+      wg.V = a.vocab;
+      wg.hdim = a.hdim;
+      wg.ignore_index = a.ignore_index;
+      wg.scale = 1.f;
+      wg.nsort = L.nsort;
+      launch_weigh(wg, stream);
+      LabelArgs la{};
+      la.keys = wg.keys;
+      la.H = a.hidden;
+      la.rows = wg.rows;
+      la.wt = wg.wt;
+      la.lsum = at<float>(a.ws, L.lsum);
+      la.slot = wg.slot;
+      la.next = at<int32_t>(a.ws, L.next);
+      la.hdim = a.hdim;
+      la.nsort = L.nsort;
+      launch_labels(la, nc, stream);
+    }
     DwArgs dw{};
     dw.Ht = GOp{Hc, a.hdim, nc, a.hdim};
     dw.Et = GOp{E, a.vocab, nc, a.vocab};
-    dw.slot = la.slot;
-    dw.next = la.next;
-    dw.lsum = la.lsum;
+    dw.slot = at<int32_t>(a.ws, L.slot);
+    dw.next = at<int32_t>(a.ws, L.next);
+    dw.lsum = at<float>(a.ws, L.lsum);
     dw.dw = a.dweight;
     dw.acc32 = at<float>(a.ws, L.acc32);
     dw.nvalid = nvalid;
@@ -635,7 +829,7 @@ hipError_t distill_run(const DistillArgs& a, hipStream_t stream) {
     dw.hdim = a.hdim;
     dw.V = a.vocab;
     dw.chunk = L.chunk;
-    launch_dw(dw, L.few && L.nchunks == 1, stream);
+    launch_dw(dw, one_few, stream);
   }
   if (need_dw && a.n == 0) launch_zero(a.dweight, a.vocab * a.hdim, stream);
   LossArgs lo{};

@@ -1173,6 +1173,7 @@ __global__ __launch_bounds__(kFewThreads) void flce_logits_few_kernel(const Logi
   constexpr int TOK = 32 * NB, STAGE = (kFewBI + TOK) * BK, NWV = kFewThreads / 64, STAGES = NB <= 2 ? 3 : 2;
   __shared__ __align__(16) bf16 smem[STAGES * STAGE];
   const int64_t i0 = (int64_t)blockIdx.x * kFewBI;
+  if (LISTS && p.slot != nullptr && threadIdx.x < kFewBI && i0 + threadIdx.x < p.V) p.slot[i0 + threadIdx.x] = 0;
   if (*p.nvalid <= p.c0) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
@@ -1432,6 +1433,52 @@ __global__ __launch_bounds__(256) void flce_dh_few_sum_kernel(const FewSumArgs a
     if (v == a.ignore_index || v < 0 || v >= p.E.cols) st_bf16x8(p.dh + r * p.hdim + col, zero_bf16x8());
   }
   if (r >= nv) return;
+  if (a.lsum != nullptr) {
+    // the first row of its label adds those of all (at most kFewRows), in order: group q every eighth of them
+    __shared__ int16_t same[kFewRows];
+    __shared__ int count[2];
+    const int64_t v = p.y[r];
+    const int j = threadIdx.x;
+    const bool match = j < nv && p.y[min((int64_t)j, nv - 1)] == v;
+    const uint64_t m = __ballot(match);
+    if (j < kFewRows && (j & 63) == 0) count[j >> 6] = __popcll(m);
+    const bool later = __syncthreads_or(match && j < r);
+    if (!later) {
+      if (match) same[(j >= 64 ? count[0] : 0) + __popcll(m & ((j & 63) ? ~0ull >> (64 - (j & 63)) : 0ull))] = (int16_t)j;
+      __syncthreads();
+      const int n = count[0] + count[1];
+      float acc[8] = {};
+      if (col < p.hdim) {
+#pragma unroll 4
+        for (int s = q; s < n; s += 8) {
+          const int k = same[s];
+          const int64_t row = p.rows[p.c0 + k];
+          const float w = a.w0[k] * (a.g != nullptr ? a.scale * a.g[row] : a.scale);
+          const bf16x8 x = ld_bf16x8(a.H + row * p.hdim + col);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w, (float)x[i], acc[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sh[q][g][i] = acc[i];
+      __syncthreads();
+      if (q == 0 && col < p.hdim) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] += sh[k][g][i];
+        float* dst = a.lsum + r * p.hdim + col;
+        *reinterpret_cast<f32x4*>(dst) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
+        if (blockIdx.x == 0 && g == 0) {
+          a.slot[v] = (int32_t)r + 1;
+          a.next[r] = 0;
+        }
+      }
+      __syncthreads();
+    }
+    if (p.dh == nullptr) return;
+  }
   f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
   if (col < p.hdim) {
     const float* src = p.part + r * p.hdim + col;
@@ -1711,8 +1758,7 @@ void launch_row(RowArgs& rw, bool few, bool lists, hipStream_t stream) {
   rw.parts = rw.grads ? (int)std::max<int64_t>(kRowGroups / groups, 1) : 1;
   const dim3 grid((unsigned)(rw.nsort + groups * rw.parts));
   if (few)
-    hipLaunchKernelGGL((lists ? flce_row_kernel<kFewRowRows, true> : flce_row_kernel<kFewRowRows, false>), grid,
-                       dim3(kRowThreads), 0, stream, rw);
+    hipLaunchKernelGGL((flce_row_kernel<kFewRowRows, false>), grid, dim3(kRowThreads), 0, stream, rw);
   else
     hipLaunchKernelGGL((lists ? flce_row_kernel<kRowRows, true> : flce_row_kernel<kRowRows, false>), grid,
                        dim3(kRowThreads), 0, stream, rw);
@@ -1741,10 +1787,12 @@ void launch_dh_few(FewSumArgs& a, hipStream_t stream) {
   DhArgs& dh = a.dh;
   dh.nI = (int)((dh.hdim + kFewBI - 1) / kFewBI);
   const dim3 grid((unsigned)(dh.nI * dh.splits));
-  if (dh.nc <= 64)
-    hipLaunchKernelGGL(flce_dh_few_kernel<2>, grid, dim3(kFewThreads), 0, stream, dh);
-  else
-    hipLaunchKernelGGL(flce_dh_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, dh);
+  if (dh.dh != nullptr) {
+    if (dh.nc <= 64)
+      hipLaunchKernelGGL(flce_dh_few_kernel<2>, grid, dim3(kFewThreads), 0, stream, dh);
+    else
+      hipLaunchKernelGGL(flce_dh_few_kernel<4>, grid, dim3(kFewThreads), 0, stream, dh);
+  }
   hipLaunchKernelGGL(flce_dh_few_sum_kernel, dim3((unsigned)((dh.hdim + 255) / 256), (unsigned)dh.nc), dim3(256), 0, stream,
                      a);
 }

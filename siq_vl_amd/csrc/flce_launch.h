@@ -45,6 +45,7 @@ struct LogitsArgs {
   float* zk;              // [nc, ldk] the listed tokens' logits in log2 units, relative to ref, in the list's order
   int64_t ldm, ldb;
   int ldk;
+  int32_t* slot;          // [V] cleared (few rows with lists), or nullptr
 };
 
 struct RowArgs {
@@ -142,6 +143,12 @@ struct FewSumArgs {
   const int64_t* labels;  // of all rows, or nullptr: nothing is cleared
   int64_t ignore_index;
   float scale;
+  // the label terms of dW, too (dh.dh may be nullptr then): sums of w H over the rows of each
+  // label, as flce_label_kernel's (slots cleared before)
+  const bf16* H;          // [n, hdim] all rows
+  float* lsum;            // [nc, hdim] or nullptr
+  int32_t* slot;          // [V]
+  int32_t* next;          // [nc]
 };
 
 // dH: vocab ranges, rows of a run, and slots of partial sums that rows [c0, c0 + nc) need.
@@ -173,7 +180,7 @@ void launch_compact(const CompactArgs& a, hipStream_t stream);
 
 // `few`: the kernels of few rows (nc <= kFewRows, tiles of kFewBI columns).
 void launch_logits(LogitsArgs& lg, bool few, bool lists, hipStream_t stream);
-void launch_row(RowArgs& rw, bool few, bool lists, hipStream_t stream);
+void launch_row(RowArgs& rw, bool few, bool lists, hipStream_t stream);  // (lists: not with few)
 void launch_weigh(const WeighArgs& wg, hipStream_t stream);
 void launch_labels(const LabelArgs& la, int64_t nc, hipStream_t stream);
 void launch_dh(DhArgs& dh, hipStream_t stream);
