@@ -294,6 +294,10 @@ int siq_flp_bwd(const void* hidden, const void* weight, const int64_t* labels, c
  * (and then an exact 1.0 writes nothing); any other overlap is undefined. */
 int siq_scale_bf16(const void* src, void* dst, int64_t numel, const float* scalar, void* stream);
 
+/* Two tensors by the same scalar in one launch. */
+int siq_scale2_bf16(const void* src0, void* dst0, int64_t numel0, const void* src1, void* dst1, int64_t numel1,
+                    const float* scalar, void* stream);
+
 /* siq_scale_bf16(data, data, numel, scalar, stream). */
 int siq_scale_bf16_inplace(void* data, int64_t numel, const float* scalar, void* stream);
 

@@ -800,6 +800,22 @@ int siq_scale_bf16(const void* src, void* dst, int64_t numel, const float* scala
   return ok();
 }
 
+int siq_scale2_bf16(const void* src0, void* dst0, int64_t numel0, const void* src1, void* dst1, int64_t numel1,
+                    const float* scalar, void* stream) {
+  if (numel0 < 0 || numel1 < 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "numel must be >= 0");
+  if (numel0 == 0) return siq_scale_bf16(src1, dst1, numel1, scalar, stream);
+  if (numel1 == 0) return siq_scale_bf16(src0, dst0, numel0, scalar, stream);
+  if (src0 == nullptr || dst0 == nullptr || src1 == nullptr || dst1 == nullptr || scalar == nullptr)
+    return fail(SIQ_ERR_INVALID_ARGUMENT, "src, dst and scalar must not be NULL");
+  if (!aligned16(src0) || !aligned16(dst0) || !aligned16(src1) || !aligned16(dst1))
+    return fail(SIQ_ERR_ALIGNMENT, "src / dst not 16-byte aligned");
+  const hipError_t e = siq::launch_scale2_bf16(static_cast<const siq::bf16*>(src0), static_cast<siq::bf16*>(dst0), numel0,
+                                               static_cast<const siq::bf16*>(src1), static_cast<siq::bf16*>(dst1), numel1,
+                                               scalar, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(SIQ_ERR_LAUNCH, "scale launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
 int siq_probe_clock(uint64_t* out, int64_t spin_ticks, void* stream) {
   if (out == nullptr || (reinterpret_cast<uintptr_t>(out) & 7u))
     return fail(SIQ_ERR_ALIGNMENT, "out must be a non-NULL 8-byte aligned uint64[2]");

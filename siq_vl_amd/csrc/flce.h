@@ -51,5 +51,7 @@ hipError_t flp_bwd(const FlpArgs& a, hipStream_t stream);
 size_t flce_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk, bool need_dh, bool need_dw);
 hipError_t flce_run(const FlceArgs& a, hipStream_t stream);
 hipError_t launch_scale_bf16(const bf16* src, bf16* dst, int64_t numel, const float* scalar, hipStream_t stream);
+hipError_t launch_scale2_bf16(const bf16* x0, bf16* y0, int64_t n0, const bf16* x1, bf16* y1, int64_t n1,
+                              const float* scalar, hipStream_t stream);
 
 }  // namespace siq

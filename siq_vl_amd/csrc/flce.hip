@@ -1003,9 +1003,7 @@ __global__ __launch_bounds__(1024) void flce_loss_kernel(const float* __restrict
 
 // y = x * scalar in bf16 (rounded once from fp32).  x == y scales in place,
 // and then an exact 1.0 returns at once; out of place it is a copy.
-__global__ __launch_bounds__(256) void scale_bf16_kernel(const bf16* x, bf16* y, int64_t nvec, int64_t numel,
-                                                         const float* __restrict__ scalar) {
-  const float s = *scalar;
+__device__ __forceinline__ void scale_bf16(const bf16* x, bf16* y, int64_t nvec, int64_t numel, float s) {
   if (s == 1.f && x == y) return;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nvec; i += (int64_t)gridDim.x * 256) {
     if (8 * i + 8 <= numel) {
@@ -1017,6 +1015,17 @@ __global__ __launch_bounds__(256) void scale_bf16_kernel(const bf16* x, bf16* y,
       for (int64_t k = 8 * i; k < numel; ++k) y[k] = (bf16)((float)x[k] * s);
     }
   }
+}
+__global__ __launch_bounds__(256) void scale_bf16_kernel(const bf16* x, bf16* y, int64_t nvec, int64_t numel,
+                                                         const float* __restrict__ scalar) {
+  scale_bf16(x, y, nvec, numel, *scalar);
+}
+// Two tensors by the same scalar.
+__global__ __launch_bounds__(256) void scale2_bf16_kernel(const bf16* x0, bf16* y0, int64_t n0, const bf16* x1, bf16* y1,
+                                                          int64_t n1, const float* __restrict__ scalar) {
+  const float s = *scalar;
+  scale_bf16(x0, y0, (n0 + 7) / 8, n0, s);
+  scale_bf16(x1, y1, (n1 + 7) / 8, n1, s);
 }
 
 __global__ __launch_bounds__(256) void zero_bf16_kernel(bf16* __restrict__ x, int64_t nvec) {
@@ -2256,6 +2265,13 @@ hipError_t launch_scale_bf16(const bf16* src, bf16* dst, int64_t numel, const fl
   int64_t blocks = (nvec + 255) / 256;
   if (blocks > 4096) blocks = 4096;
   hipLaunchKernelGGL(scale_bf16_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, src, dst, nvec, numel, scalar);
+  return hipGetLastError();
+}
+
+hipError_t launch_scale2_bf16(const bf16* x0, bf16* y0, int64_t n0, const bf16* x1, bf16* y1, int64_t n1,
+                              const float* scalar, hipStream_t stream) {
+  const int64_t blocks = std::min<int64_t>((std::max(n0, n1) + 2047) / 2048, 4096);
+  hipLaunchKernelGGL(scale2_bf16_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, x0, y0, n0, x1, y1, n1, scalar);
   return hipGetLastError();
 }
 

@@ -614,47 +614,6 @@ __global__ __launch_bounds__(kFewThreads) void stats_grad_few_kernel(const StatG
   }
 }
 
-// dZ from the numerators that the forward kept, a workgroup 2048 columns of a row;
-// the rows that fill up a tile are zeroed, and dH of rows whose label does not
-// count.  It reads and writes 2 bytes an element where the logits take 2 hdim flops.
-struct UnpackArgs {
-  const bf16* E;          // [nc, V]
-  const f32x4* part;      // [nc, parts]
-  const f32x4* coef;      // [nc]
-  bf16* G;                // [nc, V]
-  const int64_t* nvalid;
-  const int64_t* labels;  // [n]
-  bf16* dh;               // or nullptr
-  int64_t nc, c0, V, hdim, ignore_index;
-  int parts;
-  bool few;
-};
-constexpr int kUnpackCols = 2048;
-__global__ __launch_bounds__(256) void stats_unpack_kernel(const UnpackArgs p) {
-  const int64_t nv = min(p.nc, *p.nvalid - p.c0), v = (int64_t)blockIdx.x * kUnpackCols + 8 * threadIdx.x;
-  for (int64_t k = blockIdx.y; k < p.nc; k += gridDim.y) {
-    if (blockIdx.x == 0 && p.dh != nullptr) {
-      const int64_t row = p.c0 + k, y = p.labels[row];
-      if (y == p.ignore_index || y < 0 || y >= p.V)
-        for (int64_t c = 8 * (int64_t)threadIdx.x; c < p.hdim; c += 8 * 256) st_bf16x8(p.dh + row * p.hdim + c, zero_bf16x8());
-    }
-    if (k >= nv + BJ || v >= p.V) continue;
-    bf16x8 g = zero_bf16x8();
-    if (k < nv) {
-      const bf16x8 e = ld_bf16x8(p.E + k * p.V + v);
-      const int64_t part = p.few ? v / kFewBI : 2 * (v / kVT) + (v >> 6 & 1);
-      const f32x4 c = p.coef[k];
-      const float d = p.part[k * p.parts + part][0] - c[0], f = exp2f_fast(d), a = __builtin_fmaf(c[2], d, c[1]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = (float)e[i];
-        g[i] = (bf16)(x * f * __builtin_fmaf(c[2], fmaxf(__log2f(x), -1e4f), a));
-      }
-    }
-    st_bf16x8(p.G + k * p.V + v, g);
-  }
-}
-
 // What a row's gradient needs of the forward's results and of the upstream
 // gradients: {lse, A, B} as above, and the given token's own dz (in 32 bits),
 //   A = -(g + e H) / T,  B = -e ln 2 / T,  dz_y = (g (1 - p_y) - e p_y (ln p_y + H)) / T.
@@ -662,11 +621,21 @@ struct StatCoefArgs {
   const int32_t* rows;    // [nc]
   const int64_t* nvalid;
   const float *logp, *entropy, *lse, *g, *e;  // by row; g and e may be nullptr
-  f32x4* coef;            // [nc]
+  f32x4* coef;            // [nc] (what the forward kept needs none)
   float *f, *w;           // [nc]: 1, dz_y
   int64_t nc, c0;
   float inv_t;
 };
+__device__ __forceinline__ f32x4 stat_coef(const StatCoefArgs& p, int64_t k, float& dzy) {
+  const int64_t row = p.rows[k];
+  const float lp = p.logp[row], hh = p.entropy[row];
+  const float g = (p.g != nullptr ? p.g[row] : 0.f) * p.inv_t, e = (p.e != nullptr ? p.e[row] : 0.f) * p.inv_t;
+  const float py = expf(lp);
+  dzy = -g * expm1f(lp) - (e != 0.f ? e * py * (fmaxf(lp, -1e4f) + hh) : 0.f);
+  return f32x4{p.lse[row], -__builtin_fmaf(e, hh, g), -e * kLn2, 0.f};
+}
+
+// For the logits that are formed again.
 __global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
   const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, nv = min(p.nc, *p.nvalid - p.c0);
   if (k >= p.nc) return;
@@ -674,13 +643,67 @@ __global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
     p.coef[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     return;
   }
-  const int64_t row = p.rows[k];
-  const float lp = p.logp[row], hh = p.entropy[row];
-  const float g = (p.g != nullptr ? p.g[row] : 0.f) * p.inv_t, e = (p.e != nullptr ? p.e[row] : 0.f) * p.inv_t;
-  const float py = expf(lp);
-  p.coef[k] = f32x4{p.lse[row], -__builtin_fmaf(e, hh, g), -e * kLn2, 0.f};
+  p.coef[k] = stat_coef(p, k, p.w[k]);
   p.f[k] = 1.f;
-  p.w[k] = -g * expm1f(lp) - (e != 0.f ? e * py * (fmaxf(lp, -1e4f) + hh) : 0.f);
+}
+
+
+// dZ from the numerators that the forward kept, a workgroup 2048 columns of a row;
+// the rows that fill up a tile are zeroed, and dH of rows whose label does not
+// count.  It reads and writes 2 bytes an element where the logits take 2 hdim flops.
+struct UnpackArgs {
+  StatCoefArgs c;
+  const bf16* E;          // [nc, V]
+  const f32x4* part;      // [nc, parts]
+  bf16* G;                // [nc, V]
+  const int64_t* labels;  // [n]
+  bf16* dh;               // or nullptr
+  int64_t V, hdim, ignore_index;
+  int parts;
+  bool few;
+  // few rows in one chunk, with dW: what launch_weigh leaves otherwise
+  const bf16* H;          // [n, hdim]
+  bf16* Hs;               // [nc, hdim] the counted rows, or nullptr
+  int32_t* slot;          // [V] cleared
+};
+constexpr int kUnpackCols = 2048;
+__global__ __launch_bounds__(256) void stats_unpack_kernel(const UnpackArgs p) {
+  const int64_t nc = p.c.nc, nv = min(nc, *p.c.nvalid - p.c.c0), v = (int64_t)blockIdx.x * kUnpackCols + 8 * threadIdx.x;
+  if (p.Hs != nullptr && blockIdx.y == 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (v + i < p.V) p.slot[v + i] = 0;
+  for (int64_t k = blockIdx.y; k < nc; k += gridDim.y) {
+    if (blockIdx.x == 0) {
+      const int64_t row = p.c.c0 + k, y = p.labels[row], src = k < nv ? p.c.rows[k] : 0;
+      const bool clear = p.dh != nullptr && (y == p.ignore_index || y < 0 || y >= p.V);
+      if (clear || p.Hs != nullptr)
+        for (int64_t c = 8 * (int64_t)threadIdx.x; c < p.hdim; c += 8 * 256) {
+          if (clear) st_bf16x8(p.dh + row * p.hdim + c, zero_bf16x8());
+          if (p.Hs != nullptr) st_bf16x8(p.Hs + k * p.hdim + c, k < nv ? ld_bf16x8(p.H + src * p.hdim + c) : zero_bf16x8());
+        }
+    }
+    if (k >= nv + BJ) continue;
+    bf16x8 g = zero_bf16x8();
+    if (k < nv) {
+      float dzy;
+      const f32x4 c = stat_coef(p.c, k, dzy);
+      if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.c.f[k] = 1.f;
+        p.c.w[k] = dzy;
+      }
+      if (v >= p.V) continue;
+      const bf16x8 e = ld_bf16x8(p.E + k * p.V + v);
+      const int64_t part = p.few ? v / kFewBI : 2 * (v / kVT) + (v >> 6 & 1);
+      const float d = p.part[k * p.parts + part][0] - c[0], f = exp2f_fast(d), a = __builtin_fmaf(c[2], d, c[1]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = (float)e[i];
+        g[i] = (bf16)(x * f * __builtin_fmaf(c[2], fmaxf(__log2f(x), -1e4f), a));
+      }
+    }
+    if (v < p.V) st_bf16x8(p.G + k * p.V + v, g);
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -928,6 +951,8 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
   c.ref = at<float>(a.ws, L.ref);
   c.dh = a.dhidden;
   if (!have) launch_compact(c, stream);
+  // few rows in one chunk, from what was kept: the labels' sums come with dH's
+  const bool one_few = have && need_dw && L.few && L.nchunks == 1;
   bf16* E = at<bf16>(a.ws, L.E);
   float *f0 = at<float>(a.ws, L.f0), *w0 = at<float>(a.ws, L.w0);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
@@ -947,7 +972,7 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
     co.nc = nc;
     co.c0 = c0;
     co.inv_t = (float)(1. / a.temperature);
-    hipLaunchKernelGGL(stats_coef_kernel, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, stream, co);
+    if (!have) hipLaunchKernelGGL(stats_coef_kernel, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, stream, co);
     StatGradArgs gr{};
     gr.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
     gr.H = GOp{Hc, a.hdim, nc, a.hdim};
@@ -963,18 +988,18 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
       UnpackArgs un{};
       un.E = at<bf16>(a.saved, S.E) + c0 * a.vocab;
       un.part = at<f32x4>(a.saved, S.part) + c0 * S.parts;
-      un.coef = co.coef;
+      un.c = co;
       un.G = E;
-      un.nvalid = nvalid;
       un.labels = a.labels;
       un.dh = a.dhidden;
-      un.nc = nc;
-      un.c0 = c0;
       un.V = a.vocab;
       un.hdim = a.hdim;
       un.ignore_index = a.ignore_index;
       un.parts = (int)S.parts;
       un.few = a.n <= kFewRows;
+      un.H = a.hidden;
+      un.Hs = one_few ? Hc : nullptr;
+      un.slot = at<int32_t>(a.ws, L.slot);
       const dim3 grid((unsigned)((a.vocab + kUnpackCols - 1) / kUnpackCols), (unsigned)std::min<int64_t>(nc, 32768));
       hipLaunchKernelGGL(stats_unpack_kernel, grid, dim3(256), 0, stream, un);
     } else if (L.few) {
@@ -987,7 +1012,7 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
       const int grid = ((gr.nI * gr.nJ + kXcds - 1) / kXcds) * kXcds;
       hipLaunchKernelGGL(stats_grad_kernel, dim3(grid), dim3(NT), 0, stream, gr);
     }
-    if (a.dhidden != nullptr) {
+    if (a.dhidden != nullptr || one_few) {
       DhArgs dh{};
       dh.Wt = gr.W;
       dh.E = GOp{E, a.vocab, nc, a.vocab};
@@ -1010,50 +1035,58 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
         fs.f0 = f0;
         fs.w0 = w0;
         fs.scale = 1.f;
+        if (one_few) {
+          fs.H = a.hidden;
+          fs.lsum = at<float>(a.ws, L.lsum);
+          fs.slot = at<int32_t>(a.ws, L.slot);
+          fs.next = at<int32_t>(a.ws, L.next);
+        }
         launch_dh_few(fs, stream);
       } else {
         launch_dh(dh, stream);
       }
     }
     if (!need_dw) continue;
-    WeighArgs wg{};
-    wg.H = a.hidden;
-    wg.rows = rows + c0;
-    wg.y = gr.y;
-    wg.f0 = f0;
-    wg.w0 = w0;
-    wg.nvalid = nvalid;
-    wg.Hs = Hc;  // (which the logits above have read; every factor is 1)
-    wg.f = at<float>(a.ws, L.f);
-    wg.wt = at<float>(a.ws, L.wt);
-    wg.keys = at<uint64_t>(a.ws, L.keys);
-    wg.slot = at<int32_t>(a.ws, L.slot);
-    wg.n = a.n;
-    wg.nc = nc;
-    wg.c0 = c0;
-    wg.V = a.vocab;
-    wg.hdim = a.hdim;
-    wg.ignore_index = a.ignore_index;
-    wg.scale = 1.f;
-    wg.nsort = L.nsort;
-    launch_weigh(wg, stream);
-    LabelArgs la{};
-    la.keys = wg.keys;
-    la.H = a.hidden;
-    la.rows = wg.rows;
-    la.wt = wg.wt;
-    la.lsum = at<float>(a.ws, L.lsum);
-    la.slot = wg.slot;
-    la.next = at<int32_t>(a.ws, L.next);
-    la.hdim = a.hdim;
-    la.nsort = L.nsort;
-    launch_labels(la, nc, stream);
+    if (!one_few) {
+      WeighArgs wg{};
+      wg.H = a.hidden;
+      wg.rows = rows + c0;
+      wg.y = gr.y;
+      wg.f0 = f0;
+      wg.w0 = w0;
+      wg.nvalid = nvalid;
+      wg.Hs = Hc;  // (which the logits above have read; every factor is 1)
+      wg.f = at<float>(a.ws, L.f);
+      wg.wt = at<float>(a.ws, L.wt);
+      wg.keys = at<uint64_t>(a.ws, L.keys);
+      wg.slot = at<int32_t>(a.ws, L.slot);
+      wg.n = a.n;
+      wg.nc = nc;
+      wg.c0 = c0;
+      wg.V = a.vocab;
+      wg.hdim = a.hdim;
+      wg.ignore_index = a.ignore_index;
+      wg.scale = 1.f;
+      wg.nsort = L.nsort;
+      launch_weigh(wg, stream);
+      LabelArgs la{};
+      la.keys = wg.keys;
+      la.H = a.hidden;
+      la.rows = wg.rows;
+      la.wt = wg.wt;
+      la.lsum = at<float>(a.ws, L.lsum);
+      la.slot = wg.slot;
+      la.next = at<int32_t>(a.ws, L.next);
+      la.hdim = a.hdim;
+      la.nsort = L.nsort;
+      launch_labels(la, nc, stream);
+    }
     DwArgs dw{};
     dw.Ht = GOp{Hc, a.hdim, nc, a.hdim};
     dw.Et = GOp{E, a.vocab, nc, a.vocab};
-    dw.slot = la.slot;
-    dw.next = la.next;
-    dw.lsum = la.lsum;
+    dw.slot = at<int32_t>(a.ws, L.slot);
+    dw.next = at<int32_t>(a.ws, L.next);
+    dw.lsum = at<float>(a.ws, L.lsum);
     dw.dw = a.dweight;
     dw.acc32 = at<float>(a.ws, L.acc32);
     dw.nvalid = nvalid;

@@ -34,7 +34,7 @@ using torch::autograd::variable_list;
   X(siq_pref_fwd) X(siq_pref_bwd) X(siq_policy_workspace_bytes) X(siq_policy_fwd) X(siq_policy_bwd)                 \
   X(siq_flp_saved_bytes) X(siq_flp_fwd_workspace_bytes) X(siq_flp_fwd) X(siq_flp_bwd_workspace_bytes) X(siq_flp_bwd) \
   X(siq_stats_saved_bytes) X(siq_stats_fwd_workspace_bytes) X(siq_stats_fwd) X(siq_stats_bwd_workspace_bytes)       \
-  X(siq_stats_bwd) X(siq_distill_workspace_bytes) X(siq_distill) X(siq_scale_bf16)
+  X(siq_stats_bwd) X(siq_distill_workspace_bytes) X(siq_distill) X(siq_scale2_bf16)
 
 struct Api {
 #define SIQ_MEMBER(name) decltype(&::name) name = nullptr;
@@ -697,13 +697,6 @@ variable_list distill(const Tensor& hidden, const Tensor& weight, const Tensor& 
   return {loss, div, ce, dh, dw};
 }
 
-// t times a device scalar: in place, unless the graph is kept and a second backward wants t as it is.
-Tensor scaled(const Tensor& t, const Tensor& g, bool in_place) {
-  const Tensor out = in_place ? t : at::empty(t.sizes(), t.options());
-  check(api.siq_scale_bf16(t.data_ptr(), out.data_ptr(), t.numel(), fptr(g), stream_of(t)), "siq_scale_bf16");
-  return out;
-}
-
 // The gradients are known in the forward up to the upstream one, a scalar.
 struct Distillation : torch::autograd::Function<Distillation> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
@@ -726,9 +719,17 @@ struct Distillation : torch::autograd::Function<Distillation> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor g = upstream(grads[0]);
     const c10::DeviceGuard guard(g.device());
+    // in place, unless the graph is kept and a second backward wants them as they are
     const bool in_place = !torch::autograd::get_current_graph_task_keep_graph();
-    if (ctx->needs_input_grad(0)) out[0] = scaled(s[0], g, in_place).view(ctx->saved_data["shape"].toIntVector());
-    if (ctx->needs_input_grad(1)) out[1] = scaled(s[1], g, in_place);
+    Tensor to[2];
+    for (int i = 0; i < 2; ++i)
+      if (ctx->needs_input_grad(i)) to[i] = in_place ? s[i] : at::empty(s[i].sizes(), s[i].options());
+    auto src = [&](int i) { return to[i].defined() ? s[i].data_ptr() : nullptr; };
+    auto size = [&](int i) { return to[i].defined() ? to[i].numel() : 0; };
+    check(api.siq_scale2_bf16(src(0), ptr(to[0]), size(0), src(1), ptr(to[1]), size(1), fptr(g), stream_of(g)),
+          "siq_scale2_bf16");
+    if (to[0].defined()) out[0] = to[0].view(ctx->saved_data["shape"].toIntVector());
+    out[1] = to[1];
     return out;
   }
 };

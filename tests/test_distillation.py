@@ -109,6 +109,14 @@ def test_workspace_sizes(lib):
     assert f(5, 64, 8, 129, 64, 1, 1) == 0 and f(5, 64, 8, 1, 0, 1, 1) == 0 and f(0, 64, 8, 1, 64, 1, 1) > 0
 
 
+def test_scaling_two_tensors(lib):
+    f = lib.siq_scale2_bf16
+    assert f(None, None, 0, None, None, 0, None, None) == OK
+    assert f(FAKE, FAKE, -1, FAKE, FAKE, 8, FAKE, None) == INVALID and f(FAKE, FAKE, 8, FAKE, FAKE, -1, FAKE, None) == INVALID
+    assert f(None, FAKE, 8, FAKE, FAKE, 8, FAKE, None) == INVALID and f(FAKE, FAKE, 8, FAKE, FAKE, 8, None, None) == INVALID
+    assert f(FAKE, FAKE, 8, FAKE + 8, FAKE, 8, FAKE, None) == ALIGN and f(FAKE, FAKE + 2, 8, FAKE, FAKE, 8, FAKE, None) == ALIGN
+
+
 def test_python_refusals():
     h, w, y = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16), torch.zeros(4).long()
     ids, lt = torch.zeros(4, 2).long(), torch.zeros(4, 2)
