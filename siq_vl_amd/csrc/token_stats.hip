@@ -621,7 +621,7 @@ struct StatCoefArgs {
   const int32_t* rows;    // [nc]
   const int64_t* nvalid;
   const float *logp, *entropy, *lse, *g, *e;  // by row; g and e may be nullptr
-  f32x4* coef;            // [nc] (what the forward kept needs none)
+  f32x4* coef;            // [nc]
   float *f, *w;           // [nc]: 1, dz_y
   int64_t nc, c0;
   float inv_t;
@@ -635,7 +635,6 @@ __device__ __forceinline__ f32x4 stat_coef(const StatCoefArgs& p, int64_t k, flo
   return f32x4{p.lse[row], -__builtin_fmaf(e, hh, g), -e * kLn2, 0.f};
 }
 
-// For the logits that are formed again.
 __global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
   const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, nv = min(p.nc, *p.nvalid - p.c0);
   if (k >= p.nc) return;
@@ -661,36 +660,45 @@ struct UnpackArgs {
   int64_t V, hdim, ignore_index;
   int parts;
   bool few;
-  // few rows in one chunk, with dW: what launch_weigh leaves otherwise
+  // ONE_FEW: what launch_weigh leaves otherwise
   const bf16* H;          // [n, hdim]
-  bf16* Hs;               // [nc, hdim] the counted rows, or nullptr
+  bf16* Hs;               // [nc, hdim] the counted rows
   int32_t* slot;          // [V] cleared
 };
 constexpr int kUnpackCols = 2048;
+// ONE_FEW: few rows in one chunk, with dW; it makes the rows' coefficients, too.  (For
+// many rows that costs more than a launch: each workgroup would wait for them, 2048 x 1536
+// 1.35 -> 1.40 ms, 4099 x 896 2.62 -> 2.75 ms.)
+template <bool ONE_FEW>
 __global__ __launch_bounds__(256) void stats_unpack_kernel(const UnpackArgs p) {
   const int64_t nc = p.c.nc, nv = min(nc, *p.c.nvalid - p.c.c0), v = (int64_t)blockIdx.x * kUnpackCols + 8 * threadIdx.x;
-  if (p.Hs != nullptr && blockIdx.y == 0)
+  if (ONE_FEW && blockIdx.y == 0)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (v + i < p.V) p.slot[v + i] = 0;
   for (int64_t k = blockIdx.y; k < nc; k += gridDim.y) {
     if (blockIdx.x == 0) {
-      const int64_t row = p.c.c0 + k, y = p.labels[row], src = k < nv ? p.c.rows[k] : 0;
+      const int64_t row = p.c.c0 + k, y = p.labels[row], src = ONE_FEW && k < nv ? p.c.rows[k] : 0;
       const bool clear = p.dh != nullptr && (y == p.ignore_index || y < 0 || y >= p.V);
-      if (clear || p.Hs != nullptr)
+      if (clear || ONE_FEW)
         for (int64_t c = 8 * (int64_t)threadIdx.x; c < p.hdim; c += 8 * 256) {
           if (clear) st_bf16x8(p.dh + row * p.hdim + c, zero_bf16x8());
-          if (p.Hs != nullptr) st_bf16x8(p.Hs + k * p.hdim + c, k < nv ? ld_bf16x8(p.H + src * p.hdim + c) : zero_bf16x8());
+          if (ONE_FEW) st_bf16x8(p.Hs + k * p.hdim + c, k < nv ? ld_bf16x8(p.H + src * p.hdim + c) : zero_bf16x8());
         }
     }
     if (k >= nv + BJ) continue;
     bf16x8 g = zero_bf16x8();
     if (k < nv) {
-      float dzy;
-      const f32x4 c = stat_coef(p.c, k, dzy);
-      if (blockIdx.x == 0 && threadIdx.x == 0) {
-        p.c.f[k] = 1.f;
-        p.c.w[k] = dzy;
+      f32x4 c;
+      if constexpr (ONE_FEW) {
+        float dzy;
+        c = stat_coef(p.c, k, dzy);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+          p.c.f[k] = 1.f;
+          p.c.w[k] = dzy;
+        }
+      } else {
+        c = p.c.coef[k];
       }
       if (v >= p.V) continue;
       const bf16x8 e = ld_bf16x8(p.E + k * p.V + v);
@@ -972,7 +980,7 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
     co.nc = nc;
     co.c0 = c0;
     co.inv_t = (float)(1. / a.temperature);
-    if (!have) hipLaunchKernelGGL(stats_coef_kernel, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, stream, co);
+    if (!one_few) hipLaunchKernelGGL(stats_coef_kernel, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, stream, co);
     StatGradArgs gr{};
     gr.W = GOp{a.weight, a.hdim, a.vocab, a.hdim};
     gr.H = GOp{Hc, a.hdim, nc, a.hdim};
@@ -998,10 +1006,10 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
       un.parts = (int)S.parts;
       un.few = a.n <= kFewRows;
       un.H = a.hidden;
-      un.Hs = one_few ? Hc : nullptr;
+      un.Hs = Hc;
       un.slot = at<int32_t>(a.ws, L.slot);
       const dim3 grid((unsigned)((a.vocab + kUnpackCols - 1) / kUnpackCols), (unsigned)std::min<int64_t>(nc, 32768));
-      hipLaunchKernelGGL(stats_unpack_kernel, grid, dim3(256), 0, stream, un);
+      hipLaunchKernelGGL((one_few ? stats_unpack_kernel<true> : stats_unpack_kernel<false>), grid, dim3(256), 0, stream, un);
     } else if (L.few) {
       const dim3 grid((unsigned)((a.vocab + kFewBI - 1) / kFewBI));
       hipLaunchKernelGGL((nc <= 64 ? stats_grad_few_kernel<2> : stats_grad_few_kernel<4>), grid, dim3(kFewThreads), 0, stream,
