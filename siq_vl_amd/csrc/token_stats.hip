@@ -215,7 +215,9 @@ constexpr int kFewSmem = kFewStages<NB> * (kFewBI + 32 * NB) * BK;
 template <int NB, bool TOP, bool KEEP>
 __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const StatLogitsArgs p) {
   constexpr int TOK = 32 * NB, NWV = kFewThreads / 64;
-  __shared__ __align__(16) bf16 smem[kFewSmem<NB>];
+  // behind the last step's barrier: the waves' maxima and sums, and z, which leaves by whole rows of the tile
+  constexpr int RED = 6 * NWV * TOK * 2, BYTES2 = RED + (TOP ? TOK * kFewBI * 2 : 0);
+  __shared__ __align__(16) bf16 smem[BYTES2 > kFewSmem<NB> ? BYTES2 : kFewSmem<NB>];
   const int64_t i0 = (int64_t)blockIdx.x * kFewBI;
   if (*p.nvalid <= p.c0) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h = lane >> 5, l32 = lane & 31;
@@ -235,27 +237,25 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
       for (int r = 0; r < 16; ++r)
         if (vbase + 16 * (r >> 3) + (r & 7) >= p.V) acc[b][r] = -INFINITY;
   }
-  // (behind the last step's barrier) the waves' maxima, then their sums
+  float* zt = reinterpret_cast<float*>(smem + RED);  // [TOK][128], 16-byte chunk c of row r at c ^ (r % 32)
   float *max_sh = reinterpret_cast<float*>(smem), *top_sh = max_sh + NWV * TOK;  // [NWV][TOK]
   f32x4* red = reinterpret_cast<f32x4*>(smem) + 2 * NWV * TOK / 4;               // [NWV][TOK]
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
     const bool tv = tok < p.nc;
-    if (TOP && tv) {
+    if (TOP) {
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
-        const int64_t v0 = vbase + 16 * jj;
-        if (v0 >= p.V) continue;
         f32x4 lo, hi;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           lo[i] = acc[b][8 * jj + i];
           hi[i] = acc[b][8 * jj + 4 + i];
         }
-        float* z = p.Z + tok * p.V + v0;
-        *reinterpret_cast<f32x4*>(z) = lo;
-        *reinterpret_cast<f32x4*>(z + 4) = hi;
+        const int c = 8 * w + 4 * jj + 2 * h;
+        *reinterpret_cast<f32x4*>(zt + tok * kFewBI + 4 * (c ^ l32)) = lo;
+        *reinterpret_cast<f32x4*>(zt + tok * kFewBI + 4 * ((c + 1) ^ l32)) = hi;
       }
     }
     auto get = [&](int, int r) { return acc[b][r]; };
@@ -279,6 +279,13 @@ __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const Sta
     }
   }
   __syncthreads();
+  if (TOP) {
+    const int rows = (int)min(p.nc, (int64_t)TOK), c = tid % 32;
+    if (i0 + 4 * c < p.V)
+      for (int r = tid / 32; r < rows; r += kFewThreads / 32)
+        *reinterpret_cast<f32x4*>(p.Z + r * p.V + i0 + 4 * c) =
+            *reinterpret_cast<const f32x4*>(zt + r * kFewBI + 4 * (c ^ (r & 31)));
+  }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int64_t tok = 32 * b + l32;
