@@ -456,8 +456,8 @@ int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels,
                   size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
-      (rc = check_saved(saved, saved_bytes, siq::stats_saved_bytes(n, vocab))) || (rc = check_top_k(top_k, 0, vocab)) || (rc = check_not_null(count, "count")) ||
-      (rc = check_not_null(bad_labels, "bad_labels")))
+      (rc = check_saved(saved, saved_bytes, siq::stats_saved_bytes(n, vocab))) || (rc = check_top_k(top_k, 0, vocab)) ||
+      (rc = check_not_null(count, "count")) || (rc = check_not_null(bad_labels, "bad_labels")))
     return rc;
   if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
                 (rc = check_not_null(lse, "lse"))))
