@@ -430,15 +430,25 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     }
   }
   if (p.rows == nullptr ? !counts : p.c0 + k >= *p.nvalid) return;
+  // the row's parts, read once where a vocabulary has no more than 163,840 columns
+  constexpr int R = 5;
   const f32x4* src = p.part + k * p.parts;
+  f32x4 held[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) held[u] = src[min(tid + T * u, p.parts - 1)];
+  auto each_part = [&](auto use) {
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+      if (tid + T * u < p.parts) use(tid + T * u, held[u]);
+    for (int i = tid + T * R; i < p.parts; i += T) use(i, src[i]);
+  };
   const double dy = (double)p.zy[k] * (double)p.zscale;
   float m = (float)dy;
   uint32_t best = 0;
-  for (int i = tid; i < p.parts; i += T) {
-    const f32x4 x = src[i];
+  each_part([&](int, const f32x4& x) {
     m = fmaxf(m, x[0]);
     best = max(best, order_of(x[3]));
-  }
+  });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   if (lane == 0) m_sh[w] = m;
@@ -448,14 +458,13 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
 #pragma unroll
   for (int i = 0; i < NWV; ++i) m = fmaxf(m, m_sh[i]);
   double s = 0., t = 0.;
-  for (int i = tid; i < p.parts; i += T) {
-    const f32x4 x = src[i];
-    if (x[1] == 0.f) continue;  // (nothing but minus infinities; a NaN counts)
+  each_part([&](int, const f32x4& x) {
+    if (x[1] == 0.f) return;  // (nothing but minus infinities; a NaN counts)
     // (a factor for the sums of 128 terms: its rounding is that of a sum of so many)
     const float d = x[0] - m, f = exp2f_fast(d);
     s += (double)(x[1] * f);
     t += ((double)x[2] + (double)x[1] * (double)d) * (double)f;
-  }
+  });
   s = wave_sum(s);
   t = wave_sum(t);
   if (lane == 0) {
@@ -494,11 +503,11 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     p.top_logp[row * p.K + rank] = (float)(((double)zi * (double)p.zscale - lse_sh) * kLn2d);
     p.top_ids[row * p.K + rank] = (int64_t)(uint32_t)~(uint32_t)key;
   };
-  for (int i = tid; i < p.parts; i += T)
-    if (order_of(src[i][3]) >= tau) {
-      const int at = atomicAdd(&nparts_sh, 1);  // (in any order: ranks make one)
-      if (at < kMostParts) part_sh[at] = i;
-    }
+  each_part([&](int i, const f32x4& x) {
+    if (order_of(x[3]) < tau) return;
+    const int at = atomicAdd(&nparts_sh, 1);  // (in any order: ranks make one)
+    if (at < kMostParts) part_sh[at] = i;
+  });
   __syncthreads();
   const int np = nparts_sh, c = tid & 127, off = p.few ? c : (c & 63) + 128 * (c >> 6);
   auto column = [&](int part) {
