@@ -562,13 +562,14 @@ int siq_policy_bwd(const float* grad_loss, const float* dtoken, const float* wei
  * z = hidden weight^T / temperature exist only as one chunk's.
  *
  * siq_stats_fwd: for each counted row logp = ln softmax(z) at the label,
- * entropy = -sum p ln p, and with top_k > 0 (at most 128 and vocab)
- * the largest logits' ids in order, equal ones by lower id first
- * (top_ids [n, top_k]), with their log-probabilities (top_logp).  Rows that do not
+ * entropy = -sum p ln p, and with top_k > 0 (at most 128 and vocab) the largest
+ * logits' ids in order, equal ones by lower id first (top_ids [n, top_k]), with
+ * their log-probabilities (top_logp).  Rows that do not
  * count have 0, and ids of -1.  A row with a NaN logit has NaN log-probabilities
- * and ids in [0, vocab).  logp, entropy, lse [n]; lse is what siq_stats_bwd takes
- * besides them.  top_logp and top_ids may be NULL with top_k 0.  saved (siq_stats_saved_bytes,
- * or NULL): the softmax numerators in bf16, kept for the backward.
+ * and ids in [0, vocab).  logp, entropy [n]; state [3, n] (or NULL) is what
+ * siq_stats_bwd takes of them.  top_logp and top_ids may be NULL with top_k 0.
+ * saved (siq_stats_saved_bytes, or NULL): the softmax numerators in bf16, kept for
+ * the backward.
  * siq_stats_bwd: dhidden and / or dweight (NULL: not computed) from the upstream
  * gradients dlogp and dentropy [n] (NULL: zero),
  *   dz_j = dlogp ([j = label] - p_j) - dentropy p_j (ln p_j + entropy).
@@ -603,17 +604,16 @@ size_t siq_stats_fwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int
 
 int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
                   int64_t vocab, int64_t ignore_index, double temperature, int top_k, float* logp, float* entropy,
-                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* saved,
+                  float* state, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* saved,
                   size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
 size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int64_t chunk_tokens, int need_dweight,
                                      int have_saved);
 
-int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* logp,
-                  const float* entropy, const float* lse, const float* dlogp, const float* dentropy, int64_t n,
-                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, const void* saved,
-                  size_t saved_bytes, void* dhidden, void* dweight, int64_t chunk_tokens, void* workspace,
-                  size_t workspace_bytes, void* stream);
+int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* state,
+                  const float* dlogp, const float* dentropy, int64_t n, int64_t hdim, int64_t vocab,
+                  int64_t ignore_index, double temperature, const void* saved, size_t saved_bytes, void* dhidden,
+                  void* dweight, int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
 size_t siq_distill_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int top_k, int64_t chunk_tokens,
                                    int need_grads, int need_dweight);

@@ -119,8 +119,8 @@ _PROTOS = {
     "siq_stats_bwd_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i32, _i32]),
     "siq_stats_bwd": (
         _i32,
-        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64,
-         _f64, _c_void_p, _size, _c_void_p, _c_void_p, _i64, _c_void_p, _size, _c_void_p],
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _f64, _c_void_p, _size,
+         _c_void_p, _c_void_p, _i64, _c_void_p, _size, _c_void_p],
     ),
     "siq_distill_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64, _i32, _i32]),
     "siq_distill": (

@@ -452,16 +452,14 @@ size_t siq_stats_bwd_workspace_bytes(int64_t n, int64_t hdim, int64_t vocab, int
 
 int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels, int64_t n, int64_t hdim,
                   int64_t vocab, int64_t ignore_index, double temperature, int top_k, float* logp, float* entropy,
-                  float* lse, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* saved,
+                  float* state, float* top_logp, int64_t* top_ids, int64_t* count, int64_t* bad_labels, void* saved,
                   size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
       (rc = check_saved(saved, saved_bytes, siq::stats_saved_bytes(n, vocab))) || (rc = check_top_k(top_k, 0, vocab)) ||
       (rc = check_not_null(count, "count")) || (rc = check_not_null(bad_labels, "bad_labels")))
     return rc;
-  if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
-                (rc = check_not_null(lse, "lse"))))
-    return rc;
+  if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")))) return rc;
   if (n > 0 && top_k > 0 && ((rc = check_not_null(top_logp, "top_logp")) || (rc = check_not_null(top_ids, "top_ids"))))
     return rc;
   if ((rc = check_ws(workspace, workspace_bytes,
@@ -479,7 +477,7 @@ int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels,
   a.top_k = top_k;
   a.logp = logp;
   a.entropy = entropy;
-  a.lse = lse;
+  a.state = state;
   a.top_logp = top_logp;
   a.top_ids = top_ids;
   a.count = count;
@@ -489,19 +487,16 @@ int siq_stats_fwd(const void* hidden, const void* weight, const int64_t* labels,
   return launched(siq::stats_fwd(a, static_cast<hipStream_t>(stream)), "token statistics");
 }
 
-int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* logp,
-                  const float* entropy, const float* lse, const float* dlogp, const float* dentropy, int64_t n,
-                  int64_t hdim, int64_t vocab, int64_t ignore_index, double temperature, const void* saved,
-                  size_t saved_bytes, void* dhidden, void* dweight, int64_t chunk_tokens, void* workspace,
-                  size_t workspace_bytes, void* stream) {
+int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* state,
+                  const float* dlogp, const float* dentropy, int64_t n, int64_t hdim, int64_t vocab,
+                  int64_t ignore_index, double temperature, const void* saved, size_t saved_bytes, void* dhidden,
+                  void* dweight, int64_t chunk_tokens, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_flp_call(hidden, weight, labels, n, hdim, vocab, temperature, nullptr, 0)) ||
       (rc = check_saved(saved, saved_bytes, siq::stats_saved_bytes(n, vocab))))
     return rc;
   if (chunk_tokens <= 0) return fail(SIQ_ERR_INVALID_ARGUMENT, "chunk_tokens must be positive");
-  if (n > 0 && ((rc = check_not_null(logp, "logp")) || (rc = check_not_null(entropy, "entropy")) ||
-                (rc = check_not_null(lse, "lse"))))
-    return rc;
+  if (n > 0 && (rc = check_not_null(state, "state"))) return rc;
   if ((rc = check_grads(hidden, dhidden, dweight, n, hdim))) return rc;
   if (dhidden == nullptr && dweight == nullptr) return ok();
   if ((rc = check_ws(workspace, workspace_bytes,
@@ -516,9 +511,7 @@ int siq_stats_bwd(const void* hidden, const void* weight, const int64_t* labels,
   a.vocab = vocab;
   a.ignore_index = ignore_index;
   a.temperature = temperature;
-  a.logp = const_cast<float*>(logp);
-  a.entropy = const_cast<float*>(entropy);
-  a.lse = const_cast<float*>(lse);
+  a.state = const_cast<float*>(state);
   a.dlogp = dlogp;
   a.dentropy = dentropy;
   a.saved = const_cast<void*>(saved);

@@ -19,7 +19,7 @@ struct StatsArgs {
   int top_k;
   float* logp;          // [n]
   float* entropy;       // [n]
-  float* lse;           // [n] log2 of the sum of exp(z / temperature): what the backward needs
+  float* state;         // [3, n] (or nullptr: no backward follows) log2 of the sum of exp(z / temperature), logp and entropy
   float* top_logp;      // [n, top_k]
   int64_t* top_ids;     // [n, top_k]
   int64_t* count;

@@ -338,10 +338,11 @@ struct StatRowArgs {
   const int32_t* rows;    // [nc] compacted row -> row, or nullptr: nothing was compacted (a call of few rows)
   const int64_t* nvalid;
   const int64_t* labels;  // [n]
-  float *logp, *entropy, *lse;  // [n] by row
+  float *logp, *entropy;  // [n] by row
+  float* state;           // [3, n] or nullptr
   float* top_logp;        // [n, K]
   int64_t* top_ids;
-  int64_t c0, V, ignore_index;
+  int64_t n, c0, V, ignore_index;
   int parts, K;
   bool few;               // parts of 128 columns in a row, or twice 64 of a tile
   float zscale;
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
   const int64_t k = blockIdx.x, own = p.c0 + k, y = p.labels[own];
   const bool counts = y != p.ignore_index && y >= 0 && y < p.V;
   if (!counts) {
-    if (tid == 0) p.logp[own] = p.entropy[own] = p.lse[own] = 0.f;
+    if (tid == 0) p.logp[own] = p.entropy[own] = 0.f;
     if (tid < p.K) {
       p.top_logp[own * p.K + tid] = 0.f;
       p.top_ids[own * p.K + tid] = -1;
@@ -491,9 +492,14 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     const double over = s * exp2(-d), ent = kLn2d * (l2 - (t + (ey > 0. ? ey * d : 0.)) / all);
     lse_sh = lse;
     // p_y = 1 / (1 + over): its logarithm keeps its digits where `over` is small
-    p.logp[row] = (float)(over <= 1e300 ? -log1p(over) : kLn2d * (d - l2));
-    p.entropy[row] = ent < 0. ? 0.f : (float)ent;
-    p.lse[row] = (float)lse;
+    const float lp = (float)(over <= 1e300 ? -log1p(over) : kLn2d * (d - l2)), e = ent < 0. ? 0.f : (float)ent;
+    p.logp[row] = lp;
+    p.entropy[row] = e;
+    if (p.state != nullptr) {
+      p.state[row] = (float)lse;
+      p.state[p.n + row] = lp;
+      p.state[2 * p.n + row] = e;
+    }
   }
   if (p.K == 0) return;
   const uint32_t tau = tau_sh;
@@ -655,19 +661,19 @@ __global__ __launch_bounds__(kFewThreads) void stats_grad_few_kernel(const StatG
 struct StatCoefArgs {
   const int32_t* rows;    // [nc]
   const int64_t* nvalid;
-  const float *logp, *entropy, *lse, *g, *e;  // by row; g and e may be nullptr
+  const float *state, *g, *e;  // [3, n], [n], [n]; g and e may be nullptr
   f32x4* coef;            // [nc]
   float *f, *w;           // [nc]: 1, dz_y
-  int64_t nc, c0;
+  int64_t n, nc, c0;
   float inv_t;
 };
 __device__ __forceinline__ f32x4 stat_coef(const StatCoefArgs& p, int64_t k, float& dzy) {
   const int64_t row = p.rows[k];
-  const float lp = p.logp[row], hh = p.entropy[row];
+  const float lse = p.state[row], lp = p.state[p.n + row], hh = p.state[2 * p.n + row];
   const float g = (p.g != nullptr ? p.g[row] : 0.f) * p.inv_t, e = (p.e != nullptr ? p.e[row] : 0.f) * p.inv_t;
   const float py = expf(lp);
   dzy = -g * expm1f(lp) - (e != 0.f ? e * py * (fmaxf(lp, -1e4f) + hh) : 0.f);
-  return f32x4{p.lse[row], -__builtin_fmaf(e, hh, g), -e * kLn2, 0.f};
+  return f32x4{lse, -__builtin_fmaf(e, hh, g), -e * kLn2, 0.f};
 }
 
 __global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
@@ -738,7 +744,8 @@ __global__ __launch_bounds__(256) void stats_unpack_kernel(const UnpackArgs p) {
       if (v >= p.V) continue;
       const bf16x8 e = ld_bf16x8(p.E + k * p.V + v);
       const int64_t part = p.few ? v / kFewBI : 2 * (v / kVT) + (v >> 6 & 1);
-      const float d = p.part[k * p.parts + part][0] - c[0], f = exp2f_fast(d), a = __builtin_fmaf(c[2], d, c[1]);
+      // (minus infinity: a part of nothing else)
+      const float d = fmaxf(p.part[k * p.parts + part][0] - c[0], -1e4f), f = exp2f_fast(d), a = __builtin_fmaf(c[2], d, c[1]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = (float)e[i];
@@ -962,7 +969,8 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
     rw.labels = a.labels;
     rw.logp = a.logp;
     rw.entropy = a.entropy;
-    rw.lse = a.lse;
+    rw.state = a.state;
+    rw.n = a.n;
     rw.top_logp = a.top_logp;
     rw.top_ids = a.top_ids;
     rw.c0 = c0;
@@ -1009,9 +1017,8 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
     StatCoefArgs co{};
     co.rows = rows + c0;
     co.nvalid = nvalid;
-    co.logp = a.logp;
-    co.entropy = a.entropy;
-    co.lse = a.lse;
+    co.state = a.state;
+    co.n = a.n;
     co.g = a.dlogp;
     co.e = a.dentropy;
     co.coef = at<f32x4>(a.ws, L.coef);

@@ -557,13 +557,14 @@ std::pair<Tensor, Tensor> raw_flp_bwd(const Tensor& hidden, const Tensor& weight
 }
 
 // ---------------------------------------------------------------- token statistics
-// What a call returns, and what its backward takes besides: by row of the labels' shape.
+// What a call returns (of the labels' shape), and what its backward takes: copies, so that a caller may change the
+// results in place.
 struct Stats {
-  Tensor logp, entropy, lse, top_logp, top_ids, saved;
+  Tensor logp, entropy, top_logp, top_ids, state, saved;
 };
 
 Stats stats_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels, int64_t ignore_index, double temperature,
-                int64_t top_k, bool keep, at::IntArrayRef shape, int64_t* counts) {
+                int64_t top_k, bool grads, bool keep, at::IntArrayRef shape, int64_t* counts) {
   check_head(hidden, weight, labels);
   // (as int for the library)
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= (1 << 20), "top_k must not be negative, or that large: ", top_k);
@@ -572,7 +573,10 @@ Stats stats_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels
   const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0);
   std::vector<int64_t> top = shape.vec();
   top.push_back(top_k);
-  Stats s{floats(shape, h), floats(shape, h), floats({n}, h), Tensor(), Tensor(), Tensor()};
+  Stats s;
+  s.logp = floats(shape, h);
+  s.entropy = floats(shape, h);
+  if (grads) s.state = floats({3, n}, h);
   if (top_k > 0) {
     s.top_logp = floats(top, h);
     s.top_ids = at::empty(top, h.options().dtype(at::kLong));
@@ -580,7 +584,7 @@ Stats stats_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& labels
   if (keep) s.saved = bytes(api.siq_stats_saved_bytes(n, vocab), h);
   const Tensor ws = bytes(api.siq_stats_fwd_workspace_bytes(n, hdim, vocab, (int)top_k, keep), h);
   check(api.siq_stats_fwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), n, hdim, vocab, ignore_index,
-                          temperature, (int)top_k, fptr(s.logp), fptr(s.entropy), fptr(s.lse), fptr(s.top_logp),
+                          temperature, (int)top_k, fptr(s.logp), fptr(s.entropy), fptr(s.state), fptr(s.top_logp),
                           static_cast<int64_t*>(ptr(s.top_ids)), counts, counts + 1, ptr(s.saved),
                           keep ? s.saved.numel() : 0, ptr(ws), ws.numel(), stream_of(h)),
         "siq_stats_fwd");
@@ -593,8 +597,8 @@ struct TokenStats : torch::autograd::Function<TokenStats> {
                                int64_t* counts) {
     const Tensor h = rows_2d(hidden);
     const bool keep = weight.dim() == 2 && (int64_t)api.siq_stats_saved_bytes(h.size(0), weight.size(0)) <= keep_bytes;
-    Stats s = stats_fwd(h, weight, rows_1d(labels), ignore_index, temperature, top_k, keep, labels.sizes(), counts);
-    ctx->save_for_backward({hidden, weight, labels, s.logp, s.entropy, s.lse, s.saved});
+    Stats s = stats_fwd(h, weight, rows_1d(labels), ignore_index, temperature, top_k, true, keep, labels.sizes(), counts);
+    ctx->save_for_backward({hidden, weight, labels, s.state, s.saved});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["chunk"] = chunk;
@@ -619,11 +623,11 @@ struct TokenStats : torch::autograd::Function<TokenStats> {
     const int64_t n = h.size(0), hdim = h.size(1), vocab = w.size(0), chunk = ctx->saved_data["chunk"].toInt();
     const Tensor dh = ctx->needs_input_grad(0) ? at::empty(h.sizes(), h.options()) : Tensor();
     const Tensor dw = ctx->needs_input_grad(1) ? at::empty(w.sizes(), w.options()) : Tensor();
-    const Tensor& saved = s[6];
+    const Tensor& saved = s[4];
     const bool have = saved.defined();
     const Tensor ws = bytes(api.siq_stats_bwd_workspace_bytes(n, hdim, vocab, chunk, dw.defined(), have), h);
-    check(api.siq_stats_bwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), fptr(s[3]), fptr(s[4]),
-                            fptr(s[5]), fptr(g), fptr(e), n, hdim, vocab, ctx->saved_data["ignore"].toInt(),
+    check(api.siq_stats_bwd(h.data_ptr(), w.data_ptr(), static_cast<const int64_t*>(ptr(y)), fptr(s[3]), fptr(g),
+                            fptr(e), n, hdim, vocab, ctx->saved_data["ignore"].toInt(),
                             ctx->saved_data["temperature"].toDouble(), ptr(saved), have ? saved.numel() : 0, ptr(dh), ptr(dw),
                             chunk, ptr(ws), ws.numel(), stream_of(h)),
           "siq_stats_bwd");
@@ -654,7 +658,7 @@ std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>, Tensor> token_sta
     return {o[0], o[1], o[2], o[3], counts};
   }
   const Stats s =
-      stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, false, labels.sizes(), c);
+      stats_fwd(rows_2d(hidden), weight, rows_1d(labels), ignore_index, temperature, top_k, false, false, labels.sizes(), c);
   if (top_k == 0) return {s.logp, s.entropy, std::nullopt, std::nullopt, counts};
   return {s.logp, s.entropy, s.top_logp, s.top_ids, counts};
 }

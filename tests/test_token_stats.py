@@ -49,21 +49,21 @@ def test_oracle_against_torch_and_differences(temperature):
 
 
 def _fwd(lib, **kw):
-    a = dict(h=FAKE, w=FAKE, y=FAKE, n=300, hdim=256, vocab=1000, ign=-100, t=1.0, k=5, lp=FAKE, ent=FAKE, lse=FAKE, tl=FAKE,
+    a = dict(h=FAKE, w=FAKE, y=FAKE, n=300, hdim=256, vocab=1000, ign=-100, t=1.0, k=5, lp=FAKE, ent=FAKE, state=FAKE, tl=FAKE,
              ti=FAKE, count=FAKE, bad=FAKE, saved=None, sb=0, ws=FAKE)
     a.update(kw)
     a.setdefault("wb", lib.siq_stats_fwd_workspace_bytes(300, 256, 1000, 5, int(a["saved"] is not None)))
-    return lib.siq_stats_fwd(*(a[k] for k in ("h", "w", "y", "n", "hdim", "vocab", "ign", "t", "k", "lp", "ent", "lse", "tl",
+    return lib.siq_stats_fwd(*(a[k] for k in ("h", "w", "y", "n", "hdim", "vocab", "ign", "t", "k", "lp", "ent", "state", "tl",
                                               "ti", "count", "bad", "saved", "sb", "ws", "wb")), None)
 
 
 def _bwd(lib, **kw):
-    a = dict(h=FAKE, w=FAKE, y=FAKE, lp=FAKE, ent=FAKE, lse=FAKE, g=FAKE, e=FAKE, n=300, hdim=256, vocab=1000, ign=-100, t=1.0,
+    a = dict(h=FAKE, w=FAKE, y=FAKE, state=FAKE, g=FAKE, e=FAKE, n=300, hdim=256, vocab=1000, ign=-100, t=1.0,
              saved=None, sb=0, dh=FAKE + (1 << 24), dw=FAKE, chunk=128, ws=FAKE)
     a.update(kw)
     a.setdefault("wb", lib.siq_stats_bwd_workspace_bytes(300, 256, 1000, 128, int(a["dw"] is not None),
                                                          int(a["saved"] is not None)))
-    return lib.siq_stats_bwd(*(a[k] for k in ("h", "w", "y", "lp", "ent", "lse", "g", "e", "n", "hdim", "vocab", "ign", "t",
+    return lib.siq_stats_bwd(*(a[k] for k in ("h", "w", "y", "state", "g", "e", "n", "hdim", "vocab", "ign", "t",
                                               "saved", "sb", "dh", "dw", "chunk", "ws", "wb")), None)
 
 
@@ -71,8 +71,7 @@ def _bwd(lib, **kw):
     (dict(n=-1), INVALID), (dict(n=2 ** 31), INVALID), (dict(hdim=0), INVALID), (dict(hdim=100), UNSUPPORTED),
     (dict(vocab=1001), UNSUPPORTED), (dict(vocab=2 ** 23), INVALID), (dict(h=None), INVALID), (dict(h=FAKE + 8), ALIGN),
     (dict(w=None), INVALID), (dict(w=FAKE + 2), ALIGN), (dict(y=None), INVALID), (dict(t=0.0), INVALID),
-    (dict(t=float("nan")), INVALID), (dict(t=1e-45), INVALID), (dict(lp=None), INVALID), (dict(ent=None), INVALID),
-    (dict(lse=None), INVALID), (dict(saved=FAKE, sb=100), WS), (dict(saved=FAKE + 8, sb=1 << 30), WS), (dict(ws=None), WS),
+    (dict(t=float("nan")), INVALID), (dict(t=1e-45), INVALID), (dict(saved=FAKE, sb=100), WS), (dict(saved=FAKE + 8, sb=1 << 30), WS), (dict(ws=None), WS),
     (dict(wb=64), WS),
 ])
 def test_validation_of_both_directions(lib, kw, code):
@@ -81,10 +80,11 @@ def test_validation_of_both_directions(lib, kw, code):
 
 
 def test_validation_of_one_direction(lib):
-    for kw in (dict(k=-1), dict(k=129), dict(k=9, vocab=8), dict(tl=None), dict(ti=None), dict(count=None), dict(bad=None)):
+    for kw in (dict(k=-1), dict(k=129), dict(k=9, vocab=8), dict(tl=None), dict(ti=None), dict(count=None), dict(bad=None),
+               dict(lp=None), dict(ent=None)):
         assert _fwd(lib, wb=1 << 40, **kw) == INVALID
     assert _fwd(lib, k=129) == INVALID and "top_k must be in [0, 128]" in lib.siq_last_error().decode()
-    assert _bwd(lib, chunk=0, wb=1 << 40) == INVALID
+    assert _bwd(lib, chunk=0, wb=1 << 40) == INVALID and _bwd(lib, state=None) == INVALID
     assert _bwd(lib, dh=FAKE + 8) == ALIGN and _bwd(lib, dw=FAKE + 8) == ALIGN
     assert _bwd(lib, dh=FAKE) == INVALID and _bwd(lib, dh=FAKE + 1024) == INVALID  # over hidden
     assert _bwd(lib, dh=None, dw=None) == OK  # nothing to do
