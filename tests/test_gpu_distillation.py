@@ -148,6 +148,18 @@ def test_a_certain_student_keeps_its_tails_digits(n, kind):
     check(h, w, y, ids, lt, **KINDS[kind])
 
 
+@pytest.mark.parametrize("n", [2, 128, 300])
+@pytest.mark.parametrize("kind", [0, 2, 5])
+def test_one_token_for_all_rows(n, kind):
+    """Every teacher and every label names the same token first: its gradients meet in one row of dW."""
+    h, w, y, ids, lt = make(n, 128, 1000, 3, seed=18, ignored=0.0)
+    ids = torch.where(ids == 999, 5, ids)
+    ids[:, 0] = y[:] = 999
+    lt[:, 0] += 3.0
+    lt = torch.log_softmax(lt, 1) - 0.05
+    check(h, w, y, ids, lt, **KINDS[kind])
+
+
 def test_nothing_counts_no_rows_and_bad_labels():
     h, w, y, ids, lt = make(300, 128, 1000, 5, seed=8)
     hd, wd = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()

@@ -252,6 +252,85 @@ def test_autograd_shapes_types_frozen_and_retained():
     assert (np.abs(np64(g1 - g2)).reshape(60, 128) <= 2 * ref["dh_off"]).all()
 
 
+@pytest.mark.parametrize("keep", [True, False])
+@pytest.mark.parametrize("n", [60, 300])
+def test_results_may_be_changed_in_place(n, keep):
+    h, w, y, up, ent = make(n, 128, 520, seed=16)
+    hd, wd = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+
+    def call(change):
+        out = LP.fused_linear_token_stats(hd, wd, y.to(DEV), 3, keep_bytes=1 << 32 if keep else 0)
+        a, b = out.log_probs, out.entropy
+        if change:
+            a *= 2.0
+            b += 7.0
+            out.top_log_probs.zero_()
+        else:
+            a = 2.0 * a
+        return torch.autograd.grad([a, b], [hd, wd], [up.to(DEV), ent.to(DEV)])
+
+    assert all(torch.equal(a, b) for a, b in zip(call(True), call(False)))
+
+
+@pytest.mark.parametrize("n", [2, 128, 300])
+def test_one_token_for_all_rows(n):
+    h, w, y, up, ent = make(n, 128, 1000, seed=17, ignored=0.0)
+    y[:] = 999
+    check(h, w, y, up, ent)
+
+
+@pytest.mark.parametrize("n", [3, 300])
+def test_more_columns_than_a_row_pass_holds(n):
+    """270,336 columns: rows of more parts than are read once, scores and gradients."""
+    vocab = 270_336
+    h, w, y = on_grid(n, 64, vocab, seed=n)
+    y[-1] = vocab - 1
+    hd, wd = h.to(DEV).requires_grad_(), w.to(DEV)
+    out = LP.fused_linear_token_stats(hd, wd, y.to(DEV), 40)
+    z = h.to(DEV).double() @ wd.double().T.contiguous()
+    key = (z * 4096).round().long() * 2 ** 19 + (vocab - 1 - torch.arange(vocab, device=DEV))
+    want = vocab - 1 - key.topk(40, dim=1).values.remainder(2 ** 19)
+    assert torch.equal(out.top_ids, want)
+    lp = torch.log_softmax(z, 1)
+    off = 2 * ots.SUM + 8 * ots.FP32 * lp.abs().amax(1)
+    assert bool(((out.log_probs.double() - lp.gather(1, y.to(DEV)[:, None])[:, 0]).abs() <= off).all())
+    assert bool(((out.top_log_probs.double() - lp.gather(1, want)).abs() <= off[:, None]).all())
+    H = -(lp.exp() * lp).sum(1)
+    assert bool(((out.entropy.double() - H).abs() <= 3 * off * (1 + H)).all())
+    dh, = torch.autograd.grad(out.entropy.sum(), [hd])
+    dz = -lp.exp() * (lp + H[:, None])
+    want, size = dz @ wd.double(), (2 * dz.abs() + lp.exp()) @ wd.double().abs()
+    assert bool(((dh.double() - want).abs() <= 2.0 ** -8 * (1.1 * size + want.abs())).all())
+
+
+@pytest.mark.parametrize("k", [1, 20, 128])
+@pytest.mark.parametrize("shape", ["random", "rising", "falling", "flat", "late"])
+def test_bounded_alternatives_of_a_real_vocabulary(shape, k):
+    """1,100 rows of 151,936 columns: an eighth of them (or more, for more alternatives) bounds what is written of the others.
+    Logits are exact, so ids are the definition's: ties, sorted logits, all equal ones, and all large ones at the end."""
+    n, vocab = 1100, 151_936
+    print(f"stats bounded {shape} K={k}", flush=True)
+    h, w, y = on_grid(n, 64, vocab, seed=k)
+    if shape != "random":
+        h[:], w[:] = 0, 0
+        h[:, 0] = 1.0
+        place = torch.arange(vocab)
+        w[:, 0] = {"rising": place // 1024 / 4, "falling": (vocab - 1 - place) // 1024 / 4, "flat": torch.zeros(vocab),
+                   "late": (place >= vocab - 300) * 1.0}[shape]
+    y[::7] = -100
+    out = LP.fused_linear_token_stats(h.to(DEV), w.to(DEV), y.to(DEV), k)
+    at = (y >= 0).to(DEV)
+    assert bool((out.top_ids[~at] == -1).all())
+    hd, wd = h.to(DEV).double()[at], w.to(DEV).double()
+    ids, lps = out.top_ids[at], out.top_log_probs[at]
+    for c in range(0, ids.shape[0], 200):
+        z = hd[c:c + 200] @ wd.T.contiguous()
+        key = (z * 4096).round().long() * 2 ** 18 + (vocab - 1 - torch.arange(vocab, device=DEV))
+        assert torch.equal(ids[c:c + 200], vocab - 1 - key.topk(k, dim=1).values.remainder(2 ** 18))
+        want = torch.log_softmax(z, 1).gather(1, ids[c:c + 200])
+        assert bool(((lps[c:c + 200].double() - want).abs() <= ots.SUM + 4 * ots.FP32 * want.abs()).all())
+
+
 def test_gradient_is_a_difference():
     """One direction in ``hidden``, central differences of the fp32 results."""
     h, w, y, up, ent = make(64, 128, 520, seed=12, ignored=0.1)
