@@ -80,6 +80,9 @@ constexpr float kRefLimit = 0x1p60f;
 // columns, in the order of its accumulators, and only groups of eight in which some
 // lane has one are looked at.  Tokens of a lane lie in a row in zk, so nothing is
 // looked up.
+// 11450 rows x 1536 over 151936 columns, 64 tokens a row: 4.70 ms, without lists 4.43
+// (walking the rows' lists and picking accumulators by branches, a whole training call
+// took 17.0 ms instead of 14.1).
 template <bool LISTS>
 __global__ __launch_bounds__(NT) void flce_logits_kernel(const LogitsArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
@@ -264,7 +267,7 @@ __device__ __forceinline__ void sort_labels(uint64_t* sk, const int64_t* y, int6
   sort_keys(sk, np2);
   for (int i = threadIdx.x; i < kIdChunk; i += kRowThreads) keys[base + i] = i < np2 ? sk[i] : kNoKey;
 }
-//
+
 // LISTS: rows with a list of tokens apart.  What they add is not known here: a
 // row's sum over the others is left as it is, and E of rows with redone tiles is
 // brought to the sum's own reference.

@@ -27,6 +27,12 @@
 // one pass over that makes dZ; otherwise the logits GEMM, made again, writes it.
 // The given token is left out: its term is added in fp32 by the products' kernels.
 // The two gradient products follow.
+//
+// Whole calls over 151936 columns: one row x 896 with 20 alternatives 62 us, of which
+// the table is read in 43 (6.3 TB/s); 5670 counted rows x 1536 with 64 alternatives
+// 2.48 ms, the logits alone 2.14 (1.24 PFLOP/s); 1279 counted rows x 1536, frozen
+// head, 1.33 ms, of it 0.16 the pass over what was kept; 2755 x 896 in full training
+// 2.60 ms.
 #include <algorithm>
 
 #include "few.h"
@@ -93,7 +99,10 @@ __device__ __forceinline__ f32x4 stat_part(float zscale, float m, Get z, Keep ke
   return f32x4{m, half_sum(s), half_sum(t), 0.f};
 }
 
-// TOP: Z is written; KEEP: E is.
+// TOP: Z is written; KEEP: E is.  Bounded by the matrix cores and, as nothing covers
+// it, a tile's epilogue of 65536 exponentials: 1279 rows x 1536 that keep E 0.51-0.61 ms
+// (1.0-1.16 PFLOP/s), 2755 x 896 0.75-0.82 (0.9-1.0).  Parts are 64 columns of a
+// wave, so a part's sums need no other wave's.
 template <bool TOP, bool KEEP>
 __global__ __launch_bounds__(NT) void stats_logits_kernel(const StatLogitsArgs p) {
   __shared__ __align__(16) bf16 smem[SMEM];
@@ -214,6 +223,8 @@ constexpr int kFewStages = NB <= 2 ? 3 : 2;  // (64 rows: three buffers; 128: tw
 template <int NB>
 constexpr int kFewSmem = kFewStages<NB> * (kFewBI + 32 * NB) * BK;
 
+// Bounded by memory: over 151936 x 896 one row 43 us (272 MB, 6.3 TB/s), 61 rows with Z
+// 62 us (309 MB, 4.9 TB/s: a copy's rate, reads and writes mixed).
 template <int NB, bool TOP, bool KEEP>
 __global__ __launch_bounds__(kFewThreads) void stats_logits_few_kernel(const StatLogitsArgs p) {
   constexpr int TOK = 32 * NB, NWV = kFewThreads / 64;
@@ -408,7 +419,9 @@ __global__ __launch_bounds__(kRowGroups) void stats_bound_kernel(const BoundArgs
   if (threadIdx.x == 0) p.bound[k] = tau == 0 ? -INFINITY : number_of(tau);
 }
 
-// One workgroup a row.  Columns that reach the bound are listed, usually K or
+// One workgroup a row; bounded by its chain of reads and barriers (a row alone 9 us,
+// 61 rows 8), many rows by the reads of parts (2755 rows without alternatives: 52 MB in
+// 19 us) and of the candidates' logits (3328 rows of 64: 65 us).  Columns that reach the bound are listed, usually K or
 // somewhat more, and each one's rank is how many of the others come before it.
 // Where they are too many (long ties, or a vocabulary of few parts) the K largest
 // are taken one after the other instead.
@@ -431,7 +444,8 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     }
   }
   if (p.rows == nullptr ? !counts : p.c0 + k >= *p.nvalid) return;
-  // the row's parts, read once where a vocabulary has no more than 163,840 columns
+  // the row's parts, read once where there are no more than 1280 (read again for each use: one row 64.1 us in all,
+  // 62.3 so; 61 rows 76.2 and 74.4)
   constexpr int R = 5;
   const f32x4* src = p.part + k * p.parts;
   f32x4 held[R];
@@ -679,7 +693,7 @@ __device__ __forceinline__ f32x4 stat_coef(const StatCoefArgs& p, int64_t k, flo
 __global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
   const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, nv = min(p.nc, *p.nvalid - p.c0);
   if (k >= p.nc) return;
-  if (k >= nv) {  // dZ of the rows that fill up a tile is 0 (dW multiplies it with zeros, which a NaN would survive)
+  if (k >= nv) {  // dZ of the rows that fill up dW's last k-step is 0 (dW multiplies it with zeros, which a NaN would survive)
     p.coef[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     return;
   }
@@ -689,8 +703,9 @@ __global__ __launch_bounds__(256) void stats_coef_kernel(const StatCoefArgs p) {
 
 
 // dZ from the numerators that the forward kept, a workgroup 2048 columns of a row;
-// the rows that fill up a tile are zeroed, and dH of rows whose label does not
-// count.  It reads and writes 2 bytes an element where the logits take 2 hdim flops.
+// the rows that fill up dW's last k-step are zeroed, and dH of rows whose label does
+// not count.  It reads and writes 2 bytes an element where the logits take 2 hdim flops:
+// 2755 rows 334 us (1.67 GB, 5.0 TB/s, a copy's rate), the logits' product 750 again.
 struct UnpackArgs {
   StatCoefArgs c;
   const bf16* E;          // [nc, V]
@@ -727,7 +742,7 @@ __global__ __launch_bounds__(256) void stats_unpack_kernel(const UnpackArgs p) {
           if (ONE_FEW) st_bf16x8(p.Hs + k * p.hdim + c, k < nv ? ld_bf16x8(p.H + src * p.hdim + c) : zero_bf16x8());
         }
     }
-    if (k >= nv + BJ) continue;
+    if (k >= (nv + BK - 1) / BK * BK) continue;
     bf16x8 g = zero_bf16x8();
     if (k < nv) {
       f32x4 c;
@@ -858,7 +873,9 @@ BwdLayout bwd_layout(int64_t n, int64_t hdim, int64_t V, int64_t chunk, bool nee
 
 // Tiles whose parts bound the others': at least K of them, so that the K-th largest of
 // their 2 K parts says something, and three rounds of workgroups, so that the last round
-// of a launch of its own costs little; 0: all in one launch.
+// of a launch of its own costs little; 0: all in one launch.  (5735 rows x 1536 with 64
+// alternatives 2.87 -> 2.49 ms: two fifths of the others are written.  A second bound,
+// from three eighths, costs as much as it saves: 2.48 -> 2.50.)
 int bound_tiles(int nI, int nJ, int K) {
   const int tiles = std::max({nI / 8, K, (3 * kCus + nJ - 1) / nJ});
   return 3 * tiles <= nI ? tiles : 0;
@@ -929,7 +946,8 @@ hipError_t stats_fwd(const StatsArgs& a, hipStream_t stream) {
   c.hc = at<bf16>(a.ws, L.hc);
   c.yc = keep ? at<int64_t>(a.saved, S.yc) : at<int64_t>(a.ws, L.yc);
   c.ref = at<float>(a.ws, L.ref);
-  // few rows are taken as they are, those that do not count among them: the table is read all the same
+  // few rows are taken as they are, those that do not count among them: the table is read all the same (one row 69.4 us
+  // with a compacting launch, 64.1 so; 61 rows 80.6 and 76.2)
   const bool as_is = a.n > 0 && L.few && !keep;
   if (!as_is) launch_compact(c, stream);
   for (int64_t c0 = 0; c0 < a.n; c0 += L.chunk) {
@@ -1007,7 +1025,7 @@ hipError_t stats_bwd(const StatsArgs& a, hipStream_t stream) {
   c.ref = at<float>(a.ws, L.ref);
   c.dh = a.dhidden;
   if (!have) launch_compact(c, stream);
-  // few rows in one chunk, from what was kept: the labels' sums come with dH's
+  // few rows in one chunk, from what was kept: the labels' sums come with dH's (4 rows x 64, both directions, 109 -> 98 us)
   const bool one_few = have && need_dw && L.few && L.nchunks == 1;
   bf16* E = at<bf16>(a.ws, L.E);
   float *f0 = at<float>(a.ws, L.f0), *w0 = at<float>(a.ws, L.w0);
