@@ -80,7 +80,7 @@ constexpr float kRefLimit = 0x1p60f;
 // columns, in the order of its accumulators, and only groups of eight in which some
 // lane has one are looked at.  Tokens of a lane lie in a row in zk, so nothing is
 // looked up.
-// 11450 rows x 1536 over 151936 columns, 64 tokens a row: 4.70 ms, without lists 4.43
+// 11450 rows x 1536 over 151936 columns, 64 tokens a row: 4.7 ms, without lists 4.45
 // (walking the rows' lists and picking accumulators by branches, a whole training call
 // took 17.0 ms instead of 14.1).
 template <bool LISTS>
