@@ -81,6 +81,8 @@ def fused_causal_lm_forward(self, input_ids=None, attention_mask=None, position_
         raise ValueError("return_log_probs needs labels: they say which tokens' log-probabilities are wanted")
     if top_k is not None and not return_log_probs:
         raise ValueError("top_k goes with return_log_probs")
+    if distillation is not None and teacher is None:
+        raise ValueError("distillation's options go with a teacher")
     if teacher is not None and return_log_probs:
         raise ValueError("a call gives log-probabilities or a teacher's loss, not both")
     if teacher is not None and labels is None and kwargs.get("shift_labels") is None:
