@@ -28,7 +28,7 @@
 // The given token is left out: its term is added in fp32 by the products' kernels.
 // The two gradient products follow.
 //
-// Whole calls over 151936 columns: one row x 896 with 20 alternatives 62 us, of which
+// Whole calls over 151936 columns: one row x 896 with 20 alternatives 61 us, of which
 // the table is read in 43 (6.3 TB/s); 5670 counted rows x 1536 with 64 alternatives
 // 2.48 ms, the logits alone 2.14 (1.24 PFLOP/s); 1279 counted rows x 1536, frozen
 // head, 1.33 ms, of it 0.16 the pass over what was kept; 2755 x 896 in full training
@@ -381,21 +381,29 @@ constexpr int kRowGroups = 256;               // threads of a workgroup, and gro
 constexpr int kMostParts = 1024, kMostListed = 1024;
 static_assert(kMaxTopK <= kRowGroups, "a bound is the K-th largest group's");
 
-// The K-th largest of the keys of 256 groups in LDS (behind a barrier), bit by bit, by one
-// wave.  (Every thread counting the keys above its own: 2.47 -> 2.54 ms at 8192 rows.)
+// The K-th largest of the keys of 256 groups in LDS (behind a barrier), without its last
+// eight bits, two bits at a time, by one wave.  (Every thread counting the keys above its
+// own: 2.47 -> 2.54 ms at 8192 rows.)
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t* best_sh, int K, int lane) {
   constexpr int N = kRowGroups / 64;
   uint32_t b[N], tau = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) b[i] = best_sh[64 * i + lane];
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = tau | (1u << bit);
-    int c = 0;
+#pragma unroll 1
+  for (int bit = 30; bit >= 8; bit -= 2) {
+    int c[3] = {0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < N; ++i) c += __popcll(__ballot(b[i] >= cand));
-    if (c >= K) tau = cand;
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+      for (int i = 0; i < N; ++i) c[q] += __popcll(__ballot(b[i] >= (tau | (uint32_t)(q + 1) << bit)));
+    tau |= (uint32_t)(c[2] >= K ? 3 : c[1] >= K ? 2 : c[0] >= K ? 1 : 0) << bit;
   }
   return tau;
+}
+
+// ... as a number (none, or what lost bits fell below: minus infinity).
+__device__ __forceinline__ float bound_of(uint32_t tau) {
+  return tau < 0x007fffffu ? -INFINITY : number_of(tau);
 }
 
 // The bound that the first `parts` parts of a row give.
@@ -416,12 +424,13 @@ __global__ __launch_bounds__(kRowGroups) void stats_bound_kernel(const BoundArgs
   __syncthreads();
   if (threadIdx.x >= 64) return;
   const uint32_t tau = kth_largest(best_sh, p.K, threadIdx.x);
-  if (threadIdx.x == 0) p.bound[k] = tau == 0 ? -INFINITY : number_of(tau);
+  if (threadIdx.x == 0) p.bound[k] = bound_of(tau);
 }
 
-// One workgroup a row; bounded by its chain of reads and barriers (a row alone 9 us,
-// 61 rows 8), many rows by the reads of parts (2755 rows without alternatives: 52 MB in
-// 19 us) and of the candidates' logits (3328 rows of 64: 65 us).  Columns that reach the bound are listed, usually K or
+// One workgroup a row; bounded by its chain of reads and barriers, and by instructions
+// that are read for the first time (a row alone 7 us; a branch for each part and column
+// 9), many rows by the reads of parts (2755 rows without alternatives: 52 MB in 19 us)
+// and of the candidates' logits (3328 rows of 64: 60 us).  Columns that reach the bound are listed, usually K or
 // somewhat more, and each one's rank is how many of the others come before it.
 // Where they are too many (long ties, or a vocabulary of few parts) the K largest
 // are taken one after the other instead.
@@ -523,34 +532,52 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
     p.top_logp[row * p.K + rank] = (float)(((double)zi * (double)p.zscale - lse_sh) * kLn2d);
     p.top_ids[row * p.K + rank] = (int64_t)(uint32_t)~(uint32_t)key;
   };
-  each_part([&](int i, const f32x4& x) {
-    if (order_of(x[3]) < tau) return;
-    const int at = atomicAdd(&nparts_sh, 1);  // (in any order: ranks make one)
+  // Which of a thread's parts, and of their columns, reach it is a bit each, and a loop lists them: branches of their own
+  // each wait for instructions that nothing has run before (90 alternatives of 49152: 18.8 us, 10.8 so; 54 of 151936: 13.1
+  // and 8.3).
+  auto list_part = [&](int i) {  // (in any order: ranks make one)
+    const int at = atomicAdd(&nparts_sh, 1);
     if (at < kMostParts) part_sh[at] = i;
-  });
+  };
+  const float least = bound_of(tau);
+  uint32_t reach = 0;
+#pragma unroll
+  for (int u = 0; u < R; ++u) reach |= tid + T * u < p.parts && held[u][3] >= least ? 1u << u : 0u;
+#pragma unroll 1
+  for (; reach != 0; reach &= reach - 1) list_part(tid + T * (int)__builtin_ctz(reach));
+#pragma unroll 1
+  for (int i = tid + T * R; i < p.parts; i += T)
+    if (src[i][3] >= least) list_part(i);
   __syncthreads();
-  const int np = nparts_sh, c = tid & 127, off = p.few ? c : (c & 63) + 128 * (c >> 6);
-  auto column = [&](int part) {
-    return (p.few ? 128 * (int64_t)part : 256 * (int64_t)(part >> 1) + 64 * (part & 1)) + off;
+  const int np = nparts_sh;
+  auto column = [&](int part, int c) {  // the c-th of a part
+    return p.few ? 128 * (int64_t)part + c : 256 * (int64_t)(part >> 1) + 64 * (part & 1) + (c & 63) + 128 * (c >> 6);
   };
   if (np <= kMostParts) {
-    constexpr int U = 8, STEP = T / 128;
-    for (int q0 = tid / 128; q0 < np; q0 += STEP * U) {
-      float x[U];
-      int64_t v[U];
+    constexpr int U = 8, STEP = T / 32;  // 64 parts in flight
+    for (int q0 = tid / 32; q0 < np; q0 += STEP * U) {
+      f32x4 x[U];
+      uint32_t there = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int q = q0 + STEP * u, part = part_sh[min(q, np - 1)];
-        v[u] = column(part);
-        if (q >= np || v[u] >= p.V) v[u] = -1;
-        x[u] = v[u] >= 0 ? z[v[u]] : 0.f;
+        const int q = q0 + STEP * u;
+        const int64_t v = column(part_sh[min(q, np - 1)], 4 * (tid & 31));
+        there |= q < np && v < p.V ? 15u << (4 * u) : 0u;
+        x[u] = *reinterpret_cast<const f32x4*>(z + min(v, p.V - 4));
       }
+      reach = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (v[u] >= 0 && order_of(x[u]) >= tau) {
-          const int at = atomicAdd(&n_sh, 1);
-          if (at < kMostListed) listed_sh[at] = order_of(x[u], v[u]);
-        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reach |= x[u][i] < least ? 0u : 1u << (4 * u + i);  // (what is not a number does)
+      reach &= there;
+#pragma unroll 1
+      for (; reach != 0; reach &= reach - 1) {
+        const int b = (int)__builtin_ctz(reach);
+        const int64_t vb = column(part_sh[q0 + STEP * (b / 4)], 4 * (tid & 31) + b % 4);
+        const int at = atomicAdd(&n_sh, 1);
+        if (at < kMostListed) listed_sh[at] = order_of(z[vb], vb);
+      }
     }
   }
   __syncthreads();
@@ -568,7 +595,7 @@ __global__ __launch_bounds__(kRowGroups) void stats_row_kernel(const StatRowArgs
   for (int r = 0; r < p.K; ++r) {
     uint64_t top = 0;
     for (int i = tid / 128; i < p.parts; i += T / 128) {
-      const int64_t v = column(i);
+      const int64_t v = column(i, tid & 127);
       if (v >= p.V || order_of(src[i][3]) < tau) continue;
       const uint64_t key = order_of(z[v], v);
       if (key < last && key > top) top = key;

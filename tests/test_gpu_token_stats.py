@@ -112,6 +112,22 @@ def test_rows_without_a_difference(n, vocab):
     assert float((out.top_log_probs.double() + np.log(vocab)).abs().max()) <= off
 
 
+@pytest.mark.parametrize("n", [3, 100, 300])
+@pytest.mark.parametrize("offset", [-2048.0, 2048.0])
+@pytest.mark.parametrize("features", [2, 128])
+def test_logits_with_a_large_part_in_common(n, offset, features):
+    """Logits next to +-2048, exact in fp32 (steps of 2^-12): apart by less than 0.01 all of them, or by some units."""
+    h, w, y = on_grid(n, 128, 4104, seed=n)
+    h[:, features:] = 0
+    h[:, 0], w[:, 0] = 2048.0, offset / 2048
+    for k in (1, 64):
+        ref = ots.linear_token_stats(np64(h), np64(w), y.numpy(), k)
+        out = LP.fused_linear_token_stats(h.to(DEV), w.to(DEV), y.to(DEV), k)
+        check_top(out, ref, n, True)
+        for name, got in (("logp", out.log_probs), ("entropy", out.entropy)):
+            assert (np.abs(np64(got) - ref[name]) <= ref[name + "_off"]).all(), name
+
+
 @pytest.mark.parametrize("n", [5, 200])
 def test_sorted_logits_in_either_direction(n):
     """All large logits beside one another: parts of rows that hold more than their share of the alternatives."""
