@@ -29,7 +29,7 @@
 // Bounded by the products: 11450 counted rows x 1536 over 151936 columns, 64 tokens a
 // row, all gradients, 13.95 ms (16.0 TFLOP, 1.15 PFLOP/s; what is not a product takes
 // 0.5), loss alone of 3441 rows x 896 0.95 ms.  Few rows by memory, the table read twice
-// and its gradient written: 48 rows x 896 228 us, 0.82 GB in 191 us of products.
+// and its gradient written: 48 rows x 896 228 us, 0.82 GB in 192 us of products.
 #include <algorithm>
 
 #include "distill.h"
@@ -72,14 +72,17 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
-// Workgroup k: the k-th counted row's operands, where there is one (its label, or -1),
-// and what belongs to row k where its label does not count.
-__device__ __forceinline__ int64_t few_compact(const FewPrep& p, int64_t V, int64_t& src) {
+// Workgroup k: the k-th counted row, where there is one.
+struct FewRow {
+  int nv, nbad, at;  // rows that count, bad labels, the row (-1: none)
+  bool counts;       // row k's label does
+  int64_t y;         // the label, or -1
+};
+__device__ __forceinline__ FewRow few_row(const FewPrep& p, int64_t V) {
   constexpr int G = kFewRows / 64;
-  __shared__ float dot_sh[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, k = blockIdx.x;
+  const int lane = threadIdx.x & 63, k = blockIdx.x;
   int nv = 0, nbad = 0, at = -1;
-  bool counts = false;  // row k
+  bool counts = false;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int64_t v = 64 * g + lane < p.n ? p.labels[64 * g + lane] : p.ignore_index;
@@ -92,7 +95,14 @@ __device__ __forceinline__ int64_t few_compact(const FewPrep& p, int64_t V, int6
     counts = counts || (k / 64 == g && (m >> (k % 64) & 1));
     nv += __popcll(m);
   }
-  const int64_t y = at >= 0 ? p.labels[at] : -1;
+  return {nv, nbad, at, counts, at >= 0 ? p.labels[at] : -1};
+}
+
+// Its operands, and what belongs to row k where its label does not count.
+__device__ __forceinline__ void few_compact(const FewPrep& p, const FewRow& r) {
+  __shared__ float dot_sh[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, k = blockIdx.x, at = r.at;
+  const int64_t y = r.y;
   float dot = 0.f;
   for (int64_t c = 8 * (int64_t)tid; c < p.hdim; c += 8 * 256) {
     bf16x8 x = zero_bf16x8();
@@ -103,7 +113,7 @@ __device__ __forceinline__ int64_t few_compact(const FewPrep& p, int64_t V, int6
       for (int i = 0; i < 8; ++i) dot = __builtin_fmaf((float)x[i], (float)wy[i], dot);
     }
     st_bf16x8(p.hc + k * p.hdim + c, x);
-    if (!counts && p.dh != nullptr) st_bf16x8(p.dh + k * p.hdim + c, zero_bf16x8());
+    if (!r.counts && p.dh != nullptr) st_bf16x8(p.dh + k * p.hdim + c, zero_bf16x8());
   }
   dot = wave_sum(dot);
   if (lane == 0) dot_sh[w] = dot;
@@ -113,12 +123,10 @@ __device__ __forceinline__ int64_t few_compact(const FewPrep& p, int64_t V, int6
     p.y[k] = y;
     if (at >= 0) p.rows[k] = at;
     if (k == 0) {
-      *p.nvalid = p.counts[0] = nv;
-      p.counts[1] = nbad;
+      *p.nvalid = p.counts[0] = r.nv;
+      p.counts[1] = r.nbad;
     }
   }
-  src = at;
-  return y;
 }
 
 struct ListArgs {
@@ -143,7 +151,7 @@ struct ListArgs {
 // place in the list how many other kept keys are less.  Tokens of probability zero and
 // ids of -1 are not there; of equal ids the first stays.  The bits are set in LDS,
 // kListSpan columns at a time.  Few rows are bounded by the chain of steps (48 rows,
-// compaction and all, 10 us), many by the bits (6912 rows 50 us, 145 MB).
+// compaction and all, 9 us), many by the bits (6912 rows 50 us, 145 MB).
 constexpr int kListThreads = 256, kListSpan = 1 << 17;
 static_assert(kMaxTeacher + 1 <= kListThreads, "a thread a token");
 // How many of the first n keys (in fours; the last ones none) are less than x.
@@ -168,8 +176,12 @@ __global__ __launch_bounds__(kListThreads) void distill_list_kernel(const ListAr
   const int tid = threadIdx.x, K = p.K;
   const int64_t k = blockIdx.x;
   int64_t row = -1, y = -1;
-  if (FEW && p.few.labels != nullptr) {
-    y = few_compact(p.few, p.V, row);
+  const bool prepare = FEW && p.few.labels != nullptr;
+  FewRow found{};
+  if (prepare) {
+    found = few_row(p.few, p.V);
+    row = found.at;
+    y = found.y;
   } else if (k < min(p.nc, *p.nvalid - p.c0)) {
     row = p.rows[k];
     y = p.y[k];
@@ -189,6 +201,7 @@ __global__ __launch_bounds__(kListThreads) void distill_list_kernel(const ListAr
   }
   if (id >= 0) mine = (uint32_t)(id / VT * VT + list_place(id % VT, FEW)) << 8 | (tid < K ? (uint32_t)tid : 255u);
   if (tid < kMaxTeacher + 4) key_sh[tid] = mine;
+  if (prepare) few_compact(p.few, found);
   __syncthreads();
   // a token is kept unless the same one has a lower key: no key lies between (tile, place) * 256 and its own
   const bool kept = mine != kNone && less_than(key_sh, K + 1, mine) == less_than(key_sh, K + 1, mine & ~255u);
@@ -461,7 +474,8 @@ __global__ __launch_bounds__(1024) void distill_loss_kernel(const LossArgs p) {
 
 // Few rows: a workgroup a row adds its tiles' sums (E of rows with redone tiles is
 // brought to the largest of their references, as flce_row_kernel does), one wave of it does
-// the row's math, and all scale its hidden state for dW.  A chain of latencies: 12 us.
+// the row's math, and all scale its hidden state for dW.  A chain of latencies: 10 us (12
+// where the sums were read twice, a few at a time).
 __global__ __launch_bounds__(256) void distill_row_few_kernel(const RowMathArgs p) {
   constexpr int T = 256, NWV = T / 64;
   __shared__ double s_sh[NWV];
@@ -471,25 +485,40 @@ __global__ __launch_bounds__(256) void distill_row_few_kernel(const RowMathArgs 
   if (k >= nv) return;
   const float rf = p.ref[k];
   float m = rf;  // the reference of the sum: the row's, or a redone tile's above it
+  // the sums of tiles, all on their way at once where there are no more than 1280
+  constexpr int R = 5;
+  float held[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) held[u] = p.spart[min((int64_t)(tid + T * u), p.nvt - 1) * p.ldp + k];
+  double sum = 0.;
   bool redone = false;
-  for (int64_t t = tid; t < p.nvt; t += T)
-    if (p.spart[t * p.ldp + k] < 0.f) {
-      redone = true;
-      m = fmaxf(m, p.mpart[t * p.ldp + k]);
-    }
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const float s = tid + T * u < p.nvt ? held[u] : 0.f;
+    redone = redone || s < 0.f;
+    sum += (double)s;
+  }
+#pragma unroll 1
+  for (int64_t t = tid + T * R; t < p.nvt; t += T) {
+    const float s = p.spart[t * p.ldp + k];
+    redone = redone || s < 0.f;
+    sum += (double)s;
+  }
   redone = __syncthreads_or(redone);
   if (redone) {
+    for (int64_t t = tid; t < p.nvt; t += T)
+      if (p.spart[t * p.ldp + k] < 0.f) m = fmaxf(m, p.mpart[t * p.ldp + k]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (lane == 0) m_sh[w] = m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NWV; ++i) m = fmaxf(m, m_sh[i]);
-  }
-  double sum = 0.;
-  for (int64_t t = tid; t < p.nvt; t += T) {
-    const float s = p.spart[t * p.ldp + k];
-    sum += redone ? (double)fabsf(s) * exp2((double)((s < 0.f ? p.mpart[t * p.ldp + k] : rf) - m)) : (double)s;
+    sum = 0.;
+    for (int64_t t = tid; t < p.nvt; t += T) {
+      const float s = p.spart[t * p.ldp + k];
+      sum += (double)fabsf(s) * exp2((double)((s < 0.f ? p.mpart[t * p.ldp + k] : rf) - m));
+    }
   }
   sum = wave_sum(sum);
   if (lane == 0) s_sh[w] = sum;
