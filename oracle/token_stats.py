@@ -33,8 +33,9 @@ def log_softmax(z):
 
 def linear_token_stats(hidden, weight, labels, top_k=0, dlogp=None, dentropy=None, temperature=1.0, ignore_index=-100,
                        roundings=1):
-    """dict(logp, entropy, count, bad, order, z, off): ``order`` the tokens of each counted row by falling logit (equal ones
-    by id), ``off`` what the logits of a row may be off by; ``logp_off`` and ``entropy_off`` follow from it.
+    """dict(logp, entropy, count, bad, at, z, off): ``at`` the counted rows, ``off`` what their logits may be off by;
+    ``logp_off`` and ``entropy_off`` follow from it.  With ``top_k`` also ``top_ids``, each row's tokens by falling logit
+    (equal ones by id; -1 in rows that do not count).
 
     With upstream gradients also dh and dw, and ``dh_off`` / ``dw_off``: each element of dZ but the given token's rounded
     ``roundings`` times to bf16 (the first of them before a logarithm is taken, where there are two), and the result once.

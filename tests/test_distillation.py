@@ -156,3 +156,16 @@ def test_a_model_with_a_teacher_needs_labels_and_the_gpu():
         model(input_ids=ids, labels=ids, return_log_probs=True, top_k=4)
     with pytest.raises(ValueError, match="top_k goes with return_log_probs"):
         model(input_ids=ids, labels=ids, top_k=4)
+
+
+def test_distillation_options_need_a_teacher():
+    transformers = pytest.importorskip("transformers")
+    from siq_vl_amd.text_model import enable_fused_cross_entropy
+
+    cfg = transformers.Qwen2Config(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=1,
+                                   num_attention_heads=2, num_key_value_heads=1, use_cache=False)
+    model = transformers.Qwen2ForCausalLM(cfg)
+    enable_fused_cross_entropy(model)
+    ids = torch.randint(0, 64, (1, 5))
+    with pytest.raises(ValueError, match="go with a teacher"):
+        model(input_ids=ids, labels=ids, distillation={"ce_weight": 0.5})

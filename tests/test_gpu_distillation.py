@@ -460,3 +460,12 @@ def test_a_model_learns_from_a_model():
     assert abs(float(summed.loss.detach()) - float(out.loss.detach())) <= 1e-6 * float(out.loss.detach())
     out.loss.backward()
     assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in student.parameters())
+
+
+@pytest.mark.parametrize("n", [8, 130])
+@pytest.mark.parametrize("wscale", [0.05, 2.0])
+def test_more_columns_than_a_row_pass_holds(n, wscale):
+    """270,336 columns: more tiles than a row of few takes at once, and lists of three spans; formed again or not."""
+    data = make(n, 64, 270_336, 7, seed=n, wscale=wscale)
+    data[3][0, 0], data[3][1, 1] = 270_335, 131_072  # (at a span's borders)
+    check(*data, redone=wscale > 1, **KINDS[2])
